@@ -226,6 +226,67 @@ MOE_API int moe_block_forward(moe_ctx* ctx, int layer, int T, const uint16_t* h2
 MOE_API int moe_ep_export(moe_ctx* ctx, void* buf, int cap);
 MOE_API int moe_ep_import(moe_ctx* ctx, const void* records, int world);
 
+/* ---- 8-bit floating point: e4m3 values with one fp32 scale for each 128 ----
+ *
+ * An e4m3 matrix [rows, cols] has a scale for each 128 columns of a row (activations) or of 128 rows
+ * (weights); the last block of a row or column may be partial.  The value is q * scale.  These calls
+ * keep nothing in the context but the device-side status (a bounded wait that gave up, an expert
+ * index out of range: MOE_F_SYNC or moe_status) and the launch count: their working memory is the
+ * caller's, so calls on several streams, and captured graphs, may overlap if their buffers differ.
+ * Device pointers, 16-byte aligned; workspaces 256-byte aligned, their contents of no meaning before
+ * or after a call.
+ *
+ * moe_quantize_fp8: x [batch][rows, cols] bf16 or fp32 (dtype MOE_DT_*), cols a multiple of 16; groups of
+ * 128 columns and block_rows (1 or 128) rows of one matrix.
+ *   scale [batch][ceil(rows / block_rows), ceil(cols / 128)] = the smallest power of two >= 2^-126 with
+ *     max|x| <= 448 scale, 1 for a group of zeros;   q = x / scale, rounded once to e4m3 (ties to even).
+ * Infinities and NaN become NaN and take no part in the maximum.
+ *
+ * moe_matmul_fp8: out [M, N] (bf16 or fp32) = x . w^T with fp32 sums; x [M, K] scaled per row and 128
+ * columns (x_scale [M, ceil(K / 128)]), w [N, K] per 128 x 128 block (w_scale [ceil(N / 128),
+ * ceil(K / 128)]).  Any scales, not powers of two alone.  K a multiple of 16, at most 16384.
+ *
+ * moe_experts_fp8: the routed experts on e4m3 weights, with the caller's routing (moe_route's topk_idx
+ * and topk_w [T, top_k]); H, F, E and top_k are the context's:
+ *   x_q = quantised x;  g, u = gate, up . x_q;  a = quantised g / (1 + exp(-g)) * u  (128 columns of F);
+ *   out[t] (+)= sum_k topk_w[t, k] * down . a,  bf16 or fp32
+ * gate_up [E][2][F, H] (gate rows, then up rows), gate_up_scale [E][2][ceil(F / 128), ceil(H / 128)], down
+ * [E][H, F], down_scale [E][ceil(H / 128), ceil(F / 128)].  A negative topk_idx is no
+ * expert; one of E or more is MOE_EINVAL in the device-side status, and skipped.
+ * T * top_k <= 2^20, whatever max_tokens is.  MOE_F_ACCUMULATE: out += (fp32 only).  The workspace
+ * has moe_experts_fp8_workspace bytes (-1: T out of range). */
+#define MOE_DT_BF16 0
+#define MOE_DT_F32 1
+MOE_API int moe_quantize_fp8(moe_ctx* ctx, const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols,
+                             int block_rows, uint8_t* q, float* scale, int flags, void* stream);
+MOE_API int moe_matmul_fp8(moe_ctx* ctx, int64_t M, int64_t N, int64_t K, const uint8_t* x, const float* x_scale,
+                           const uint8_t* w, const float* w_scale, void* out, int out_dtype, int flags, void* stream);
+MOE_API int64_t moe_experts_fp8_workspace(moe_ctx* ctx, int T);
+MOE_API int moe_experts_fp8(moe_ctx* ctx, int T, const uint16_t* x, const uint8_t* gate_up, const float* gate_up_scale,
+                            const uint8_t* down, const float* down_scale, const int32_t* topk_idx, const float* topk_w,
+                            void* out, int out_dtype, void* workspace, int64_t workspace_bytes, int flags, void* stream);
+
+/* ---- The router's load-balance loss, its per-expert counts and its gradient ----
+ *
+ * logits [T, E] fp32 and the choices topk_idx [T, top_k] (negative: none); E, top_k and the scoring are
+ * the context's, T is not bound by max_tokens.  offsets [B + 1] (device, non-decreasing, within [0, T])
+ * are the sequences' first tokens; NULL with B = 1 is one sequence of all T.  Tokens outside every
+ * sequence, and those with mask [T] == 0 (NULL: none), do not count and get a zero gradient; nothing
+ * of them reaches a result.  With n_b tokens that count, c_be choices of expert e among them, and p_t
+ * the softmax of the logits (sigmoid scoring: s / (sum s + 1e-20), without the correction bias):
+ *   f_be = E c_be / (top_k n_b);  P_be = sum_t p_te / n_b;  loss = mean over b with n_b > 0 of f_b . P_b
+ * (0 if there are none).  counts [B, E] = c, tokens [B + 1] = n and, last, the number of b with n_b > 0.
+ * The backward call takes both and gives dlogits [T, E] = grad[0] (NULL: 1) * d loss / d logits, the
+ * counts being constants.  Results do not depend on timing.  An index of E or more, or offsets out
+ * of order, are MOE_EINVAL in the device-side status.  workspace: moe_balance_loss_workspace bytes. */
+MOE_API int64_t moe_balance_loss_workspace(moe_ctx* ctx, int64_t T, int B);
+MOE_API int moe_balance_loss(moe_ctx* ctx, int64_t T, const float* logits, const int32_t* topk_idx, const int32_t* offsets,
+                             int B, const uint8_t* mask, float* loss, int32_t* counts, int32_t* tokens, void* workspace,
+                             int64_t workspace_bytes, int flags, void* stream);
+MOE_API int moe_balance_loss_backward(moe_ctx* ctx, int64_t T, const float* logits, const int32_t* offsets, int B,
+                                      const uint8_t* mask, const int32_t* counts, const int32_t* tokens, const float* grad,
+                                      float* dlogits, int flags, void* stream);
+
 /* The router's exponential, y[i] = exp(x[i]) rounded once to fp32 (correctly rounded), on the
  * calling thread's current device, asynchronously on `stream`; x and y are device pointers.  It is
  * the exp of the softmax numerators (host.rs.tpl:249, `(v - m).exp()`) and of the sigmoid

@@ -10,7 +10,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # torch-dependent API loaded on first use so `import npu_offload_b200` stays light
-    if name in ("MoEDataPlane", "gpu_moe", "set_threads", "as_bf16"):
+    if name in ("MoEDataPlane", "Fp8", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"):
         from . import moe
         return getattr(moe, name)
     raise AttributeError(name)

@@ -20,6 +20,7 @@ MOE_OPT_RING_STAGES, MOE_OPT_STAGE_BYTES, MOE_OPT_PREFILL_MIN_T, MOE_OPT_PREFILL
 MOE_OPT_LAYER_SLOTS, MOE_OPT_SHARED_INTER, MOE_OPT_Q8_UNIT_COST, MOE_OPT_REDUCERS, MOE_OPT_LATE_BYTES = 9, 10, 11, 12, 13
 MOE_OPT_PLANNER = 14
 MOE_EP_RECORD_BYTES = 256
+MOE_DT_BF16, MOE_DT_F32 = 0, 1
 
 STATUS_NAMES = {0: "MOE_OK", 1: "MOE_EINVAL", 2: "MOE_ENONFINITE", 3: "MOE_ECUDA", 4: "MOE_ENOMEM",
                 5: "MOE_ESTATE", 6: "MOE_ETIMEOUT", 7: "MOE_ECOMM"}
@@ -40,6 +41,7 @@ class MoEError(RuntimeError):
 
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
+_i64 = ctypes.c_int64
 _SIGS = {
     "moe_abi_version": (_i, []),
     "moe_last_error": (ctypes.c_char_p, []),
@@ -62,6 +64,13 @@ _SIGS = {
     "moe_launch_count": (ctypes.c_int64, [_vp]),
     "moe_ck_moe3_noalloc": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i, _vp]),
     "moe_router_exp": (_i, [_vp, _vp, ctypes.c_int64, _vp]),
+    "moe_quantize_fp8": (_i, [_vp, _vp, _i, _i64, _i64, _i64, _i, _vp, _vp, _i, _vp]),
+    "moe_matmul_fp8": (_i, [_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp]),
+    "moe_experts_fp8_workspace": (_i64, [_vp, _i]),
+    "moe_experts_fp8": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
+    "moe_balance_loss_workspace": (_i64, [_vp, _i64, _i]),
+    "moe_balance_loss": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
+    "moe_balance_loss_backward": (_i, [_vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "moe_load_shared": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i]),
     "moe_shared_router": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp]),
     "moe_combine_residual": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _vp]),

@@ -16,7 +16,7 @@ LIB = os.path.join(HERE, "libmoe_dp.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["moe_dp.cu", "route.cu", "experts.cu", "decode.cu", "noalloc.cu", "prefill.cu", "prefill_tc.cu",
-           "block.cu"]
+           "block.cu", "fp8_quant.cu", "fp8_gemm.cu", "balance.cu"]
 
 
 def cute_include():

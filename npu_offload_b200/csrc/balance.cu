@@ -1,0 +1,360 @@
+// Load-balance loss of a router and its gradient.
+//
+// Sequence b holds n_b tokens that count.  With c_be the pairs (token, choice) of the sequence on
+// expert e and p_t the token's scores over all experts (softmax, or sigmoid s divided by
+// S = sum s + 1e-20):
+//   f_be = E c_be / (K n_b)      P_be = (1 / n_b) sum_t p_te      L = 1/B' sum_b sum_e f_be P_be
+// over the B' sequences with n_b > 0.  The counts are constants, so
+//   softmax:  dL/dl_te = 1/(B' n_b) p_te (f_be - sum_j f_bj p_tj)
+//   sigmoid:  dL/dl_te = 1/(B' n_b) s_te (1 - s_te) / S (f_be - sum_j f_bj p_tj)
+// Nothing is kept of the scores: the backward pass computes them again from the logits, which costs
+// the same read as keeping them would.  Both passes are bounded by HBM: T E 4 bytes read, and T E 4
+// bytes written by the backward pass.
+//
+// Forward: unit u of a sequence is a run of kept chunk tokens; a CTA sums p over a unit (a warp a row,
+// a lane every 32nd expert, 32-bit sums over at most chunk / 8 rows, then the warps in order) and
+// counts its choices with integer atomics in shared memory, and stores both sums.  The second kernel,
+// a cluster of eight CTAs a sequence, adds the units in order (in 64 bits) and forms f . P; the last
+// cluster to finish adds the sequences in order.  No sum depends on timing.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "balance.h"
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace moe {
+
+constexpr int kBalThreads = 256, kBalWarps = kBalThreads / 32;
+constexpr int kBalCluster = 8;  // second kernel: CTAs a sequence, 32 experts each (E <= 256)
+
+// Tokens a unit: two rows a warp, more once there are four units for every SM.
+static int balance_chunk(int T, int sm_count) {
+    const int per = (T + 4 * sm_count - 1) / (4 * sm_count);
+    return std::max(16, (per + 15) / 16 * 16);
+}
+static int balance_units(int T, int B, int chunk) { return T / chunk + B; }
+
+struct BalanceWs {
+    float* p;          // [units, E]
+    int32_t* c;        // [units, E]
+    int32_t* n;        // [units]
+    float* loss;       // [B]
+    uint32_t* ticket;  // [1]
+    size_t bytes;
+};
+static BalanceWs balance_layout(void* ws, int E, int B, int units) {
+    BalanceWs w;
+    char* p = static_cast<char*>(ws);
+    size_t o = 0;
+    auto take = [&](size_t n) {
+        char* r = p + o;
+        o += (n + 255) / 256 * 256;
+        return r;
+    };
+    w.p = (float*)take(sizeof(float) * units * E);
+    w.c = (int32_t*)take(sizeof(int32_t) * units * E);
+    w.n = (int32_t*)take(sizeof(int32_t) * units);
+    w.loss = (float*)take(sizeof(float) * B);
+    w.ticket = (uint32_t*)take(sizeof(uint32_t));
+    w.bytes = o;
+    return w;
+}
+size_t balance_workspace(int T, int E, int B, int sm_count) {
+    return balance_layout(nullptr, E, B, balance_units(T, B, balance_chunk(T, sm_count))).bytes;
+}
+
+// Sequence b's tokens [first, last), clipped to the T there are; an offset that is out of order or
+// out of range is an error (and the sequence empty).
+__device__ __forceinline__ void sequence(const int32_t* offsets, int b, int T, int& first, int& last) {
+    if (!offsets) {
+        first = 0, last = T;
+        return;
+    }
+    first = __ldg(offsets + b), last = __ldg(offsets + b + 1);
+    if (first < 0 || last < first || last > T) first = last = 0;
+}
+__device__ __forceinline__ bool offsets_bad(const int32_t* offsets, int b, int T) {
+    if (!offsets) return false;
+    const int first = __ldg(offsets + b), last = __ldg(offsets + b + 1);
+    return first < 0 || last < first || last > T;
+}
+// The unit of chunk j of sequence b is offsets[b] / chunk + b + j: it grows with (b, j), and no two
+// have the same one, since a sequence has at most offsets[b + 1] / chunk - offsets[b] / chunk + 1.
+__device__ __forceinline__ int first_unit(const int32_t* offsets, int b, int chunk) {
+    return offsets ? max(__ldg(offsets + b), 0) / chunk + b : 0;
+}
+
+// Scores of one token: e[j] = exp(l - max l) or sigmoid(l) of expert lane + 32 j (0 behind the last),
+// and 1 / their sum.
+template <int NE, bool SIG>
+__device__ __forceinline__ float scores(const float (&l)[NE], int E, float (&e)[NE]) {
+    const int lane = threadIdx.x & 31;
+    float sum = 0.f;
+    if (SIG) {
+#pragma unroll
+        for (int j = 0; j < NE; j++) {
+            e[j] = lane + 32 * j < E ? 1.f / (1.f + expf(-l[j])) : 0.f;
+            sum += e[j];
+        }
+        return 1.f / (warp_sum(sum) + 1e-20f);
+    }
+    float m = -__int_as_float(0x7f800000);
+#pragma unroll
+    for (int j = 0; j < NE; j++)
+        if (lane + 32 * j < E) m = fmaxf(m, l[j]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+#pragma unroll
+    for (int j = 0; j < NE; j++) {
+        e[j] = lane + 32 * j < E ? expf(l[j] - m) : 0.f;
+        sum += e[j];
+    }
+    return 1.f / warp_sum(sum);
+}
+
+template <int NE>
+__device__ __forceinline__ void load_row(const float* row, int E, float (&l)[NE]) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int j = 0; j < NE; j++) l[j] = lane + 32 * j < E ? __ldg(row + lane + 32 * j) : 0.f;
+}
+
+template <int NE, bool SIG>
+__global__ void __launch_bounds__(kBalThreads) balance_units_kernel(BalanceArgs a, BalanceWs w, int chunk) {
+    __shared__ float p_s[kBalWarps][NE * 32];
+    __shared__ int32_t c_s[NE * 32];
+    __shared__ int32_t n_s[kBalWarps];
+    griddep_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = blockIdx.x, E = a.E, K = a.K;
+    if (u == 0 && tid == 0) *w.ticket = 0;
+    // the last sequence whose first unit is at most u
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first_unit(a.offsets, mid, chunk) <= u) lo = mid;
+        else hi = mid - 1;
+    }
+    int first, last;
+    sequence(a.offsets, lo, a.T, first, last);
+    const long t0 = first + (long)(u - first_unit(a.offsets, lo, chunk)) * chunk;
+    if (t0 < first || t0 >= last) return;  // no such chunk
+    const int t1 = (int)min(t0 + chunk, (long)last);
+    for (int e = tid; e < NE * 32; e += kBalThreads) c_s[e] = 0;
+    __syncthreads();
+    float acc[NE];
+#pragma unroll
+    for (int j = 0; j < NE; j++) acc[j] = 0.f;
+    int n = 0;
+    bool bad = false;
+    for (int t = (int)t0 + warp; t < t1; t += kBalWarps) {
+        if (a.mask && !a.mask[t]) continue;
+        float l[NE], e[NE];
+        load_row<NE>(a.logits + (size_t)t * E, E, l);
+        if (lane < K) {
+            const int x = __ldg(a.idx + (size_t)t * K + lane);
+            if (x >= E) bad = true;
+            else if (x >= 0) atomicAdd(&c_s[x], 1);
+        }
+        const float r = scores<NE, SIG>(l, E, e);
+#pragma unroll
+        for (int j = 0; j < NE; j++) acc[j] = fmaf(e[j], r, acc[j]);
+        n++;
+    }
+    if (bad) atomicOr(a.err, kErrBadIndex);
+#pragma unroll
+    for (int j = 0; j < NE; j++) p_s[warp][lane + 32 * j] = acc[j];
+    if (lane == 0) n_s[warp] = n;
+    __syncthreads();
+    for (int e = tid; e < E; e += kBalThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < kBalWarps; k++) v += p_s[k][e];
+        w.p[(size_t)u * E + e] = v;
+        w.c[(size_t)u * E + e] = c_s[e];
+    }
+    if (tid == 0) {
+        int v = 0;
+#pragma unroll
+        for (int k = 0; k < kBalWarps; k++) v += n_s[k];
+        w.n[u] = v;
+    }
+}
+
+// A cluster of eight CTAs a sequence: CTA r adds the units of experts [32 r, 32 r + 32).
+__global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalThreads)
+    balance_sum_kernel(BalanceArgs a, BalanceWs w, int chunk) {
+    __shared__ double p_s[kBalWarps][32];
+    __shared__ int32_t c_s[kBalWarps][32], n_s[kBalWarps];
+    __shared__ double dot_s[kBalCluster];
+    __shared__ int last_s;
+    cg::cluster_group cl = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = (int)cl.block_rank(), E = a.E;
+    const int e = r * 32 + lane, clusters = gridDim.x / kBalCluster;
+    griddep_wait();
+    for (int b = blockIdx.x / kBalCluster; b < a.B; b += clusters) {
+        int first, last;
+        sequence(a.offsets, b, a.T, first, last);
+        if (r == 0 && tid == 0 && offsets_bad(a.offsets, b, a.T)) atomicOr(a.err, kErrBadIndex);
+        const int u0 = first_unit(a.offsets, b, chunk), nu = (last - first + chunk - 1) / chunk;
+        double p = 0.0;
+        int32_t c = 0, n = 0;
+        for (int u = warp; u < nu; u += kBalWarps) {
+            if (e < E) {
+                p += w.p[(size_t)(u0 + u) * E + e];
+                c += w.c[(size_t)(u0 + u) * E + e];
+            }
+            n += w.n[u0 + u];
+        }
+        p_s[warp][lane] = p;
+        c_s[warp][lane] = c;
+        if (lane == 0) n_s[warp] = n;
+        __syncthreads();
+        if (warp == 0) {
+            p = 0.0, c = 0, n = 0;
+#pragma unroll
+            for (int k = 0; k < kBalWarps; k++) p += p_s[k][lane], c += c_s[k][lane], n += n_s[k];
+            if (e < E) a.counts[(size_t)b * E + e] = c;
+            double v = n > 0 && e < E ? (double)c * p : 0.0;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+            // f . P of these experts, to the cluster's first CTA
+            if (lane == 0) *cl.map_shared_rank(&dot_s[r], 0) = n > 0 ? v * E / ((double)a.K * n * n) : 0.0;
+            if (r == 0 && lane == 0) a.tokens[b] = n;
+        }
+        cl.sync();
+        if (r == 0 && tid == 0) {
+            double v = 0.0;
+            for (int k = 0; k < kBalCluster; k++) v += dot_s[k];
+            w.loss[b] = (float)v;
+        }
+        cl.sync();
+    }
+    if (r != 0) return;
+    if (tid == 0) {
+        __threadfence();
+        last_s = atomicAdd(w.ticket, 1u) == (unsigned)clusters - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    if (!last_s) return;
+    // the last cluster: the mean over the sequences that have tokens
+    double v = 0.0;
+    int full = 0;
+    for (int b = tid; b < a.B; b += kBalThreads) {
+        v += __ldcg(w.loss + b);
+        full += __ldcg(a.tokens + b) > 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+        full += __shfl_xor_sync(0xffffffffu, full, o);
+    }
+    if (lane == 0) p_s[warp][0] = v, n_s[warp] = full;
+    __syncthreads();
+    if (tid == 0) {
+        v = 0.0, full = 0;
+        for (int k = 0; k < kBalWarps; k++) v += p_s[k][0], full += n_s[k];
+        *a.loss = full ? (float)(v / full) : 0.f;
+        a.tokens[a.B] = full;
+    }
+}
+
+// A warp a row; rows of a warp are neighbours, so that it keeps its sequence's f in registers.
+template <int NE, bool SIG>
+__global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceArgs a, int per_warp) {
+    const int lane = threadIdx.x & 31, E = a.E;
+    const long t0 = ((long)blockIdx.x * kBalWarps + (threadIdx.x >> 5)) * per_warp;
+    const long t1 = min(t0 + per_warp, (long)a.T);
+    float f[NE];
+    int have = -1;
+    const int full = __ldg(a.tokens + a.B);
+    const float grad = a.grad ? __ldg(a.grad) : 1.f;
+    for (long t = t0; t < t1; t++) {
+        int b = 0;
+        if (a.offsets) {  // the last sequence that begins at or before t
+            int lo = 0, hi = a.B;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (__ldg(a.offsets + mid) <= t) lo = mid + 1;
+                else hi = mid;
+            }
+            b = lo - 1;
+            if (b >= 0 && __ldg(a.offsets + b + 1) <= t) b = -1;
+        }
+        float* d = a.dlogits + (size_t)t * E;
+        const int n = b >= 0 ? __ldg(a.tokens + b) : 0;
+        if (n <= 0 || (a.mask && !a.mask[t])) {  // a token of no sequence, or one that does not count
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                if (lane + 32 * j < E) d[lane + 32 * j] = 0.f;
+            continue;
+        }
+        if (b != have) {
+            const float k = grad * (float)((double)E / ((double)a.K * n * (double)n * full));
+#pragma unroll
+            for (int j = 0; j < NE; j++)
+                f[j] = lane + 32 * j < E ? k * (float)__ldg(a.counts + (size_t)b * E + lane + 32 * j) : 0.f;
+            have = b;
+        }
+        float l[NE], e[NE], inner = 0.f;
+        load_row<NE>(a.logits + (size_t)t * E, E, l);
+        const float r = scores<NE, SIG>(l, E, e);
+#pragma unroll
+        for (int j = 0; j < NE; j++) inner = fmaf(f[j], e[j], inner);
+        inner = warp_sum(inner) * r;
+#pragma unroll
+        for (int j = 0; j < NE; j++)
+            if (lane + 32 * j < E) d[lane + 32 * j] = (SIG ? e[j] * (1.f - e[j]) : e[j]) * r * (f[j] - inner);
+    }
+}
+
+template <int NE>
+static cudaError_t units_launch(const BalanceArgs& a, const BalanceWs& w, int chunk, int units, cudaStream_t st) {
+    if (a.scoring) balance_units_kernel<NE, true><<<units, kBalThreads, 0, st>>>(a, w, chunk);
+    else balance_units_kernel<NE, false><<<units, kBalThreads, 0, st>>>(a, w, chunk);
+    return cudaGetLastError();
+}
+template <int NE>
+static cudaError_t backward_launch(const BalanceArgs& a, int grid, int per_warp, cudaStream_t st) {
+    if (a.scoring) balance_backward_kernel<NE, true><<<grid, kBalThreads, 0, st>>>(a, per_warp);
+    else balance_backward_kernel<NE, false><<<grid, kBalThreads, 0, st>>>(a, per_warp);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_balance_loss(const BalanceArgs& a, int sm_count, cudaStream_t st) {
+    const int chunk = balance_chunk(a.T, sm_count), units = balance_units(a.T, a.B, chunk);
+    const BalanceWs w = balance_layout(a.ws, a.E, a.B, units);
+    cudaError_t e;
+    if (a.E <= 32) e = units_launch<1>(a, w, chunk, units, st);
+    else if (a.E <= 64) e = units_launch<2>(a, w, chunk, units, st);
+    else if (a.E <= 128) e = units_launch<4>(a, w, chunk, units, st);
+    else e = units_launch<8>(a, w, chunk, units, st);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(kBalCluster * std::min(a.B, sm_count / kBalCluster));
+    cfg.blockDim = dim3(kBalThreads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, balance_sum_kernel, a, w, chunk);
+}
+
+cudaError_t launch_balance_backward(const BalanceArgs& a, int sm_count, cudaStream_t st) {
+    if (a.T <= 0) return cudaSuccess;
+    // sixteen warps an SM at the least before a warp takes a second row
+    const int per_warp = std::max(1, std::min(32, a.T / (sm_count * 16)));
+    const int grid = (a.T + kBalWarps * per_warp - 1) / (kBalWarps * per_warp);
+    if (a.E <= 32) return backward_launch<1>(a, grid, per_warp, st);
+    if (a.E <= 64) return backward_launch<2>(a, grid, per_warp, st);
+    if (a.E <= 128) return backward_launch<4>(a, grid, per_warp, st);
+    return backward_launch<8>(a, grid, per_warp, st);
+}
+
+}  // namespace moe

@@ -8,6 +8,12 @@ namespace moe {
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 16;
 constexpr int kMaxTokens = 4096;
+// Limits of the e4m3 and balance-loss calls, whose working memory is the caller's.
+constexpr int kF8MaxK = 16384;             // inner size of a scaled product
+constexpr int kF8MaxRows = 1 << 24;        // its M and N
+constexpr int kF8MaxPairs = 1 << 20;       // (token, expert) pairs of an expert call
+constexpr int kBalanceMaxTokens = 1 << 24;
+constexpr int kBalanceMaxSeqs = 1 << 16;
 
 // Latched device-side error bits (ctx->dev_err); host maps them to MOE_E* codes.
 constexpr uint32_t kErrNonFinite = 1u;

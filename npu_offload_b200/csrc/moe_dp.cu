@@ -11,10 +11,12 @@
 
 #include "../../include/moe_dp.h"
 #include "common.cuh"
+#include "balance.h"
 #include "decode.h"
 #include "prefill_tc.h"
 #include "block.h"
 #include "experts.h"
+#include "fp8.h"
 #include "route.h"
 
 using namespace moe;
@@ -1551,6 +1553,133 @@ int moe_block_forward(moe_ctx* c, int layer, int T, const uint16_t* h2, const ui
         if (logits_out) CUDA_TRY(cudaMemcpyAsync(logits_out, lg, (size_t)T * E * 4, cudaMemcpyDeviceToHost, s));
     }
     return (host || (flags & MOE_F_SYNC)) ? block_sync(c, s) : MOE_OK;
+}
+
+// ---------------- 8-bit floating point (e4m3 with one scale for each 128 values) ----------------
+
+int moe_quantize_fp8(moe_ctx* c, const void* x, int dtype, int64_t batch, int64_t rows, int64_t cols, int block_rows,
+                     uint8_t* q, float* scale, int flags, void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "moe_quantize_fp8 takes device pointers and no flag but MOE_F_SYNC");
+    if (dtype != MOE_DT_BF16 && dtype != MOE_DT_F32) return fail(MOE_EINVAL, "dtype %d is neither MOE_DT_BF16 nor MOE_DT_F32", dtype);
+    if (block_rows != 1 && block_rows != 128) return fail(MOE_EINVAL, "block_rows %d is neither 1 nor 128", block_rows);
+    if (batch < 0 || rows < 0 || cols < 0 || batch > INT32_MAX || rows > INT32_MAX || cols > INT32_MAX)
+        return fail(MOE_EINVAL, "batch, rows and cols must be in [0, 2^31)");
+    if (cols % 16) return fail(MOE_EINVAL, "cols %lld is not a multiple of 16", (long long)cols);
+    // [batch * rows, cols] values of a tensor: their number, and so that of the groups, is a 40-bit one at most
+    if (batch && rows && cols && (batch * rows > INT64_MAX / cols || batch * rows * cols > (1ll << 38)))
+        return fail(MOE_EINVAL, "batch * rows * cols is more than 2^38");
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (batch && rows && cols) {
+        if (!x || !q || !scale) return fail(MOE_EINVAL, "null x / q / scale");
+        if (!aligned16(x) || !aligned16(q) || (uintptr_t)scale & 3) return fail(MOE_EINVAL, "x and q must be 16-byte aligned");
+        CUDA_TRY(launch_quantize_fp8(x, dtype == MOE_DT_F32, batch, rows, cols, block_rows, q, scale, c->sm_count, st));
+        c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+int moe_matmul_fp8(moe_ctx* c, int64_t M, int64_t N, int64_t K, const uint8_t* x, const float* x_scale, const uint8_t* w,
+                   const float* w_scale, void* out, int out_dtype, int flags, void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "moe_matmul_fp8 takes device pointers and no flag but MOE_F_SYNC");
+    if (out_dtype != MOE_DT_BF16 && out_dtype != MOE_DT_F32) return fail(MOE_EINVAL, "out_dtype %d is neither MOE_DT_BF16 nor MOE_DT_F32", out_dtype);
+    if (M < 0 || N < 0 || M > kF8MaxRows || N > kF8MaxRows) return fail(MOE_EINVAL, "M and N must be in [0, %d]", kF8MaxRows);
+    if (K < 16 || K % 16 || K > kF8MaxK) return fail(MOE_EINVAL, "K %lld is not a multiple of 16 in [16, %d]", (long long)K, kF8MaxK);
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (M && N) {
+        if (!x || !x_scale || !w || !w_scale || !out) return fail(MOE_EINVAL, "null operand");
+        if (!aligned16(x) || !aligned16(w) || !aligned16(out)) return fail(MOE_EINVAL, "x, w and out must be 16-byte aligned");
+        MatmulF8 a{x, x_scale, w, w_scale, M, N, (int)K, out, out_dtype == MOE_DT_F32, c->d_err, c->timeout_ns};
+        CUDA_TRY(launch_matmul_fp8(a, c->sm_count, st));
+        c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+int64_t moe_experts_fp8_workspace(moe_ctx* c, int T) {
+    if (!c || T < 0 || (int64_t)T * c->cfg.top_k > kF8MaxPairs) return -1;
+    return (int64_t)experts_fp8_workspace(T, c->cfg.top_k, c->cfg.hidden, c->cfg.inter, c->cfg.n_experts);
+}
+
+int moe_experts_fp8(moe_ctx* c, int T, const uint16_t* x, const uint8_t* gate_up, const float* gate_up_scale, const uint8_t* down,
+                    const float* down_scale, const int32_t* topk_idx, const float* topk_w, void* out, int out_dtype,
+                    void* workspace, int64_t workspace_bytes, int flags, void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~(MOE_F_SYNC | MOE_F_ACCUMULATE)) return fail(MOE_EINVAL, "moe_experts_fp8 takes device pointers");
+    if (out_dtype != MOE_DT_BF16 && out_dtype != MOE_DT_F32) return fail(MOE_EINVAL, "out_dtype %d is neither MOE_DT_BF16 nor MOE_DT_F32", out_dtype);
+    if ((flags & MOE_F_ACCUMULATE) && out_dtype != MOE_DT_F32) return fail(MOE_EINVAL, "MOE_F_ACCUMULATE needs an fp32 output");
+    const int64_t need = moe_experts_fp8_workspace(c, T);
+    if (need < 0) return fail(MOE_EINVAL, "T=%d: T * top_k must be in [0, %d]", T, kF8MaxPairs);
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T) {
+        if (!x || !gate_up || !gate_up_scale || !down || !down_scale || !topk_idx || !topk_w || !out || !workspace)
+            return fail(MOE_EINVAL, "null argument");
+        if (!aligned16(x) || !aligned16(gate_up) || !aligned16(down) || !aligned16(out) || (uintptr_t)workspace & 255)
+            return fail(MOE_EINVAL, "x, weights and out must be 16-byte, the workspace 256-byte aligned");
+        if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+        ExpertsF8 a{x, gate_up, gate_up_scale, down, down_scale, topk_idx, topk_w, T, c->cfg.hidden, c->cfg.inter,
+                    c->cfg.n_experts, c->cfg.top_k, out, out_dtype == MOE_DT_F32, (flags & MOE_F_ACCUMULATE) != 0, workspace,
+                    c->d_err, c->timeout_ns};
+        int n = 0;
+        CUDA_TRY(launch_experts_fp8(a, c->sm_count, st, &n));
+        c->launches += n;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+// ---------------- router load-balance loss ----------------
+
+static int balance_checks(moe_ctx* c, int64_t T, int B, const int32_t* offsets, int flags) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "the balance loss takes device pointers and no flag but MOE_F_SYNC");
+    if (T < 0 || T > kBalanceMaxTokens) return fail(MOE_EINVAL, "T=%lld not in [0,%d]", (long long)T, kBalanceMaxTokens);
+    if (B < 1 || B > kBalanceMaxSeqs) return fail(MOE_EINVAL, "B=%d not in [1,%d]", B, kBalanceMaxSeqs);
+    if (B > 1 && !offsets) return fail(MOE_EINVAL, "%d sequences need their offsets", B);
+    return MOE_OK;
+}
+
+int64_t moe_balance_loss_workspace(moe_ctx* c, int64_t T, int B) {
+    if (!c || T < 0 || T > kBalanceMaxTokens || B < 1 || B > kBalanceMaxSeqs) return -1;
+    return (int64_t)balance_workspace((int)T, c->cfg.n_experts, B, c->sm_count);
+}
+
+int moe_balance_loss(moe_ctx* c, int64_t T, const float* logits, const int32_t* topk_idx, const int32_t* offsets, int B,
+                     const uint8_t* mask, float* loss, int32_t* counts, int32_t* tokens, void* workspace,
+                     int64_t workspace_bytes, int flags, void* stream) {
+    int r = balance_checks(c, T, B, offsets, flags);
+    if (r) return r;
+    if (!loss || !counts || !tokens || !workspace || (T && (!logits || !topk_idx))) return fail(MOE_EINVAL, "null argument");
+    if ((uintptr_t)workspace & 255) return fail(MOE_EINVAL, "the workspace must be 256-byte aligned");
+    const int64_t need = moe_balance_loss_workspace(c, T, B);
+    if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    BalanceArgs a{logits, topk_idx, offsets, mask, (int)T, c->cfg.n_experts, c->cfg.top_k, B, c->cfg.scoring, counts, tokens, loss,
+                  nullptr, nullptr, workspace, c->d_err};
+    CUDA_TRY(launch_balance_loss(a, c->sm_count, st));
+    c->launches += 2;
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+int moe_balance_loss_backward(moe_ctx* c, int64_t T, const float* logits, const int32_t* offsets, int B, const uint8_t* mask,
+                              const int32_t* counts, const int32_t* tokens, const float* grad, float* dlogits, int flags,
+                              void* stream) {
+    int r = balance_checks(c, T, B, offsets, flags);
+    if (r) return r;
+    if (!counts || !tokens || (T && (!logits || !dlogits))) return fail(MOE_EINVAL, "null argument");
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T) {
+        BalanceArgs a{logits, nullptr, offsets, mask, (int)T, c->cfg.n_experts, c->cfg.top_k, B, c->cfg.scoring,
+                      const_cast<int32_t*>(counts), const_cast<int32_t*>(tokens), nullptr, grad, dlogits, nullptr, c->d_err};
+        CUDA_TRY(launch_balance_backward(a, c->sm_count, st));
+        c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
 }
 
 int moe_router_exp(const float* x, float* y, int64_t n, void* stream) {
