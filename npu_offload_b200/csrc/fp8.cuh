@@ -47,6 +47,20 @@ __device__ __forceinline__ uint2 f8_pack8(const float (&f)[8], float inv) {
     return make_uint2(f8_pack2(v[0], v[1]) | f8_pack2(v[2], v[3]) << 16, f8_pack2(v[4], v[5]) | f8_pack2(v[6], v[7]) << 16);
 }
 
+__device__ __forceinline__ uint32_t f8_pack1(float f, float inv) {
+    float v = f * inv;
+    if (fabsf(v) == __int_as_float(0x7f800000)) v = __int_as_float(0x7fffffff);
+    return f8_pack2(v, 0.f) & 0xffu;
+}
+
+// Two floats rounded to bf16 (ties to even, NaN stays NaN), lo in the low half.
+__device__ __forceinline__ uint32_t f8_bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint16_t f8_bf16(float v) { return (uint16_t)f8_bf16x2(v, 0.f); }
+
 // The two e4m3 values of a 16-bit word as floats (both conversions exact).
 __device__ __forceinline__ void f8_unpack2(uint32_t w, float& lo, float& hi) {
     asm("{\n\t.reg .b32 h;\n\t.reg .b16 a, b, c;\n\t"

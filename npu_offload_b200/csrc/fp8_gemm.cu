@@ -1,108 +1,270 @@
-// Products of e4m3 operands with one scale for each 128 values, and the routed-expert FFN built on them.
-//
-//   out[m, n] = sum_kb xs[m, kb] ws[n / 128, kb] sum_{k in block kb} x[m, k] w[n, k]
-//
-// The products of two e4m3 values are exact in fp32; all sums are fp32.
+// Scaled products of e4m3 operands and the routed-expert FFN built on them: choice of kernel, tensor maps,
+// launches, and the small kernels around the products (token quantiser with the grouping, combine).
 #include <algorithm>
 
 #include "common.cuh"
 #include "fp8.h"
 #include "fp8.cuh"
+#include "fp8_tc.cuh"
 
 namespace moe {
+namespace {
 
-// One warp's dot product of an activation row and a weight row; every lane gets the sum.
-__device__ __forceinline__ float dot_row(const uint8_t* x, const float* xs, const uint8_t* w, const float* ws, int K) {
-    float acc = 0.f;
-    for (int k = (threadIdx.x & 31) * 16; k < K; k += 512) {
-        float a[16], b[16], d = 0.f;
-        f8_unpack16(__ldg(reinterpret_cast<const uint4*>(x + k)), a);
-        f8_unpack16(__ldg(reinterpret_cast<const uint4*>(w + k)), b);
-#pragma unroll
-        for (int i = 0; i < 16; i++) d = fmaf(a[i], b[i], d);
-        acc = fmaf(d, xs[k / kF8Block] * ws[k / kF8Block], acc);
+// [mats][rows][cols] bytes, boxes of 128 columns x box_rows rows of one matrix, 128-byte swizzle
+bool encode3(EncodeTiledFn enc, CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int64_t mats, int box_rows) {
+    const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)mats};
+    const cuuint64_t strides[2] = {(cuuint64_t)cols, (cuuint64_t)(cols * rows)};
+    const cuuint32_t box[3] = {128, (cuuint32_t)box_rows, 1}, es[3] = {1, 1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+bool encode2(EncodeTiledFn enc, CUtensorMap* m, const void* base, int64_t cols, int64_t rows, int box_rows) {
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)cols};
+    const cuuint32_t box[2] = {128, (cuuint32_t)box_rows}, es[2] = {1, 1};
+    return enc(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, on every device that it runs on.
+template <auto kernel>
+cudaError_t allow_smem(int bytes) {
+    static unsigned long long done = 0;  // a bit a device; setting it twice does no harm
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+    return e;
+}
+
+// Launch with an optional cluster split and, where `pdl`, ahead of the end of the kernel before it.
+template <class K>
+cudaError_t launch(K kernel, int grid, int threads, int smem, int cluster, bool pdl, cudaStream_t st, const CUtensorMap& mw,
+                   const CUtensorMap& mx, const F8Gemm& g) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    int n = 0;
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    n++;
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        n++;
     }
-    return warp_sum(acc);
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    return cudaLaunchKernelEx(&cfg, kernel, mw, mx, g);
 }
 
-__device__ __forceinline__ void store_out(void* out, bool f32, size_t i, float v) {
-    if (f32) static_cast<float*>(out)[i] = v;
-    else static_cast<uint16_t*>(out)[i] = f2bf(v);
-}
-
-__global__ void __launch_bounds__(256) matmul_fp8_kernel(const uint8_t* x, const float* xs, const uint8_t* w, const float* ws,
-                                                         int64_t M, int64_t N, int K, void* out, bool f32) {
-    const int kb = (K + kF8Block - 1) / kF8Block;
-    for (int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < M * N; i += gridDim.x * 8ll) {
-        const int64_t m = i / N, n = i - m * N;
-        const float v = dot_row(x + m * K, xs + m * kb, w + n * K, ws + n / kF8Block * kb, K);
-        if ((threadIdx.x & 31) == 0) store_out(out, f32, i, v);
+template <int MODE, int NQ>
+struct Few {
+    using C = FewCfg<MODE, NQ>;
+    // tiles: upper bound of the tiles there may be
+    static cudaError_t run(const CUtensorMap& mw, const CUtensorMap& mx, const F8Gemm& g, int64_t tiles, int sm_count, bool pdl,
+                           cudaStream_t st) {
+        constexpr auto k = f8_few_kernel<MODE, NQ>;
+        const cudaError_t e = allow_smem<k>(C::kSmem);
+        if (e != cudaSuccess) return e;
+        const int slots = sm_count * C::kMinCtas;
+        int cs = 1;  // split the inner dimension while all CTAs are still on the GPU at once
+        while (C::kRed && cs < 8 && tiles * cs * 2 <= slots && cs * 2 <= g.nkb) cs *= 2;
+        const int clusters = (int)std::min<int64_t>(tiles, slots / cs);
+        return launch(k, clusters * cs, kFewThreads, C::kSmem, cs, pdl, st, mw, mx, g);
     }
-}
+};
 
-cudaError_t launch_matmul_fp8(const MatmulF8& a, int sm_count, cudaStream_t st) {
-    if (a.M <= 0 || a.N <= 0) return cudaSuccess;
-    const int64_t ctas = (a.M * a.N + 7) / 8;
-    matmul_fp8_kernel<<<(int)std::min<int64_t>(ctas, sm_count * 64ll), 256, 0, st>>>(a.x, a.xs, a.w, a.ws, a.M, a.N, a.K, a.out,
-                                                                                    a.out_f32);
-    return cudaGetLastError();
+template <int MODE, int NB>
+struct Many {
+    using C = ManyCfg<MODE, NB>;
+    static cudaError_t run(const CUtensorMap& mw, const CUtensorMap& mx, const F8Gemm& g, int64_t tiles, int sm_count, bool pdl,
+                           cudaStream_t st) {
+        constexpr auto k = f8_many_kernel<MODE, NB>;
+        const cudaError_t e = allow_smem<k>(C::kSmem);
+        if (e != cudaSuccess) return e;
+        // the register split of the kernel draws on what the launch gives: 256 x 216 + 128 x 72 at most
+        static const int regs = [&] {
+            cudaFuncAttributes at;
+            return cudaFuncGetAttributes(&at, k) == cudaSuccess ? at.numRegs : 0;
+        }();
+        if (regs * kManyThreads < 256 * 216 + 128 * 72) return cudaErrorInvalidConfiguration;
+        return launch(k, (int)std::min<int64_t>(tiles, sm_count), kManyThreads, C::kSmem, 1, pdl, st, mw, mx, g);
+    }
+};
+
+}  // namespace
+
+cudaError_t launch_matmul_fp8(const MatmulF8& m, int sm_count, cudaStream_t st) {
+    if (m.M <= 0 || m.N <= 0) return cudaSuccess;
+    EncodeTiledFn enc = tc_encode_fn();
+    if (!enc) return cudaErrorNotSupported;
+    F8Gemm g{};
+    g.xs = m.xs;
+    g.ws = m.ws;
+    g.nkb = (m.K + 127) / 128;
+    g.nb = (int)((m.N + 127) / 128);
+    g.nt = g.nb;
+    g.M = (int)m.M;
+    g.N = (int)m.N;
+    g.out = m.out;
+    g.out_f32 = m.out_f32;
+    g.err = m.err;
+    g.timeout_ns = m.timeout_ns;
+    const int nq = m.M <= 16 ? 16 : m.M <= 32 ? 32 : m.M <= 64 ? 64 : 128;
+    CUtensorMap mw, mx;
+    if (!encode3(enc, &mw, m.w, m.K, m.N, 1, 128) || !encode2(enc, &mx, m.x, m.K, m.M, nq)) return cudaErrorInvalidValue;
+    if (nq == 16) return Few<kF8Dense, 16>::run(mw, mx, g, g.nt, sm_count, false, st);
+    if (nq == 32) return Few<kF8Dense, 32>::run(mw, mx, g, g.nt, sm_count, false, st);
+    if (nq == 64) return Few<kF8Dense, 64>::run(mw, mx, g, g.nt, sm_count, false, st);
+    const int64_t mt = (m.M + 127) / 128;
+    if (mt * ((m.N + 255) / 256) < sm_count) return Many<kF8Dense, 128>::run(mw, mx, g, mt * g.nt, sm_count, false, st);
+    g.nt = (int)((m.N + 255) / 256);
+    return Many<kF8Dense, 256>::run(mw, mx, g, mt * g.nt, sm_count, false, st);
 }
 
 // ---- routed experts ----
 
-__global__ void __launch_bounds__(256) gate_up_fp8_kernel(ExpertsF8 a, const uint8_t* xq, const float* xs, float* act) {
-    const int hb = (a.H + kF8Block - 1) / kF8Block, fb = (a.F + kF8Block - 1) / kF8Block;
-    const int64_t n = (int64_t)a.T * a.K * a.F;
-    for (int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < n; i += gridDim.x * 8ll) {
-        const int64_t p = i / a.F;
-        const int f = (int)(i - p * a.F), e = a.idx[p];
-        if (e < 0 || e >= a.E) {
-            if (e >= a.E && (threadIdx.x & 31) == 0) atomicOr(a.err, kErrBadIndex);
-            continue;
-        }
-        const int64_t t = p / a.K;
-        float v[2];
+constexpr int kPrepThreads = 1024;
+
+struct PrepArgs {
+    const uint16_t* x;
+    const int32_t* idx;
+    int T, H, E, K, height;  // height: token rows of a group
+    uint8_t* xq;
+    float* xs;
+    int32_t* pos;            // [T * K] slot of each pair, -1: none
+    int32_t* perm;           // [T * K] token of each slot
+    F8Group* groups;
+    int* n_groups;
+    uint32_t* err;
+};
+
+// CTA 0 groups the pairs by expert; the others quantise the tokens.  A pair's place among its expert's
+// slots may differ from run to run: a slot's row is computed from that row alone, so no result does.
+__global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
+    griddep_launch_dependents();
+    const int tid = threadIdx.x;
+    if (blockIdx.x > 0) {
+        const uint32_t per_row = (uint32_t)(a.H + 127) / 128, groups = (uint32_t)a.T * per_row, sub = tid & 15;
+        const uint32_t stride = (gridDim.x - 1) * (kPrepThreads / 16);
+        for (uint32_t g = (blockIdx.x - 1) * (kPrepThreads / 16) + tid / 16; g - tid / 16 < groups; g += stride) {
+            const uint32_t row = g / per_row, c = (g - row * per_row) * 128 + sub * 8;
+            const bool in = g < groups && c < (uint32_t)a.H;
+            const uint4 w = in ? ldg_stream(a.x + (size_t)row * a.H + c) : make_uint4(0, 0, 0, 0);
+            const float f[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
+            uint32_t top = f8_top(f);
 #pragma unroll
-        for (int h = 0; h < 2; h++)
-            v[h] = dot_row(xq + t * a.H, xs + t * hb, a.gu + (((int64_t)e * 2 + h) * a.F + f) * a.H,
-                           a.gus + (((int64_t)e * 2 + h) * fb + f / kF8Block) * hb, a.H);
-        if ((threadIdx.x & 31) == 0) act[i] = v[0] / (1.f + expf(-v[0])) * v[1];
-    }
-}
-
-__global__ void __launch_bounds__(256) down_fp8_kernel(ExpertsF8 a, const uint8_t* aq, const float* as, float* y) {
-    const int hb = (a.H + kF8Block - 1) / kF8Block, fb = (a.F + kF8Block - 1) / kF8Block;
-    const int64_t n = (int64_t)a.T * a.K * a.H;
-    for (int64_t i = blockIdx.x * 8ll + (threadIdx.x >> 5); i < n; i += gridDim.x * 8ll) {
-        const int64_t p = i / a.H;
-        const int h = (int)(i - p * a.H), e = a.idx[p];
-        if (e < 0 || e >= a.E) continue;
-        const float v = dot_row(aq + p * a.F, as + p * fb, a.d + ((int64_t)e * a.H + h) * a.F,
-                                a.ds + ((int64_t)e * hb + h / kF8Block) * fb, a.F);
-        if ((threadIdx.x & 31) == 0) y[i] = v;
-    }
-}
-
-__global__ void __launch_bounds__(256) combine_fp8_kernel(ExpertsF8 a, const float* y) {
-    const int64_t n = (int64_t)a.T * a.H;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-        const int64_t t = i / a.H, h = i - t * a.H;
-        float v = a.accumulate ? static_cast<const float*>(a.out)[i] : 0.f;
-        for (int k = 0; k < a.K; k++) {
-            const int e = a.idx[t * a.K + k];
-            if (e >= 0 && e < a.E) v = fmaf(a.w[t * a.K + k], y[(t * a.K + k) * a.H + h], v);
+            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const uint32_t se = f8_scale_exp(top);
+            if (in) *reinterpret_cast<uint2*>(a.xq + (size_t)row * a.H + c) = f8_pack8(f, f8_inverse(se));
+            if (sub == 0 && g < groups) a.xs[g] = __uint_as_float(se << 23);
         }
-        store_out(a.out, a.out_f32, i, v);
+        return;
+    }
+    __shared__ int cnt[kMaxExperts], off[kMaxExperts], goff[kMaxExperts + 1];
+    const int P = a.T * a.K, E = a.E;
+    for (int e = tid; e < kMaxExperts; e += kPrepThreads) cnt[e] = 0;
+    __syncthreads();
+    constexpr int U = 8;  // index loads in flight
+    bool bad = false;
+    for (int p0 = tid; p0 < P; p0 += U * kPrepThreads) {
+        int e[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) e[u] = p0 + u * kPrepThreads < P ? __ldg(a.idx + p0 + u * kPrepThreads) : -1;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = p0 + u * kPrepThreads;
+            bad |= e[u] >= E;
+            if (p < P) a.pos[p] = e[u] >= 0 && e[u] < E ? atomicAdd(&cnt[e[u]], 1) : -1;
+        }
+    }
+    if (bad) atomicOr(a.err, kErrBadIndex);
+    __syncthreads();
+    if (tid < 32) {  // exclusive sums of the counts and of the groups, eight experts a lane
+        int c = 0, g = 0;
+        for (int e = tid * 8; e < tid * 8 + 8; e++) c += cnt[e], g += (cnt[e] + a.height - 1) / a.height;
+        int ci = c, gi = g;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, ci, o), z = __shfl_up_sync(0xffffffffu, gi, o);
+            if (tid >= o) ci += y, gi += z;
+        }
+        c = ci - c, g = gi - g;
+        for (int e = tid * 8; e < tid * 8 + 8; e++) {
+            off[e] = c, goff[e] = g;
+            c += cnt[e], g += (cnt[e] + a.height - 1) / a.height;
+        }
+        if (tid == 31) *a.n_groups = gi;
+    }
+    __syncthreads();
+    for (int p0 = tid; p0 < P; p0 += U * kPrepThreads) {
+        int e[U], r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int p = p0 + u * kPrepThreads;
+            r[u] = p < P ? a.pos[p] : -1;
+            e[u] = p < P ? __ldg(a.idx + p) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (r[u] >= 0) {
+                const int p = p0 + u * kPrepThreads, slot = off[e[u]] + r[u];
+                a.pos[p] = slot;
+                a.perm[slot] = p / a.K;
+            }
+    }
+    for (int e = tid; e < E; e += kPrepThreads)
+        for (int g = 0; g * a.height < cnt[e]; g++)
+            a.groups[goff[e] + g] = F8Group{off[e] + g * a.height, min(a.height, cnt[e] - g * a.height), e, 0};
+}
+
+// out[t] = (out[t] +) sum_k w[t, k] y[slot of (t, k)], in order of k; four columns a thread.
+__global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ pos,
+                                                         const float* __restrict__ w, int T, int K, int H, void* out, bool f32,
+                                                         bool accumulate) {
+    griddep_wait();
+    const int per = H / 4;
+    const int64_t n = (int64_t)T * per;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        const int64_t t = i / per;
+        const int h = (int)(i - t * per) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (accumulate) v = *reinterpret_cast<const float4*>(static_cast<const float*>(out) + t * H + h);
+        for (int k = 0; k < K; k++) {
+            const int s = __ldg(pos + t * K + k);
+            if (s < 0) continue;
+            const float c = __ldg(w + t * K + k);
+            const float4 a = *reinterpret_cast<const float4*>(y + (size_t)s * H + h);
+            v.x = fmaf(c, a.x, v.x), v.y = fmaf(c, a.y, v.y), v.z = fmaf(c, a.z, v.z), v.w = fmaf(c, a.w, v.w);
+        }
+        if (f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + t * H + h) = v;
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + t * H + h) = make_uint2(f8_bf16x2(v.x, v.y), f8_bf16x2(v.z, v.w));
     }
 }
 
 namespace {
+
+// Token rows of a group: the smallest height that takes an expert's tokens, on average, in one group.
+int group_height(int64_t pairs, int E) {
+    const int64_t a = pairs / E;
+    return a <= 8 ? 16 : a <= 24 ? 32 : a <= 40 ? 64 : 128;
+}
+
 struct Ws {
     uint8_t *xq, *aq;
-    float *xs, *as, *act, *y;
+    float *xs, *as, *y;
+    int32_t *pos, *perm;
+    F8Group* groups;
+    int* n_groups;
     size_t bytes;
 };
-Ws experts_layout(void* ws, int T, int K, int H, int F) {
+Ws experts_layout(void* ws, int T, int K, int H, int F, int E) {
     Ws w;
     char* p = static_cast<char*>(ws);
     size_t o = 0;
@@ -111,33 +273,90 @@ Ws experts_layout(void* ws, int T, int K, int H, int F) {
         o += (n + 255) / 256 * 256;
         return r;
     };
-    const size_t P = (size_t)T * K, hb = (H + kF8Block - 1) / kF8Block, fb = (F + kF8Block - 1) / kF8Block;
+    const size_t P = (size_t)T * K, hb = (H + 127) / 128, fb = (F + 127) / 128;
     w.xq = (uint8_t*)take((size_t)T * H);
     w.xs = (float*)take(4 * (size_t)T * hb);
-    w.act = (float*)take(4 * P * F);
     w.aq = (uint8_t*)take(P * F);
     w.as = (float*)take(4 * P * fb);
     w.y = (float*)take(4 * P * H);
+    w.pos = (int32_t*)take(4 * P);
+    w.perm = (int32_t*)take(4 * P);
+    w.groups = (F8Group*)take(sizeof(F8Group) * (P / 16 + std::min<size_t>(E, P)));
+    w.n_groups = (int*)take(4);
     w.bytes = o;
     return w;
 }
+
+template <int NQ>
+cudaError_t products_few(const CUtensorMap (&m)[4], F8Gemm gu, F8Gemm dn, int64_t groups, int sm_count, cudaStream_t st) {
+    const cudaError_t e = Few<kF8GateUp, NQ>::run(m[0], m[1], gu, groups * gu.nt, sm_count, true, st);
+    return e != cudaSuccess ? e : Few<kF8Down, NQ>::run(m[2], m[3], dn, groups * dn.nt, sm_count, true, st);
+}
+
 }  // namespace
 
-size_t experts_fp8_workspace(int T, int K, int H, int F, int E) { return experts_layout(nullptr, T, K, H, F).bytes; }
+size_t experts_fp8_workspace(int T, int K, int H, int F, int E) { return experts_layout(nullptr, T, K, H, F, E).bytes; }
 
 cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st, int* launches) {
     if (a.T <= 0) return cudaSuccess;
-    const Ws w = experts_layout(a.ws, a.T, a.K, a.H, a.F);
-    cudaError_t e = launch_quantize_fp8(a.x, false, 1, a.T, a.H, 1, w.xq, w.xs, sm_count, st);
+    EncodeTiledFn enc = tc_encode_fn();
+    if (!enc) return cudaErrorNotSupported;
+    const Ws w = experts_layout(a.ws, a.T, a.K, a.H, a.F, a.E);
+    const int64_t P = (int64_t)a.T * a.K;
+    const int height = group_height(P, a.E);
+    const int64_t groups = std::min<int64_t>(a.E, P) + P / height;  // at most
+    CUtensorMap m[4];
+    if (!encode3(enc, &m[0], a.gu, a.H, a.F, 2 * (int64_t)a.E, 128) || !encode2(enc, &m[1], w.xq, a.H, a.T, 1) ||
+        !encode3(enc, &m[2], a.d, a.F, a.H, a.E, 128) || !encode2(enc, &m[3], w.aq, a.F, P, height))
+        return cudaErrorInvalidValue;
+    PrepArgs pa{a.x, a.idx, a.T, a.H, a.E, a.K, height, w.xq, w.xs, w.pos, w.perm, w.groups, w.n_groups, a.err};
+    const int64_t qctas = ((int64_t)a.T * ((a.H + 127) / 128) + kPrepThreads / 16 - 1) / (kPrepThreads / 16);
+    f8_prep_kernel<<<1 + (int)std::min<int64_t>(qctas, 2 * sm_count), kPrepThreads, 0, st>>>(pa);
+    cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    const int grid = sm_count * 16;
-    gate_up_fp8_kernel<<<grid, 256, 0, st>>>(a, w.xq, w.xs, w.act);
-    e = launch_quantize_fp8(w.act, true, 1, (int64_t)a.T * a.K, a.F, 1, w.aq, w.as, sm_count, st);
+
+    F8Gemm gu{}, dn{};
+    gu.xs = w.xs;
+    gu.ws = a.gus;
+    gu.nkb = (a.H + 127) / 128;
+    gu.nb = gu.nt = (a.F + 127) / 128;
+    gu.N = a.F;
+    gu.groups = w.groups;
+    gu.n_groups = w.n_groups;
+    gu.perm = w.perm;
+    gu.aq = w.aq;
+    gu.as = w.as;
+    gu.err = a.err;
+    gu.timeout_ns = a.timeout_ns;
+    dn = gu;
+    dn.xs = w.as;
+    dn.ws = a.ds;
+    dn.nkb = (a.F + 127) / 128;
+    dn.nb = dn.nt = (a.H + 127) / 128;
+    dn.N = a.H;
+    dn.out = w.y;
+    dn.out_f32 = 1;
+    if (height == 16) e = products_few<16>(m, gu, dn, groups, sm_count, st);
+    else if (height == 32) e = products_few<32>(m, gu, dn, groups, sm_count, st);
+    else if (height == 64) e = products_few<64>(m, gu, dn, groups, sm_count, st);
+    else {
+        e = Many<kF8GateUp, 256>::run(m[0], m[1], gu, groups * gu.nt, sm_count, true, st);
+        dn.nt = (a.H + 255) / 256;
+        if (e == cudaSuccess) e = Many<kF8Down, 256>::run(m[2], m[3], dn, groups * dn.nt, sm_count, true, st);
+    }
     if (e != cudaSuccess) return e;
-    down_fp8_kernel<<<grid, 256, 0, st>>>(a, w.aq, w.as, w.y);
-    combine_fp8_kernel<<<grid, 256, 0, st>>>(a, w.y);
-    *launches += 5;
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((int)std::min<int64_t>(((int64_t)a.T * a.H / 4 + 255) / 256, sm_count * 8));
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    *launches += 4;
+    return cudaLaunchKernelEx(&cfg, f8_combine_kernel, (const float*)w.y, (const int32_t*)w.pos, a.w, a.T, a.K, a.H, a.out, a.out_f32,
+                              a.accumulate);
 }
 
 }  // namespace moe

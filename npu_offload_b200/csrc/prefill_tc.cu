@@ -21,15 +21,12 @@
 // Weights are read in place from the unit tables through a 3-D tensor map (unit element, f, expert
 // slot); the A rows through a 2-D map.  Every wait is bounded; a CTA that gives up raises kErrTimeout,
 // lets its in-flight copies and MMAs finish and frees its TMEM before returning.
-#include <cuda.h>
-
 #include <algorithm>
-
-#include <cute/arch/mma_sm100_desc.hpp>
 
 #include "common.cuh"
 #include "prefill_tc.h"
 #include "ptx.cuh"
+#include "tc.cuh"
 
 namespace moe {
 
@@ -47,81 +44,6 @@ struct TcCtrl {
     uint32_t tmem;
     int abort;
 };
-__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, int* abort, uint32_t* err, uint64_t deadline) {
-    while (!mbar_try_wait_sleep(bar, parity, 20000u)) {
-        if (*(volatile int*)abort) return false;
-        if (globaltimer_ns() > deadline) {
-            *(volatile int*)abort = 1;
-            atomicOr(err, kErrTimeout);
-            return false;
-        }
-    }
-    return true;
-}
-
-// K-major operand in the 128-byte swizzle layout TMA writes for a 64-element (128-byte) inner box:
-// rows 128 bytes apart, 8-row (1 KB) swizzle atoms stacked at 1 KB (SBO); the K-slice of a K=16 MMA
-// starts 32 bytes further per step inside the atom.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-    cute::UMMA::SmemDescriptor d;
-    d.desc_ = 0;
-    d.start_address_ = (uint16_t)(saddr >> 4);
-    d.leading_byte_offset_ = 1;
-    d.stride_byte_offset_ = 1024 >> 4;
-    d.version_ = 1;
-    d.base_offset_ = 0;
-    d.lbo_mode_ = 0;
-    d.layout_type_ = (uint8_t)cute::UMMA::LayoutType::SWIZZLE_128B;
-    return d.desc_;
-}
-
-__device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int x, int y, uint64_t* bar,
-                                            uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4}], "
-        "[%2], %5;" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "l"(policy)
-        : "memory");
-}
-
-__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar,
-                                            uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, "
-        "%5}], [%2], %6;" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "l"(policy)
-        : "memory");
-}
-
-__device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(da), "l"(db), "r"(idesc), "r"(acc));
-}
-
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
-          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
-          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
-          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-        : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
-
 // MN-major operand (down columns): 64 outputs (128 bytes) contiguous per f row as TMA writes a
 // [64 f x 64 h] box with 128-byte swizzle; 8-row swizzle atoms 1 KB apart along K (SBO), the
 // 64-output chunks 8 KB apart along N (LBO); a K=16 step advances two whole atoms (2 KB).
@@ -437,11 +359,7 @@ cudaError_t launch_tc_items(const Job* jobs, const int* n_jobs, int E, const voi
 
 // ---- host side ----
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn encode_fn() {
+EncodeTiledFn tc_encode_fn() {
     static EncodeTiledFn fn = nullptr;
     static bool tried = false;
     if (!tried) {
@@ -457,7 +375,7 @@ static EncodeTiledFn encode_fn() {
     return fn;
 }
 
-bool tc_available() { return encode_fn() != nullptr; }
+bool tc_available() { return tc_encode_fn() != nullptr; }
 
 cudaError_t tc_set_smem_limit() {
     cudaError_t e = cudaFuncSetAttribute(tc_gemm_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kTcSmem);
@@ -491,7 +409,7 @@ cudaError_t launch_down_tc(const uint16_t* act, int arows, const void* arena, in
                            const TcItem* items, int n_items, const int* n_items_dev, int H, int F, float* y,
                            uint32_t* sched, uint32_t* err, uint64_t timeout_ns, int grid_max, uint32_t* mt_done,
                            cudaStream_t st) {
-    EncodeTiledFn enc = encode_fn();
+    EncodeTiledFn enc = tc_encode_fn();
     if (!enc) return cudaErrorNotSupported;
     if (H % 256 || F % kTcBK || slot_bytes % 16 || ((uintptr_t)act | (uintptr_t)arena) & 15) return cudaErrorInvalidValue;
     CUtensorMap ma, md;
@@ -525,7 +443,7 @@ cudaError_t launch_gateup_tc(const uint16_t* xg, int xrows, const void* arena, i
                              const TcItem* items, int n_items, const int* n_items_dev, int H, int F, uint16_t* act,
                              uint32_t* sched, uint32_t* err, uint64_t timeout_ns, int grid_max, uint32_t* mt_done,
                              cudaStream_t st) {
-    EncodeTiledFn enc = encode_fn();
+    EncodeTiledFn enc = tc_encode_fn();
     if (!enc) return cudaErrorNotSupported;
     if (H % kTcBK || F % 128 || slot_bytes % 16 || ((uintptr_t)xg | (uintptr_t)arena) & 15) return cudaErrorInvalidValue;
     CUtensorMap mx, mw;
