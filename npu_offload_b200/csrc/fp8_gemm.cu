@@ -88,12 +88,6 @@ struct Many {
         constexpr auto k = f8_many_kernel<MODE, NB>;
         const cudaError_t e = allow_smem<k>(C::kSmem);
         if (e != cudaSuccess) return e;
-        // the register split of the kernel draws on what the launch gives: 256 x 216 + 128 x 72 at most
-        static const int regs = [&] {
-            cudaFuncAttributes at;
-            return cudaFuncGetAttributes(&at, k) == cudaSuccess ? at.numRegs : 0;
-        }();
-        if (regs * kManyThreads < 256 * 216 + 128 * 72) return cudaErrorInvalidConfiguration;
         return launch(k, (int)std::min<int64_t>(tiles, sm_count), kManyThreads, C::kSmem, 1, pdl, st, mw, mx, g);
     }
 };
@@ -224,24 +218,35 @@ __global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
             a.groups[goff[e] + g] = F8Group{off[e] + g * a.height, min(a.height, cnt[e] - g * a.height), e, 0};
 }
 
-// out[t] = (out[t] +) sum_k w[t, k] y[slot of (t, k)], in order of k; four columns a thread.
+// out[t] = (out[t] +) sum_k w[t, k] y[slot of (t, k)], in order of k; four columns a thread.  Eight slots are
+// looked up, and then eight rows read, at a time: two round trips to memory instead of two for each expert.
 __global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ pos,
                                                          const float* __restrict__ w, int T, int K, int H, void* out, bool f32,
                                                          bool accumulate) {
-    griddep_wait();
     const int per = H / 4;
     const int64_t n = (int64_t)T * per;
+    griddep_wait();
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
         const int64_t t = i / per;
         const int h = (int)(i - t * per) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         if (accumulate) v = *reinterpret_cast<const float4*>(static_cast<const float*>(out) + t * H + h);
-        for (int k = 0; k < K; k++) {
-            const int s = __ldg(pos + t * K + k);
-            if (s < 0) continue;
-            const float c = __ldg(w + t * K + k);
-            const float4 a = *reinterpret_cast<const float4*>(y + (size_t)s * H + h);
-            v.x = fmaf(c, a.x, v.x), v.y = fmaf(c, a.y, v.y), v.z = fmaf(c, a.z, v.z), v.w = fmaf(c, a.w, v.w);
+        for (int k0 = 0; k0 < K; k0 += 8) {
+            int s[8];
+            float c[8];
+            float4 a[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                s[k] = k0 + k < K ? __ldg(pos + t * K + k0 + k) : -1;
+                c[k] = k0 + k < K ? __ldg(w + t * K + k0 + k) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (s[k] >= 0) a[k] = *reinterpret_cast<const float4*>(y + (size_t)s[k] * H + h);
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (s[k] >= 0)
+                    v.x = fmaf(c[k], a[k].x, v.x), v.y = fmaf(c[k], a[k].y, v.y), v.z = fmaf(c[k], a[k].z, v.z), v.w = fmaf(c[k], a[k].w, v.w);
         }
         if (f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + t * H + h) = v;
         else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + t * H + h) = make_uint2(f8_bf16x2(v.x, v.y), f8_bf16x2(v.z, v.w));
@@ -274,7 +279,7 @@ Ws experts_layout(void* ws, int T, int K, int H, int F, int E) {
         return r;
     };
     const size_t P = (size_t)T * K, hb = (H + 127) / 128, fb = (F + 127) / 128;
-    w.xq = (uint8_t*)take((size_t)T * H);
+    w.xq = (uint8_t*)take(((size_t)T + kF8PadRows) * H);
     w.xs = (float*)take(4 * (size_t)T * hb);
     w.aq = (uint8_t*)take(P * F);
     w.as = (float*)take(4 * P * fb);
@@ -306,7 +311,7 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     const int height = group_height(P, a.E);
     const int64_t groups = std::min<int64_t>(a.E, P) + P / height;  // at most
     CUtensorMap m[4];
-    if (!encode3(enc, &m[0], a.gu, a.H, a.F, 2 * (int64_t)a.E, 128) || !encode2(enc, &m[1], w.xq, a.H, a.T, 1) ||
+    if (!encode3(enc, &m[0], a.gu, a.H, a.F, 2 * (int64_t)a.E, 128) || !encode2(enc, &m[1], w.xq, a.H, a.T + kF8PadRows, 1) ||
         !encode3(enc, &m[2], a.d, a.F, a.H, a.E, 128) || !encode2(enc, &m[3], w.aq, a.F, P, height))
         return cudaErrorInvalidValue;
     PrepArgs pa{a.x, a.idx, a.T, a.H, a.E, a.K, height, w.xq, w.xs, w.pos, w.perm, w.groups, w.n_groups, a.err};
@@ -320,6 +325,7 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     gu.ws = a.gus;
     gu.nkb = (a.H + 127) / 128;
     gu.nb = gu.nt = (a.F + 127) / 128;
+    gu.M = a.T;
     gu.N = a.F;
     gu.groups = w.groups;
     gu.n_groups = w.n_groups;

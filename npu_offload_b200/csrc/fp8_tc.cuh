@@ -36,7 +36,7 @@ struct F8Gemm {
     const float* xs;         // token scales [rows, nkb]
     const float* ws;         // weight scales [.., ceil(N / 128), nkb] (gate / up: [E][2][..])
     int nkb, nt, nb;         // inner blocks; weight tiles a group (nt) and 128-row scale blocks a matrix (nb)
-    int M, N;                // dense: tokens; weight rows of a matrix (dense N, gate/up F, down H)
+    int M, N;                // tokens; weight rows of a matrix (dense N, gate/up F, down H)
     const F8Group* groups;   // experts: token groups
     const int* n_groups;     //   and their number (device); dense: null
     const int32_t* perm;     // gate/up: token of each slot
@@ -48,13 +48,14 @@ struct F8Gemm {
     uint64_t timeout_ns;
 };
 
-// Bounded wait of all lanes (or of one thread): the clock is read only where the first try fails.
+// Bounded wait of all lanes (or of one thread).  The limit is counted in SM cycles (reading the global timer
+// takes long beside a wait); 2 cycles a ns are at least the limit's time at any clock below 2 GHz.
 __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, int* abort, const F8Gemm& a) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
+    if (mbar_try_wait(bar, parity) || mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+    const long long t0 = clock64();
     while (!mbar_try_wait_sleep(bar, parity, 20000u)) {
         if (*(volatile int*)abort) return false;
-        if (globaltimer_ns() - t0 > a.timeout_ns) {
+        if ((uint64_t)(clock64() - t0) > 2 * a.timeout_ns) {
             *(volatile int*)abort = 1;
             atomicOr(a.err, kErrTimeout);
             return false;
@@ -146,6 +147,71 @@ __device__ __forceinline__ bool f8_wait_cluster(uint64_t* bar, uint32_t parity, 
     }
 }
 
+// Scales travel ahead of the epilogue in a ring of their own: a slot holds CHUNK blocks' scales of a
+// tile's R token rows and of its (two) weight blocks.  One warp copies them asynchronously.
+template <int R, int CHUNK, int SLOTS>
+struct F8Scales {
+    static constexpr int kChunk = CHUNK, kSlots = SLOTS;
+    alignas(16) float tok[SLOTS][CHUNK][R];
+    float wt[SLOTS][CHUNK][2];
+    uint64_t full[SLOTS], empty[SLOTS];
+};
+__device__ __forceinline__ void cp_async4(float* dst, const float* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Arrives on bar once this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+template <int R, int CH, int SL>
+__device__ __forceinline__ void scales_init(F8Scales<R, CH, SL>& sc, int readers) {
+    for (int i = 0; i < SL; i++) mbar_init(&sc.full[i], 32), mbar_init(&sc.empty[i], readers);
+}
+// One item's scales of blocks [kb0, kb1); `chunk` counts on over the items.  All lanes of a warp.
+template <int MODE, int WB, int R, int CH, int SL>
+__device__ __forceinline__ bool scales_load(F8Scales<R, CH, SL>& sc, const F8Gemm& a, const F8Group& grp, const float* const (&wsp)[WB], int kb0,
+                                            int kb1, uint32_t& chunk, int* abort) {
+    constexpr int N = (R + 31) / 32;
+    const int lane = threadIdx.x & 31;
+    const float* xsp[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int r = lane + 32 * i;
+        xsp[i] = nullptr;
+        if (r < R && r < grp.rows)
+            xsp[i] = a.xs + (size_t)(MODE == kF8GateUp ? __ldg(a.perm + grp.row0 + r) : grp.row0 + r) * a.nkb;
+    }
+    for (int kb = kb0; kb < kb1; kb += CH, chunk++) {
+        const int s = chunk % SL;
+        bool ok = true;
+        if (chunk >= SL) ok = f8_wait(&sc.empty[s], ((chunk / SL) & 1) ^ 1, abort, a);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (xsp[i])
+#pragma unroll
+                for (int k = 0; k < CH; k++)
+                    if (kb + k < kb1) cp_async4(&sc.tok[s][k][lane + 32 * i], xsp[i] + kb + k);
+        if (lane < WB * CH) {
+            const int h = lane / CH, k = lane % CH;
+            if (kb + k < kb1) cp_async4(&sc.wt[s][k][h], wsp[h] + kb + k);
+        }
+        cp_async_arrive(&sc.full[s]);
+    }
+    return true;
+}
+
+// The tokens of slots c0 .. c0 + 3 of a group.  Behind the last slot the four rows are filled up with pad rows
+// of the token buffer, other ones in each CTA: the last token's own row again, in all CTAs at once, made one
+// line of L2 the busiest of all.
+constexpr int kF8PadRows = 512;
+__device__ __forceinline__ int4 f8_gather_rows(const F8Gemm& a, const F8Group& grp, int c0) {
+    const int32_t* p = a.perm + grp.row0;
+    const int pad = a.M + (blockIdx.x * 3) % (kF8PadRows - 2);
+    return make_int4(__ldg(p + c0), c0 + 1 < grp.rows ? __ldg(p + c0 + 1) : pad, c0 + 2 < grp.rows ? __ldg(p + c0 + 2) : pad + 1,
+                     c0 + 3 < grp.rows ? __ldg(p + c0 + 3) : pad + 2);
+}
+
 // SwiGLU as the other expert paths form it, in fp32.
 __device__ __forceinline__ float swiglu_f32(float g, float u) { return g / (1.f + expf(-g)) * u; }
 
@@ -168,6 +234,8 @@ __device__ __forceinline__ const float* f8_wscale(const F8Gemm& a, int expert, i
 
 // ---------------------------------------------------------------- few rows
 
+constexpr int kFewScales = 16;  // floats a token column of the scale ring and the maxima
+
 template <int MODE, int NQ>
 struct FewCfg {
     static constexpr int WB = MODE == kF8GateUp ? 2 : 1;  // weight tiles a stage: gate and up, or one
@@ -175,21 +243,22 @@ struct FewCfg {
     // two CTAs an SM; one where 64 rows of gate and up sums fill the registers
     static constexpr int kMinCtas = NQ == 64 && WB == 2 ? 1 : 2;
     static constexpr int kRed = NQ == 64 && WB == 2 ? 0 : WB * NQ * 128 * 4;  // partial sums of a cluster (none: no split)
-    static constexpr int kBudget = (kMinCtas == 2 ? 112 : 224) * 1024 - 2048;
+    static constexpr int kBudget = (kMinCtas == 2 ? 112 : 224) * 1024 - 2048 - (kFewScales) * NQ * 4;
     static constexpr int kStages = (kBudget - kRed) / kStage > 8 ? 8 : (kBudget - kRed) / kStage;
     static constexpr int kTmemCols = 2 * WB * NQ < 32 ? 32 : 2 * WB * NQ;
     static constexpr int kSmem = kStages * kStage + kRed + 1024;  // 1 KB: alignment of the ring
-    static_assert(kStages >= 2 && kSmem + 1024 <= 227 * 1024 / kMinCtas, "stages");
+    static_assert(kStages >= 2 && kSmem + 1024 + (kFewScales) * NQ * 4 <= 227 * 1024 / kMinCtas, "stages");
 };
 
-constexpr int kFewThreads = 192;  // 4 epilogue warps, the TMA warp, the MMA warp
+constexpr int kFewChunk = 4, kFewSlots = 3;
+constexpr int kFewThreads = 224;  // 4 epilogue warps, the TMA, the MMA and the scale warp
 
 template <int NQ>
 struct FewCtrl {
     uint64_t full[8], empty[8], dfull[2], dempty[2], red_full, red_free, done;
     uint32_t tmem;
     int abort;
-    float sq[2][NQ];         // token scales of a block
+    F8Scales<NQ, kFewChunk, kFewSlots> sc;
     float top[4][NQ];        // per-warp maxima of the activations
 };
 
@@ -212,6 +281,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
         mbar_init(&c.red_full, 4 * CS);
         mbar_init(&c.red_free, 4 * CS);
         mbar_init(&c.done, 1);
+        scales_init(c.sc, 4);
         c.abort = 0;
         fence_mbar_init();
     }
@@ -222,23 +292,22 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
     tc_fence_after();
     const uint32_t tmem = c.tmem;
     griddep_launch_dependents();
-    if (MODE != kF8Dense) griddep_wait();
+    griddep_wait();
     const int items = f8_groups<MODE>(a, NQ) * a.nt;
 
     if (warp == 4) {
         uint32_t g = 0;
         bool ok = true;
         const uint64_t pol_w = l2_evict_first(), pol_x = l2_evict_last();
-        if (MODE == kF8Dense) griddep_wait();
         for (int item = cid; ok && item < items; item += n_clusters) {
             const int n = item % a.nt;
             const F8Group grp = f8_group<MODE>(a, item / a.nt, NQ);
+            // gate/up: lane l gathers the tokens of slots 4 l ..; rows of the stage behind them keep what was there,
+            // and only columns that nobody reads come of them
             int4 rows = make_int4(0, 0, 0, 0);
-            if (MODE == kF8GateUp && lane < NQ / 4) {  // the tokens of four slots; the first slot's again behind the last
-                const int c0 = 4 * lane;
-                const int32_t* p = a.perm + grp.row0;
-                rows = make_int4(__ldg(p + (c0 < grp.rows ? c0 : 0)), __ldg(p + (c0 + 1 < grp.rows ? c0 + 1 : 0)),
-                                 __ldg(p + (c0 + 2 < grp.rows ? c0 + 2 : 0)), __ldg(p + (c0 + 3 < grp.rows ? c0 + 3 : 0)));
+            const int gathers = MODE == kF8GateUp ? (grp.rows + 3) / 4 : 0;
+            if (lane < gathers) {
+                rows = f8_gather_rows(a, grp, 4 * lane);
             }
             for (int kb = kb0; kb < kb1; kb++, g++) {
                 const int s = g % S;
@@ -247,7 +316,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                 if (!ok) break;
                 unsigned char* st = ring + (size_t)s * C::kStage;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&c.full[s], C::kStage);
+                    mbar_arrive_expect_tx(&c.full[s], MODE == kF8GateUp ? WB * 16384 + gathers * 512 : C::kStage);
                     if (MODE == kF8GateUp) {
                         tma_load_3d(st, &map_w, kb * 128, n * 128, grp.expert * 2, &c.full[s], pol_w);
                         tma_load_3d(st + 16384, &map_w, kb * 128, n * 128, grp.expert * 2 + 1, &c.full[s], pol_w);
@@ -258,7 +327,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                 }
                 if (MODE == kF8GateUp) {
                     __syncwarp();
-                    if (lane < NQ / 4) tma_gather4(st + 32768 + lane * 512, &map_x, kb * 128, rows, &c.full[s], pol_x);
+                    if (lane < gathers) tma_gather4(st + 32768 + lane * 512, &map_x, kb * 128, rows, &c.full[s], pol_x);
                 }
             }
         }
@@ -301,49 +370,48 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
             }
         }
         __syncwarp();
-    } else {
-        // epilogue: warp w holds weight rows [32 w, 32 w + 32) of the tile, one a lane, all token columns
-        const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
-        uint32_t g = 0, it = 0;
+    } else if (warp == 6) {
+        uint32_t chunk = 0;
         bool ok = true;
-        if (MODE == kF8Dense) griddep_wait();
-        for (int item = cid; item < items; item += n_clusters, it++) {
-            const int n = item % a.nt;
+        for (int item = cid; ok && item < items; item += n_clusters) {
             const F8Group grp = f8_group<MODE>(a, item / a.nt, NQ);
             const float* wsp[WB];
 #pragma unroll
-            for (int h = 0; h < WB; h++) wsp[h] = f8_wscale<MODE>(a, grp.expert, h, n);
-            const float* xsp = nullptr;  // scales of token column tid
-            if (tid < NQ && tid < grp.rows)
-                xsp = a.xs + (size_t)(MODE == kF8GateUp ? __ldg(a.perm + grp.row0 + tid) : grp.row0 + tid) * a.nkb;
+            for (int h = 0; h < WB; h++) wsp[h] = f8_wscale<MODE>(a, grp.expert, h, item % a.nt);
+            ok = scales_load<MODE, WB>(c.sc, a, grp, wsp, kb0, kb1, chunk, &c.abort);
+        }
+        cp_async_wait_all();
+    } else {
+        // epilogue: warp w holds weight rows [32 w, 32 w + 32) of the tile, one a lane, all token columns
+        const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+        uint32_t g = 0, it = 0, chunk = 0;
+        bool ok = true;
+        for (int item = cid; item < items; item += n_clusters, it++) {
+            const int n = item % a.nt;
+            const F8Group grp = f8_group<MODE>(a, item / a.nt, NQ);
             float acc[WB][NQ];
 #pragma unroll
             for (int h = 0; h < WB; h++)
 #pragma unroll
                 for (int j = 0; j < NQ; j++) acc[h][j] = 0.f;
-            if (tid < NQ) c.sq[g & 1][tid] = xsp && kb0 < kb1 ? __ldg(xsp + kb0) : 0.f;
-            float sw[WB];
-#pragma unroll
-            for (int h = 0; h < WB; h++) sw[h] = kb0 < kb1 ? __ldg(wsp[h] + kb0) : 0.f;
             for (int kb = kb0; kb < kb1; kb++, g++) {
-                const int b = g & 1;
-                const float next = xsp && kb + 1 < kb1 ? __ldg(xsp + kb + 1) : 0.f;
-                float sw_next[WB];
-#pragma unroll
-                for (int h = 0; h < WB; h++) sw_next[h] = kb + 1 < kb1 ? __ldg(wsp[h] + kb + 1) : 0.f;
+                const int b = g & 1, s = chunk % kFewSlots, k = (kb - kb0) % kFewChunk;
+                if (k == 0) ok = ok && f8_wait(&c.sc.full[s], (chunk / kFewSlots) & 1, &c.abort, a);
                 ok = ok && f8_wait(&c.dfull[b], (g >> 1) & 1, &c.abort, a);
-                named_bar_sync(1, 128);  // the block's token scales are in c.sq[b]; its last readers are past it
+                __syncwarp();
                 tc_fence_after();
+                float sw[WB];
+#pragma unroll
+                for (int h = 0; h < WB; h++) sw[h] = c.sc.wt[s][k][h];
 #pragma unroll
                 for (int j0 = 0; j0 < NQ; j0 += 16) {
                     uint32_t v[WB][16];
-                    __syncwarp();
 #pragma unroll
                     for (int h = 0; h < WB; h++) tmem_ld16(taddr + (b * WB + h) * NQ + j0, v[h]);
                     tmem_wait_ld();
 #pragma unroll
                     for (int j = 0; j < 16; j += 4) {
-                        const float4 q = *reinterpret_cast<const float4*>(&c.sq[b][j0 + j]);
+                        const float4 q = *reinterpret_cast<const float4*>(&c.sc.tok[s][k][j0 + j]);
                         const float qq[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                         for (int i = 0; i < 4; i++)
@@ -355,9 +423,10 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.dempty[b]);
-                if (tid < NQ) c.sq[b ^ 1][tid] = next;
-#pragma unroll
-                for (int h = 0; h < WB; h++) sw[h] = sw_next[h];
+                if (k == kFewChunk - 1 || kb + 1 == kb1) {
+                    if (lane == 0) mbar_arrive(&c.sc.empty[s]);
+                    chunk++;
+                }
             }
             // columns this CTA finishes: j -> token rank + CS j
             int mine = grp.rows;
@@ -410,7 +479,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                         if (i < a.N) a.aq[slot * a.N + i] = (uint8_t)f8_pack1(acc[0][j], f8_inverse(se));
                         if (tid == 0) a.as[slot * a.nb + n] = __uint_as_float(se << 23);
                     }
-                // the next item's first barrier comes before c.top is written again
+                named_bar_sync(1, 128);  // c.top is read before the next item's is written
             } else if (i < a.N) {
 #pragma unroll
                 for (int j = 0; j < NQ; j++)
@@ -433,21 +502,26 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
 
 // ---------------------------------------------------------------- many rows
 
+constexpr int kManyEpi = 16;                         // epilogue warps: 128 rows x four column quarters
+constexpr int kManyThreads = (kManyEpi + 3) * 32;    // and the TMA, the MMA and the scale warp
+
+template <int MODE>
+struct ManyCtrl {
+    uint64_t full[5], empty[5], dfull[2], dempty[2], done;
+    uint32_t tmem;
+    int abort;
+    F8Scales<128, 2, 2> sc;
+    uint32_t top[MODE == kF8GateUp ? 4 : 1][MODE == kF8GateUp ? 128 : 1];  // row maxima of the column quarters
+};
+
 template <int MODE, int NB>
 struct ManyCfg {
     static constexpr int kStage = 16384 + NB * 128;
-    static constexpr int kStages = NB == 256 ? 4 : 6;
-    static constexpr int kSmem = kStages * kStage + 1024;
+    static constexpr int kStages = NB == 256 ? 4 : 5;
+    static constexpr int kTurn = MODE == kF8GateUp ? 0 : 2048;  // a warp's 32 rows x 64 bytes on their way to memory
+    static constexpr int kSmem = kStages * kStage + kManyEpi * kTurn + (int)sizeof(ManyCtrl<MODE>);
     static_assert(MODE == kF8Dense || NB == 256, "the expert products use 256-row tiles");
-};
-
-constexpr int kManyThreads = 384;  // 8 epilogue warps, the TMA warp, the MMA warp, two idle ones
-
-struct ManyCtrl {
-    uint64_t full[6], empty[6], dfull[2], dempty[2], done;
-    uint32_t tmem;
-    int abort;
-    uint32_t top[2][128];  // gate/up: row maxima of the two column halves
+    static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 // Dense tiles in bands of 16 token tiles, weight tiles along the band: the tiles that run at a time share
@@ -464,23 +538,64 @@ __device__ __forceinline__ void many_tile(const F8Gemm& a, int item, int groups,
     }
 }
 
+// Stores a warp's 32 rows x 64 bytes (lane l holds row l as four 16-byte words) so that four lanes write a
+// row's 64 bytes: through shared memory, word w of row r at place w ^ (r / 2 & 3), conflict-free both ways.
+// Rows from `rows` and words from `words` on are left out.  (Each lane writing its own row, a store
+// instruction touched 32 rows: the last product of 2048 tokens took 259 us, 209 so.)
+__device__ __forceinline__ void turn_rows(unsigned char* turn, const uint4 (&w)[4], char* dst, size_t pitch, int rows, int words) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(turn + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) = w[k];
+    __syncwarp();
+    const int k = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int r = i * 8 + (lane >> 2);
+        const uint4 v = *reinterpret_cast<const uint4*>(turn + r * 64 + ((k ^ (r >> 1 & 3)) << 4));
+        if (r < rows && k < words) *reinterpret_cast<uint4*>(dst + r * pitch + k * 16) = v;
+    }
+}
+// A segment's 32 columns from column n0 on as fp32 or bf16, row0 = the warp's first row.
+template <bool F32>
+__device__ __forceinline__ void turn_store(unsigned char* turn, const float (&v)[32], void* out, size_t row0, int n0, int N, int rows) {
+    constexpr int B = F32 ? 4 : 2, W = 16 / B;  // bytes a value, values a word
+    char* dst = static_cast<char*>(out) + (row0 * N + n0) * B;
+#pragma unroll
+    for (int c = 0; c < 32; c += 4 * W) {
+        uint4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float* q = v + c + k * W;
+            if (F32) w[k] = make_uint4(__float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3]));
+            else w[k] = make_uint4(f8_bf16x2(q[0], q[1]), f8_bf16x2(q[2], q[3]), f8_bf16x2(q[W - 4], q[W - 3]), f8_bf16x2(q[W - 2], q[W - 1]));
+        }
+        turn_rows(turn, w, dst + c * B, (size_t)N * B, rows, (N - n0 - c) / W);
+    }
+}
+
 template <int MODE, int NB>
 __global__ void __launch_bounds__(kManyThreads, 1)
     f8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8Gemm a) {
     using C = ManyCfg<MODE, NB>;
-    constexpr int S = C::kStages;
+    constexpr int S = C::kStages, SEG = NB / 128;
     extern __shared__ __align__(1024) unsigned char f8_smem[];
-    __shared__ ManyCtrl c;
-    unsigned char* ring = reinterpret_cast<unsigned char*>(((uintptr_t)f8_smem + 1023) & ~(uintptr_t)1023);
+    unsigned char* ring = f8_smem;
+    ManyCtrl<MODE>& c = *reinterpret_cast<ManyCtrl<MODE>*>(ring + S * C::kStage + kManyEpi * C::kTurn);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(ring) & 1023) {  // the swizzled operands need it; the array is declared so
+        if (tid == 0) atomicOr(a.err, kErrTimeout);
+        return;
+    }
     if (tid == 0) {
         for (int s = 0; s < S; s++) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
-        for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1), mbar_init(&c.dempty[b], 8);
+        for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1), mbar_init(&c.dempty[b], kManyEpi);
         mbar_init(&c.done, 1);
+        scales_init(c.sc, kManyEpi);
         c.abort = 0;
         fence_mbar_init();
     }
-    if (warp == 9) tmem_alloc(&c.tmem, 2 * NB);
+    if (warp == kManyEpi + 1) tmem_alloc(&c.tmem, 2 * NB);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -489,222 +604,186 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     griddep_wait();
     const int groups = f8_groups<MODE>(a, 128), items = groups * a.nt, nkb = a.nkb;
 
-    if (warp >= 8) {
-        setmaxnreg_dec<72>();
-        if (warp == 8) {
+    if (warp == kManyEpi) {
+        uint32_t g = 0;
+        bool ok = true;
+        const uint64_t pol_w = MODE == kF8Dense ? l2_evict_last() : l2_evict_first(), pol_x = l2_evict_last();
+        for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            int gi, n;
+            many_tile<MODE>(a, item, groups, gi, n);
+            const F8Group grp = f8_group<MODE>(a, gi, 128);
+            int4 rows = make_int4(0, 0, 0, 0);  // as in the other form
+            const int gathers = MODE == kF8GateUp ? (grp.rows + 3) / 4 : 0;
+            if (lane < gathers) rows = f8_gather_rows(a, grp, 4 * lane);
+            for (int kb = 0; kb < nkb; kb++, g++) {
+                const int s = g % S;
+                if (g >= (uint32_t)S) ok = f8_wait(&c.empty[s], ((g / S) & 1) ^ 1, &c.abort, a);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                unsigned char* st = ring + (size_t)s * C::kStage;
+                unsigned char* sw = st + 16384;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&c.full[s], MODE == kF8GateUp ? 32768 + gathers * 512 : C::kStage);
+                    if (MODE == kF8GateUp) {
+                        tma_load_3d(sw, &map_w, kb * 128, n * 128, grp.expert * 2, &c.full[s], pol_w);
+                        tma_load_3d(sw + 16384, &map_w, kb * 128, n * 128, grp.expert * 2 + 1, &c.full[s], pol_w);
+                    } else {
+                        tma_load_2d(st, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
+#pragma unroll
+                        for (int h = 0; h < SEG; h++)
+                            tma_load_3d(sw + h * 16384, &map_w, kb * 128, n * NB + h * 128, grp.expert, &c.full[s], pol_w);
+                    }
+                }
+                if (MODE == kF8GateUp) {
+                    __syncwarp();
+                    if (lane < gathers) tma_gather4(st + lane * 512, &map_x, kb * 128, rows, &c.full[s], pol_x);
+                }
+            }
+        }
+        if (lane == 0) {  // every issued copy lands before the CTA may exit
+            const uint64_t t0 = globaltimer_ns();
+            for (uint32_t q = g > (uint32_t)S ? g - S : 0; q < g; q++)
+                while (!mbar_try_wait(&c.full[q % S], (q / S) & 1))
+                    if (globaltimer_ns() - t0 > a.timeout_ns) break;
+        }
+        __syncwarp();
+    } else if (warp == kManyEpi + 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = f8_idesc(NB);
             uint32_t g = 0;
             bool ok = true;
-            const uint64_t pol_w = MODE == kF8Dense ? l2_evict_last() : l2_evict_first(), pol_x = l2_evict_last();
             for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-                int gi, n;
-                many_tile<MODE>(a, item, groups, gi, n);
-                const F8Group grp = f8_group<MODE>(a, gi, 128);
-                int4 rows = make_int4(0, 0, 0, 0);
-                if (MODE == kF8GateUp) {
-                    const int c0 = 4 * lane;
-                    const int32_t* p = a.perm + grp.row0;
-                    rows = make_int4(__ldg(p + (c0 < grp.rows ? c0 : 0)), __ldg(p + (c0 + 1 < grp.rows ? c0 + 1 : 0)),
-                                     __ldg(p + (c0 + 2 < grp.rows ? c0 + 2 : 0)), __ldg(p + (c0 + 3 < grp.rows ? c0 + 3 : 0)));
-                }
                 for (int kb = 0; kb < nkb; kb++, g++) {
-                    const int s = g % S;
-                    if (g >= (uint32_t)S) ok = f8_wait(&c.empty[s], ((g / S) & 1) ^ 1, &c.abort, a);
-                    ok = __all_sync(0xffffffffu, ok);
+                    const int s = g % S, b = g & 1;
+                    ok = f8_wait(&c.full[s], (g / S) & 1, &c.abort, a);
+                    if (g >= 2) ok = ok && f8_wait(&c.dempty[b], ((g >> 1) & 1) ^ 1, &c.abort, a);
                     if (!ok) break;
-                    unsigned char* st = ring + (size_t)s * C::kStage;
-                    unsigned char* sw = st + 16384;
-                    if (lane == 0) {
-                        mbar_arrive_expect_tx(&c.full[s], C::kStage);
-                        if (MODE == kF8GateUp) {
-                            tma_load_3d(sw, &map_w, kb * 128, n * 128, grp.expert * 2, &c.full[s], pol_w);
-                            tma_load_3d(sw + 16384, &map_w, kb * 128, n * 128, grp.expert * 2 + 1, &c.full[s], pol_w);
-                        } else {
-                            tma_load_2d(st, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
+                    tc_fence_after();
+                    const uint32_t sx = smem_u32(ring + (size_t)s * C::kStage), sw = sx + 16384;
 #pragma unroll
-                            for (int h = 0; h < NB / 128; h++)
-                                tma_load_3d(sw + h * 16384, &map_w, kb * 128, n * NB + h * 128, grp.expert, &c.full[s], pol_w);
-                        }
-                    }
-                    if (MODE == kF8GateUp) {
-                        __syncwarp();
-                        tma_gather4(st + lane * 512, &map_x, kb * 128, rows, &c.full[s], pol_x);
-                    }
+                    for (int kk = 0; kk < 4; kk++)
+                        umma_f8(tmem + b * NB, sw128_desc(sx + kk * 32), sw128_desc(sw + kk * 32), idesc, kk > 0);
+                    umma_commit(&c.empty[s]);
+                    umma_commit(&c.dfull[b]);
                 }
             }
-            if (lane == 0) {
+            if (*(volatile int*)&c.abort) {
+                umma_commit(&c.done);
                 const uint64_t t0 = globaltimer_ns();
-                for (uint32_t q = g > (uint32_t)S ? g - S : 0; q < g; q++)
-                    while (!mbar_try_wait(&c.full[q % S], (q / S) & 1))
-                        if (globaltimer_ns() - t0 > a.timeout_ns) break;
+                while (!mbar_try_wait(&c.done, 0))
+                    if (globaltimer_ns() - t0 > a.timeout_ns) break;
             }
-            __syncwarp();
-        } else if (warp == 9) {
-            if (lane == 0) {
-                constexpr uint32_t idesc = f8_idesc(NB);
-                uint32_t g = 0;
-                bool ok = true;
-                for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
-                    for (int kb = 0; kb < nkb; kb++, g++) {
-                        const int s = g % S, b = g & 1;
-                        if (g >= 2) ok = f8_wait(&c.dempty[b], ((g >> 1) & 1) ^ 1, &c.abort, a);
-                        ok = ok && f8_wait(&c.full[s], (g / S) & 1, &c.abort, a);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t sx = smem_u32(ring + (size_t)s * C::kStage), sw = sx + 16384;
-#pragma unroll
-                        for (int kk = 0; kk < 4; kk++)
-                            umma_f8(tmem + b * NB, sw128_desc(sx + kk * 32), sw128_desc(sw + kk * 32), idesc, kk > 0);
-                        umma_commit(&c.empty[s]);
-                        umma_commit(&c.dfull[b]);
-                    }
-                }
-                if (*(volatile int*)&c.abort) {
-                    umma_commit(&c.done);
-                    const uint64_t t0 = globaltimer_ns();
-                    while (!mbar_try_wait(&c.done, 0))
-                        if (globaltimer_ns() - t0 > a.timeout_ns) break;
-                }
-            }
-            __syncwarp();
         }
-    } else {
-        setmaxnreg_inc<216>();
-        // epilogue: warp w holds token rows [32 (w % 4), ..), one a lane, and half the columns: segments of 64
-        constexpr int SEG = NB / 128;
-        const int q = warp & 3, half = warp >> 2, r = q * 32 + lane;
-        int col[SEG];
+        __syncwarp();
+    } else if (warp == kManyEpi + 2) {
+        uint32_t chunk = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            int gi, n;
+            many_tile<MODE>(a, item, groups, gi, n);
+            const F8Group grp = f8_group<MODE>(a, gi, 128);
+            const float* wsp[SEG];
 #pragma unroll
-        for (int i = 0; i < SEG; i++) col[i] = MODE == kF8GateUp ? i * 128 + half * 64 : (half * SEG + i) * 64;
-        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16);
-        uint32_t g = 0;
+            for (int h = 0; h < SEG; h++)
+                wsp[h] = f8_wscale<MODE>(a, grp.expert, h, MODE == kF8GateUp ? n : min(n * SEG + h, a.nb - 1));
+            ok = scales_load<MODE, SEG>(c.sc, a, grp, wsp, 0, nkb, chunk, &c.abort);
+        }
+        cp_async_wait_all();
+    } else {
+        // epilogue: warp w holds token rows [32 (w % 4), ..), one a lane, and a quarter of the columns in segments
+        // of 32 (gate/up: one of gate and the same of up).  Sixteen warps, since the scaled sums are bound by
+        // latency: eight, with 128 columns each, took 507 cycles a block where these take 320 (the MMAs: 512).
+        const int q = warp & 3, quarter = warp >> 2, r = q * 32 + lane;
+        unsigned char* turn = ring + S * C::kStage + warp * C::kTurn;
+        const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (MODE == kF8GateUp ? 32 : NB / 4) * quarter;
+        constexpr int SEGSTEP = MODE == kF8GateUp ? 128 : 32;  // accumulator columns between a warp's segments
+        const int wsel = MODE != kF8GateUp && NB == 256 ? quarter >> 1 : 0;
+        uint32_t g = 0, chunk = 0;
         bool ok = true;
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
             int gi, n;
             many_tile<MODE>(a, item, groups, gi, n);
             const F8Group grp = f8_group<MODE>(a, gi, 128);
-            const bool live = r < grp.rows;
-            const int slot = grp.row0 + (live ? r : 0);
-            const float* xsp = a.xs + (size_t)(MODE == kF8GateUp ? __ldg(a.perm + slot) : slot) * nkb;
-            const float* wsp[SEG];
-#pragma unroll
-            for (int i = 0; i < SEG; i++) {
-                const int block = MODE == kF8GateUp ? n : min((n * NB + col[i]) / 128, a.nb - 1);
-                wsp[i] = f8_wscale<MODE>(a, grp.expert, i, block);
-            }
-            f32x2 acc[SEG][32];
+            float acc[SEG][32];
 #pragma unroll
             for (int i = 0; i < SEG; i++)
 #pragma unroll
-                for (int j = 0; j < 32; j++) acc[i][j] = 0ull;
-            float sx = __ldg(xsp), sw[SEG];
-#pragma unroll
-            for (int i = 0; i < SEG; i++) sw[i] = __ldg(wsp[i]);
+                for (int j = 0; j < 32; j++) acc[i][j] = 0.f;
             for (int kb = 0; kb < nkb; kb++, g++) {
-                const int b = g & 1;
-                f32x2 s[SEG];
+                const int b = g & 1, sl = chunk & 1, k = kb & 1;
+                if (k == 0) ok = ok && f8_wait(&c.sc.full[sl], (chunk >> 1) & 1, &c.abort, a);
+                const float sx = c.sc.tok[sl][k][r];
+                float sw[SEG];
 #pragma unroll
-                for (int i = 0; i < SEG; i++) s[i] = pack_f32x2(sx * sw[i], sx * sw[i]);
-                if (kb + 1 < nkb) {
-                    sx = __ldg(xsp + kb + 1);
-#pragma unroll
-                    for (int i = 0; i < SEG; i++) sw[i] = __ldg(wsp[i] + kb + 1);
-                }
+                for (int i = 0; i < SEG; i++) sw[i] = sx * c.sc.wt[sl][k][MODE == kF8GateUp ? i : wsel];
                 ok = ok && f8_wait(&c.dfull[b], (g >> 1) & 1, &c.abort, a);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t v[2][32];
-                tmem_ld32(taddr + b * NB + col[0], v[0]);
+                uint32_t v[2][16];
+                tmem_ld16(taddr + b * NB, v[0]);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 2 * SEG; i++) {  // chunks of 32 columns; the next one is read while this one is added
-                    if (i + 1 < 2 * SEG) tmem_ld32(taddr + b * NB + col[(i + 1) / 2] + ((i + 1) & 1) * 32, v[(i + 1) & 1]);
+                for (int i = 0; i < 2 * SEG; i++) {  // the next sixteen columns are read while these are added
+                    if (i + 1 < 2 * SEG) tmem_ld16(taddr + b * NB + (i + 1) / 2 * SEGSTEP + ((i + 1) & 1) * 16, v[(i + 1) & 1]);
 #pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        acc[i / 2][(i & 1) * 16 + j] =
-                            ffma2(pack_f32x2(__uint_as_float(v[i & 1][2 * j]), __uint_as_float(v[i & 1][2 * j + 1])), s[i / 2],
-                                  acc[i / 2][(i & 1) * 16 + j]);
+                    for (int j = 0; j < 16; j++) {
+                        float& d = acc[i / 2][(i & 1) * 16 + j];
+                        d = fmaf(__uint_as_float(v[i & 1][j]), sw[i / 2], d);
+                    }
                     if (i + 1 < 2 * SEG) tmem_wait_ld();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.dempty[b]);
+                if (k == 1 || kb + 1 == nkb) {
+                    if (lane == 0) mbar_arrive(&c.sc.empty[sl]);
+                    chunk++;
+                }
             }
+            const bool live = r < grp.rows;
+            const size_t slot = (size_t)grp.row0 + r;
             if (MODE == kF8GateUp) {
                 uint32_t top = 0;
 #pragma unroll
                 for (int j = 0; j < 32; j++) {
-                    float g0, g1, u0, u1;
-                    unpack_f32x2(acc[0][j], g0, g1);
-                    unpack_f32x2(acc[SEG - 1][j], u0, u1);
-                    const float v0 = swiglu_f32(g0, u0), v1 = swiglu_f32(g1, u1);
-                    acc[0][j] = pack_f32x2(v0, v1);
-                    const uint32_t t0 = __float_as_uint(v0) & 0x7fffffffu, t1 = __float_as_uint(v1) & 0x7fffffffu;
-                    top = max(top, t0 < 0x7f800000u ? t0 : 0u);
-                    top = max(top, t1 < 0x7f800000u ? t1 : 0u);
+                    acc[0][j] = swiglu_f32(acc[0][j], acc[SEG - 1][j]);
+                    const uint32_t t = __float_as_uint(acc[0][j]) & 0x7fffffffu;
+                    top = max(top, t < 0x7f800000u ? t : 0u);
                 }
-                c.top[half][r] = top;
-                named_bar_sync(1, 256);
-                top = max(c.top[0][r], c.top[1][r]);
-                named_bar_sync(1, 256);  // read before the next item writes
+                c.top[quarter][r] = top;
+                named_bar_sync(1, kManyEpi * 32);
+                top = max(max(c.top[0][r], c.top[1 % (sizeof(c.top) / sizeof(c.top[0]))][r]),
+                          max(c.top[2 % (sizeof(c.top) / sizeof(c.top[0]))][r], c.top[3 % (sizeof(c.top) / sizeof(c.top[0]))][r]));
+                named_bar_sync(1, kManyEpi * 32);  // read before the next item writes
                 const uint32_t se = f8_scale_exp(top);
                 const float inv = f8_inverse(se);
-                const int f0 = n * 128 + half * 64;
-                if (live) {
-                    uint8_t* dst = a.aq + (size_t)slot * a.N + f0;
+                const int f0 = n * 128 + quarter * 32;
+                if (live && f0 < a.N) {  // F is a multiple of 64
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {  // sixteen values at a time (F is a multiple of 64)
-                        float v[16];
-#pragma unroll
-                        for (int i = 0; i < 8; i++) unpack_f32x2(acc[0][8 * j + i], v[2 * i], v[2 * i + 1]);
-                        const uint2 lo = f8_pack8(reinterpret_cast<const float(&)[8]>(v[0]), inv);
-                        const uint2 hi = f8_pack8(reinterpret_cast<const float(&)[8]>(v[8]), inv);
-                        if (f0 < a.N) reinterpret_cast<uint4*>(dst)[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                    for (int j = 0; j < 2; j++) {
+                        const uint2 lo = f8_pack8(reinterpret_cast<const float(&)[8]>(acc[0][16 * j]), inv);
+                        const uint2 hi = f8_pack8(reinterpret_cast<const float(&)[8]>(acc[0][16 * j + 8]), inv);
+                        reinterpret_cast<uint4*>(a.aq + slot * a.N + f0)[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
                     }
-                    if (half == 0) a.as[(size_t)slot * a.nb + n] = __uint_as_float(se << 23);
                 }
-            } else if (live) {
+                if (live && quarter == 0) a.as[slot * a.nb + n] = __uint_as_float(se << 23);
+            } else {
+                const int rows = min(32, grp.rows - q * 32);  // of this warp
+                const bool f32 = MODE == kF8Down || a.out_f32;
+                const size_t row0 = (size_t)grp.row0 + q * 32;
 #pragma unroll
                 for (int i = 0; i < SEG; i++) {
-                    const int n0 = n * NB + col[i];
-                    const size_t at = (size_t)slot * a.N + n0;
-                    if (MODE == kF8Down || a.out_f32) {
-                        float* dst = static_cast<float*>(a.out) + at;
-                        if (n0 + 64 <= a.N && a.N % 4 == 0) {
+                    const int n0 = n * NB + quarter * (NB / 4) + i * 32;
+                    if (a.N % (f32 ? 4 : 8) == 0) {
+                        if (f32) turn_store<true>(turn, acc[i], a.out, row0, n0, a.N, rows);
+                        else turn_store<false>(turn, acc[i], a.out, row0, n0, a.N, rows);
+                    } else if (live) {  // rows that are not 16-byte aligned
 #pragma unroll
-                            for (int j = 0; j < 16; j++)
-                                reinterpret_cast<ulonglong2*>(dst)[j] = make_ulonglong2(acc[i][2 * j], acc[i][2 * j + 1]);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; j++) {
-                                float v0, v1;
-                                unpack_f32x2(acc[i][j], v0, v1);
-                                if (n0 + 2 * j < a.N) dst[2 * j] = v0;
-                                if (n0 + 2 * j + 1 < a.N) dst[2 * j + 1] = v1;
+                        for (int j = 0; j < 32; j++)
+                            if (n0 + j < a.N) {
+                                if (f32) static_cast<float*>(a.out)[slot * a.N + n0 + j] = acc[i][j];
+                                else static_cast<uint16_t*>(a.out)[slot * a.N + n0 + j] = f8_bf16(acc[i][j]);
                             }
-                        }
-                    } else {
-                        uint16_t* dst = static_cast<uint16_t*>(a.out) + at;
-                        if (n0 + 64 <= a.N && a.N % 8 == 0) {
-#pragma unroll
-                            for (int j = 0; j < 8; j++) {
-                                uint32_t o[4];
-#pragma unroll
-                                for (int k = 0; k < 4; k++) {
-                                    float v0, v1;
-                                    unpack_f32x2(acc[i][4 * j + k], v0, v1);
-                                    o[k] = f8_bf16x2(v0, v1);
-                                }
-                                reinterpret_cast<uint4*>(dst)[j] = make_uint4(o[0], o[1], o[2], o[3]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 32; j++) {
-                                float v0, v1;
-                                unpack_f32x2(acc[i][j], v0, v1);
-                                if (n0 + 2 * j < a.N) dst[2 * j] = f8_bf16(v0);
-                                if (n0 + 2 * j + 1 < a.N) dst[2 * j + 1] = f8_bf16(v1);
-                            }
-                        }
                     }
                 }
             }
@@ -712,7 +791,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 9) {
+    if (warp == kManyEpi + 1) {
         tc_fence_after();
         tmem_dealloc(tmem, 2 * NB);
     }

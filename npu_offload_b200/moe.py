@@ -11,6 +11,7 @@
 PyTorch only provides device memory and streams here; every computation runs in libmoe_dp.so.
 """
 import ctypes
+import math
 from typing import NamedTuple
 
 import numpy as np
@@ -23,6 +24,8 @@ from ._lib import (MOE_DT_BF16, MOE_DT_F32, MOE_F_ACCUMULATE, MOE_F_HOST, MOE_F_
 __all__ = ["MoEDataPlane", "Fp8", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"]
 
 _DTYPES = {torch.bfloat16: MOE_DT_BF16, torch.float32: MOE_DT_F32}
+_F8 = torch.float8_e4m3fn
+_E4M3, _BF16, _F32, _I32, _MASK = (_F8,), (torch.bfloat16,), (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
 
 
 class Fp8(NamedTuple):
@@ -378,6 +381,8 @@ class MoEDataPlane:
         return q, sc, rs
 
     # ---- 8-bit floating point: e4m3 values with one scale for each 128 ----
+    # These calls take a few microseconds on the GPU at one token, so the host's share counts: checks
+    # cost an attribute each, and messages are made only when one fails.
     def quantize_fp8(self, x, block_rows=1, stream=None):
         """x [..., rows, cols] bf16 or fp32 -> Fp8(q, scale): one scale for each 128 columns of a row
         (block_rows=1, activations) or of 128 rows (block_rows=128, weights).  Scales are powers of two;
@@ -385,16 +390,17 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.quantize_fp8(x, block_rows)
-        x = self._operand("x", x, tuple(_DTYPES), None, 16)
-        _need(x.dim() >= 2 and block_rows in (1, 128), "quantize_fp8 takes [..., rows, cols] and block_rows 1 or 128")
-        *lead, rows, cols = x.shape
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=self.device)
-        scale = torch.empty(*lead, -(-rows // block_rows), -(-cols // 128), dtype=torch.float32, device=self.device)
-        batch = 1
-        for n in lead:
-            batch *= n
-        check(lib().moe_quantize_fp8(self._h, x.data_ptr(), _DTYPES[x.dtype], batch, rows, cols, block_rows, q.data_ptr(),
-                                     scale.data_ptr(), 0, self._raw_stream()))
+        x = self._operand("x", x, _DTYPES, None, 16)
+        shape = x.shape
+        if len(shape) < 2 or block_rows not in (1, 128):
+            raise ValueError("quantize_fp8 takes [..., rows, cols] and block_rows 1 or 128")
+        rows, cols = shape[-2:]
+        q = torch.empty_like(x, dtype=_F8)
+        scale = torch.empty((*shape[:-2], -(-rows // block_rows), -(-cols // 128)), dtype=torch.float32, device=self.device)
+        status = lib().moe_quantize_fp8(self._h, x.data_ptr(), _DTYPES[x.dtype], math.prod(shape[:-2]), rows, cols, block_rows,
+                                        q.data_ptr(), scale.data_ptr(), 0, self._raw_stream())
+        if status:
+            check(status)
         return Fp8(q, scale)
 
     def matmul_fp8(self, x, w, out_dtype=torch.bfloat16, out=None, stream=None):
@@ -403,15 +409,18 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.matmul_fp8(x, w, out_dtype, out)
-        if not isinstance(x, Fp8):
+        if type(x) is not Fp8:
             x = self.quantize_fp8(x)
         xq, xs = self._fp8("x", x, 2, 1)
         wq, ws = self._fp8("w", w, 2, 128)
-        (M, K), N = xq.shape, wq.shape[0]
-        _need(wq.shape[1] == K, f"x has {K} columns, w {wq.shape[1]}")
-        out = self._output(out, (M, N), out_dtype)
-        check(lib().moe_matmul_fp8(self._h, M, N, K, xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), out.data_ptr(),
-                                   _DTYPES[out.dtype], 0, self._raw_stream()))
+        (M, K), (N, wk) = xq.shape, wq.shape
+        if wk != K:
+            raise ValueError(f"x has {K} columns, w {wk}")
+        out = self._output(out, (M, N), out_dtype, _DTYPES)
+        status = lib().moe_matmul_fp8(self._h, M, N, K, xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), out.data_ptr(),
+                                      _DTYPES[out.dtype], 0, self._raw_stream())
+        if status:
+            check(status)
         return out
 
     def experts_fp8(self, x, gate_up, down, idx, w, out_dtype=torch.float32, out=None, accumulate=False, stream=None):
@@ -423,24 +432,32 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.experts_fp8(x, gate_up, down, idx, w, out_dtype, out, accumulate)
-        x = self._operand("x", x, (torch.bfloat16,), 2, 16)
-        T, H, F, E, K = x.shape[0], self.H, self.F, self.E, self.K
-        _need(x.shape[1] == H, f"x has {x.shape[1]} columns, the context {H}")
+        x = self._operand("x", x, _BF16, 2, 16)
+        H, F, E, K = self.H, self.F, self.E, self.K
+        T, cols = x.shape
+        if cols != H:
+            raise ValueError(f"x has {cols} columns, the context {H}")
         gq, gs = self._fp8("gate_up", gate_up, 4, 128)
         dq, ds = self._fp8("down", down, 3, 128)
-        _need(gq.shape == (E, 2, F, H), f"gate_up is {tuple(gq.shape)}, not {(E, 2, F, H)}")
-        _need(dq.shape == (E, H, F), f"down is {tuple(dq.shape)}, not {(E, H, F)}")
-        idx = self._operand("idx", idx, (torch.int32,), 2)
-        w = self._operand("w", w, (torch.float32,), 2)
-        _need(idx.shape == (T, K) and w.shape == (T, K), f"idx {tuple(idx.shape)} and w {tuple(w.shape)} must be {(T, K)}")
-        _need(out is not None or not accumulate, "accumulate needs an out to add to")
-        out = self._output(out, (T, H), out_dtype)
+        if gq.shape != (E, 2, F, H):
+            raise ValueError(f"gate_up is {tuple(gq.shape)}, not {(E, 2, F, H)}")
+        if dq.shape != (E, H, F):
+            raise ValueError(f"down is {tuple(dq.shape)}, not {(E, H, F)}")
+        idx = self._operand("idx", idx, _I32, 2)
+        w = self._operand("w", w, _F32, 2)
+        if idx.shape != (T, K) or w.shape != (T, K):
+            raise ValueError(f"idx {tuple(idx.shape)} and w {tuple(w.shape)} must be {(T, K)}")
+        if accumulate and out is None:
+            raise ValueError("accumulate needs an out to add to")
+        out = self._output(out, (T, H), out_dtype, _DTYPES)
         L = lib()
         n = L.moe_experts_fp8_workspace(self._h, T)
         ws = torch.empty(max(n, 0), dtype=torch.uint8, device=self.device)  # from the stream's pool, alive until enqueued
-        check(L.moe_experts_fp8(self._h, T, x.data_ptr(), gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(),
-                                idx.data_ptr(), w.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], ws.data_ptr(), n,
-                                MOE_F_ACCUMULATE if accumulate else 0, self._raw_stream()))
+        status = L.moe_experts_fp8(self._h, T, x.data_ptr(), gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(),
+                                   idx.data_ptr(), w.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], ws.data_ptr(), n,
+                                   MOE_F_ACCUMULATE if accumulate else 0, self._raw_stream())
+        if status:
+            check(status)
         return out
 
     def route_topk(self, logits, bias=None, stream=None):
@@ -449,13 +466,15 @@ class MoEDataPlane:
             with torch.cuda.stream(stream):
                 return self.route_topk(logits, bias)
         lg = _as(logits, torch.float32, self.device)
+        if lg.dim() != 2 or lg.shape[1] != self.E:
+            raise ValueError(f"logits are {tuple(lg.shape)}, the context has {self.E} experts")
         T = lg.shape[0]
-        _need(lg.dim() == 2 and lg.shape[1] == self.E, f"logits are {tuple(lg.shape)}, the context has {self.E} experts")
         b = None if bias is None else _as(bias, torch.float32, self.device)
         idx = torch.empty(T, self.K, dtype=torch.int32, device=self.device)
         w = torch.empty(T, self.K, dtype=torch.float32, device=self.device)
-        n = torch.empty(2 * self.E + 1 + max(1, T * self.K) + self.E + 1, dtype=torch.int32, device=self.device)
-        counts, offsets, perm, order, jobs = n.split([self.E, self.E + 1, max(1, T * self.K), self.E, 1])
+        pairs = max(1, T * self.K)
+        n = torch.empty(3 * self.E + 2 + pairs, dtype=torch.int32, device=self.device)
+        counts, offsets, perm, order, jobs = n.split([self.E, self.E + 1, pairs, self.E, 1])
         check(lib().moe_route(self._h, T, _vp(lg), _vp(b), _vp(idx), _vp(w), _vp(counts), _vp(offsets), _vp(perm), _vp(order),
                               _vp(jobs), 0, self._raw_stream()))
         return idx, w
@@ -471,19 +490,21 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.balance_loss(logits, idx, offsets, mask)
-        logits, offsets, mask = self._balance_inputs(logits, offsets, mask)
-        T, B = logits.shape[0], 1 if offsets is None else offsets.shape[0] - 1
-        idx = self._operand("idx", idx, (torch.int32,), 2)
-        _need(idx.shape == (T, self.K), f"idx is {tuple(idx.shape)}, not {(T, self.K)}")
-        loss = torch.empty((), dtype=torch.float32, device=self.device)
-        counts = torch.empty(B, self.E, dtype=torch.int32, device=self.device)
-        tokens = torch.empty(B + 1, dtype=torch.int32, device=self.device)
+        logits, offsets, mask, B, po, pm = self._balance_inputs(logits, offsets, mask)
+        T, E = logits.shape
+        idx = self._operand("idx", idx, _I32, 2)
+        if idx.shape != (T, self.K):
+            raise ValueError(f"idx is {tuple(idx.shape)}, not {(T, self.K)}")
         L = lib()
+        loss = torch.empty((), dtype=torch.float32, device=self.device)
+        counts = torch.empty((B, E), dtype=torch.int32, device=self.device)
+        tokens = torch.empty(B + 1, dtype=torch.int32, device=self.device)
         n = L.moe_balance_loss_workspace(self._h, T, B)
         ws = torch.empty(max(n, 0), dtype=torch.uint8, device=self.device)
-        check(L.moe_balance_loss(self._h, T, logits.data_ptr(), idx.data_ptr(), offsets.data_ptr() if offsets is not None else None, B,
-                                 mask.data_ptr() if mask is not None else None, loss.data_ptr(), counts.data_ptr(),
-                                 tokens.data_ptr(), ws.data_ptr(), n, 0, self._raw_stream()))
+        status = L.moe_balance_loss(self._h, T, logits.data_ptr(), idx.data_ptr(), po, B, pm, loss.data_ptr(), counts.data_ptr(),
+                                    tokens.data_ptr(), ws.data_ptr(), n, 0, self._raw_stream())
+        if status:
+            check(status)
         return loss, BalanceStats(counts, tokens, offsets, mask)
 
     def balance_loss_backward(self, logits, stats, grad=None, out=None, stream=None):
@@ -492,56 +513,75 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.balance_loss_backward(logits, stats, grad, out)
-        logits, offsets, mask = self._balance_inputs(logits, stats.offsets, stats.mask)
-        T, B = logits.shape[0], 1 if offsets is None else offsets.shape[0] - 1
-        counts = self._operand("stats.counts", stats.counts, (torch.int32,), 2)
-        tokens = self._operand("stats.tokens", stats.tokens, (torch.int32,), 1)
-        _need(counts.shape == (B, self.E) and tokens.shape == (B + 1,), "stats are of other sequences")
+        counts, tokens, offsets, mask = stats
+        logits, offsets, mask, B, po, pm = self._balance_inputs(logits, offsets, mask)
+        counts = self._operand("stats.counts", counts, _I32, 2)
+        tokens = self._operand("stats.tokens", tokens, _I32, 1)
+        T, E = logits.shape
+        if counts.shape != (B, E) or tokens.shape != (B + 1,):
+            raise ValueError("stats are of other sequences")
         if grad is not None:
-            grad = self._operand("grad", grad, (torch.float32,), 0)
-        out = self._output(out, (T, self.E), torch.float32, (torch.float32,))
-        check(lib().moe_balance_loss_backward(self._h, T, logits.data_ptr(), offsets.data_ptr() if offsets is not None else None, B,
-                                              mask.data_ptr() if mask is not None else None, counts.data_ptr(), tokens.data_ptr(),
-                                              grad.data_ptr() if grad is not None else None, out.data_ptr(), 0,
-                                              self._raw_stream()))
+            grad = self._operand("grad", grad, _F32, 0)
+        out = self._output(out, (T, E), torch.float32, _F32)
+        status = lib().moe_balance_loss_backward(self._h, T, logits.data_ptr(), po, B, pm, counts.data_ptr(), tokens.data_ptr(),
+                                                 None if grad is None else grad.data_ptr(), out.data_ptr(), 0, self._raw_stream())
+        if status:
+            check(status)
         return out
 
     def _balance_inputs(self, logits, offsets, mask):
-        logits = self._operand("logits", logits, (torch.float32,), 2)
-        _need(not (torch.is_grad_enabled() and logits.requires_grad),
-              "balance_loss records no autograd graph: pass logits.detach() and use balance_loss_backward")
-        _need(logits.shape[1] == self.E, f"logits have {logits.shape[1]} columns, the context {self.E} experts")
+        logits = self._operand("logits", logits, _F32, 2)
+        if logits.requires_grad and torch.is_grad_enabled():
+            raise ValueError("balance_loss records no autograd graph: pass logits.detach() and use balance_loss_backward")
+        if logits.shape[1] != self.E:
+            raise ValueError(f"logits have {logits.shape[1]} columns, the context {self.E} experts")
+        B, po, pm = 1, None, None
         if offsets is not None:
-            offsets = self._operand("offsets", offsets, (torch.int32,), 1)
-            _need(offsets.shape[0] >= 2, "offsets need two entries at least")
+            offsets = self._operand("offsets", offsets, _I32, 1)
+            B, po = offsets.shape[0] - 1, offsets.data_ptr()
+            if B < 1:
+                raise ValueError("offsets need two entries at least")
         if mask is not None:
-            mask = self._operand("mask", mask, (torch.bool, torch.uint8), 1)
-            _need(mask.shape[0] == logits.shape[0], f"mask has {mask.shape[0]} tokens, logits {logits.shape[0]}")
-        return logits, offsets, mask
+            mask = self._operand("mask", mask, _MASK, 1)
+            pm = mask.data_ptr()
+            if mask.shape[0] != logits.shape[0]:
+                raise ValueError(f"mask has {mask.shape[0]} tokens, logits {logits.shape[0]}")
+        return logits, offsets, mask, B, po, pm
 
     def _operand(self, name, t, dtypes, dims, align=1):
         """t as a contiguous tensor of this device, at a multiple of align bytes; other types and ranks are refused."""
-        _need(isinstance(t, torch.Tensor) and t.device == self.device, f"{name} must be a tensor on {self.device}")
-        _need(t.dtype in dtypes, f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
-        _need(dims is None or t.dim() == dims, f"{name} has {t.dim()} dimensions, not {dims}")
-        t = t.contiguous()
-        return t if t.data_ptr() % align == 0 else t.clone()
+        if not isinstance(t, torch.Tensor) or t.device != self.device:
+            raise ValueError(f"{name} must be a tensor on {self.device}")
+        if t.dtype not in dtypes:
+            raise ValueError(f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
+        if dims is not None and t.dim() != dims:
+            raise ValueError(f"{name} has {t.dim()} dimensions, not {dims}")
+        if not t.is_contiguous():
+            t = t.contiguous()
+        return t.clone() if align > 1 and t.data_ptr() % align else t
 
     def _fp8(self, name, m, dims, block_rows):
-        _need(isinstance(m, Fp8), f"{name} must be an Fp8, as quantize_fp8 gives it")
-        _need(block_rows == 1 or isinstance(m.q, torch.Tensor) and m.q.is_contiguous(), f"{name}.q must be contiguous")
-        q = self._operand(name + ".q", m.q, (torch.float8_e4m3fn,), dims, 16)
-        s = self._operand(name + ".scale", m.scale, (torch.float32,), dims)
-        want = (*q.shape[:-2], -(-q.shape[-2] // block_rows), -(-q.shape[-1] // 128))
-        _need(s.shape == want, f"{name}.scale is {tuple(s.shape)}, not {want}")
+        if type(m) is not Fp8:
+            raise ValueError(f"{name} must be an Fp8, as quantize_fp8 gives it")
+        q, s = m
+        if block_rows > 1 and isinstance(q, torch.Tensor) and not q.is_contiguous():
+            raise ValueError(f"{name}.q must be contiguous")
+        q = self._operand(name + ".q", q, _E4M3, dims, 16)
+        s = self._operand(name + ".scale", s, _F32, dims)
+        *lead, rows, cols = q.shape
+        want = (*lead, -(-rows // block_rows), -(-cols // 128))
+        if s.shape != want:
+            raise ValueError(f"{name}.scale is {tuple(s.shape)}, not {want}")
         return q, s
 
-    def _output(self, out, shape, dtype, dtypes=tuple(_DTYPES)):
+    def _output(self, out, shape, dtype, dtypes):
         if out is None:
-            _need(dtype in dtypes, f"out_dtype {dtype} is neither torch.bfloat16 nor torch.float32")
+            if dtype not in dtypes:
+                raise ValueError(f"out_dtype {dtype} is neither torch.bfloat16 nor torch.float32")
             return torch.empty(shape, dtype=dtype, device=self.device)
-        _need(out.device == self.device and out.dtype in dtypes and out.shape == shape and out.is_contiguous() and
-              out.data_ptr() % 16 == 0, f"out must be a contiguous, 16-byte aligned {shape} tensor on {self.device}")
+        if (out.device != self.device or out.dtype not in dtypes or out.shape != shape or not out.is_contiguous() or
+                out.data_ptr() % 16):
+            raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} tensor on {self.device}")
         return out
 
     def _raw_stream(self):
@@ -575,11 +615,6 @@ class MoEDataPlane:
         n = ctypes.c_int64()
         check(lib().moe_profile_read(self._h, ms, n_stages, ctypes.byref(n)))
         return list(ms), int(n.value)
-
-
-def _need(ok, message):
-    if not ok:
-        raise ValueError(message)
 
 
 def _cpu(t):
