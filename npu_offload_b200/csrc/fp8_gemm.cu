@@ -1,11 +1,15 @@
 // Scaled products of e4m3 operands and the routed-expert FFN built on them: choice of kernel, tensor maps,
 // launches, and the small kernels around the products (token quantiser with the grouping, combine).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 
 #include "common.cuh"
 #include "fp8.h"
 #include "fp8.cuh"
 #include "fp8_tc.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace moe {
 namespace {
@@ -63,6 +67,21 @@ cudaError_t launch(K kernel, int grid, int threads, int smem, int cluster, bool 
     return cudaLaunchKernelEx(&cfg, kernel, mw, mx, g);
 }
 
+// Launch ahead of the end of the kernel before it (which it waits for itself).
+template <class K, class... A>
+cudaError_t launch_after(K kernel, int grid, int threads, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 template <int MODE, int NQ>
 struct Few {
     using C = FewCfg<MODE, NQ>;
@@ -74,7 +93,7 @@ struct Few {
         if (e != cudaSuccess) return e;
         const int slots = sm_count * C::kMinCtas;
         int cs = 1;  // split the inner dimension while all CTAs are still on the GPU at once
-        while (C::kRed && cs < 8 && tiles * cs * 2 <= slots && cs * 2 <= g.nkb) cs *= 2;
+        while (cs < 8 && tiles * cs * 2 <= slots && cs * 2 <= g.nkb) cs *= 2;
         const int clusters = (int)std::min<int64_t>(tiles, slots / cs);
         return launch(k, clusters * cs, kFewThreads, C::kSmem, cs, pdl, st, mw, mx, g);
     }
@@ -125,97 +144,194 @@ cudaError_t launch_matmul_fp8(const MatmulF8& m, int sm_count, cudaStream_t st) 
 // ---- routed experts ----
 
 constexpr int kPrepThreads = 1024;
+constexpr int kPrepPairs = 1024;   // up to here every CTA of the token quantiser groups the pairs itself
+constexpr int kPlanCluster = 8;
 
 struct PrepArgs {
     const uint16_t* x;
     const int32_t* idx;
     int T, H, E, K, height;  // height: token rows of a group
-    uint8_t* xq;
-    float* xs;
+    uint8_t* xq;             // [slots, H]: each pair's token, an expert's pairs one after the other
+    float* xs;               // [slots, ceil(H / 128)]
     int32_t* pos;            // [T * K] slot of each pair, -1: none
-    int32_t* perm;           // [T * K] token of each slot
     F8Group* groups;
     int* n_groups;
     uint32_t* err;
 };
 
-// CTA 0 groups the pairs by expert; the others quantise the tokens.  A pair's place among its expert's
-// slots may differ from run to run: a slot's row is computed from that row alone, so no result does.
-__global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
-    griddep_launch_dependents();
-    const int tid = threadIdx.x;
-    if (blockIdx.x > 0) {
-        const uint32_t per_row = (uint32_t)(a.H + 127) / 128, groups = (uint32_t)a.T * per_row, sub = tid & 15;
-        const uint32_t stride = (gridDim.x - 1) * (kPrepThreads / 16);
-        for (uint32_t g = (blockIdx.x - 1) * (kPrepThreads / 16) + tid / 16; g - tid / 16 < groups; g += stride) {
-            const uint32_t row = g / per_row, c = (g - row * per_row) * 128 + sub * 8;
-            const bool in = g < groups && c < (uint32_t)a.H;
-            const uint4 w = in ? ldg_stream(a.x + (size_t)row * a.H + c) : make_uint4(0, 0, 0, 0);
-            const float f[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
-            uint32_t top = f8_top(f);
+// off, goff = exclusive sums of the experts' pairs and groups (one warp, eight experts a lane); returns the
+// number of groups in lane 31.
+__device__ __forceinline__ int prep_scan(const int* cnt, int* off, int* goff, int height) {
+    const int lane = threadIdx.x & 31;
+    int c = 0, g = 0;
+    for (int e = lane * 8; e < lane * 8 + 8; e++) c += cnt[e], g += (cnt[e] + height - 1) / height;
+    int ci = c, gi = g;
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const uint32_t se = f8_scale_exp(top);
-            if (in) *reinterpret_cast<uint2*>(a.xq + (size_t)row * a.H + c) = f8_pack8(f, f8_inverse(se));
-            if (sub == 0 && g < groups) a.xs[g] = __uint_as_float(se << 23);
-        }
-        return;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, ci, o), z = __shfl_up_sync(0xffffffffu, gi, o);
+        if (lane >= o) ci += y, gi += z;
     }
-    __shared__ int cnt[kMaxExperts], off[kMaxExperts], goff[kMaxExperts + 1];
-    const int P = a.T * a.K, E = a.E;
-    for (int e = tid; e < kMaxExperts; e += kPrepThreads) cnt[e] = 0;
+    c = ci - c, g = gi - g;
+    for (int e = lane * 8; e < lane * 8 + 8; e++) {
+        off[e] = c, goff[e] = g;
+        c += cnt[e], g += (cnt[e] + height - 1) / height;
+    }
+    return gi;
+}
+
+// Quantises the tokens, sixteen lanes a group of 128 values, and stores each to the slots of its K pairs: the
+// products then read an expert's rows as one matrix.  (Gathering the rows in the products, by TMA, took them
+// 1.6 us a block of 128 rows where whole tiles take 0.8.)  slots[p - first] = slot of pair p; `v`, `g`: the
+// thread's first values and group, already loaded.
+struct PrepLoad {
+    uint32_t g, stride, groups, per_row;
+    uint4 v;
+};
+__device__ __forceinline__ uint4 prep_load(const PrepArgs& a, const PrepLoad& l, uint32_t g) {
+    const uint32_t row = g / l.per_row, c = (g - row * l.per_row) * 128 + (threadIdx.x & 15) * 8;
+    return g < l.groups && c < (uint32_t)a.H ? ldg_stream(a.x + (size_t)row * a.H + c) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ PrepLoad prep_begin(const PrepArgs& a) {
+    PrepLoad l;
+    l.per_row = (uint32_t)(a.H + 127) / 128;
+    l.groups = (uint32_t)a.T * l.per_row;
+    l.stride = gridDim.x * (kPrepThreads / 16);
+    l.g = blockIdx.x * (kPrepThreads / 16) + threadIdx.x / 16;
+    l.v = prep_load(a, l, l.g);
+    return l;
+}
+__device__ __forceinline__ void prep_rows(const PrepArgs& a, PrepLoad l, const int* slots) {
+    const uint32_t sub = threadIdx.x & 15;
+    for (uint32_t g = l.g; g - threadIdx.x / 16 < l.groups; g += l.stride) {
+        const uint32_t row = g / l.per_row, c = (g - row * l.per_row) * 128 + sub * 8;
+        const bool in = g < l.groups && c < (uint32_t)a.H;
+        const uint4 w = l.v;
+        l.v = prep_load(a, l, g + l.stride);
+        const float f[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
+        uint32_t top = f8_top(f);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint32_t se = f8_scale_exp(top);
+        const uint2 q = f8_pack8(f, f8_inverse(se));
+        if (g < l.groups)
+            for (int k = 0; k < a.K; k++) {
+                const int s = slots[row * a.K + k];
+                if (s < 0) continue;
+                if (in) *reinterpret_cast<uint2*>(a.xq + (size_t)s * a.H + c) = q;
+                if (sub == 0) a.xs[(size_t)s * l.per_row + (g - row * l.per_row)] = __uint_as_float(se << 23);
+            }
+    }
+}
+
+// Few pairs: every CTA finds all pairs' slots itself, in the pairs' order within each expert (so that all
+// agree), and quantises its share of the tokens; CTA 0 stores the slots and groups.
+__global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
+    __shared__ int wc[kPrepPairs / 32][kMaxExperts];  // pairs of each warp on each expert, then their exclusive sums
+    __shared__ int cnt[kMaxExperts], off[kMaxExperts], goff[kMaxExperts], slots[kPrepPairs];
+    griddep_launch_dependents();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, P = a.T * a.K, warps = (P + 31) / 32;
+    const int e = tid < P ? __ldg(a.idx + tid) : -1;
+    const PrepLoad l = prep_begin(a);
+    for (int i = tid; i < warps * kMaxExperts; i += kPrepThreads) (&wc[0][0])[i] = 0;
     __syncthreads();
-    constexpr int U = 8;  // index loads in flight
+    const bool ok = e >= 0 && e < a.E;
+    const uint32_t same = __match_any_sync(0xffffffffu, ok ? e : -1);
+    const int before = __popc(same & ((1u << lane) - 1));
+    if (ok && before == 0) wc[warp][e] = __popc(same);
+    if (e >= a.E && blockIdx.x == 0) atomicOr(a.err, kErrBadIndex);
+    __syncthreads();
+    if (tid < kMaxExperts) {
+        int n = 0;
+        for (int w = 0; w < warps; w++) {
+            const int t = wc[w][tid];
+            wc[w][tid] = n;
+            n += t;
+        }
+        cnt[tid] = n;
+    }
+    __syncthreads();
+    if (tid < 32) {
+        const int n = prep_scan(cnt, off, goff, a.height);
+        if (tid == 31 && blockIdx.x == 0) *a.n_groups = n;
+    }
+    __syncthreads();
+    const int slot = ok ? off[e] + wc[warp][e] + before : -1;
+    if (tid < P) {
+        slots[tid] = slot;
+        if (blockIdx.x == 0) a.pos[tid] = slot;
+    }
+    if (blockIdx.x == 0 && tid < a.E)
+        for (int g = 0; g * a.height < cnt[tid]; g++)
+            a.groups[goff[tid] + g] = F8Group{off[tid] + g * a.height, min(a.height, cnt[tid] - g * a.height), tid, 0};
+    __syncthreads();
+    prep_rows(a, l, slots);
+}
+
+// Many pairs: one cluster finds the slots, an eighth of the pairs a CTA.  A pair's place among its CTA's pairs
+// on the expert may differ from run to run: a slot's row is computed from that row alone, so no result does.
+__global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPrepThreads) f8_plan_kernel(PrepArgs a) {
+    __shared__ int mine[kMaxExperts], cnt[kMaxExperts], off[kMaxExperts], goff[kMaxExperts];
+    cg::cluster_group cl = cg::this_cluster();
+    griddep_launch_dependents();
+    const int tid = threadIdx.x, rank = (int)cl.block_rank(), E = a.E;
+    const int P = a.T * a.K, share = (P + kPlanCluster - 1) / kPlanCluster, first = min(P, rank * share), last = min(P, first + share);
+    if (tid < kMaxExperts) mine[tid] = 0;
+    __syncthreads();
+    constexpr int U = 4;  // index loads in flight
     bool bad = false;
-    for (int p0 = tid; p0 < P; p0 += U * kPrepThreads) {
+    for (int p0 = first + tid; p0 < last; p0 += U * kPrepThreads) {
         int e[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) e[u] = p0 + u * kPrepThreads < P ? __ldg(a.idx + p0 + u * kPrepThreads) : -1;
+        for (int u = 0; u < U; u++) e[u] = p0 + u * kPrepThreads < last ? __ldg(a.idx + p0 + u * kPrepThreads) : -1;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int p = p0 + u * kPrepThreads;
             bad |= e[u] >= E;
-            if (p < P) a.pos[p] = e[u] >= 0 && e[u] < E ? atomicAdd(&cnt[e[u]], 1) : -1;
+            if (p < last) a.pos[p] = e[u] >= 0 && e[u] < E ? atomicAdd(&mine[e[u]], 1) : -1;
         }
     }
     if (bad) atomicOr(a.err, kErrBadIndex);
-    __syncthreads();
-    if (tid < 32) {  // exclusive sums of the counts and of the groups, eight experts a lane
-        int c = 0, g = 0;
-        for (int e = tid * 8; e < tid * 8 + 8; e++) c += cnt[e], g += (cnt[e] + a.height - 1) / a.height;
-        int ci = c, gi = g;
+    cl.sync();
+    int before = 0;  // pairs on expert tid of the CTAs before this one
+    if (tid < kMaxExperts) {
+        int n = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, ci, o), z = __shfl_up_sync(0xffffffffu, gi, o);
-            if (tid >= o) ci += y, gi += z;
+        for (int r = 0; r < kPlanCluster; r++) {
+            const int c = cl.map_shared_rank(mine, r)[tid];
+            if (r < rank) before += c;
+            n += c;
         }
-        c = ci - c, g = gi - g;
-        for (int e = tid * 8; e < tid * 8 + 8; e++) {
-            off[e] = c, goff[e] = g;
-            c += cnt[e], g += (cnt[e] + a.height - 1) / a.height;
-        }
-        if (tid == 31) *a.n_groups = gi;
+        cnt[tid] = n;
     }
     __syncthreads();
-    for (int p0 = tid; p0 < P; p0 += U * kPrepThreads) {
+    if (tid < 32) {
+        const int n = prep_scan(cnt, off, goff, a.height);
+        if (tid == 31 && rank == 0) *a.n_groups = n;
+    }
+    cl.sync();  // every CTA has read the others' counts
+    if (tid < kMaxExperts) mine[tid] = off[tid] + before;
+    __syncthreads();
+    for (int p0 = first + tid; p0 < last; p0 += U * kPrepThreads) {
         int e[U], r[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int p = p0 + u * kPrepThreads;
-            r[u] = p < P ? a.pos[p] : -1;
-            e[u] = p < P ? __ldg(a.idx + p) : -1;
+            r[u] = p < last ? a.pos[p] : -1;
+            e[u] = p < last ? __ldg(a.idx + p) : -1;
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (r[u] >= 0) {
-                const int p = p0 + u * kPrepThreads, slot = off[e[u]] + r[u];
-                a.pos[p] = slot;
-                a.perm[slot] = p / a.K;
-            }
+            if (r[u] >= 0) a.pos[p0 + u * kPrepThreads] = mine[e[u]] + r[u];
     }
-    for (int e = tid; e < E; e += kPrepThreads)
-        for (int g = 0; g * a.height < cnt[e]; g++)
-            a.groups[goff[e] + g] = F8Group{off[e] + g * a.height, min(a.height, cnt[e] - g * a.height), e, 0};
+    if (tid < E)
+        for (int g = rank; g * a.height < cnt[tid]; g += kPlanCluster)
+            a.groups[goff[tid] + g] = F8Group{off[tid] + g * a.height, min(a.height, cnt[tid] - g * a.height), tid, 0};
+}
+__global__ void __launch_bounds__(kPrepThreads) f8_scatter_kernel(PrepArgs a) {
+    griddep_launch_dependents();
+    const PrepLoad l = prep_begin(a);
+    griddep_wait();
+    prep_rows(a, l, a.pos);
 }
 
 // out[t] = (out[t] +) sum_k w[t, k] y[slot of (t, k)], in order of k; four columns a thread.  Eight slots are
@@ -264,7 +380,7 @@ int group_height(int64_t pairs, int E) {
 struct Ws {
     uint8_t *xq, *aq;
     float *xs, *as, *y;
-    int32_t *pos, *perm;
+    int32_t* pos;
     F8Group* groups;
     int* n_groups;
     size_t bytes;
@@ -279,13 +395,12 @@ Ws experts_layout(void* ws, int T, int K, int H, int F, int E) {
         return r;
     };
     const size_t P = (size_t)T * K, hb = (H + 127) / 128, fb = (F + 127) / 128;
-    w.xq = (uint8_t*)take(((size_t)T + kF8PadRows) * H);
-    w.xs = (float*)take(4 * (size_t)T * hb);
+    w.xq = (uint8_t*)take(P * H);
+    w.xs = (float*)take(4 * P * hb);
     w.aq = (uint8_t*)take(P * F);
     w.as = (float*)take(4 * P * fb);
     w.y = (float*)take(4 * P * H);
     w.pos = (int32_t*)take(4 * P);
-    w.perm = (int32_t*)take(4 * P);
     w.groups = (F8Group*)take(sizeof(F8Group) * (P / 16 + std::min<size_t>(E, P)));
     w.n_groups = (int*)take(4);
     w.bytes = o;
@@ -311,13 +426,22 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     const int height = group_height(P, a.E);
     const int64_t groups = std::min<int64_t>(a.E, P) + P / height;  // at most
     CUtensorMap m[4];
-    if (!encode3(enc, &m[0], a.gu, a.H, a.F, 2 * (int64_t)a.E, 128) || !encode2(enc, &m[1], w.xq, a.H, a.T + kF8PadRows, 1) ||
+    if (!encode3(enc, &m[0], a.gu, a.H, a.F, 2 * (int64_t)a.E, 128) || !encode2(enc, &m[1], w.xq, a.H, P, height) ||
         !encode3(enc, &m[2], a.d, a.F, a.H, a.E, 128) || !encode2(enc, &m[3], w.aq, a.F, P, height))
         return cudaErrorInvalidValue;
-    PrepArgs pa{a.x, a.idx, a.T, a.H, a.E, a.K, height, w.xq, w.xs, w.pos, w.perm, w.groups, w.n_groups, a.err};
-    const int64_t qctas = ((int64_t)a.T * ((a.H + 127) / 128) + kPrepThreads / 16 - 1) / (kPrepThreads / 16);
-    f8_prep_kernel<<<1 + (int)std::min<int64_t>(qctas, 2 * sm_count), kPrepThreads, 0, st>>>(pa);
-    cudaError_t e = cudaGetLastError();
+    const PrepArgs pa{a.x, a.idx, a.T, a.H, a.E, a.K, height, w.xq, w.xs, w.pos, w.groups, w.n_groups, a.err};
+    const int qctas = (int)std::min<int64_t>(((int64_t)a.T * ((a.H + 127) / 128) + kPrepThreads / 16 - 1) / (kPrepThreads / 16),
+                                             2 * sm_count);
+    cudaError_t e;
+    if (P <= kPrepPairs) {
+        f8_prep_kernel<<<qctas, kPrepThreads, 0, st>>>(pa);
+        e = cudaGetLastError();
+    } else {
+        f8_plan_kernel<<<kPlanCluster, kPrepThreads, 0, st>>>(pa);
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = launch_after(f8_scatter_kernel, qctas, kPrepThreads, st, pa);
+        ++*launches;
+    }
     if (e != cudaSuccess) return e;
 
     F8Gemm gu{}, dn{};
@@ -325,11 +449,9 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     gu.ws = a.gus;
     gu.nkb = (a.H + 127) / 128;
     gu.nb = gu.nt = (a.F + 127) / 128;
-    gu.M = a.T;
     gu.N = a.F;
     gu.groups = w.groups;
     gu.n_groups = w.n_groups;
-    gu.perm = w.perm;
     gu.aq = w.aq;
     gu.as = w.as;
     gu.err = a.err;
@@ -351,18 +473,9 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
         if (e == cudaSuccess) e = Many<kF8Down, 256>::run(m[2], m[3], dn, groups * dn.nt, sm_count, true, st);
     }
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((int)std::min<int64_t>(((int64_t)a.T * a.H / 4 + 255) / 256, sm_count * 8));
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
     *launches += 4;
-    return cudaLaunchKernelEx(&cfg, f8_combine_kernel, (const float*)w.y, (const int32_t*)w.pos, a.w, a.T, a.K, a.H, a.out, a.out_f32,
-                              a.accumulate);
+    return launch_after(f8_combine_kernel, (int)std::min<int64_t>(((int64_t)a.T * a.H / 4 + 255) / 256, sm_count * 8), 256, st,
+                        (const float*)w.y, (const int32_t*)w.pos, a.w, a.T, a.K, a.H, a.out, a.out_f32, a.accumulate);
 }
 
 }  // namespace moe

@@ -39,7 +39,6 @@ struct F8Gemm {
     int M, N;                // tokens; weight rows of a matrix (dense N, gate/up F, down H)
     const F8Group* groups;   // experts: token groups
     const int* n_groups;     //   and their number (device); dense: null
-    const int32_t* perm;     // gate/up: token of each slot
     void* out;               // dense: [M, N]; down: y [slots, N] fp32
     int out_f32;
     uint8_t* aq;             // gate/up: quantised activations [slots, N]
@@ -62,15 +61,6 @@ __device__ __forceinline__ bool f8_wait(uint64_t* bar, uint32_t parity, int* abo
         }
     }
     return true;
-}
-
-// Four 128-byte rows r0..r3 at byte column x of a [rows, cols] byte matrix (boxes one row high).
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* map, int x, int4 r, uint64_t* bar, uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint [%0], "
-        "[%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(smem_u32(dst)),
-        "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w), "l"(policy)
-        : "memory");
 }
 
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc) {
@@ -100,6 +90,18 @@ __device__ __forceinline__ void tmem_dealloc(uint32_t taddr, int cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols));
 }
 
+// True in one lane of a converged warp.  The MMA warp runs its loop as a whole and one lane issues: descriptors
+// stay in uniform registers (issued by one diverged thread, the four MMAs of a block took 800 cycles).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -127,7 +129,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
 }
 // As f8_wait, acquiring what other CTAs of the cluster wrote before they arrived.
 __device__ __forceinline__ bool f8_wait_cluster(uint64_t* bar, uint32_t parity, int* abort, const F8Gemm& a) {
-    const uint64_t t0 = globaltimer_ns();
+    const long long t0 = clock64();
     while (true) {
         uint32_t ok;
         asm volatile(
@@ -139,7 +141,7 @@ __device__ __forceinline__ bool f8_wait_cluster(uint64_t* bar, uint32_t parity, 
             : "memory");
         if (ok) return true;
         if (*(volatile int*)abort) return false;
-        if (globaltimer_ns() - t0 > a.timeout_ns) {
+        if ((uint64_t)(clock64() - t0) > 2 * a.timeout_ns) {
             *(volatile int*)abort = 1;
             atomicOr(a.err, kErrTimeout);
             return false;
@@ -168,7 +170,7 @@ __device__ __forceinline__ void scales_init(F8Scales<R, CH, SL>& sc, int readers
     for (int i = 0; i < SL; i++) mbar_init(&sc.full[i], 32), mbar_init(&sc.empty[i], readers);
 }
 // One item's scales of blocks [kb0, kb1); `chunk` counts on over the items.  All lanes of a warp.
-template <int MODE, int WB, int R, int CH, int SL>
+template <int WB, int R, int CH, int SL>
 __device__ __forceinline__ bool scales_load(F8Scales<R, CH, SL>& sc, const F8Gemm& a, const F8Group& grp, const float* const (&wsp)[WB], int kb0,
                                             int kb1, uint32_t& chunk, int* abort) {
     constexpr int N = (R + 31) / 32;
@@ -179,7 +181,7 @@ __device__ __forceinline__ bool scales_load(F8Scales<R, CH, SL>& sc, const F8Gem
         const int r = lane + 32 * i;
         xsp[i] = nullptr;
         if (r < R && r < grp.rows)
-            xsp[i] = a.xs + (size_t)(MODE == kF8GateUp ? __ldg(a.perm + grp.row0 + r) : grp.row0 + r) * a.nkb;
+            xsp[i] = a.xs + (size_t)(grp.row0 + r) * a.nkb;
     }
     for (int kb = kb0; kb < kb1; kb += CH, chunk++) {
         const int s = chunk % SL;
@@ -199,17 +201,6 @@ __device__ __forceinline__ bool scales_load(F8Scales<R, CH, SL>& sc, const F8Gem
         cp_async_arrive(&sc.full[s]);
     }
     return true;
-}
-
-// The tokens of slots c0 .. c0 + 3 of a group.  Behind the last slot the four rows are filled up with pad rows
-// of the token buffer, other ones in each CTA: the last token's own row again, in all CTAs at once, made one
-// line of L2 the busiest of all.
-constexpr int kF8PadRows = 512;
-__device__ __forceinline__ int4 f8_gather_rows(const F8Gemm& a, const F8Group& grp, int c0) {
-    const int32_t* p = a.perm + grp.row0;
-    const int pad = a.M + (blockIdx.x * 3) % (kF8PadRows - 2);
-    return make_int4(__ldg(p + c0), c0 + 1 < grp.rows ? __ldg(p + c0 + 1) : pad, c0 + 2 < grp.rows ? __ldg(p + c0 + 2) : pad + 1,
-                     c0 + 3 < grp.rows ? __ldg(p + c0 + 3) : pad + 2);
 }
 
 // SwiGLU as the other expert paths form it, in fp32.
@@ -242,7 +233,7 @@ struct FewCfg {
     static constexpr int kStage = WB * 16384 + NQ * 128;
     // two CTAs an SM; one where 64 rows of gate and up sums fill the registers
     static constexpr int kMinCtas = NQ == 64 && WB == 2 ? 1 : 2;
-    static constexpr int kRed = NQ == 64 && WB == 2 ? 0 : WB * NQ * 128 * 4;  // partial sums of a cluster (none: no split)
+    static constexpr int kRed = WB * NQ * 128 * 4;  // the sums on their way to the CTA that finishes them
     static constexpr int kBudget = (kMinCtas == 2 ? 112 : 224) * 1024 - 2048 - (kFewScales) * NQ * 4;
     static constexpr int kStages = (kBudget - kRed) / kStage > 8 ? 8 : (kBudget - kRed) / kStage;
     static constexpr int kTmemCols = 2 * WB * NQ < 32 ? 32 : 2 * WB * NQ;
@@ -259,7 +250,7 @@ struct FewCtrl {
     uint32_t tmem;
     int abort;
     F8Scales<NQ, kFewChunk, kFewSlots> sc;
-    float top[4][NQ];        // per-warp maxima of the activations
+    uint32_t top[4][NQ];     // per-warp maxima of the activations
 };
 
 template <int MODE, int NQ>
@@ -302,13 +293,6 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
         for (int item = cid; ok && item < items; item += n_clusters) {
             const int n = item % a.nt;
             const F8Group grp = f8_group<MODE>(a, item / a.nt, NQ);
-            // gate/up: lane l gathers the tokens of slots 4 l ..; rows of the stage behind them keep what was there,
-            // and only columns that nobody reads come of them
-            int4 rows = make_int4(0, 0, 0, 0);
-            const int gathers = MODE == kF8GateUp ? (grp.rows + 3) / 4 : 0;
-            if (lane < gathers) {
-                rows = f8_gather_rows(a, grp, 4 * lane);
-            }
             for (int kb = kb0; kb < kb1; kb++, g++) {
                 const int s = g % S;
                 if (g >= (uint32_t)S) ok = f8_wait(&c.empty[s], ((g / S) & 1) ^ 1, &c.abort, a);
@@ -316,18 +300,11 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                 if (!ok) break;
                 unsigned char* st = ring + (size_t)s * C::kStage;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&c.full[s], MODE == kF8GateUp ? WB * 16384 + gathers * 512 : C::kStage);
-                    if (MODE == kF8GateUp) {
-                        tma_load_3d(st, &map_w, kb * 128, n * 128, grp.expert * 2, &c.full[s], pol_w);
-                        tma_load_3d(st + 16384, &map_w, kb * 128, n * 128, grp.expert * 2 + 1, &c.full[s], pol_w);
-                    } else {
-                        tma_load_3d(st, &map_w, kb * 128, n * 128, grp.expert, &c.full[s], pol_w);
-                        tma_load_2d(st + 16384, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
-                    }
-                }
-                if (MODE == kF8GateUp) {
-                    __syncwarp();
-                    if (lane < gathers) tma_gather4(st + 32768 + lane * 512, &map_x, kb * 128, rows, &c.full[s], pol_x);
+                    mbar_arrive_expect_tx(&c.full[s], C::kStage);
+#pragma unroll
+                    for (int h = 0; h < WB; h++)
+                        tma_load_3d(st + h * 16384, &map_w, kb * 128, n * 128, grp.expert * WB + h, &c.full[s], pol_w);
+                    tma_load_2d(st + WB * 16384, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
                 }
             }
         }
@@ -340,8 +317,10 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
         }
         __syncwarp();
     } else if (warp == 5) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = f8_idesc(NQ);
+        constexpr uint32_t idesc = f8_idesc(NQ);
+        const bool leader = elect_one();
+        const uint64_t desc0 = sw128_desc(smem_u32(ring));
+        {
             uint32_t g = 0;
             bool ok = true;
             for (int item = cid; ok && item < items; item += n_clusters) {
@@ -351,18 +330,20 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                     ok = ok && f8_wait(&c.full[s], (g / S) & 1, &c.abort, a);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sw = smem_u32(ring + (size_t)s * C::kStage), sx = sw + WB * 16384;
+                    const uint64_t dw = desc0 + (uint64_t)(s * (C::kStage >> 4)), dx = dw + WB * 1024;
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
+                        for (int kk = 0; kk < 4; kk++)
 #pragma unroll
-                        for (int h = 0; h < WB; h++)
-                            umma_f8(tmem + (b * WB + h) * NQ, sw128_desc(sw + h * 16384 + kk * 32), sw128_desc(sx + kk * 32),
-                                    idesc, kk > 0);
-                    umma_commit(&c.empty[s]);
-                    umma_commit(&c.dfull[b]);
+                            for (int h = 0; h < WB; h++)
+                                umma_f8(tmem + (b * WB + h) * NQ, dw + h * 1024 + kk * 2, dx + kk * 2, idesc, kk > 0);
+                        umma_commit(&c.empty[s]);
+                        umma_commit(&c.dfull[b]);
+                    }
+                    __syncwarp();
                 }
             }
-            if (*(volatile int*)&c.abort) {  // MMAs that no warp waited for
+            if (leader && *(volatile int*)&c.abort) {  // MMAs that no warp waited for
                 umma_commit(&c.done);
                 const uint64_t t0 = globaltimer_ns();
                 while (!mbar_try_wait(&c.done, 0))
@@ -378,7 +359,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
             const float* wsp[WB];
 #pragma unroll
             for (int h = 0; h < WB; h++) wsp[h] = f8_wscale<MODE>(a, grp.expert, h, item % a.nt);
-            ok = scales_load<MODE, WB>(c.sc, a, grp, wsp, kb0, kb1, chunk, &c.abort);
+            ok = scales_load<WB>(c.sc, a, grp, wsp, kb0, kb1, chunk, &c.abort);
         }
         cp_async_wait_all();
     } else {
@@ -428,11 +409,12 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                     chunk++;
                 }
             }
-            // columns this CTA finishes: j -> token rank + CS j
-            int mine = grp.rows;
-            if (C::kRed && CS > 1) {
-                const int per = NQ / CS;
-                mine = grp.rows > rank ? (grp.rows - rank + CS - 1) / CS : 0;
+            // The sums go through shared memory, a cluster's to the CTA that finishes the column: token column j
+            // to CTA j % CS.  What follows runs once an item: short loops, since as unrolled code (registers
+            // cannot be indexed) it cost 4 us in instruction fetches alone.
+            const int per = NQ / CS;
+            const int mine = grp.rows > rank ? (grp.rows - rank + CS - 1) / CS : 0;  // columns of this CTA
+            if (CS > 1) {
                 if (it > 0) ok = ok && f8_wait_cluster(&c.red_free, (it - 1) & 1, &c.abort, a);
                 const uint32_t base = smem_u32(red) + (uint32_t)(rank * per * WB * 128 + tid) * 4;
 #pragma unroll
@@ -445,49 +427,49 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                 __syncwarp();
                 if (lane < CS) mbar_arrive_cluster(cluster_map(smem_u32(&c.red_full), lane));
                 ok = ok && f8_wait_cluster(&c.red_full, it & 1, &c.abort, a);
+            } else {  // each thread reads its own alone
 #pragma unroll
-                for (int j = 0; j < NQ / 2; j++)  // CS >= 2
-                    if (j < mine)
+                for (int j = 0; j < NQ; j++)
+                    if (j < grp.rows)
 #pragma unroll
-                        for (int h = 0; h < WB; h++) {
-                            float v = 0.f;
-                            for (int r = 0; r < CS; r++) v += red[((r * per + j) * WB + h) * 128 + tid];
-                            acc[h][j] = v;
-                        }
+                        for (int h = 0; h < WB; h++) red[(j * WB + h) * 128 + tid] = acc[h][j];
+            }
+            const int i = n * 128 + tid;  // weight row
+#pragma unroll 1
+            for (int j = 0; j < mine; j++) {
+                float v[WB];
+#pragma unroll
+                for (int h = 0; h < WB; h++) {
+                    v[h] = red[(j * WB + h) * 128 + tid];
+#pragma unroll 1
+                    for (int r = 1; r < CS; r++) v[h] += red[((r * per + j) * WB + h) * 128 + tid];
+                }
+                if (MODE == kF8GateUp) {
+                    v[0] = swiglu_f32(v[0], v[WB - 1]);
+                    red[j * WB * 128 + tid] = v[0];
+                    uint32_t t = __float_as_uint(v[0]) & 0x7fffffffu;
+                    t = __reduce_max_sync(0xffffffffu, t < 0x7f800000u ? t : 0u);
+                    if (lane == 0) c.top[warp][j] = t;
+                } else if (i < a.N) {
+                    const size_t at = ((size_t)grp.row0 + rank + CS * j) * a.N + i;
+                    if (MODE == kF8Down || a.out_f32) static_cast<float*>(a.out)[at] = v[0];
+                    else static_cast<uint16_t*>(a.out)[at] = f8_bf16(v[0]);
+                }
+            }
+            if (MODE == kF8GateUp) {
+                named_bar_sync(1, 128);
+#pragma unroll 1
+                for (int j = 0; j < mine; j++) {
+                    const uint32_t se = f8_scale_exp(max(max(c.top[0][j], c.top[1][j]), max(c.top[2][j], c.top[3][j])));
+                    const size_t slot = (size_t)grp.row0 + rank + CS * j;
+                    if (i < a.N) a.aq[slot * a.N + i] = (uint8_t)f8_pack1(red[j * WB * 128 + tid], f8_inverse(se));
+                    if (tid == 0) a.as[slot * a.nb + n] = __uint_as_float(se << 23);
+                }
+                named_bar_sync(1, 128);  // c.top is read before the next item's is written
+            }
+            if (CS > 1) {
                 __syncwarp();
                 if (lane < CS) mbar_arrive_cluster(cluster_map(smem_u32(&c.red_free), lane));
-            }
-            const int step = C::kRed && CS > 1 ? CS : 1, first = C::kRed && CS > 1 ? rank : 0;
-            const int i = n * 128 + tid;  // weight row
-            if (MODE == kF8GateUp) {
-#pragma unroll
-                for (int j = 0; j < NQ; j++)
-                    if (j < mine) {
-                        const float v = swiglu_f32(acc[0][j], acc[WB - 1][j]);
-                        acc[0][j] = v;
-                        uint32_t t = __float_as_uint(v) & 0x7fffffffu;
-                        t = __reduce_max_sync(0xffffffffu, t < 0x7f800000u ? t : 0u);
-                        if (lane == 0) c.top[warp][j] = __uint_as_float(t);
-                    }
-                named_bar_sync(1, 128);
-#pragma unroll
-                for (int j = 0; j < NQ; j++)
-                    if (j < mine) {
-                        const float t = fmaxf(fmaxf(c.top[0][j], c.top[1][j]), fmaxf(c.top[2][j], c.top[3][j]));
-                        const uint32_t se = f8_scale_exp(__float_as_uint(t));
-                        const size_t slot = (size_t)grp.row0 + first + step * j;
-                        if (i < a.N) a.aq[slot * a.N + i] = (uint8_t)f8_pack1(acc[0][j], f8_inverse(se));
-                        if (tid == 0) a.as[slot * a.nb + n] = __uint_as_float(se << 23);
-                    }
-                named_bar_sync(1, 128);  // c.top is read before the next item's is written
-            } else if (i < a.N) {
-#pragma unroll
-                for (int j = 0; j < NQ; j++)
-                    if (j < mine) {
-                        const size_t at = ((size_t)grp.row0 + first + step * j) * a.N + i;
-                        if (MODE == kF8Down || a.out_f32) static_cast<float*>(a.out)[at] = acc[0][j];
-                        else static_cast<uint16_t*>(a.out)[at] = f8_bf16(acc[0][j]);
-                    }
             }
         }
     }
@@ -612,9 +594,6 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             int gi, n;
             many_tile<MODE>(a, item, groups, gi, n);
             const F8Group grp = f8_group<MODE>(a, gi, 128);
-            int4 rows = make_int4(0, 0, 0, 0);  // as in the other form
-            const int gathers = MODE == kF8GateUp ? (grp.rows + 3) / 4 : 0;
-            if (lane < gathers) rows = f8_gather_rows(a, grp, 4 * lane);
             for (int kb = 0; kb < nkb; kb++, g++) {
                 const int s = g % S;
                 if (g >= (uint32_t)S) ok = f8_wait(&c.empty[s], ((g / S) & 1) ^ 1, &c.abort, a);
@@ -623,20 +602,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 unsigned char* st = ring + (size_t)s * C::kStage;
                 unsigned char* sw = st + 16384;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&c.full[s], MODE == kF8GateUp ? 32768 + gathers * 512 : C::kStage);
-                    if (MODE == kF8GateUp) {
-                        tma_load_3d(sw, &map_w, kb * 128, n * 128, grp.expert * 2, &c.full[s], pol_w);
-                        tma_load_3d(sw + 16384, &map_w, kb * 128, n * 128, grp.expert * 2 + 1, &c.full[s], pol_w);
-                    } else {
-                        tma_load_2d(st, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
+                    mbar_arrive_expect_tx(&c.full[s], C::kStage);
+                    tma_load_2d(st, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
 #pragma unroll
-                        for (int h = 0; h < SEG; h++)
-                            tma_load_3d(sw + h * 16384, &map_w, kb * 128, n * NB + h * 128, grp.expert, &c.full[s], pol_w);
+                    for (int h = 0; h < SEG; h++) {
+                        if (MODE == kF8GateUp) tma_load_3d(sw + h * 16384, &map_w, kb * 128, n * 128, grp.expert * 2 + h, &c.full[s], pol_w);
+                        else tma_load_3d(sw + h * 16384, &map_w, kb * 128, n * NB + h * 128, grp.expert, &c.full[s], pol_w);
                     }
-                }
-                if (MODE == kF8GateUp) {
-                    __syncwarp();
-                    if (lane < gathers) tma_gather4(st + lane * 512, &map_x, kb * 128, rows, &c.full[s], pol_x);
                 }
             }
         }
@@ -648,8 +620,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         __syncwarp();
     } else if (warp == kManyEpi + 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = f8_idesc(NB);
+        constexpr uint32_t idesc = f8_idesc(NB);
+        const bool leader = elect_one();
+        const uint64_t desc0 = sw128_desc(smem_u32(ring));
+        {
             uint32_t g = 0;
             bool ok = true;
             for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
@@ -659,15 +633,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     if (g >= 2) ok = ok && f8_wait(&c.dempty[b], ((g >> 1) & 1) ^ 1, &c.abort, a);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sx = smem_u32(ring + (size_t)s * C::kStage), sw = sx + 16384;
+                    const uint64_t dx = desc0 + (uint64_t)(s * (C::kStage >> 4)), dw = dx + 1024;
+                    if (leader) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        umma_f8(tmem + b * NB, sw128_desc(sx + kk * 32), sw128_desc(sw + kk * 32), idesc, kk > 0);
-                    umma_commit(&c.empty[s]);
-                    umma_commit(&c.dfull[b]);
+                        for (int kk = 0; kk < 4; kk++) umma_f8(tmem + b * NB, dx + kk * 2, dw + kk * 2, idesc, kk > 0);
+                        umma_commit(&c.empty[s]);
+                        umma_commit(&c.dfull[b]);
+                    }
+                    __syncwarp();
                 }
             }
-            if (*(volatile int*)&c.abort) {
+            if (leader && *(volatile int*)&c.abort) {
                 umma_commit(&c.done);
                 const uint64_t t0 = globaltimer_ns();
                 while (!mbar_try_wait(&c.done, 0))
@@ -686,7 +662,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
             for (int h = 0; h < SEG; h++)
                 wsp[h] = f8_wscale<MODE>(a, grp.expert, h, MODE == kF8GateUp ? n : min(n * SEG + h, a.nb - 1));
-            ok = scales_load<MODE, SEG>(c.sc, a, grp, wsp, 0, nkb, chunk, &c.abort);
+            ok = scales_load<SEG>(c.sc, a, grp, wsp, 0, nkb, chunk, &c.abort);
         }
         cp_async_wait_all();
     } else {
