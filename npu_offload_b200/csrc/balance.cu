@@ -28,13 +28,14 @@ namespace cg = cooperative_groups;
 
 namespace moe {
 
-constexpr int kBalThreads = 256, kBalWarps = kBalThreads / 32;
+constexpr int kBalThreads = 512, kBalWarps = kBalThreads / 32;
+constexpr int kSumThreads = 1024, kSumWarps = kSumThreads / 32;
 constexpr int kBalCluster = 8;  // second kernel: CTAs a sequence, 32 experts each (E <= 256)
 
-// Tokens a unit: two rows a warp, more once there are four units for every SM.
+// Tokens a unit: a row a warp, more once there are two units for every SM.
 static int balance_chunk(int T, int sm_count) {
-    const int per = (T + 4 * sm_count - 1) / (4 * sm_count);
-    return std::max(16, (per + 15) / 16 * 16);
+    const int per = (T + 2 * sm_count - 1) / (2 * sm_count);
+    return std::max(kBalWarps, per);
 }
 static int balance_units(int T, int B, int chunk) { return T / chunk + B; }
 
@@ -88,42 +89,72 @@ __device__ __forceinline__ int first_unit(const int32_t* offsets, int b, int chu
     return offsets ? max(__ldg(offsets + b), 0) / chunk + b : 0;
 }
 
-// Scores of one token: e[j] = exp(l - max l) or sigmoid(l) of expert lane + 32 j (0 behind the last),
-// and 1 / their sum.
-template <int NE, bool SIG>
-__device__ __forceinline__ float scores(const float (&l)[NE], int E, float (&e)[NE]) {
+// 2^x of the hardware (2 ulp).  exp(d) is taken as 2^(d log2 e), which is off by |d| 2^-24, relative, at most: as
+// much as the rounding of d = l - m itself.  (The fused l log2 e - m log2 e overflows where d does not.)
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.44269504f;
+
+// The expert of a lane's value k: every 32nd, or (V: rows of 16-byte words) four neighbours of every 128.
+template <bool V>
+__device__ __forceinline__ int expert_of(int k) {
     const int lane = threadIdx.x & 31;
+    return V ? (k >> 2) * 128 + lane * 4 + (k & 3) : lane + 32 * k;
+}
+
+// One token's logits as they come from memory, and whether it counts; a token ahead of the one worked on, so
+// that a warp always has a row's loads in flight (without: 4.7 TB/s at best with 32 warps an SM).
+template <int NE, bool V, bool FULL>
+struct Row {
+    float l[NE];
+    bool counts;
+    __device__ __forceinline__ void load(const BalanceArgs& a, long t) {
+        counts = !a.mask || a.mask[t];
+        const float* row = a.logits + (size_t)t * a.E;
+#pragma unroll
+        for (int k = 0; k < NE; k += V ? 4 : 1) {
+            const int e = expert_of<V>(k);
+            if (V) {
+                const float4 v = FULL || e < a.E ? __ldcs(reinterpret_cast<const float4*>(row + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                l[k] = v.x, l[k + 1 < NE ? k + 1 : k] = v.y, l[k + 2 < NE ? k + 2 : k] = v.z, l[k + 3 < NE ? k + 3 : k] = v.w;
+            } else {
+                l[k] = FULL || e < a.E ? __ldcs(row + e) : 0.f;
+            }
+        }
+    }
+};
+
+// Scores of one token: e[k] = exp(l - max l) or sigmoid(l) of the lane's expert k (0 behind the last),
+// and 1 / their sum.
+template <int NE, bool SIG, bool V, bool FULL>
+__device__ __forceinline__ float scores(const float (&l)[NE], int E, float (&e)[NE]) {
     float sum = 0.f;
     if (SIG) {
 #pragma unroll
-        for (int j = 0; j < NE; j++) {
-            e[j] = lane + 32 * j < E ? 1.f / (1.f + expf(-l[j])) : 0.f;
-            sum += e[j];
+        for (int k = 0; k < NE; k++) {
+            e[k] = FULL || expert_of<V>(k) < E ? 1.f / (1.f + exp2_approx(-kLog2e * l[k])) : 0.f;
+            sum += e[k];
         }
         return 1.f / (warp_sum(sum) + 1e-20f);
     }
     float m = -__int_as_float(0x7f800000);
 #pragma unroll
-    for (int j = 0; j < NE; j++)
-        if (lane + 32 * j < E) m = fmaxf(m, l[j]);
+    for (int k = 0; k < NE; k++)
+        if (FULL || expert_of<V>(k) < E) m = fmaxf(m, l[k]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
 #pragma unroll
-    for (int j = 0; j < NE; j++) {
-        e[j] = lane + 32 * j < E ? expf(l[j] - m) : 0.f;
-        sum += e[j];
+    for (int k = 0; k < NE; k++) {
+        e[k] = FULL || expert_of<V>(k) < E ? exp2_approx((l[k] - m) * kLog2e) : 0.f;
+        sum += e[k];
     }
     return 1.f / warp_sum(sum);
 }
 
-template <int NE>
-__device__ __forceinline__ void load_row(const float* row, int E, float (&l)[NE]) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int j = 0; j < NE; j++) l[j] = lane + 32 * j < E ? __ldg(row + lane + 32 * j) : 0.f;
-}
-
-template <int NE, bool SIG>
+template <int NE, bool SIG, bool V, bool FULL>
 __global__ void __launch_bounds__(kBalThreads) balance_units_kernel(BalanceArgs a, BalanceWs w, int chunk) {
     __shared__ float p_s[kBalWarps][NE * 32];
     __shared__ int32_t c_s[NE * 32];
@@ -147,26 +178,34 @@ __global__ void __launch_bounds__(kBalThreads) balance_units_kernel(BalanceArgs 
     __syncthreads();
     float acc[NE];
 #pragma unroll
-    for (int j = 0; j < NE; j++) acc[j] = 0.f;
+    for (int k = 0; k < NE; k++) acc[k] = 0.f;
     int n = 0;
     bool bad = false;
-    for (int t = (int)t0 + warp; t < t1; t += kBalWarps) {
-        if (a.mask && !a.mask[t]) continue;
-        float l[NE], e[NE];
-        load_row<NE>(a.logits + (size_t)t * E, E, l);
-        if (lane < K) {
-            const int x = __ldg(a.idx + (size_t)t * K + lane);
-            if (x >= E) bad = true;
-            else if (x >= 0) atomicAdd(&c_s[x], 1);
-        }
-        const float r = scores<NE, SIG>(l, E, e);
+    Row<NE, V, FULL> next;
+    int next_x = -1;
+    int t = (int)t0 + warp;
+    auto ahead = [&](int q) {
+        if (q >= t1) return;
+        next.load(a, q);
+        next_x = lane < K ? __ldcs(a.idx + (size_t)q * K + lane) : -1;
+    };
+    ahead(t);
+    for (; t < t1; t += kBalWarps) {
+        const Row<NE, V, FULL> row = next;
+        const int x = next_x;
+        ahead(t + kBalWarps);
+        if (!row.counts) continue;
+        float e[NE];
+        if (x >= E) bad = true;
+        else if (x >= 0) atomicAdd(&c_s[x], 1);
+        const float r = scores<NE, SIG, V, FULL>(row.l, E, e);
 #pragma unroll
-        for (int j = 0; j < NE; j++) acc[j] = fmaf(e[j], r, acc[j]);
+        for (int k = 0; k < NE; k++) acc[k] = fmaf(e[k], r, acc[k]);
         n++;
     }
     if (bad) atomicOr(a.err, kErrBadIndex);
 #pragma unroll
-    for (int j = 0; j < NE; j++) p_s[warp][lane + 32 * j] = acc[j];
+    for (int k = 0; k < NE; k++) p_s[warp][expert_of<V>(k)] = acc[k];
     if (lane == 0) n_s[warp] = n;
     __syncthreads();
     for (int e = tid; e < E; e += kBalThreads) {
@@ -185,10 +224,10 @@ __global__ void __launch_bounds__(kBalThreads) balance_units_kernel(BalanceArgs 
 }
 
 // A cluster of eight CTAs a sequence: CTA r adds the units of experts [32 r, 32 r + 32).
-__global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalThreads)
+__global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThreads)
     balance_sum_kernel(BalanceArgs a, BalanceWs w, int chunk) {
-    __shared__ double p_s[kBalWarps][32];
-    __shared__ int32_t c_s[kBalWarps][32], n_s[kBalWarps];
+    __shared__ double p_s[kSumWarps][32];
+    __shared__ int32_t c_s[kSumWarps][32], n_s[kSumWarps];
     __shared__ double dot_s[kBalCluster];
     __shared__ int last_s;
     cg::cluster_group cl = cg::this_cluster();
@@ -202,7 +241,8 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalThread
         const int u0 = first_unit(a.offsets, b, chunk), nu = (last - first + chunk - 1) / chunk;
         double p = 0.0;
         int32_t c = 0, n = 0;
-        for (int u = warp; u < nu; u += kBalWarps) {
+#pragma unroll 4
+        for (int u = warp; u < nu; u += kSumWarps) {
             if (e < E) {
                 p += w.p[(size_t)(u0 + u) * E + e];
                 c += w.c[(size_t)(u0 + u) * E + e];
@@ -216,7 +256,7 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalThread
         if (warp == 0) {
             p = 0.0, c = 0, n = 0;
 #pragma unroll
-            for (int k = 0; k < kBalWarps; k++) p += p_s[k][lane], c += c_s[k][lane], n += n_s[k];
+            for (int k = 0; k < kSumWarps; k++) p += p_s[k][lane], c += c_s[k][lane], n += n_s[k];
             if (e < E) a.counts[(size_t)b * E + e] = c;
             double v = n > 0 && e < E ? (double)c * p : 0.0;
 #pragma unroll
@@ -244,7 +284,7 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalThread
     // the last cluster: the mean over the sequences that have tokens
     double v = 0.0;
     int full = 0;
-    for (int b = tid; b < a.B; b += kBalThreads) {
+    for (int b = tid; b < a.B; b += kSumThreads) {
         v += __ldcg(w.loss + b);
         full += __ldcg(a.tokens + b) > 0;
     }
@@ -257,86 +297,106 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kBalThread
     __syncthreads();
     if (tid == 0) {
         v = 0.0, full = 0;
-        for (int k = 0; k < kBalWarps; k++) v += p_s[k][0], full += n_s[k];
+        for (int k = 0; k < kSumWarps; k++) v += p_s[k][0], full += n_s[k];
         *a.loss = full ? (float)(v / full) : 0.f;
         a.tokens[a.B] = full;
     }
 }
 
 // A warp a row; rows of a warp are neighbours, so that it keeps its sequence's f in registers.
-template <int NE, bool SIG>
+template <int NE, bool SIG, bool V, bool FULL>
 __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceArgs a, int per_warp) {
-    const int lane = threadIdx.x & 31, E = a.E;
+    const int E = a.E;
     const long t0 = ((long)blockIdx.x * kBalWarps + (threadIdx.x >> 5)) * per_warp;
     const long t1 = min(t0 + per_warp, (long)a.T);
-    float f[NE];
-    int have = -1;
+    if (t0 >= t1) return;
+    Row<NE, V, FULL> next;
+    next.load(a, t0);
     const int full = __ldg(a.tokens + a.B);
     const float grad = a.grad ? __ldg(a.grad) : 1.f;
+    int b = 0;  // the sequence of token t is the last that begins at or before t, -1: none does
+    if (a.offsets) {
+        int lo = 0, hi = a.B;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (__ldg(a.offsets + mid) <= t0) lo = mid + 1;
+            else hi = mid;
+        }
+        b = lo - 1;
+    }
+    float f[NE];
+    int have = -1, n = 0;
     for (long t = t0; t < t1; t++) {
-        int b = 0;
-        if (a.offsets) {  // the last sequence that begins at or before t
-            int lo = 0, hi = a.B;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (__ldg(a.offsets + mid) <= t) lo = mid + 1;
-                else hi = mid;
+        const Row<NE, V, FULL> row = next;
+        if (t + 1 < t1) next.load(a, t + 1);
+        bool in = true;
+        if (a.offsets) {
+            while (b + 1 < a.B && __ldg(a.offsets + b + 1) <= t) b++;
+            in = b >= 0 && __ldg(a.offsets + b + 1) > t;
+        }
+        if (in && b != have) {
+            n = __ldg(a.tokens + b);
+            const float k = n > 0 && full > 0 ? grad * (float)((double)E / ((double)a.K * n * (double)n * full)) : 0.f;
+#pragma unroll
+            for (int j = 0; j < NE; j++) {
+                const int e = expert_of<V>(j);
+                f[j] = FULL || e < E ? k * (float)__ldg(a.counts + (size_t)b * E + e) : 0.f;
             }
-            b = lo - 1;
-            if (b >= 0 && __ldg(a.offsets + b + 1) <= t) b = -1;
-        }
-        float* d = a.dlogits + (size_t)t * E;
-        const int n = b >= 0 ? __ldg(a.tokens + b) : 0;
-        if (n <= 0 || (a.mask && !a.mask[t])) {  // a token of no sequence, or one that does not count
-#pragma unroll
-            for (int j = 0; j < NE; j++)
-                if (lane + 32 * j < E) d[lane + 32 * j] = 0.f;
-            continue;
-        }
-        if (b != have) {
-            const float k = grad * (float)((double)E / ((double)a.K * n * (double)n * full));
-#pragma unroll
-            for (int j = 0; j < NE; j++)
-                f[j] = lane + 32 * j < E ? k * (float)__ldg(a.counts + (size_t)b * E + lane + 32 * j) : 0.f;
             have = b;
         }
-        float l[NE], e[NE], inner = 0.f;
-        load_row<NE>(a.logits + (size_t)t * E, E, l);
-        const float r = scores<NE, SIG>(l, E, e);
+        float d[NE];
+        if (!in || n <= 0 || !row.counts) {  // a token of no sequence, or one that does not count
 #pragma unroll
-        for (int j = 0; j < NE; j++) inner = fmaf(f[j], e[j], inner);
-        inner = warp_sum(inner) * r;
+            for (int j = 0; j < NE; j++) d[j] = 0.f;
+        } else {
+            float e[NE], inner = 0.f;
+            const float r = scores<NE, SIG, V, FULL>(row.l, E, e);
 #pragma unroll
-        for (int j = 0; j < NE; j++)
-            if (lane + 32 * j < E) d[lane + 32 * j] = (SIG ? e[j] * (1.f - e[j]) : e[j]) * r * (f[j] - inner);
+            for (int j = 0; j < NE; j++) inner = fmaf(f[j], e[j], inner);
+            inner = warp_sum(inner) * r;
+#pragma unroll
+            for (int j = 0; j < NE; j++) d[j] = (SIG ? e[j] * (1.f - e[j]) : e[j]) * r * (f[j] - inner);
+        }
+        float* out = a.dlogits + (size_t)t * E;
+#pragma unroll
+        for (int j = 0; j < NE; j += V ? 4 : 1) {
+            const int e = expert_of<V>(j);
+            if (!FULL && e >= E) continue;
+            if (V) __stcs(reinterpret_cast<float4*>(out + e), make_float4(d[j], d[j + 1 < NE ? j + 1 : j], d[j + 2 < NE ? j + 2 : j], d[j + 3 < NE ? j + 3 : j]));
+            else __stcs(out + e, d[j]);
+        }
     }
 }
 
-template <int NE>
+template <int NE, bool V, bool FULL>
 static cudaError_t units_launch(const BalanceArgs& a, const BalanceWs& w, int chunk, int units, cudaStream_t st) {
-    if (a.scoring) balance_units_kernel<NE, true><<<units, kBalThreads, 0, st>>>(a, w, chunk);
-    else balance_units_kernel<NE, false><<<units, kBalThreads, 0, st>>>(a, w, chunk);
+    if (a.scoring) balance_units_kernel<NE, true, V, FULL><<<units, kBalThreads, 0, st>>>(a, w, chunk);
+    else balance_units_kernel<NE, false, V, FULL><<<units, kBalThreads, 0, st>>>(a, w, chunk);
     return cudaGetLastError();
 }
-template <int NE>
+template <int NE, bool V, bool FULL>
 static cudaError_t backward_launch(const BalanceArgs& a, int grid, int per_warp, cudaStream_t st) {
-    if (a.scoring) balance_backward_kernel<NE, true><<<grid, kBalThreads, 0, st>>>(a, per_warp);
-    else balance_backward_kernel<NE, false><<<grid, kBalThreads, 0, st>>>(a, per_warp);
+    if (a.scoring) balance_backward_kernel<NE, true, V, FULL><<<grid, kBalThreads, 0, st>>>(a, per_warp);
+    else balance_backward_kernel<NE, false, V, FULL><<<grid, kBalThreads, 0, st>>>(a, per_warp);
     return cudaGetLastError();
 }
 
+// Rows of 16-byte words where the sizes and addresses allow them; without bounds in a row of 128 or 256.
 cudaError_t launch_balance_loss(const BalanceArgs& a, int sm_count, cudaStream_t st) {
     const int chunk = balance_chunk(a.T, sm_count), units = balance_units(a.T, a.B, chunk);
     const BalanceWs w = balance_layout(a.ws, a.E, a.B, units);
+    const bool words = a.E % 4 == 0 && ((uintptr_t)a.logits & 15) == 0;
     cudaError_t e;
-    if (a.E <= 32) e = units_launch<1>(a, w, chunk, units, st);
-    else if (a.E <= 64) e = units_launch<2>(a, w, chunk, units, st);
-    else if (a.E <= 128) e = units_launch<4>(a, w, chunk, units, st);
-    else e = units_launch<8>(a, w, chunk, units, st);
+    if (words && a.E == 128) e = units_launch<4, true, true>(a, w, chunk, units, st);
+    else if (words && a.E == 256) e = units_launch<8, true, true>(a, w, chunk, units, st);
+    else if (words && a.E <= 128) e = units_launch<4, true, false>(a, w, chunk, units, st);
+    else if (words) e = units_launch<8, true, false>(a, w, chunk, units, st);
+    else if (a.E <= 128) e = units_launch<4, false, false>(a, w, chunk, units, st);
+    else e = units_launch<8, false, false>(a, w, chunk, units, st);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(kBalCluster * std::min(a.B, sm_count / kBalCluster));
-    cfg.blockDim = dim3(kBalThreads);
+    cfg.blockDim = dim3(kSumThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -348,13 +408,16 @@ cudaError_t launch_balance_loss(const BalanceArgs& a, int sm_count, cudaStream_t
 
 cudaError_t launch_balance_backward(const BalanceArgs& a, int sm_count, cudaStream_t st) {
     if (a.T <= 0) return cudaSuccess;
-    // sixteen warps an SM at the least before a warp takes a second row
-    const int per_warp = std::max(1, std::min(32, a.T / (sm_count * 16)));
+    // thirty-two warps an SM at the least before a warp takes a second row
+    const int per_warp = std::max(1, std::min(16, a.T / (sm_count * 32)));
     const int grid = (a.T + kBalWarps * per_warp - 1) / (kBalWarps * per_warp);
-    if (a.E <= 32) return backward_launch<1>(a, grid, per_warp, st);
-    if (a.E <= 64) return backward_launch<2>(a, grid, per_warp, st);
-    if (a.E <= 128) return backward_launch<4>(a, grid, per_warp, st);
-    return backward_launch<8>(a, grid, per_warp, st);
+    const bool words = a.E % 4 == 0 && (((uintptr_t)a.logits | (uintptr_t)a.dlogits) & 15) == 0;
+    if (words && a.E == 128) return backward_launch<4, true, true>(a, grid, per_warp, st);
+    if (words && a.E == 256) return backward_launch<8, true, true>(a, grid, per_warp, st);
+    if (words && a.E <= 128) return backward_launch<4, true, false>(a, grid, per_warp, st);
+    if (words) return backward_launch<8, true, false>(a, grid, per_warp, st);
+    if (a.E <= 128) return backward_launch<4, false, false>(a, grid, per_warp, st);
+    return backward_launch<8, false, false>(a, grid, per_warp, st);
 }
 
 }  // namespace moe

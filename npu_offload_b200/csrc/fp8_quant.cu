@@ -48,43 +48,41 @@ struct Eight<true> {
     }
 };
 
-// Rows: sixteen lanes hold a group, eight values each, and share its maximum by shuffles.
+// Rows: sixteen lanes hold a group, eight values each, and share its maximum by shuffles; N groups' loads
+// in flight for each half warp.
 template <bool F32, int N>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, uint32_t groups, uint32_t per_row,
                                                             uint32_t cols, uint8_t* __restrict__ q, float* __restrict__ s) {
-    const uint32_t sub = threadIdx.x & 15;
-    const uint32_t stride = gridDim.x * 16;
-    for (uint32_t g0 = blockIdx.x * 16 + (threadIdx.x >> 4); g0 - (threadIdx.x >> 4) < groups; g0 += N * stride) {
-        Eight<F32> v[N];
-        size_t at[N];
-        bool in[N];
+    const uint32_t sub = threadIdx.x & 15, g0 = blockIdx.x * 16 * N + (threadIdx.x >> 4);
+    Eight<F32> v[N];
+    size_t at[N];
+    bool in[N];
 #pragma unroll
-        for (int n = 0; n < N; n++) {  // N groups' loads in flight
-            const uint32_t g = g0 + n * stride, row = g / per_row, c = (g - row * per_row) * kF8Block + sub * 8;
-            in[n] = g < groups && c < cols;
-            at[n] = (size_t)row * cols + c;
-            if (in[n]) v[n].load(x, at[n]);
-            else v[n].zero();
-        }
+    for (int n = 0; n < N; n++) {
+        const uint32_t g = g0 + n * 16, row = g / per_row, c = (g - row * per_row) * kF8Block + sub * 8;
+        in[n] = g < groups && c < cols;
+        at[n] = (size_t)row * cols + c;
+        if (in[n]) v[n].load(x, at[n]);
+        else v[n].zero();
+    }
 #pragma unroll
-        for (int n = 0; n < N; n++) {
-            float f[8];
-            v[n].get(f);
-            uint32_t top = f8_top(f);
+    for (int n = 0; n < N; n++) {
+        float f[8];
+        v[n].get(f);
+        uint32_t top = f8_top(f);
 #pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const uint32_t se = f8_scale_exp(top);
-            const uint2 r = f8_pack8(f, f8_inverse(se));
-            if (in[n]) *reinterpret_cast<uint2*>(q + at[n]) = r;
-            const uint32_t g = g0 + n * stride;
-            if (sub == 0 && g < groups) s[g] = __uint_as_float(se << 23);
-        }
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const uint32_t se = f8_scale_exp(top);
+        const uint2 r = f8_pack8(f, f8_inverse(se));
+        if (in[n]) *reinterpret_cast<uint2*>(q + at[n]) = r;
+        const uint32_t g = g0 + n * 16;
+        if (sub == 0 && g < groups) s[g] = __uint_as_float(se << 23);
     }
 }
 
 // 128 x 128 blocks: one CTA a block, thread t columns 8 (t % 16) .. of rows t / 16 + 16 i.
 template <bool F32>
-__global__ void __launch_bounds__(256) quantize_blocks_kernel(const void* __restrict__ x, uint32_t rows, uint32_t cols,
+__global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const void* __restrict__ x, uint32_t rows, uint32_t cols,
                                                               uint32_t rb, uint32_t cb, uint8_t* __restrict__ q,
                                                               float* __restrict__ s) {
     __shared__ uint32_t top_s[8];
@@ -129,16 +127,14 @@ cudaError_t launch_quantize_fp8(const void* x, bool f32, int64_t batch, int64_t 
     if (block_rows == 1) {
         const int64_t groups = batch * rows * cb;
         if (groups >= (1ll << 31) || cols >= (1ll << 31)) return cudaErrorInvalidValue;
-        const int64_t ctas = (groups + 15) / 16;
-        // few groups: one a half warp, spread over the SMs
-        if (ctas <= 4 * sm_count) {
-            if (f32) quantize_rows_kernel<true, 1><<<(int)ctas, 256, 0, st>>>(x, (uint32_t)groups, (uint32_t)cb, (uint32_t)cols, q, s);
-            else quantize_rows_kernel<false, 1><<<(int)ctas, 256, 0, st>>>(x, (uint32_t)groups, (uint32_t)cb, (uint32_t)cols, q, s);
-        } else {
-            const int grid = (int)std::min<int64_t>((ctas + 3) / 4, (int64_t)sm_count * 8);
-            if (f32) quantize_rows_kernel<true, 4><<<grid, 256, 0, st>>>(x, (uint32_t)groups, (uint32_t)cb, (uint32_t)cols, q, s);
-            else quantize_rows_kernel<false, 4><<<grid, 256, 0, st>>>(x, (uint32_t)groups, (uint32_t)cb, (uint32_t)cols, q, s);
-        }
+        // few groups: one a half warp, spread over the SMs; else two (fp32) or four (bf16)
+        const int n = groups <= 64ll * sm_count ? 1 : f32 ? 2 : 4;
+        const int grid = (int)((groups + 16 * n - 1) / (16 * n));
+        const uint32_t ng = (uint32_t)groups, per_row = (uint32_t)cb, nc = (uint32_t)cols;
+        if (n == 1 && f32) quantize_rows_kernel<true, 1><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
+        else if (n == 1) quantize_rows_kernel<false, 1><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
+        else if (f32) quantize_rows_kernel<true, 2><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
+        else quantize_rows_kernel<false, 4><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
         return cudaGetLastError();
     }
     const int64_t rb = (rows + kF8Block - 1) / kF8Block, blocks = batch * rb * cb;
