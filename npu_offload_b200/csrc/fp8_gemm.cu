@@ -3,6 +3,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "common.cuh"
 #include "fp8.h"
@@ -267,6 +268,52 @@ __global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
     prep_rows(a, l, slots);
 }
 
+// A few tokens (up to 32 pairs, one a lane): each warp finds the slots by comparing its lanes, with no trip
+// through shared memory, and quantises its share (of a lone token, a 4 us chain of barriers otherwise).
+constexpr int kTinyThreads = 128;
+__global__ void __launch_bounds__(kTinyThreads) f8_prep_tiny_kernel(PrepArgs a) {
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31, P = a.T * a.K;
+    int e = lane < P ? __ldg(a.idx + lane) : -1;
+    const uint32_t per_row = (uint32_t)(a.H + 127) / 128, groups = (uint32_t)a.T * per_row, sub = threadIdx.x & 15;
+    const uint32_t g = blockIdx.x * (kTinyThreads / 16) + threadIdx.x / 16, row = g / per_row, c = (g - row * per_row) * 128 + sub * 8;
+    const bool in = g < groups && c < (uint32_t)a.H;
+    const uint4 w = in ? ldg_stream(a.x + (size_t)row * a.H + c) : make_uint4(0, 0, 0, 0);
+    const bool bad = e >= a.E;
+    if (bad || e < 0) e = INT_MAX;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int rank = __popc(same & ((1u << lane) - 1)), of = __popc(same);
+    // slots and groups of the experts before this one; a group holds up to `height` of an expert's pairs
+    int slot = rank, group = 0;
+#pragma unroll
+    for (int i = 0; i < 32; i++) {
+        const int o = __shfl_sync(0xffffffffu, e, i), r = __shfl_sync(0xffffffffu, rank, i);
+        if (o < e) slot++, group += r % a.height == 0;
+    }
+    const bool ok = e != INT_MAX;
+    if (blockIdx.x == 0 && threadIdx.x < 32) {
+        if (bad) atomicOr(a.err, kErrBadIndex);
+        if (lane < P) a.pos[lane] = ok ? slot : -1;
+        const bool head = ok && rank % a.height == 0;
+        if (head) a.groups[group + rank / a.height] = F8Group{slot, min(a.height, of - rank), e, 0};
+        const int n = __popc(__ballot_sync(0xffffffffu, head));
+        if (lane == 0) *a.n_groups = n;
+    }
+    const float f[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
+    uint32_t top = f8_top(f);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const uint32_t se = f8_scale_exp(top);
+    const uint2 q = f8_pack8(f, f8_inverse(se));
+    for (int k = 0; k < a.K; k++) {
+        const int p = min((int)(row * a.K) + k, 31);  // rows behind the last token store nothing
+        const int s = __shfl_sync(0xffffffffu, ok ? slot : -1, p);
+        if (s < 0 || g >= groups) continue;
+        if (in) *reinterpret_cast<uint2*>(a.xq + (size_t)s * a.H + c) = q;
+        if (sub == 0) a.xs[(size_t)s * per_row + (g - row * per_row)] = __uint_as_float(se << 23);
+    }
+}
+
 // Many pairs: one cluster finds the slots, an eighth of the pairs a CTA.  A pair's place among its CTA's pairs
 // on the expert may differ from run to run: a slot's row is computed from that row alone, so no result does.
 __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPrepThreads) f8_plan_kernel(PrepArgs a) {
@@ -341,7 +388,7 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict
                                                          bool accumulate) {
     const int per = H / 4;
     const int64_t n = (int64_t)T * per;
-    griddep_wait();
+    bool waited = false;  // the slots are there when this kernel starts, the rows after the wait
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
         const int64_t t = i / per;
         const int h = (int)(i - t * per) * 4;
@@ -356,6 +403,8 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict
                 s[k] = k0 + k < K ? __ldg(pos + t * K + k0 + k) : -1;
                 c[k] = k0 + k < K ? __ldg(w + t * K + k0 + k) : 0.f;
             }
+            if (!waited) griddep_wait();
+            waited = true;
 #pragma unroll
             for (int k = 0; k < 8; k++)
                 if (s[k] >= 0) a[k] = *reinterpret_cast<const float4*>(y + (size_t)s[k] * H + h);
@@ -367,6 +416,7 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict
         if (f32) *reinterpret_cast<float4*>(static_cast<float*>(out) + t * H + h) = v;
         else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + t * H + h) = make_uint2(f8_bf16x2(v.x, v.y), f8_bf16x2(v.z, v.w));
     }
+    if (!waited) griddep_wait();
 }
 
 namespace {
@@ -433,7 +483,10 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     const int qctas = (int)std::min<int64_t>(((int64_t)a.T * ((a.H + 127) / 128) + kPrepThreads / 16 - 1) / (kPrepThreads / 16),
                                              2 * sm_count);
     cudaError_t e;
-    if (P <= kPrepPairs) {
+    if (P <= 32) {
+        f8_prep_tiny_kernel<<<(int)(((int64_t)a.T * ((a.H + 127) / 128) * 16 + kTinyThreads - 1) / kTinyThreads), kTinyThreads, 0, st>>>(pa);
+        e = cudaGetLastError();
+    } else if (P <= kPrepPairs) {
         f8_prep_kernel<<<qctas, kPrepThreads, 0, st>>>(pa);
         e = cudaGetLastError();
     } else {

@@ -102,6 +102,10 @@ __device__ __forceinline__ bool elect_one() {
     return p != 0;
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+}
+
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -266,6 +270,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
     const int CS = (int)cluster_size(), rank = (int)cluster_rank();
     const int n_clusters = gridDim.x / CS, cid = blockIdx.x / CS;
     const int kb0 = a.nkb * rank / CS, kb1 = a.nkb * (rank + 1) / CS;
+    if (warp == 4 && lane == 0) prefetch_map(&map_w), prefetch_map(&map_x);
     if (tid == 0) {
         for (int s = 0; s < S; s++) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
         for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1), mbar_init(&c.dempty[b], 4);
@@ -282,8 +287,11 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
     if (CS > 1) cluster_sync_all();  // every CTA's barriers are initialised before another arrives on them
     tc_fence_after();
     const uint32_t tmem = c.tmem;
-    griddep_launch_dependents();
-    griddep_wait();
+    // The down product's kernel starts when every CTA of the gate / up product has let it, which is after the
+    // groups are there: it may read them, and the weights, before it waits for the activations.
+    if (MODE == kF8Down) griddep_launch_dependents();
+    if (MODE != kF8Down || warp != 4) griddep_wait();
+    if (MODE != kF8Down) griddep_launch_dependents();
     const int items = f8_groups<MODE>(a, NQ) * a.nt;
 
     if (warp == 4) {
@@ -293,18 +301,36 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
         for (int item = cid; ok && item < items; item += n_clusters) {
             const int n = item % a.nt;
             const F8Group grp = f8_group<MODE>(a, item / a.nt, NQ);
-            for (int kb = kb0; kb < kb1; kb++, g++) {
+            auto load_w = [&](int kb, int s) {
+                unsigned char* st = ring + (size_t)s * C::kStage;
+                mbar_arrive_expect_tx(&c.full[s], C::kStage);
+#pragma unroll
+                for (int h = 0; h < WB; h++)
+                    tma_load_3d(st + h * 16384, &map_w, kb * 128, n * 128, grp.expert * WB + h, &c.full[s], pol_w);
+            };
+            auto load_x = [&](int kb, int s) {
+                tma_load_2d(ring + (size_t)s * C::kStage + WB * 16384, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
+            };
+            int kb = kb0;
+            if (MODE == kF8Down && g == 0) {  // the first stages' weights ahead of the wait
+                const int ahead = min(S, kb1 - kb0);
+                if (lane == 0)
+                    for (int k = 0; k < ahead; k++) load_w(kb0 + k, k);
+                griddep_wait();
+                if (lane == 0)
+                    for (int k = 0; k < ahead; k++) load_x(kb0 + k, k);
+                __syncwarp();
+                kb += ahead;
+                g += ahead;
+            }
+            for (; kb < kb1; kb++, g++) {
                 const int s = g % S;
                 if (g >= (uint32_t)S) ok = f8_wait(&c.empty[s], ((g / S) & 1) ^ 1, &c.abort, a);
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
-                unsigned char* st = ring + (size_t)s * C::kStage;
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&c.full[s], C::kStage);
-#pragma unroll
-                    for (int h = 0; h < WB; h++)
-                        tma_load_3d(st + h * 16384, &map_w, kb * 128, n * 128, grp.expert * WB + h, &c.full[s], pol_w);
-                    tma_load_2d(st + WB * 16384, &map_x, kb * 128, grp.row0, &c.full[s], pol_x);
+                    load_w(kb, s);
+                    load_x(kb, s);
                 }
             }
         }
@@ -569,6 +595,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         if (tid == 0) atomicOr(a.err, kErrTimeout);
         return;
     }
+    if (warp == kManyEpi && lane == 0) prefetch_map(&map_w), prefetch_map(&map_x);
     if (tid == 0) {
         for (int s = 0; s < S; s++) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
         for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1), mbar_init(&c.dempty[b], kManyEpi);
@@ -582,8 +609,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = c.tmem;
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const int groups = f8_groups<MODE>(a, 128), items = groups * a.nt, nkb = a.nkb;
 
     if (warp == kManyEpi) {

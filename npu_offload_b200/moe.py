@@ -396,7 +396,7 @@ class MoEDataPlane:
             raise ValueError("quantize_fp8 takes [..., rows, cols] and block_rows 1 or 128")
         rows, cols = shape[-2:]
         q = torch.empty_like(x, dtype=_F8)
-        scale = torch.empty((*shape[:-2], -(-rows // block_rows), -(-cols // 128)), dtype=torch.float32, device=self.device)
+        scale = x.new_empty((*shape[:-2], -(-rows // block_rows), -(-cols // 128)), dtype=torch.float32)
         status = lib().moe_quantize_fp8(self._h, x.data_ptr(), _DTYPES[x.dtype], math.prod(shape[:-2]), rows, cols, block_rows,
                                         q.data_ptr(), scale.data_ptr(), 0, self._raw_stream())
         if status:
@@ -416,7 +416,7 @@ class MoEDataPlane:
         (M, K), (N, wk) = xq.shape, wq.shape
         if wk != K:
             raise ValueError(f"x has {K} columns, w {wk}")
-        out = self._output(out, (M, N), out_dtype, _DTYPES)
+        out = self._output(out, xs, (M, N), out_dtype, _DTYPES)
         status = lib().moe_matmul_fp8(self._h, M, N, K, xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), out.data_ptr(),
                                       _DTYPES[out.dtype], 0, self._raw_stream())
         if status:
@@ -449,10 +449,10 @@ class MoEDataPlane:
             raise ValueError(f"idx {tuple(idx.shape)} and w {tuple(w.shape)} must be {(T, K)}")
         if accumulate and out is None:
             raise ValueError("accumulate needs an out to add to")
-        out = self._output(out, (T, H), out_dtype, _DTYPES)
+        out = self._output(out, x, (T, H), out_dtype, _DTYPES)
         L = lib()
         n = L.moe_experts_fp8_workspace(self._h, T)
-        ws = torch.empty(max(n, 0), dtype=torch.uint8, device=self.device)  # from the stream's pool, alive until enqueued
+        ws = x.new_empty(max(n, 0), dtype=torch.uint8)  # from the stream's pool, alive until enqueued
         status = L.moe_experts_fp8(self._h, T, x.data_ptr(), gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(),
                                    idx.data_ptr(), w.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], ws.data_ptr(), n,
                                    MOE_F_ACCUMULATE if accumulate else 0, self._raw_stream())
@@ -496,11 +496,11 @@ class MoEDataPlane:
         if idx.shape != (T, self.K):
             raise ValueError(f"idx is {tuple(idx.shape)}, not {(T, self.K)}")
         L = lib()
-        loss = torch.empty((), dtype=torch.float32, device=self.device)
-        counts = torch.empty((B, E), dtype=torch.int32, device=self.device)
-        tokens = torch.empty(B + 1, dtype=torch.int32, device=self.device)
+        loss = logits.new_empty(())
+        counts = idx.new_empty((B, E))
+        tokens = idx.new_empty(B + 1)
         n = L.moe_balance_loss_workspace(self._h, T, B)
-        ws = torch.empty(max(n, 0), dtype=torch.uint8, device=self.device)
+        ws = idx.new_empty(max(n, 0) // 4)
         status = L.moe_balance_loss(self._h, T, logits.data_ptr(), idx.data_ptr(), po, B, pm, loss.data_ptr(), counts.data_ptr(),
                                     tokens.data_ptr(), ws.data_ptr(), n, 0, self._raw_stream())
         if status:
@@ -522,7 +522,7 @@ class MoEDataPlane:
             raise ValueError("stats are of other sequences")
         if grad is not None:
             grad = self._operand("grad", grad, _F32, 0)
-        out = self._output(out, (T, E), torch.float32, _F32)
+        out = self._output(out, logits, (T, E), torch.float32, _F32)
         status = lib().moe_balance_loss_backward(self._h, T, logits.data_ptr(), po, B, pm, counts.data_ptr(), tokens.data_ptr(),
                                                  None if grad is None else grad.data_ptr(), out.data_ptr(), 0, self._raw_stream())
         if status:
@@ -574,11 +574,11 @@ class MoEDataPlane:
             raise ValueError(f"{name}.scale is {tuple(s.shape)}, not {want}")
         return q, s
 
-    def _output(self, out, shape, dtype, dtypes):
+    def _output(self, out, like, shape, dtype, dtypes):
         if out is None:
             if dtype not in dtypes:
                 raise ValueError(f"out_dtype {dtype} is neither torch.bfloat16 nor torch.float32")
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return torch.empty_like(like, dtype=dtype) if like.shape == shape else like.new_empty(shape, dtype=dtype)
         if (out.device != self.device or out.dtype not in dtypes or out.shape != shape or not out.is_contiguous() or
                 out.data_ptr() % 16):
             raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} tensor on {self.device}")
