@@ -23,6 +23,7 @@ from ._lib import (MOE_DT_BF16, MOE_DT_F32, MOE_F_ACCUMULATE, MOE_F_HOST, MOE_F_
 
 __all__ = ["MoEDataPlane", "Fp8", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"]
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (a torch without CUDA has none, and no GPU path)
 _DTYPES = {torch.bfloat16: MOE_DT_BF16, torch.float32: MOE_DT_F32}
 _F8 = torch.float8_e4m3fn
 _E4M3, _BF16, _F32, _I32, _MASK = (_F8,), (torch.bfloat16,), (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
@@ -32,6 +33,12 @@ class Fp8(NamedTuple):
     """e4m3 values with one fp32 scale for each 128 columns of one row, or of 128 rows; value = q * scale."""
     q: torch.Tensor      # [..., rows, cols] torch.float8_e4m3fn
     scale: torch.Tensor  # [..., ceil(rows / block_rows), ceil(cols / 128)] torch.float32
+
+
+class _Likes(NamedTuple):
+    f32: torch.Tensor
+    i32: torch.Tensor
+    u8: torch.Tensor
 
 
 class BalanceStats(NamedTuple):
@@ -91,6 +98,7 @@ class MoEDataPlane:
         if self.device.index is None:
             self.device = torch.device("cuda", 0)
         self._index = self.device.index
+        self._likes = None
         self.scoring = scoring
         sc = {"softmax": MOE_SCORING_SOFTMAX, "sigmoid": MOE_SCORING_SIGMOID}[scoring]
         self._shard = None
@@ -391,14 +399,13 @@ class MoEDataPlane:
             with torch.cuda.stream(stream):
                 return self.quantize_fp8(x, block_rows)
         x = self._operand("x", x, _DTYPES, None, 16)
-        shape = x.shape
-        if len(shape) < 2 or block_rows not in (1, 128):
+        if x.dim() < 2 or block_rows not in (1, 128):
             raise ValueError("quantize_fp8 takes [..., rows, cols] and block_rows 1 or 128")
-        rows, cols = shape[-2:]
+        *lead, rows, cols = x.shape
         q = torch.empty_like(x, dtype=_F8)
-        scale = x.new_empty((*shape[:-2], -(-rows // block_rows), -(-cols // 128)), dtype=torch.float32)
-        status = lib().moe_quantize_fp8(self._h, x.data_ptr(), _DTYPES[x.dtype], math.prod(shape[:-2]), rows, cols, block_rows,
-                                        q.data_ptr(), scale.data_ptr(), 0, self._raw_stream())
+        scale = self._like().f32.new_empty((*lead, -(-rows // block_rows), -(-cols // 128)))
+        status = lib().moe_quantize_fp8(self._h, x.data_ptr(), _DTYPES[x.dtype], math.prod(lead), rows, cols, block_rows,
+                                        q.data_ptr(), scale.data_ptr(), 0, _raw_stream(self._index))
         if status:
             check(status)
         return Fp8(q, scale)
@@ -418,7 +425,7 @@ class MoEDataPlane:
             raise ValueError(f"x has {K} columns, w {wk}")
         out = self._output(out, xs, (M, N), out_dtype, _DTYPES)
         status = lib().moe_matmul_fp8(self._h, M, N, K, xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), out.data_ptr(),
-                                      _DTYPES[out.dtype], 0, self._raw_stream())
+                                      _DTYPES[out.dtype], 0, _raw_stream(self._index))
         if status:
             check(status)
         return out
@@ -452,10 +459,10 @@ class MoEDataPlane:
         out = self._output(out, x, (T, H), out_dtype, _DTYPES)
         L = lib()
         n = L.moe_experts_fp8_workspace(self._h, T)
-        ws = x.new_empty(max(n, 0), dtype=torch.uint8)  # from the stream's pool, alive until enqueued
+        ws = self._like().u8.new_empty(max(n, 0))  # from the stream's pool, alive until enqueued
         status = L.moe_experts_fp8(self._h, T, x.data_ptr(), gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(),
                                    idx.data_ptr(), w.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], ws.data_ptr(), n,
-                                   MOE_F_ACCUMULATE if accumulate else 0, self._raw_stream())
+                                   MOE_F_ACCUMULATE if accumulate else 0, _raw_stream(self._index))
         if status:
             check(status)
         return out
@@ -476,7 +483,7 @@ class MoEDataPlane:
         n = torch.empty(3 * self.E + 2 + pairs, dtype=torch.int32, device=self.device)
         counts, offsets, perm, order, jobs = n.split([self.E, self.E + 1, pairs, self.E, 1])
         check(lib().moe_route(self._h, T, _vp(lg), _vp(b), _vp(idx), _vp(w), _vp(counts), _vp(offsets), _vp(perm), _vp(order),
-                              _vp(jobs), 0, self._raw_stream()))
+                              _vp(jobs), 0, _raw_stream(self._index)))
         return idx, w
 
     # ---- the router's load-balance loss ----
@@ -502,7 +509,7 @@ class MoEDataPlane:
         n = L.moe_balance_loss_workspace(self._h, T, B)
         ws = idx.new_empty(max(n, 0) // 4)
         status = L.moe_balance_loss(self._h, T, logits.data_ptr(), idx.data_ptr(), po, B, pm, loss.data_ptr(), counts.data_ptr(),
-                                    tokens.data_ptr(), ws.data_ptr(), n, 0, self._raw_stream())
+                                    tokens.data_ptr(), ws.data_ptr(), n, 0, _raw_stream(self._index))
         if status:
             check(status)
         return loss, BalanceStats(counts, tokens, offsets, mask)
@@ -524,7 +531,7 @@ class MoEDataPlane:
             grad = self._operand("grad", grad, _F32, 0)
         out = self._output(out, logits, (T, E), torch.float32, _F32)
         status = lib().moe_balance_loss_backward(self._h, T, logits.data_ptr(), po, B, pm, counts.data_ptr(), tokens.data_ptr(),
-                                                 None if grad is None else grad.data_ptr(), out.data_ptr(), 0, self._raw_stream())
+                                                 None if grad is None else grad.data_ptr(), out.data_ptr(), 0, _raw_stream(self._index))
         if status:
             check(status)
         return out
@@ -584,8 +591,11 @@ class MoEDataPlane:
             raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} tensor on {self.device}")
         return out
 
-    def _raw_stream(self):
-        return torch._C._cuda_getCurrentRawStream(self._index)
+    def _like(self):
+        """Empty tensors of this device: new_empty() of one costs half of torch.empty() with a type and a device."""
+        if self._likes is None:
+            self._likes = _Likes(*(torch.empty(0, dtype=t, device=self.device) for t in (torch.float32, torch.int32, torch.uint8)))
+        return self._likes
 
     def status(self, stream=None):
         return lib().moe_status(self._h, _stream_ptr(stream, self.device))
