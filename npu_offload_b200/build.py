@@ -1,9 +1,10 @@
-"""Build libmoe_dp.so (the C-ABI library) in-tree with nvcc for sm_100a.
+"""Build libmoe_dp.so (the C-ABI library) in-tree with nvcc for sm_100a, and _torch_binding.so (the torch
+side of the e4m3 and balance-loss calls) with the host compiler.
 
     python -m npu_offload_b200.build [--force]
 
-The library lands next to this file (npu_offload_b200/libmoe_dp.so), so it travels with the source
-tree to a GPU host; nothing is installed into site-packages or a JIT cache.
+Both land next to this file, so they travel with the source tree to a GPU host; nothing is installed
+into site-packages or a JIT cache.
 """
 import os
 import subprocess
@@ -13,6 +14,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libmoe_dp.so")
+BINDING = os.path.join(HERE, "_torch_binding.so")
+BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
+CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["moe_dp.cu", "route.cu", "experts.cu", "decode.cu", "noalloc.cu", "prefill.cu", "prefill_tc.cu",
@@ -50,7 +54,35 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in sources()[1])
 
 
+def build_binding(force=False):
+    """Compiles _torch_binding.so, linked to the library beside it, where it is older than what it is made of."""
+    deps = [BINDING_SOURCE, os.path.join(ROOT, "include", "moe_dp.h")]
+    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
+        return BINDING
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+    cmd = [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_binding"]
+    for d in [*ext.include_paths(), sysconfig.get_paths()["include"]]:
+        cmd += ["-isystem", d]
+    cmd += [BINDING_SOURCE, "-o", BINDING + ".tmp", *["-L" + d for d in ext.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu",
+            "-ltorch_python", "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    subprocess.check_call(cmd)
+    os.replace(BINDING + ".tmp", BINDING)
+    return BINDING
+
+
 def build(force=False, verbose=False, extra=(), out=None):
+    """Builds the library (build_library) and, in-tree, the torch binding beside it."""
+    lib = build_library(force, verbose, extra, out)
+    if out is None:
+        build_binding(force)
+    return lib
+
+
+def build_library(force=False, verbose=False, extra=(), out=None):
     """Compiles every source to an object in parallel (objects under _build/), then links the library.
     extra: additional nvcc flags; out: library path (default: the in-tree libmoe_dp.so)."""
     lib = out or LIB

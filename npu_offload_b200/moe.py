@@ -11,34 +11,25 @@
 PyTorch only provides device memory and streams here; every computation runs in libmoe_dp.so.
 """
 import ctypes
-import math
 from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (MOE_DT_BF16, MOE_DT_F32, MOE_F_ACCUMULATE, MOE_F_HOST, MOE_F_SYNC, MOE_SCORING_SIGMOID, MOE_SCORING_SOFTMAX,
+from ._lib import (MOE_F_ACCUMULATE, MOE_F_HOST, MOE_F_SYNC, MOE_SCORING_SIGMOID, MOE_SCORING_SOFTMAX,
                    MoeConfig, check, lib)
 
 __all__ = ["MoEDataPlane", "Fp8", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"]
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (a torch without CUDA has none, and no GPU path)
-_DTYPES = {torch.bfloat16: MOE_DT_BF16, torch.float32: MOE_DT_F32}
-_F8 = torch.float8_e4m3fn
-_E4M3, _BF16, _F32, _I32, _MASK = (_F8,), (torch.bfloat16,), (torch.float32,), (torch.int32,), (torch.bool, torch.uint8)
+_calls = None  # the module _torch_binding, from its first use on
 
 
 class Fp8(NamedTuple):
     """e4m3 values with one fp32 scale for each 128 columns of one row, or of 128 rows; value = q * scale."""
     q: torch.Tensor      # [..., rows, cols] torch.float8_e4m3fn
     scale: torch.Tensor  # [..., ceil(rows / block_rows), ceil(cols / 128)] torch.float32
-
-
-class _Likes(NamedTuple):
-    f32: torch.Tensor
-    i32: torch.Tensor
-    u8: torch.Tensor
 
 
 class BalanceStats(NamedTuple):
@@ -98,7 +89,7 @@ class MoEDataPlane:
         if self.device.index is None:
             self.device = torch.device("cuda", 0)
         self._index = self.device.index
-        self._likes = None
+        self._plane = None
         self.scoring = scoring
         sc = {"softmax": MOE_SCORING_SOFTMAX, "sigmoid": MOE_SCORING_SIGMOID}[scoring]
         self._shard = None
@@ -131,7 +122,7 @@ class MoEDataPlane:
     def close(self):
         if getattr(self, "_h", None):
             lib().moe_destroy(self._h)
-            self._h = None
+            self._h = self._plane = None
 
     def __del__(self):
         try:
@@ -389,8 +380,8 @@ class MoEDataPlane:
         return q, sc, rs
 
     # ---- 8-bit floating point: e4m3 values with one scale for each 128 ----
-    # These calls take a few microseconds on the GPU at one token, so the host's share counts: checks
-    # cost an attribute each, and messages are made only when one fails.
+    # Checks, allocation and the C calls of these methods are in _torch_binding: at one token the GPU takes a few
+    # microseconds, and Python with ctypes took longer than that.
     def quantize_fp8(self, x, block_rows=1, stream=None):
         """x [..., rows, cols] bf16 or fp32 -> Fp8(q, scale): one scale for each 128 columns of a row
         (block_rows=1, activations) or of 128 rows (block_rows=128, weights).  Scales are powers of two;
@@ -398,17 +389,8 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.quantize_fp8(x, block_rows)
-        x = self._operand("x", x, _DTYPES, None, 16)
-        if x.dim() < 2 or block_rows not in (1, 128):
-            raise ValueError("quantize_fp8 takes [..., rows, cols] and block_rows 1 or 128")
-        *lead, rows, cols = x.shape
-        q = torch.empty_like(x, dtype=_F8)
-        scale = self._like().f32.new_empty((*lead, -(-rows // block_rows), -(-cols // 128)))
-        status = lib().moe_quantize_fp8(self._h, x.data_ptr(), _DTYPES[x.dtype], math.prod(lead), rows, cols, block_rows,
-                                        q.data_ptr(), scale.data_ptr(), 0, _raw_stream(self._index))
-        if status:
-            check(status)
-        return Fp8(q, scale)
+        p = self._plane or self._bind()
+        return Fp8(*_calls.quantize_fp8(p, _tensor("x", x), block_rows, _raw_stream(self._index)))
 
     def matmul_fp8(self, x, w, out_dtype=torch.bfloat16, out=None, stream=None):
         """out [M, N] = x [M, K] . w [N, K]^T with fp32 sums.  x: Fp8 with a scale per row and 128 columns
@@ -418,17 +400,8 @@ class MoEDataPlane:
                 return self.matmul_fp8(x, w, out_dtype, out)
         if type(x) is not Fp8:
             x = self.quantize_fp8(x)
-        xq, xs = self._fp8("x", x, 2, 1)
-        wq, ws = self._fp8("w", w, 2, 128)
-        (M, K), (N, wk) = xq.shape, wq.shape
-        if wk != K:
-            raise ValueError(f"x has {K} columns, w {wk}")
-        out = self._output(out, xs, (M, N), out_dtype, _DTYPES)
-        status = lib().moe_matmul_fp8(self._h, M, N, K, xq.data_ptr(), xs.data_ptr(), wq.data_ptr(), ws.data_ptr(), out.data_ptr(),
-                                      _DTYPES[out.dtype], 0, _raw_stream(self._index))
-        if status:
-            check(status)
-        return out
+        p = self._plane or self._bind()
+        return _calls.matmul_fp8(p, x.q, x.scale, *_fp8("w", w), out_dtype, out, _raw_stream(self._index))
 
     def experts_fp8(self, x, gate_up, down, idx, w, out_dtype=torch.float32, out=None, accumulate=False, stream=None):
         """The routed experts on e4m3 weights: out [T, H] = sum_k w[t, k] expert_idx[t, k](x[t]).
@@ -439,33 +412,9 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.experts_fp8(x, gate_up, down, idx, w, out_dtype, out, accumulate)
-        x = self._operand("x", x, _BF16, 2, 16)
-        H, F, E, K = self.H, self.F, self.E, self.K
-        T, cols = x.shape
-        if cols != H:
-            raise ValueError(f"x has {cols} columns, the context {H}")
-        gq, gs = self._fp8("gate_up", gate_up, 4, 128)
-        dq, ds = self._fp8("down", down, 3, 128)
-        if gq.shape != (E, 2, F, H):
-            raise ValueError(f"gate_up is {tuple(gq.shape)}, not {(E, 2, F, H)}")
-        if dq.shape != (E, H, F):
-            raise ValueError(f"down is {tuple(dq.shape)}, not {(E, H, F)}")
-        idx = self._operand("idx", idx, _I32, 2)
-        w = self._operand("w", w, _F32, 2)
-        if idx.shape != (T, K) or w.shape != (T, K):
-            raise ValueError(f"idx {tuple(idx.shape)} and w {tuple(w.shape)} must be {(T, K)}")
-        if accumulate and out is None:
-            raise ValueError("accumulate needs an out to add to")
-        out = self._output(out, x, (T, H), out_dtype, _DTYPES)
-        L = lib()
-        n = L.moe_experts_fp8_workspace(self._h, T)
-        ws = self._like().u8.new_empty(max(n, 0))  # from the stream's pool, alive until enqueued
-        status = L.moe_experts_fp8(self._h, T, x.data_ptr(), gq.data_ptr(), gs.data_ptr(), dq.data_ptr(), ds.data_ptr(),
-                                   idx.data_ptr(), w.data_ptr(), out.data_ptr(), _DTYPES[out.dtype], ws.data_ptr(), n,
-                                   MOE_F_ACCUMULATE if accumulate else 0, _raw_stream(self._index))
-        if status:
-            check(status)
-        return out
+        p = self._plane or self._bind()
+        return _calls.experts_fp8(p, x, *_fp8("gate_up", gate_up), *_fp8("down", down), idx, w, out_dtype, out, accumulate,
+                                  _raw_stream(self._index))
 
     def route_topk(self, logits, bias=None, stream=None):
         """The router alone, on the device and without a wait: (idx [T, top_k] int32, w [T, top_k] fp32)."""
@@ -497,22 +446,9 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.balance_loss(logits, idx, offsets, mask)
-        logits, offsets, mask, B, po, pm = self._balance_inputs(logits, offsets, mask)
-        T, E = logits.shape
-        idx = self._operand("idx", idx, _I32, 2)
-        if idx.shape != (T, self.K):
-            raise ValueError(f"idx is {tuple(idx.shape)}, not {(T, self.K)}")
-        L = lib()
-        loss = logits.new_empty(())
-        counts = idx.new_empty((B, E))
-        tokens = idx.new_empty(B + 1)
-        n = L.moe_balance_loss_workspace(self._h, T, B)
-        ws = idx.new_empty(max(n, 0) // 4)
-        status = L.moe_balance_loss(self._h, T, logits.data_ptr(), idx.data_ptr(), po, B, pm, loss.data_ptr(), counts.data_ptr(),
-                                    tokens.data_ptr(), ws.data_ptr(), n, 0, _raw_stream(self._index))
-        if status:
-            check(status)
-        return loss, BalanceStats(counts, tokens, offsets, mask)
+        p = self._plane or self._bind()
+        loss, *stats = _calls.balance_loss(p, logits, idx, offsets, mask, _raw_stream(self._index))
+        return loss, BalanceStats(*stats)
 
     def balance_loss_backward(self, logits, stats, grad=None, out=None, stream=None):
         """dlogits [T, E] fp32 = grad * d loss / d logits (grad: a device fp32 scalar; None: 1), zero for
@@ -520,82 +456,17 @@ class MoEDataPlane:
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.balance_loss_backward(logits, stats, grad, out)
-        counts, tokens, offsets, mask = stats
-        logits, offsets, mask, B, po, pm = self._balance_inputs(logits, offsets, mask)
-        counts = self._operand("stats.counts", counts, _I32, 2)
-        tokens = self._operand("stats.tokens", tokens, _I32, 1)
-        T, E = logits.shape
-        if counts.shape != (B, E) or tokens.shape != (B + 1,):
-            raise ValueError("stats are of other sequences")
-        if grad is not None:
-            grad = self._operand("grad", grad, _F32, 0)
-        out = self._output(out, logits, (T, E), torch.float32, _F32)
-        status = lib().moe_balance_loss_backward(self._h, T, logits.data_ptr(), po, B, pm, counts.data_ptr(), tokens.data_ptr(),
-                                                 None if grad is None else grad.data_ptr(), out.data_ptr(), 0, _raw_stream(self._index))
-        if status:
-            check(status)
-        return out
+        p = self._plane or self._bind()
+        return _calls.balance_loss_backward(p, logits, *stats, grad, out, _raw_stream(self._index))
 
-    def _balance_inputs(self, logits, offsets, mask):
-        logits = self._operand("logits", logits, _F32, 2)
-        if logits.requires_grad and torch.is_grad_enabled():
-            raise ValueError("balance_loss records no autograd graph: pass logits.detach() and use balance_loss_backward")
-        if logits.shape[1] != self.E:
-            raise ValueError(f"logits have {logits.shape[1]} columns, the context {self.E} experts")
-        B, po, pm = 1, None, None
-        if offsets is not None:
-            offsets = self._operand("offsets", offsets, _I32, 1)
-            B, po = offsets.shape[0] - 1, offsets.data_ptr()
-            if B < 1:
-                raise ValueError("offsets need two entries at least")
-        if mask is not None:
-            mask = self._operand("mask", mask, _MASK, 1)
-            pm = mask.data_ptr()
-            if mask.shape[0] != logits.shape[0]:
-                raise ValueError(f"mask has {mask.shape[0]} tokens, logits {logits.shape[0]}")
-        return logits, offsets, mask, B, po, pm
-
-    def _operand(self, name, t, dtypes, dims, align=1):
-        """t as a contiguous tensor of this device, at a multiple of align bytes; other types and ranks are refused."""
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
-            raise ValueError(f"{name} must be a tensor on {self.device}")
-        if t.dtype not in dtypes:
-            raise ValueError(f"{name} is {t.dtype}, not {' or '.join(map(str, dtypes))}")
-        if dims is not None and t.dim() != dims:
-            raise ValueError(f"{name} has {t.dim()} dimensions, not {dims}")
-        if not t.is_contiguous():
-            t = t.contiguous()
-        return t.clone() if align > 1 and t.data_ptr() % align else t
-
-    def _fp8(self, name, m, dims, block_rows):
-        if type(m) is not Fp8:
-            raise ValueError(f"{name} must be an Fp8, as quantize_fp8 gives it")
-        q, s = m
-        if block_rows > 1 and isinstance(q, torch.Tensor) and not q.is_contiguous():
-            raise ValueError(f"{name}.q must be contiguous")
-        q = self._operand(name + ".q", q, _E4M3, dims, 16)
-        s = self._operand(name + ".scale", s, _F32, dims)
-        *lead, rows, cols = q.shape
-        want = (*lead, -(-rows // block_rows), -(-cols // 128))
-        if s.shape != want:
-            raise ValueError(f"{name}.scale is {tuple(s.shape)}, not {want}")
-        return q, s
-
-    def _output(self, out, like, shape, dtype, dtypes):
-        if out is None:
-            if dtype not in dtypes:
-                raise ValueError(f"out_dtype {dtype} is neither torch.bfloat16 nor torch.float32")
-            return torch.empty_like(like, dtype=dtype) if like.shape == shape else like.new_empty(shape, dtype=dtype)
-        if (out.device != self.device or out.dtype not in dtypes or out.shape != shape or not out.is_contiguous() or
-                out.data_ptr() % 16):
-            raise ValueError(f"out must be a contiguous, 16-byte aligned {shape} tensor on {self.device}")
-        return out
-
-    def _like(self):
-        """Empty tensors of this device: new_empty() of one costs half of torch.empty() with a type and a device."""
-        if self._likes is None:
-            self._likes = _Likes(*(torch.empty(0, dtype=t, device=self.device) for t in (torch.float32, torch.int32, torch.uint8)))
-        return self._likes
+    def _bind(self):
+        """What the calls of _torch_binding need of this context; dropped with it by close()."""
+        global _calls
+        if _calls is None:
+            lib()  # the library first: the binding is linked to it
+            from . import _torch_binding as _calls
+        self._plane = _calls.Plane(self._h.value if self._h else 0, self.device, self.H, self.F, self.E, self.K)
+        return self._plane
 
     def status(self, stream=None):
         return lib().moe_status(self._h, _stream_ptr(stream, self.device))
@@ -625,6 +496,18 @@ class MoEDataPlane:
         n = ctypes.c_int64()
         check(lib().moe_profile_read(self._h, ms, n_stages, ctypes.byref(n)))
         return list(ms), int(n.value)
+
+
+def _tensor(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name} must be a tensor on the GPU, not {type(t).__name__}")
+    return t
+
+
+def _fp8(name, m):
+    if type(m) is not Fp8:
+        raise ValueError(f"{name} must be an Fp8, as quantize_fp8 gives it")
+    return m
 
 
 def _cpu(t):

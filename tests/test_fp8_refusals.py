@@ -14,7 +14,7 @@ F8 = torch.float8_e4m3fn
 def plane(monkeypatch):
     """A plane of the host's memory whose C calls get a null context."""
     p = object.__new__(nob.MoEDataPlane)
-    p.H, p.F, p.E, p.K, p._h, p._index, p._likes = 256, 64, 8, 2, None, 0, None
+    p.H, p.F, p.E, p.K, p._h, p._index, p._plane = 256, 64, 8, 2, None, 0, None
     p.device = torch.device("cpu")
     from npu_offload_b200 import moe
     monkeypatch.setattr(moe, "_raw_stream", lambda index: 0)
