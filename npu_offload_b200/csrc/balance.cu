@@ -22,6 +22,7 @@
 
 #include "balance.h"
 #include "common.cuh"
+#include "launch.cuh"
 #include "ptx.cuh"
 
 namespace cg = cooperative_groups;
@@ -160,6 +161,7 @@ __global__ void __launch_bounds__(kBalThreads) balance_units_kernel(BalanceArgs 
     __shared__ int32_t c_s[NE * 32];
     __shared__ int32_t n_s[kBalWarps];
     griddep_launch_dependents();
+    griddep_wait();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, u = blockIdx.x, E = a.E, K = a.K;
     if (u == 0 && tid == 0) *w.ticket = 0;
     // the last sequence whose first unit is at most u
@@ -233,6 +235,7 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThread
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = (int)cl.block_rank(), E = a.E;
     const int e = r * 32 + lane, clusters = gridDim.x / kBalCluster;
+    griddep_launch_dependents();
     griddep_wait();
     for (int b = blockIdx.x / kBalCluster; b < a.B; b += clusters) {
         int first, last;
@@ -306,6 +309,8 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThread
 // A warp a row; rows of a warp are neighbours, so that it keeps its sequence's f in registers.
 template <int NE, bool SIG, bool V, bool FULL>
 __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceArgs a, int per_warp) {
+    griddep_launch_dependents();
+    griddep_wait();
     const int E = a.E;
     const long t0 = ((long)blockIdx.x * kBalWarps + (threadIdx.x >> 5)) * per_warp;
     const long t1 = min(t0 + per_warp, (long)a.T);
@@ -370,15 +375,13 @@ __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceAr
 
 template <int NE, bool V, bool FULL>
 static cudaError_t units_launch(const BalanceArgs& a, const BalanceWs& w, int chunk, int units, cudaStream_t st) {
-    if (a.scoring) balance_units_kernel<NE, true, V, FULL><<<units, kBalThreads, 0, st>>>(a, w, chunk);
-    else balance_units_kernel<NE, false, V, FULL><<<units, kBalThreads, 0, st>>>(a, w, chunk);
-    return cudaGetLastError();
+    return launch_after(a.scoring ? balance_units_kernel<NE, true, V, FULL> : balance_units_kernel<NE, false, V, FULL>, units,
+                        kBalThreads, 0, 0, st, a, w, chunk);
 }
 template <int NE, bool V, bool FULL>
 static cudaError_t backward_launch(const BalanceArgs& a, int grid, int per_warp, cudaStream_t st) {
-    if (a.scoring) balance_backward_kernel<NE, true, V, FULL><<<grid, kBalThreads, 0, st>>>(a, per_warp);
-    else balance_backward_kernel<NE, false, V, FULL><<<grid, kBalThreads, 0, st>>>(a, per_warp);
-    return cudaGetLastError();
+    return launch_after(a.scoring ? balance_backward_kernel<NE, true, V, FULL> : balance_backward_kernel<NE, false, V, FULL>, grid,
+                        kBalThreads, 0, 0, st, a, per_warp);
 }
 
 // Rows of 16-byte words where the sizes and addresses allow them; without bounds in a row of 128 or 256.
@@ -394,16 +397,7 @@ cudaError_t launch_balance_loss(const BalanceArgs& a, int sm_count, cudaStream_t
     else if (a.E <= 128) e = units_launch<4, false, false>(a, w, chunk, units, st);
     else e = units_launch<8, false, false>(a, w, chunk, units, st);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(kBalCluster * std::min(a.B, sm_count / kBalCluster));
-    cfg.blockDim = dim3(kSumThreads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, balance_sum_kernel, a, w, chunk);
+    return launch_after(balance_sum_kernel, kBalCluster * std::min(a.B, sm_count / kBalCluster), kSumThreads, 0, 0, st, a, w, chunk);
 }
 
 cudaError_t launch_balance_backward(const BalanceArgs& a, int sm_count, cudaStream_t st) {

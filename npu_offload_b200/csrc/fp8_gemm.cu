@@ -9,6 +9,7 @@
 #include "fp8.h"
 #include "fp8.cuh"
 #include "fp8_tc.cuh"
+#include "launch.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -43,51 +44,11 @@ cudaError_t allow_smem(int bytes) {
     return e;
 }
 
-// Launch with an optional cluster split and, where `pdl`, ahead of the end of the kernel before it.
-template <class K>
-cudaError_t launch(K kernel, int grid, int threads, int smem, int cluster, bool pdl, cudaStream_t st, const CUtensorMap& mw,
-                   const CUtensorMap& mx, const F8Gemm& g) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    int n = 0;
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = cluster;
-    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
-    n++;
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n].val.programmaticStreamSerializationAllowed = 1;
-        n++;
-    }
-    cfg.attrs = attr;
-    cfg.numAttrs = n;
-    return cudaLaunchKernelEx(&cfg, kernel, mw, mx, g);
-}
-
-// Launch ahead of the end of the kernel before it (which it waits for itself).
-template <class K, class... A>
-cudaError_t launch_after(K kernel, int grid, int threads, cudaStream_t st, A... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int MODE, int NQ>
 struct Few {
     using C = FewCfg<MODE, NQ>;
     // tiles: upper bound of the tiles there may be
-    static cudaError_t run(const CUtensorMap& mw, const CUtensorMap& mx, const F8Gemm& g, int64_t tiles, int sm_count, bool pdl,
+    static cudaError_t run(const CUtensorMap& mw, const CUtensorMap& mx, const F8Gemm& g, int64_t tiles, int sm_count,
                            cudaStream_t st) {
         constexpr auto k = f8_few_kernel<MODE, NQ>;
         const cudaError_t e = allow_smem<k>(C::kSmem);
@@ -96,19 +57,19 @@ struct Few {
         int cs = 1;  // split the inner dimension while all CTAs are still on the GPU at once
         while (cs < 8 && tiles * cs * 2 <= slots && cs * 2 <= g.nkb) cs *= 2;
         const int clusters = (int)std::min<int64_t>(tiles, slots / cs);
-        return launch(k, clusters * cs, kFewThreads, C::kSmem, cs, pdl, st, mw, mx, g);
+        return launch_after(k, clusters * cs, kFewThreads, C::kSmem, cs, st, mw, mx, g);
     }
 };
 
 template <int MODE, int NB>
 struct Many {
     using C = ManyCfg<MODE, NB>;
-    static cudaError_t run(const CUtensorMap& mw, const CUtensorMap& mx, const F8Gemm& g, int64_t tiles, int sm_count, bool pdl,
+    static cudaError_t run(const CUtensorMap& mw, const CUtensorMap& mx, const F8Gemm& g, int64_t tiles, int sm_count,
                            cudaStream_t st) {
         constexpr auto k = f8_many_kernel<MODE, NB>;
         const cudaError_t e = allow_smem<k>(C::kSmem);
         if (e != cudaSuccess) return e;
-        return launch(k, (int)std::min<int64_t>(tiles, sm_count), kManyThreads, C::kSmem, 1, pdl, st, mw, mx, g);
+        return launch_after(k, (int)std::min<int64_t>(tiles, sm_count), kManyThreads, C::kSmem, 0, st, mw, mx, g);
     }
 };
 
@@ -133,13 +94,13 @@ cudaError_t launch_matmul_fp8(const MatmulF8& m, int sm_count, cudaStream_t st) 
     const int nq = m.M <= 16 ? 16 : m.M <= 32 ? 32 : m.M <= 64 ? 64 : 128;
     CUtensorMap mw, mx;
     if (!encode3(enc, &mw, m.w, m.K, m.N, 1, 128) || !encode2(enc, &mx, m.x, m.K, m.M, nq)) return cudaErrorInvalidValue;
-    if (nq == 16) return Few<kF8Dense, 16>::run(mw, mx, g, g.nt, sm_count, false, st);
-    if (nq == 32) return Few<kF8Dense, 32>::run(mw, mx, g, g.nt, sm_count, false, st);
-    if (nq == 64) return Few<kF8Dense, 64>::run(mw, mx, g, g.nt, sm_count, false, st);
+    if (nq == 16) return Few<kF8Dense, 16>::run(mw, mx, g, g.nt, sm_count, st);
+    if (nq == 32) return Few<kF8Dense, 32>::run(mw, mx, g, g.nt, sm_count, st);
+    if (nq == 64) return Few<kF8Dense, 64>::run(mw, mx, g, g.nt, sm_count, st);
     const int64_t mt = (m.M + 127) / 128;
-    if (mt * ((m.N + 255) / 256) < sm_count) return Many<kF8Dense, 128>::run(mw, mx, g, mt * g.nt, sm_count, false, st);
+    if (mt * ((m.N + 255) / 256) < sm_count) return Many<kF8Dense, 128>::run(mw, mx, g, mt * g.nt, sm_count, st);
     g.nt = (int)((m.N + 255) / 256);
-    return Many<kF8Dense, 256>::run(mw, mx, g, mt * g.nt, sm_count, false, st);
+    return Many<kF8Dense, 256>::run(mw, mx, g, mt * g.nt, sm_count, st);
 }
 
 // ---- routed experts ----
@@ -230,6 +191,7 @@ __global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
     __shared__ int wc[kPrepPairs / 32][kMaxExperts];  // pairs of each warp on each expert, then their exclusive sums
     __shared__ int cnt[kMaxExperts], off[kMaxExperts], goff[kMaxExperts], slots[kPrepPairs];
     griddep_launch_dependents();
+    griddep_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, P = a.T * a.K, warps = (P + 31) / 32;
     const int e = tid < P ? __ldg(a.idx + tid) : -1;
     const PrepLoad l = prep_begin(a);
@@ -273,6 +235,7 @@ __global__ void __launch_bounds__(kPrepThreads) f8_prep_kernel(PrepArgs a) {
 constexpr int kTinyThreads = 128;
 __global__ void __launch_bounds__(kTinyThreads) f8_prep_tiny_kernel(PrepArgs a) {
     griddep_launch_dependents();
+    griddep_wait();
     const int lane = threadIdx.x & 31, P = a.T * a.K;
     int e = lane < P ? __ldg(a.idx + lane) : -1;
     const uint32_t per_row = (uint32_t)(a.H + 127) / 128, groups = (uint32_t)a.T * per_row, sub = threadIdx.x & 15;
@@ -319,7 +282,8 @@ __global__ void __launch_bounds__(kTinyThreads) f8_prep_tiny_kernel(PrepArgs a) 
 __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPrepThreads) f8_plan_kernel(PrepArgs a) {
     __shared__ int mine[kMaxExperts], cnt[kMaxExperts], off[kMaxExperts], goff[kMaxExperts];
     cg::cluster_group cl = cg::this_cluster();
-    griddep_launch_dependents();
+    griddep_wait();
+    griddep_launch_dependents();  // after the wait: the scatter kernel reads the tokens ahead of its own
     const int tid = threadIdx.x, rank = (int)cl.block_rank(), E = a.E;
     const int P = a.T * a.K, share = (P + kPlanCluster - 1) / kPlanCluster, first = min(P, rank * share), last = min(P, first + share);
     if (tid < kMaxExperts) mine[tid] = 0;
@@ -459,8 +423,8 @@ Ws experts_layout(void* ws, int T, int K, int H, int F, int E) {
 
 template <int NQ>
 cudaError_t products_few(const CUtensorMap (&m)[4], F8Gemm gu, F8Gemm dn, int64_t groups, int sm_count, cudaStream_t st) {
-    const cudaError_t e = Few<kF8GateUp, NQ>::run(m[0], m[1], gu, groups * gu.nt, sm_count, true, st);
-    return e != cudaSuccess ? e : Few<kF8Down, NQ>::run(m[2], m[3], dn, groups * dn.nt, sm_count, true, st);
+    const cudaError_t e = Few<kF8GateUp, NQ>::run(m[0], m[1], gu, groups * gu.nt, sm_count, st);
+    return e != cudaSuccess ? e : Few<kF8Down, NQ>::run(m[2], m[3], dn, groups * dn.nt, sm_count, st);
 }
 
 }  // namespace
@@ -484,15 +448,13 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
                                              2 * sm_count);
     cudaError_t e;
     if (P <= 32) {
-        f8_prep_tiny_kernel<<<(int)(((int64_t)a.T * ((a.H + 127) / 128) * 16 + kTinyThreads - 1) / kTinyThreads), kTinyThreads, 0, st>>>(pa);
-        e = cudaGetLastError();
+        e = launch_after(f8_prep_tiny_kernel, (int)(((int64_t)a.T * ((a.H + 127) / 128) * 16 + kTinyThreads - 1) / kTinyThreads),
+                         kTinyThreads, 0, 0, st, pa);
     } else if (P <= kPrepPairs) {
-        f8_prep_kernel<<<qctas, kPrepThreads, 0, st>>>(pa);
-        e = cudaGetLastError();
+        e = launch_after(f8_prep_kernel, qctas, kPrepThreads, 0, 0, st, pa);
     } else {
-        f8_plan_kernel<<<kPlanCluster, kPrepThreads, 0, st>>>(pa);
-        e = cudaGetLastError();
-        if (e == cudaSuccess) e = launch_after(f8_scatter_kernel, qctas, kPrepThreads, st, pa);
+        e = launch_after(f8_plan_kernel, kPlanCluster, kPrepThreads, 0, 0, st, pa);
+        if (e == cudaSuccess) e = launch_after(f8_scatter_kernel, qctas, kPrepThreads, 0, 0, st, pa);
         ++*launches;
     }
     if (e != cudaSuccess) return e;
@@ -521,13 +483,13 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     else if (height == 32) e = products_few<32>(m, gu, dn, groups, sm_count, st);
     else if (height == 64) e = products_few<64>(m, gu, dn, groups, sm_count, st);
     else {
-        e = Many<kF8GateUp, 256>::run(m[0], m[1], gu, groups * gu.nt, sm_count, true, st);
+        e = Many<kF8GateUp, 256>::run(m[0], m[1], gu, groups * gu.nt, sm_count, st);
         dn.nt = (a.H + 255) / 256;
-        if (e == cudaSuccess) e = Many<kF8Down, 256>::run(m[2], m[3], dn, groups * dn.nt, sm_count, true, st);
+        if (e == cudaSuccess) e = Many<kF8Down, 256>::run(m[2], m[3], dn, groups * dn.nt, sm_count, st);
     }
     if (e != cudaSuccess) return e;
     *launches += 4;
-    return launch_after(f8_combine_kernel, (int)std::min<int64_t>(((int64_t)a.T * a.H / 4 + 255) / 256, sm_count * 8), 256, st,
+    return launch_after(f8_combine_kernel, (int)std::min<int64_t>(((int64_t)a.T * a.H / 4 + 255) / 256, sm_count * 8), 256, 0, 0, st,
                         (const float*)w.y, (const int32_t*)w.pos, a.w, a.T, a.K, a.H, a.out, a.out_f32, a.accumulate);
 }
 

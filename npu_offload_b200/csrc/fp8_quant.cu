@@ -14,6 +14,8 @@
 #include "common.cuh"
 #include "fp8.h"
 #include "fp8.cuh"
+#include "launch.cuh"
+#include "ptx.cuh"
 
 namespace moe {
 
@@ -53,6 +55,8 @@ struct Eight<true> {
 template <bool F32, int N>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, uint32_t groups, uint32_t per_row,
                                                             uint32_t cols, uint8_t* __restrict__ q, float* __restrict__ s) {
+    griddep_launch_dependents();
+    griddep_wait();
     const uint32_t sub = threadIdx.x & 15, g0 = blockIdx.x * 16 * N + (threadIdx.x >> 4);
     Eight<F32> v[N];
     size_t at[N];
@@ -86,6 +90,8 @@ __global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const
                                                               uint32_t rb, uint32_t cb, uint8_t* __restrict__ q,
                                                               float* __restrict__ s) {
     __shared__ uint32_t top_s[8];
+    griddep_launch_dependents();
+    griddep_wait();
     const uint32_t b = blockIdx.x / cb, kb = blockIdx.x - b * cb, mat = b / rb, r0 = (b - mat * rb) * kF8Block;
     const uint32_t c = kb * kF8Block + (threadIdx.x & 15) * 8;
     const size_t base = (size_t)mat * rows * cols;
@@ -131,17 +137,15 @@ cudaError_t launch_quantize_fp8(const void* x, bool f32, int64_t batch, int64_t 
         const int n = groups <= 64ll * sm_count ? 1 : f32 ? 2 : 4;
         const int grid = (int)((groups + 16 * n - 1) / (16 * n));
         const uint32_t ng = (uint32_t)groups, per_row = (uint32_t)cb, nc = (uint32_t)cols;
-        if (n == 1 && f32) quantize_rows_kernel<true, 1><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
-        else if (n == 1) quantize_rows_kernel<false, 1><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
-        else if (f32) quantize_rows_kernel<true, 2><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
-        else quantize_rows_kernel<false, 4><<<grid, 256, 0, st>>>(x, ng, per_row, nc, q, s);
-        return cudaGetLastError();
+        if (n == 1 && f32) return launch_after(quantize_rows_kernel<true, 1>, grid, 256, 0, 0, st, x, ng, per_row, nc, q, s);
+        if (n == 1) return launch_after(quantize_rows_kernel<false, 1>, grid, 256, 0, 0, st, x, ng, per_row, nc, q, s);
+        if (f32) return launch_after(quantize_rows_kernel<true, 2>, grid, 256, 0, 0, st, x, ng, per_row, nc, q, s);
+        return launch_after(quantize_rows_kernel<false, 4>, grid, 256, 0, 0, st, x, ng, per_row, nc, q, s);
     }
     const int64_t rb = (rows + kF8Block - 1) / kF8Block, blocks = batch * rb * cb;
     if (blocks >= (1ll << 31) || rows >= (1ll << 31) || cols >= (1ll << 31)) return cudaErrorInvalidValue;
-    if (f32) quantize_blocks_kernel<true><<<(int)blocks, 256, 0, st>>>(x, (uint32_t)rows, (uint32_t)cols, (uint32_t)rb, (uint32_t)cb, q, s);
-    else quantize_blocks_kernel<false><<<(int)blocks, 256, 0, st>>>(x, (uint32_t)rows, (uint32_t)cols, (uint32_t)rb, (uint32_t)cb, q, s);
-    return cudaGetLastError();
+    if (f32) return launch_after(quantize_blocks_kernel<true>, (int)blocks, 256, 0, 0, st, x, (uint32_t)rows, (uint32_t)cols, (uint32_t)rb, (uint32_t)cb, q, s);
+    return launch_after(quantize_blocks_kernel<false>, (int)blocks, 256, 0, 0, st, x, (uint32_t)rows, (uint32_t)cols, (uint32_t)rb, (uint32_t)cb, q, s);
 }
 
 }  // namespace moe
