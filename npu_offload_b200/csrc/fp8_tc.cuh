@@ -564,6 +564,24 @@ __device__ __forceinline__ void turn_rows(unsigned char* turn, const uint4 (&w)[
         if (r < rows && k < words) *reinterpret_cast<uint4*>(dst + r * pitch + k * 16) = v;
     }
 }
+// The same where rows are not 16-byte aligned: the values of a row (B bytes each, `left` of them) by as many
+// neighbouring lanes.
+template <int B>
+__device__ __forceinline__ void turn_values(unsigned char* turn, const uint4 (&w)[4], char* dst, size_t pitch, int rows, int left) {
+    constexpr int L = 64 / B;  // lanes a row
+    const int lane = threadIdx.x & 31, e = lane % L;
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < 4; k++) *reinterpret_cast<uint4*>(turn + lane * 64 + ((k ^ (lane >> 1 & 3)) << 4)) = w[k];
+    __syncwarp();
+#pragma unroll 4
+    for (int r = lane / L; r < 32; r += 32 / L) {
+        const unsigned char* v = turn + r * 64 + (((e * B >> 4) ^ (r >> 1 & 3)) << 4) + (e * B & 15);
+        if (r >= rows || e >= left) continue;
+        if (B == 4) *reinterpret_cast<uint32_t*>(dst + r * pitch + e * 4) = *reinterpret_cast<const uint32_t*>(v);
+        else *reinterpret_cast<uint16_t*>(dst + r * pitch + e * 2) = *reinterpret_cast<const uint16_t*>(v);
+    }
+}
 // A segment's 32 columns from column n0 on as fp32 or bf16, row0 = the warp's first row.
 template <bool F32>
 __device__ __forceinline__ void turn_store(unsigned char* turn, const float (&v)[32], void* out, size_t row0, int n0, int N, int rows) {
@@ -578,7 +596,8 @@ __device__ __forceinline__ void turn_store(unsigned char* turn, const float (&v)
             if (F32) w[k] = make_uint4(__float_as_uint(q[0]), __float_as_uint(q[1]), __float_as_uint(q[2]), __float_as_uint(q[3]));
             else w[k] = make_uint4(f8_bf16x2(q[0], q[1]), f8_bf16x2(q[2], q[3]), f8_bf16x2(q[W - 4], q[W - 3]), f8_bf16x2(q[W - 2], q[W - 1]));
         }
-        turn_rows(turn, w, dst + c * B, (size_t)N * B, rows, (N - n0 - c) / W);
+        if (N % W == 0) turn_rows(turn, w, dst + c * B, (size_t)N * B, rows, (N - n0 - c) / W);
+        else turn_values<B>(turn, w, dst + c * B, (size_t)N * B, rows, N - n0 - c);
     }
 }
 
@@ -777,17 +796,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                 for (int i = 0; i < SEG; i++) {
                     const int n0 = n * NB + quarter * (NB / 4) + i * 32;
-                    if (a.N % (f32 ? 4 : 8) == 0) {
-                        if (f32) turn_store<true>(turn, acc[i], a.out, row0, n0, a.N, rows);
-                        else turn_store<false>(turn, acc[i], a.out, row0, n0, a.N, rows);
-                    } else if (live) {  // rows that are not 16-byte aligned
-#pragma unroll
-                        for (int j = 0; j < 32; j++)
-                            if (n0 + j < a.N) {
-                                if (f32) static_cast<float*>(a.out)[slot * a.N + n0 + j] = acc[i][j];
-                                else static_cast<uint16_t*>(a.out)[slot * a.N + n0 + j] = f8_bf16(acc[i][j]);
-                            }
-                    }
+                    if (rows <= 0) break;
+                    if (f32) turn_store<true>(turn, acc[i], a.out, row0, n0, a.N, rows);
+                    else turn_store<false>(turn, acc[i], a.out, row0, n0, a.N, rows);
                 }
             }
         }
