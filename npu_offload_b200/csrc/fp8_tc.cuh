@@ -461,35 +461,61 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                         for (int h = 0; h < WB; h++) red[(j * WB + h) * 128 + tid] = acc[h][j];
             }
             const int i = n * 128 + tid;  // weight row
+            constexpr int U = 4;          // columns at a time (one behind the other, 64 of them took 7 us)
+            if (MODE == kF8Down || (MODE == kF8Dense && i < a.N)) {
+                const size_t at = ((size_t)grp.row0 + rank) * a.N + i, step = (size_t)CS * a.N;
 #pragma unroll 1
-            for (int j = 0; j < mine; j++) {
-                float v[WB];
+                for (int j = 0; j < mine; j += U) {
+                    float v[U];
 #pragma unroll
-                for (int h = 0; h < WB; h++) {
-                    v[h] = red[(j * WB + h) * 128 + tid];
+                    for (int u = 0; u < U; u++) v[u] = red[(j + u) * 128 + tid];
 #pragma unroll 1
-                    for (int r = 1; r < CS; r++) v[h] += red[((r * per + j) * WB + h) * 128 + tid];
-                }
-                if (MODE == kF8GateUp) {
-                    v[0] = swiglu_f32(v[0], v[WB - 1]);
-                    red[j * WB * 128 + tid] = v[0];
-                    uint32_t t = __float_as_uint(v[0]) & 0x7fffffffu;
-                    t = __reduce_max_sync(0xffffffffu, t < 0x7f800000u ? t : 0u);
-                    if (lane == 0) c.top[warp][j] = t;
-                } else if (i < a.N) {
-                    const size_t at = ((size_t)grp.row0 + rank + CS * j) * a.N + i;
-                    if (MODE == kF8Down || a.out_f32) static_cast<float*>(a.out)[at] = v[0];
-                    else static_cast<uint16_t*>(a.out)[at] = f8_bf16(v[0]);
+                    for (int r = 1; r < CS; r++)
+#pragma unroll
+                        for (int u = 0; u < U; u++) v[u] += j + u < mine ? red[(r * per + j + u) * 128 + tid] : 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        if (j + u < mine && i < a.N) {
+                            if (MODE == kF8Down || a.out_f32) static_cast<float*>(a.out)[at + (j + u) * step] = v[u];
+                            else static_cast<uint16_t*>(a.out)[at + (j + u) * step] = f8_bf16(v[u]);
+                        }
                 }
             }
             if (MODE == kF8GateUp) {
+#pragma unroll 1
+                for (int j = 0; j < mine; j += U) {
+                    float v[U][WB];
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int h = 0; h < WB; h++) v[u][h] = red[((j + u) * WB + h) * 128 + tid];
+#pragma unroll 1
+                    for (int r = 1; r < CS; r++)
+#pragma unroll
+                        for (int u = 0; u < U; u++)
+#pragma unroll
+                            for (int h = 0; h < WB; h++) v[u][h] += j + u < mine ? red[((r * per + j + u) * WB + h) * 128 + tid] : 0.f;
+#pragma unroll
+                    for (int u = 0; u < U; u++) {  // columns behind the last are of no use and harmless
+                        v[u][0] = swiglu_f32(v[u][0], v[u][WB - 1]);
+                        if (j + u < mine) red[(j + u) * WB * 128 + tid] = v[u][0];
+                        uint32_t t = __float_as_uint(v[u][0]) & 0x7fffffffu;
+                        t = __reduce_max_sync(0xffffffffu, t < 0x7f800000u ? t : 0u);
+                        if (lane == 0 && j + u < mine) c.top[warp][j + u] = t;
+                    }
+                }
                 named_bar_sync(1, 128);
 #pragma unroll 1
-                for (int j = 0; j < mine; j++) {
-                    const uint32_t se = f8_scale_exp(max(max(c.top[0][j], c.top[1][j]), max(c.top[2][j], c.top[3][j])));
-                    const size_t slot = (size_t)grp.row0 + rank + CS * j;
-                    if (i < a.N) a.aq[slot * a.N + i] = (uint8_t)f8_pack1(red[j * WB * 128 + tid], f8_inverse(se));
-                    if (tid == 0) a.as[slot * a.nb + n] = __uint_as_float(se << 23);
+                for (int j = 0; j < mine; j += U) {
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+                        if (j + u < mine) {
+                            const int k = j + u;
+                            const uint32_t se = f8_scale_exp(max(max(c.top[0][k], c.top[1][k]), max(c.top[2][k], c.top[3][k])));
+                            const size_t slot = (size_t)grp.row0 + rank + CS * k;
+                            if (i < a.N) a.aq[slot * a.N + i] = (uint8_t)f8_pack1(red[k * WB * 128 + tid], f8_inverse(se));
+                            if (tid == 0) a.as[slot * a.nb + n] = __uint_as_float(se << 23);
+                        }
                 }
                 named_bar_sync(1, 128);  // c.top is read before the next item's is written
             }
