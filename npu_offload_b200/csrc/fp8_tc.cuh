@@ -552,6 +552,9 @@ template <int MODE, int NB>
 struct ManyCfg {
     static constexpr int kStage = 16384 + NB * 128;
     static constexpr int kStages = NB == 256 ? 4 : 5;
+    // Blocks the two roles hand over at a time, each with an accumulator of its own: a hand-over costs the epilogue
+    // some 400 cycles, as much as adding up a block of 128 columns.
+    static constexpr int kPhase = 256 / NB;
     static constexpr int kTurn = MODE == kF8GateUp ? 0 : 2048;  // a warp's 32 rows x 64 bytes on their way to memory
     static constexpr int kSmem = kStages * kStage + kManyEpi * kTurn + (int)sizeof(ManyCtrl<MODE>);
     static_assert(MODE == kF8Dense || NB == 256, "the expert products use 256-row tiles");
@@ -631,7 +634,7 @@ template <int MODE, int NB>
 __global__ void __launch_bounds__(kManyThreads, 1)
     f8_many_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const F8Gemm a) {
     using C = ManyCfg<MODE, NB>;
-    constexpr int S = C::kStages, SEG = NB / 128;
+    constexpr int S = C::kStages, SEG = NB / 128, KP = C::kPhase;
     extern __shared__ __align__(1024) unsigned char f8_smem[];
     unsigned char* ring = f8_smem;
     ManyCtrl<MODE>& c = *reinterpret_cast<ManyCtrl<MODE>*>(ring + S * C::kStage + kManyEpi * C::kTurn);
@@ -649,7 +652,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         c.abort = 0;
         fence_mbar_init();
     }
-    if (warp == kManyEpi + 1) tmem_alloc(&c.tmem, 2 * NB);
+    if (warp == kManyEpi + 1) tmem_alloc(&c.tmem, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -696,22 +699,23 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const bool leader = elect_one();
         const uint64_t desc0 = sw128_desc(smem_u32(ring));
         {
-            uint32_t g = 0;
+            uint32_t g = 0, ph = 0;  // blocks, phases
             bool ok = true;
             for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
                 for (int kb = 0; kb < nkb; kb++, g++) {
-                    const int s = g % S, b = g & 1;
+                    const int s = g % S, b = ph & 1, p = kb % KP;
                     ok = f8_wait(&c.full[s], (g / S) & 1, &c.abort, a);
-                    if (g >= 2) ok = ok && f8_wait(&c.dempty[b], ((g >> 1) & 1) ^ 1, &c.abort, a);
+                    if (p == 0 && ph >= 2) ok = ok && f8_wait(&c.dempty[b], ((ph >> 1) & 1) ^ 1, &c.abort, a);
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t dx = desc0 + (uint64_t)(s * (C::kStage >> 4)), dw = dx + 1024;
                     if (leader) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++) umma_f8(tmem + b * NB, dx + kk * 2, dw + kk * 2, idesc, kk > 0);
+                        for (int kk = 0; kk < 4; kk++) umma_f8(tmem + (b * KP + p) * NB, dx + kk * 2, dw + kk * 2, idesc, kk > 0);
                         umma_commit(&c.empty[s]);
-                        umma_commit(&c.dfull[b]);
+                        if (p == KP - 1 || kb + 1 == nkb) umma_commit(&c.dfull[b]);
                     }
+                    if (p == KP - 1 || kb + 1 == nkb) ph++;
                     __syncwarp();
                 }
             }
@@ -746,7 +750,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t taddr = tmem + ((uint32_t)(q * 32) << 16) + (MODE == kF8GateUp ? 32 : NB / 4) * quarter;
         constexpr int SEGSTEP = MODE == kF8GateUp ? 128 : 32;  // accumulator columns between a warp's segments
         const int wsel = MODE != kF8GateUp && NB == 256 ? quarter >> 1 : 0;
-        uint32_t g = 0, chunk = 0;
+        uint32_t ph = 0, chunk = 0;
         bool ok = true;
         for (int item = blockIdx.x; item < items; item += gridDim.x) {
             int gi, n;
@@ -757,33 +761,41 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (int i = 0; i < SEG; i++)
 #pragma unroll
                 for (int j = 0; j < 32; j++) acc[i][j] = 0.f;
-            for (int kb = 0; kb < nkb; kb++, g++) {
-                const int b = g & 1, sl = chunk & 1, k = kb & 1;
+            for (int kb = 0; kb < nkb; kb += KP, ph++) {
+                const int b = ph & 1, sl = chunk & 1, k = kb & 1;
                 if (k == 0) ok = ok && f8_wait(&c.sc.full[sl], (chunk >> 1) & 1, &c.abort, a);
-                const float sx = c.sc.tok[sl][k][r];
-                float sw[SEG];
+                float sw[KP][SEG];
 #pragma unroll
-                for (int i = 0; i < SEG; i++) sw[i] = sx * c.sc.wt[sl][k][MODE == kF8GateUp ? i : wsel];
-                ok = ok && f8_wait(&c.dfull[b], (g >> 1) & 1, &c.abort, a);
+                for (int p = 0; p < KP; p++) {  // (a block behind the last: what is there is not used)
+                    const float sx = c.sc.tok[sl][k + p][r];
+#pragma unroll
+                    for (int i = 0; i < SEG; i++) sw[p][i] = sx * c.sc.wt[sl][k + p][MODE == kF8GateUp ? i : wsel];
+                }
+                ok = ok && f8_wait(&c.dfull[b], (ph >> 1) & 1, &c.abort, a);
                 __syncwarp();
                 tc_fence_after();
-                uint32_t v[2][16];
-                tmem_ld16(taddr + b * NB, v[0]);
-                tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 2 * SEG; i++) {  // the next sixteen columns are read while these are added
-                    if (i + 1 < 2 * SEG) tmem_ld16(taddr + b * NB + (i + 1) / 2 * SEGSTEP + ((i + 1) & 1) * 16, v[(i + 1) & 1]);
+                for (int p = 0; p < KP; p++) {
+                    if (p > 0 && kb + p >= nkb) break;
+                    const uint32_t t0 = taddr + (b * KP + p) * NB;
+                    uint32_t v[2][16];
+                    tmem_ld16(t0, v[0]);
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        float& d = acc[i / 2][(i & 1) * 16 + j];
-                        d = fmaf(__uint_as_float(v[i & 1][j]), sw[i / 2], d);
+                    for (int i = 0; i < 2 * SEG; i++) {  // the next sixteen columns are read while these are added
+                        if (i + 1 < 2 * SEG) tmem_ld16(t0 + (i + 1) / 2 * SEGSTEP + ((i + 1) & 1) * 16, v[(i + 1) & 1]);
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            float& d = acc[i / 2][(i & 1) * 16 + j];
+                            d = fmaf(__uint_as_float(v[i & 1][j]), sw[p][i / 2], d);
+                        }
+                        if (i + 1 < 2 * SEG) tmem_wait_ld();
                     }
-                    if (i + 1 < 2 * SEG) tmem_wait_ld();
                 }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.dempty[b]);
-                if (k == 1 || kb + 1 == nkb) {
+                if (KP == 2 || k == 1 || kb + 1 == nkb) {
                     if (lane == 0) mbar_arrive(&c.sc.empty[sl]);
                     chunk++;
                 }
@@ -833,7 +845,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     __syncthreads();
     if (warp == kManyEpi + 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * NB);
+        tmem_dealloc(tmem, 512);
     }
 }
 
