@@ -307,7 +307,8 @@ MOE_API int64_t moe_launch_count(moe_ctx* ctx);
  *   MOE_OPT_WAIT_TIMEOUT_US     bound on every device-side wait of the fused kernel (default 1 s);
  *                               a wait that runs out makes the call report MOE_ETIMEOUT.
  *   MOE_OPT_INJECT_WAIT_TIMEOUT test hook: 1 makes the fused kernel's grid-wide arrival wait for one
- *                               CTA more than the grid has, so the bounded-wait error path can be
+ *                               CTA more than the grid has, and the e4m3 products' waits for their
+ *                               accumulators run out, so the bounded-wait error paths can be
  *                               tested without faulting or hanging the GPU.
  *   MOE_OPT_RING_STAGES         tuning: cap on the fused kernel's shared-memory ring depth (2..16;
  *                               0 = as deep as shared memory allows, the default).

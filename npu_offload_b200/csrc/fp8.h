@@ -28,6 +28,7 @@ struct MatmulF8 {
     bool out_f32;
     uint32_t* err;
     uint64_t timeout_ns;
+    int inject;        // test hook (MOE_OPT_INJECT_WAIT_TIMEOUT)
 };
 cudaError_t launch_matmul_fp8(const MatmulF8& a, int sm_count, cudaStream_t st);
 
@@ -47,6 +48,7 @@ struct ExpertsF8 {
     void* ws;                    // experts_fp8_workspace bytes, 256-byte aligned
     uint32_t* err;
     uint64_t timeout_ns;
+    int inject;                  // test hook (MOE_OPT_INJECT_WAIT_TIMEOUT)
 };
 size_t experts_fp8_workspace(int T, int K, int H, int F, int E);
 cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st, int* launches);

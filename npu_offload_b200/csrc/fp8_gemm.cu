@@ -91,7 +91,12 @@ cudaError_t launch_matmul_fp8(const MatmulF8& m, int sm_count, cudaStream_t st) 
     g.out_f32 = m.out_f32;
     g.err = m.err;
     g.timeout_ns = m.timeout_ns;
-    const int nq = m.M <= 16 ? 16 : m.M <= 32 ? 32 : m.M <= 64 ? 64 : 128;
+    g.inject = m.inject;
+    // Few rows: the cluster's exchange of partial sums costs 2 us (16 rows) to 8 us (64), a block of the many-row
+    // kernel 0.3 us: it wins where there are few blocks.  us, many / few, at N = 2560: 16 rows, K 1024 5.7 / 6.6, K 2048
+    // 8.3 / 6.9; 32 rows, K 2048 8.3 / 8.9, K 4096 13.4 / 9.8; 64 rows, K 4096 13.5 / 14.7, K 8192 23.6 / 17.1.
+    const int few = m.M <= 8 ? 0 : m.M <= 16 ? 10 : m.M <= 32 ? 16 : 32;
+    const int nq = m.M > 64 || g.nkb <= few ? 128 : m.M <= 16 ? 16 : m.M <= 32 ? 32 : 64;
     CUtensorMap mw, mx;
     if (!encode3(enc, &mw, m.w, m.K, m.N, 1, 128) || !encode2(enc, &mx, m.x, m.K, m.M, nq)) return cudaErrorInvalidValue;
     if (nq == 16) return Few<kF8Dense, 16>::run(mw, mx, g, g.nt, sm_count, st);
@@ -388,11 +393,11 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict
 
 namespace {
 
-// Token rows of a group: the smallest height that takes an expert's tokens, on average, in one group.
-int group_height(int64_t pairs, int E) {
-    const int64_t a = pairs / E;
-    return a <= 8 ? 16 : a <= 24 ? 32 : a <= 40 ? 64 : 128;
-}
+// Token rows of a group, by the pairs an expert gets on average: the few-row kernel on 16 or 32 of them, the many-row
+// kernel on 128.  128 experts of 4096 x 1280, 8 a token, evenly (unevenly) routed, us at heights 16 / 32 / 128:
+//   64 tokens 306 / 302 / 375 (156 / 161 / 189), 128 tokens 312 / 309 / 390 (213 / 210 / 235),
+//   400 tokens 465 / 355 / 421 (430 / 366 / 368), 600 tokens 625 / 523 / 432 (575 / 466 / 435).
+int group_height(int64_t pairs, int E) { return pairs <= 6ll * E ? 16 : pairs <= 28ll * E ? 32 : 128; }
 
 struct Ws {
     uint8_t *xq, *aq;
@@ -474,6 +479,7 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     gu.as = w.as;
     gu.err = a.err;
     gu.timeout_ns = a.timeout_ns;
+    gu.inject = a.inject;
     dn = gu;
     dn.xs = w.as;
     dn.ws = a.ds;
@@ -484,7 +490,6 @@ cudaError_t launch_experts_fp8(const ExpertsF8& a, int sm_count, cudaStream_t st
     dn.out_f32 = 1;
     if (height == 16) e = products_few<16>(m, gu, dn, groups, sm_count, st);
     else if (height == 32) e = products_few<32>(m, gu, dn, groups, sm_count, st);
-    else if (height == 64) e = products_few<64>(m, gu, dn, groups, sm_count, st);
     else {
         e = Many<kF8GateUp, 256>::run(m[0], m[1], gu, groups * gu.nt, sm_count, st);
         dn.nt = (a.H + 255) / 256;

@@ -8,11 +8,13 @@
 // applied that way in fp32 (the scaled MMA forms take powers of two only).
 //
 // Two forms, by the number of token rows:
-//   few rows   P = 128 weight rows (lanes), Q = 16..64 token rows: each weight byte is loaded once, by
+//   few rows   P = 128 weight rows (lanes), Q = 16, 32 or 64 token rows: each weight byte is loaded once, by
 //              TMA straight to the tensor core's shared memory, whatever the number of tokens.  A cluster
 //              of CTAs splits the inner dimension and adds its partial sums, in order, through distributed
 //              shared memory: enough loads are in flight with few tiles, and no sum depends on timing.
-//   many rows  P = 128 token rows, Q = 256 (or 128) weight rows, one persistent CTA an SM.
+//   many rows  P = 128 token rows, Q = 256 (or 128) weight rows, one persistent CTA an SM.  A block of the 128 x
+//              256 tile writes 48 KB and reads 48 KB of shared memory, 768 cycles where its MMAs take 512; the
+//              hand-overs between MMAs and epilogue (two accumulators fill tensor memory) make it about 1000.
 //
 // Roles: one warp issues the TMA loads of a ring of stages (a block of both operands each), one thread
 // issues the MMAs, the other warps are the epilogue.  All waits are bounded; after one that gave up, the
@@ -45,6 +47,7 @@ struct F8Gemm {
     float* as;               //   and their scales [slots, nb]
     uint32_t* err;
     uint64_t timeout_ns;
+    int inject;              // test hook: 1 makes the waits for finished accumulators run out
 };
 
 // Bounded wait of all lanes (or of one thread).  The limit is counted in SM cycles (reading the global timer
@@ -235,10 +238,9 @@ template <int MODE, int NQ>
 struct FewCfg {
     static constexpr int WB = MODE == kF8GateUp ? 2 : 1;  // weight tiles a stage: gate and up, or one
     static constexpr int kStage = WB * 16384 + NQ * 128;
-    // two CTAs an SM; one where 64 rows of gate and up sums fill the registers
-    static constexpr int kMinCtas = NQ == 64 && WB == 2 ? 1 : 2;
+    static constexpr int kMinCtas = 2;  // an SM
     static constexpr int kRed = WB * NQ * 128 * 4;  // the sums on their way to the CTA that finishes them
-    static constexpr int kBudget = (kMinCtas == 2 ? 112 : 224) * 1024 - 2048 - (kFewScales) * NQ * 4;
+    static constexpr int kBudget = 112 * 1024 - 2048 - (kFewScales) * NQ * 4;
     static constexpr int kStages = (kBudget - kRed) / kStage > 8 ? 8 : (kBudget - kRed) / kStage;
     static constexpr int kTmemCols = 2 * WB * NQ < 32 ? 32 : 2 * WB * NQ;
     static constexpr int kSmem = kStages * kStage + kRed + 1024;  // 1 KB: alignment of the ring
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
     if (warp == 4 && lane == 0) prefetch_map(&map_w), prefetch_map(&map_x);
     if (tid == 0) {
         for (int s = 0; s < S; s++) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
-        for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1), mbar_init(&c.dempty[b], 4);
+        for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1 + a.inject), mbar_init(&c.dempty[b], 4);
         mbar_init(&c.red_full, 4 * CS);
         mbar_init(&c.red_free, 4 * CS);
         mbar_init(&c.done, 1);
@@ -646,7 +648,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (warp == kManyEpi && lane == 0) prefetch_map(&map_w), prefetch_map(&map_x);
     if (tid == 0) {
         for (int s = 0; s < S; s++) mbar_init(&c.full[s], 1), mbar_init(&c.empty[s], 1);
-        for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1), mbar_init(&c.dempty[b], kManyEpi);
+        for (int b = 0; b < 2; b++) mbar_init(&c.dfull[b], 1 + a.inject), mbar_init(&c.dempty[b], kManyEpi);
         mbar_init(&c.done, 1);
         scales_init(c.sc, kManyEpi);
         c.abort = 0;

@@ -1592,7 +1592,8 @@ int moe_matmul_fp8(moe_ctx* c, int64_t M, int64_t N, int64_t K, const uint8_t* x
     if (M && N) {
         if (!x || !x_scale || !w || !w_scale || !out) return fail(MOE_EINVAL, "null operand");
         if (!aligned16(x) || !aligned16(w) || !aligned16(out)) return fail(MOE_EINVAL, "x, w and out must be 16-byte aligned");
-        MatmulF8 a{x, x_scale, w, w_scale, M, N, (int)K, out, out_dtype == MOE_DT_F32, c->d_err, c->timeout_ns};
+        MatmulF8 a{x, x_scale, w, w_scale, M, N, (int)K, out, out_dtype == MOE_DT_F32, c->d_err, c->timeout_ns,
+                   c->inject_timeout};
         CUDA_TRY(launch_matmul_fp8(a, c->sm_count, st));
         c->launches++;
     }
@@ -1623,7 +1624,7 @@ int moe_experts_fp8(moe_ctx* c, int T, const uint16_t* x, const uint8_t* gate_up
         if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
         ExpertsF8 a{x, gate_up, gate_up_scale, down, down_scale, topk_idx, topk_w, T, c->cfg.hidden, c->cfg.inter,
                     c->cfg.n_experts, c->cfg.top_k, out, out_dtype == MOE_DT_F32, (flags & MOE_F_ACCUMULATE) != 0, workspace,
-                    c->d_err, c->timeout_ns};
+                    c->d_err, c->timeout_ns, c->inject_timeout};
         int n = 0;
         CUDA_TRY(launch_experts_fp8(a, c->sm_count, st, &n));
         c->launches += n;

@@ -380,3 +380,158 @@ def test_calls_leave_the_current_device_and_do_not_wait(planes):
     n = p.launch_count
     p.quantize_fp8(torch.ones(2, 32, device="cuda"))
     assert torch.cuda.current_device() == before and p.launch_count == n + 1
+
+
+# ---------------------------------------------------------------- sizes at which another kernel takes over
+
+@pytest.mark.parametrize("M,K", [(8, 512), (8, 640), (9, 1280), (9, 1296), (16, 1408), (17, 2048), (17, 2064), (32, 2176), (33, 4096),
+                                 (33, 4112), (64, 4096), (64, 4224), (65, 4224)])
+def test_matmul_either_side_of_a_change_of_kernel(planes, M, K):
+    product(planes(), M, 385, K, torch.float32, M + K)
+
+
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(2049, 1921, 16), (2049, 1922, 144), (2048, 2560, 272), (1025, 6148, 400), (1, 65537, 48), (5000, 24, 160)])
+def test_matmul_of_many_tiles_and_few_blocks(planes, M, N, K, out_dtype):
+    """Rows of every alignment, tiles of either width, one to four blocks a tile and more tiles than SMs."""
+    product(planes(), M, N, K, out_dtype, N + K)
+
+
+@pytest.mark.parametrize("M", [3, 12, 40, 100])
+def test_nan_and_infinity_stay_what_they_are_in_bf16(planes, M):
+    from npu_offload_b200 import Fp8
+    p, g = planes(), gen(M)
+    x = p.quantize_fp8(randn(g, M, 256))
+    w = weight(g, 136, 256)
+    bad = x.q.clone()
+    bad.view(torch.uint8)[1] = 0x7f
+    scale = x.scale.clone()
+    scale[2] = 3e38  # products beyond the largest bf16
+    out = p.matmul_fp8(Fp8(bad, scale), Fp8(*w))
+    assert out[1].isnan().all()
+    # a block's sum beyond the largest number: the result is not finite; of one sign, it is that infinity (of both,
+    # the infinity of the one added first or NaN, as the second is added by a fused operation or a plain one)
+    blocks = [matmul64(bad[:, k:k + 128], scale[:, k // 128:k // 128 + 1], w[0][:, k:k + 128], w[1][:, k // 128:k // 128 + 1])[0][2]
+              for k in (0, 128)]
+    far = [b.abs() >= (2 - 2.0 ** -24) * 2.0 ** 127 for b in blocks]  # what rounds beyond the largest number
+    assert far[0].any() and far[1].any()
+    sums = sum(torch.where(f, b.sign() * float("inf"), 0.0) for f, b in zip(far, blocks))
+    over = far[0] | far[1]
+    assert not out[2][over].isfinite().any()
+    assert torch.equal(out[2][sums.isinf()].double(), sums[sums.isinf()])
+    assert torch.equal(out[0], p.matmul_fp8(x, Fp8(*w))[0])
+
+
+@pytest.mark.parametrize("T,H,F,E,K", [(520, 128, 64, 8, 2), (300, 128, 128, 128, 8), (1100, 64, 64, 60, 1), (129, 64, 64, 3, 8 // 4),
+                                       (2049, 64, 64, 1, 1), (1024, 64, 64, 256, 1), (1025, 64, 64, 256, 1)])
+def test_experts_of_many_pairs(planes, T, H, F, E, K):
+    """More pairs than one CTA groups, experts with many groups of rows and with none."""
+    check_experts(planes(H, F, E, K), *expert_case(T + E, T, H, F, E, K))
+
+
+def test_experts_of_many_pairs_with_choices_left_out(planes):
+    from npu_offload_b200._lib import MOE_EINVAL
+    from npu_offload_b200 import Fp8
+    p = planes(64, 64, 8, 4)
+    x, gu, d, idx, w = expert_case(3, 500, 64, 64, 8, 4)
+    g = gen(12)
+    idx[torch.rand(500, 4, generator=g, device="cuda") < 0.4] = -1
+    idx[100:140] = -1
+    out = check_experts(p, x, gu, d, idx, w)
+    assert bool((out[100:140] == 0).all())
+    bad = idx.clone()
+    bad[7, 1] = 8
+    assert torch.equal(p.experts_fp8(x, Fp8(*gu), Fp8(*d), bad, w)[8:], out[8:]) and p.status() == MOE_EINVAL
+    idx[:] = -1
+    assert bool((check_experts(p, x, gu, d, idx, w) == 0).all())
+
+
+# ---------------------------------------------------------------- order, waits
+
+def test_results_follow_the_order_of_the_stream(planes):
+    """Kernels are launched ahead of the end of the ones before them: inputs written just before a call, and
+    overwritten just after it, are the call's own; so are weights, results and working memory taken over."""
+    from npu_offload_b200 import Fp8
+    p, g = planes(512, 256, 16, 4), gen(21)
+    for T in (2, 30, 300):
+        cases = [expert_case(900 + i, T, 512, 256, 16, 4) for i in range(3)]
+        want = [p.experts_fp8(x, Fp8(*gu), Fp8(*d), idx, w) for x, gu, d, idx, w in cases]
+        torch.cuda.synchronize()
+        buf = [[t.clone() if isinstance(t, torch.Tensor) else [u.clone() for u in t] for t in c] for c in cases[:1]][0]
+        got = []
+        for _ in range(4):
+            for c in cases:
+                for dst, src in zip(buf, c):
+                    for a, b in zip(*(([dst], [src]) if isinstance(dst, torch.Tensor) else (dst, src))):
+                        a.view(torch.uint8).copy_(b.view(torch.uint8)) if a.dtype == F8 else a.copy_(b)
+                got.append(p.experts_fp8(buf[0], Fp8(*buf[1]), Fp8(*buf[2]), buf[3], buf[4]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(got))
+    xs = [randn(g, 40, 2048) for _ in range(3)]
+    w = Fp8(*weight(g, 300, 2048))
+    want = [p.matmul_fp8(x, w) for x in xs]
+    buf, got = torch.empty_like(xs[0]), []
+    for i in range(12):
+        buf.copy_(xs[i % 3])
+        got.append(p.matmul_fp8(buf, w))
+    assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(got))
+
+
+def test_a_wait_that_runs_out_is_reported_and_the_context_stays_usable():
+    """The test hook makes the kernels wait for an arrival that nothing makes: they give up and return."""
+    from npu_offload_b200 import Fp8, MoEDataPlane
+    from npu_offload_b200._lib import MOE_ETIMEOUT, MOE_OK, MOE_OPT_INJECT_WAIT_TIMEOUT, MOE_OPT_WAIT_TIMEOUT_US
+    g = gen(5)
+    with MoEDataPlane(512, 256, 8, 2, n_layers=1, max_tokens=16) as p:
+        p.set_option(MOE_OPT_WAIT_TIMEOUT_US, 2000)
+        w = Fp8(*weight(g, 1500, 2048))
+        xs = [p.quantize_fp8(randn(g, M, 2048)) for M in (1, 20, 40, 300)]
+        calls = [lambda x=x: p.matmul_fp8(x, w) for x in xs]
+        for T in (2, 20, 400):
+            x, gu, d, idx, ws = expert_case(T, T, 512, 256, 8, 2)
+            calls.append(lambda a=(x, Fp8(*gu), Fp8(*d), idx, ws): p.experts_fp8(*a))
+        want = [c() for c in calls]
+        assert p.status() == MOE_OK
+        for c, v in zip(calls, want):
+            p.set_option(MOE_OPT_INJECT_WAIT_TIMEOUT, 1)
+            c()
+            assert p.status() == MOE_ETIMEOUT
+            p.set_option(MOE_OPT_INJECT_WAIT_TIMEOUT, 0)
+            assert torch.equal(c(), v) and p.status() == MOE_OK
+
+
+def test_a_closed_plane_refuses():
+    from npu_offload_b200 import MoEDataPlane
+    from npu_offload_b200._lib import MoEError
+    p = MoEDataPlane(256, 64, 8, 2, n_layers=1, max_tokens=16)
+    x = torch.zeros(2, 32, device="cuda")
+    p.quantize_fp8(x)
+    p.close()
+    with pytest.raises(MoEError, match="null context"):
+        p.quantize_fp8(x)
+
+
+def test_calls_of_several_threads(planes):
+    """Calls that share a plane, each thread on a stream of its own."""
+    import threading
+    from npu_offload_b200 import Fp8
+    p = planes(512, 256, 16, 4)
+    cases = [expert_case(40 + i, 3 + 90 * i, 512, 256, 16, 4) for i in range(3)]
+    args = [(x, Fp8(*gu), Fp8(*d), idx, w) for x, gu, d, idx, w in cases]
+    want = [p.experts_fp8(*a) for a in args]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        s = torch.cuda.Stream()
+        for _ in range(20):
+            o = p.experts_fp8(*args[i], stream=s)
+            s.synchronize()
+            if not torch.equal(o, want[i]):
+                bad.append(i)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert not bad and p.status() == 0
