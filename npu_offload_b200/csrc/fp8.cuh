@@ -5,12 +5,13 @@
 
 namespace moe {
 
-// Bits of the largest finite |f| of eight values (0 if there is none).
-__device__ __forceinline__ uint32_t f8_top(const float (&f)[8]) {
+// Bits of the largest finite |f| of eight values (0 if there is none); special: an infinity or NaN is among them.
+__device__ __forceinline__ uint32_t f8_top(const float (&f)[8], bool& special) {
     uint32_t top = 0;
 #pragma unroll
     for (int k = 0; k < 8; k++) top = max(top, __float_as_uint(f[k]) & 0x7fffffffu);
-    if (top >= 0x7f800000u) {  // an infinity or NaN among them
+    special = top >= 0x7f800000u;
+    if (special) {
         top = 0;
 #pragma unroll
         for (int k = 0; k < 8; k++) {
@@ -19,6 +20,23 @@ __device__ __forceinline__ uint32_t f8_top(const float (&f)[8]) {
         }
     }
     return top;
+}
+// The same of eight bf16 values, two at a time.
+__device__ __forceinline__ uint32_t f8_top(uint4 v, bool& special) {
+    const uint32_t w[4] = {v.x & 0x7fff7fffu, v.y & 0x7fff7fffu, v.z & 0x7fff7fffu, v.w & 0x7fff7fffu};
+    const uint32_t m = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
+    uint32_t top = max(m >> 16, m & 0xffffu);
+    special = top >= 0x7f80u;
+    if (special) {
+        top = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t lo = w[k] & 0xffffu, hi = w[k] >> 16;
+            if (lo < 0x7f80u) top = max(top, lo);
+            if (hi < 0x7f80u) top = max(top, hi);
+        }
+    }
+    return top << 16;
 }
 
 // Biased exponent of the smallest power of two s >= 2^-126 with the value of bits `top` <= 448 s
@@ -36,17 +54,17 @@ __device__ __forceinline__ uint32_t f8_pack2(float lo, float hi) {
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// x * inv rounded to e4m3; an infinity becomes NaN instead of saturating.
-__device__ __forceinline__ uint2 f8_pack8(const float (&f)[8], float inv) {
+// x * inv rounded to e4m3; where `special`, an infinity becomes NaN instead of saturating.
+__device__ __forceinline__ uint2 f8_pack8(const float (&f)[8], float inv, bool special) {
     float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
-        v[k] = f[k] * inv;
-        if (fabsf(v[k]) == __int_as_float(0x7f800000)) v[k] = __int_as_float(0x7fffffff);
-    }
+    for (int k = 0; k < 8; k++) v[k] = f[k] * inv;
+    if (special)
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (fabsf(v[k]) == __int_as_float(0x7f800000)) v[k] = __int_as_float(0x7fffffff);
     return make_uint2(f8_pack2(v[0], v[1]) | f8_pack2(v[2], v[3]) << 16, f8_pack2(v[4], v[5]) | f8_pack2(v[6], v[7]) << 16);
 }
-
 __device__ __forceinline__ uint32_t f8_pack1(float f, float inv) {
     float v = f * inv;
     if (fabsf(v) == __int_as_float(0x7f800000)) v = __int_as_float(0x7fffffff);

@@ -106,7 +106,7 @@ cudaError_t launch_matmul_fp8(const MatmulF8& m, int sm_count, cudaStream_t st) 
     // 2048 x 2560 x 4096 (320 or 160 tiles): 46 or 53 us; 1024 x 2560 x 4096 (160 or 80): 28 or 24 us.
     const int64_t mt = (m.M + 127) / 128, wide = (m.N + 255) / 256;
     const auto rounds = [&](int64_t tiles) { return (tiles + sm_count - 1) / sm_count; };
-    if (4 * rounds(mt * g.nb) <= 7 * rounds(mt * wide)) return Many<kF8Dense, 128>::run(mw, mx, g, mt * g.nb, sm_count, st);
+    if (4 * rounds(mt * g.nb) < 7 * rounds(mt * wide)) return Many<kF8Dense, 128>::run(mw, mx, g, mt * g.nb, sm_count, st);
     g.nt = (int)wide;
     return Many<kF8Dense, 256>::run(mw, mx, g, mt * wide, sm_count, st);
 }
@@ -178,11 +178,12 @@ __device__ __forceinline__ void prep_rows(const PrepArgs& a, PrepLoad l, const i
         const uint4 w = l.v;
         l.v = prep_load(a, l, g + l.stride);
         const float f[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
-        uint32_t top = f8_top(f);
+        bool special;
+        uint32_t top = f8_top(w, special);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const uint32_t se = f8_scale_exp(top);
-        const uint2 q = f8_pack8(f, f8_inverse(se));
+        const uint2 q = f8_pack8(f, f8_inverse(se), special);
         if (g < l.groups)
             for (int k = 0; k < a.K; k++) {
                 const int s = slots[row * a.K + k];
@@ -271,11 +272,12 @@ __global__ void __launch_bounds__(kTinyThreads) f8_prep_tiny_kernel(PrepArgs a) 
         if (lane == 0) *a.n_groups = n;
     }
     const float f[8] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y), bf_lo(w.z), bf_hi(w.z), bf_lo(w.w), bf_hi(w.w)};
-    uint32_t top = f8_top(f);
+    bool special;
+    uint32_t top = f8_top(w, special);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
     const uint32_t se = f8_scale_exp(top);
-    const uint2 q = f8_pack8(f, f8_inverse(se));
+    const uint2 q = f8_pack8(f, f8_inverse(se), special);
     for (int k = 0; k < a.K; k++) {
         const int p = min((int)(row * a.K) + k, 31);  // rows behind the last token store nothing
         const int s = __shfl_sync(0xffffffffu, ok ? slot : -1, p);

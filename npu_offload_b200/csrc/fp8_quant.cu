@@ -34,6 +34,7 @@ struct Eight<false> {
 #pragma unroll
         for (int k = 0; k < 4; k++) f[2 * k] = bf_lo(w[k]), f[2 * k + 1] = bf_hi(w[k]);
     }
+    __device__ __forceinline__ uint32_t top(bool& special) const { return f8_top(v, special); }
 };
 template <>
 struct Eight<true> {
@@ -47,6 +48,11 @@ struct Eight<true> {
         const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int k = 0; k < 8; k++) f[k] = __uint_as_float(w[k]);
+    }
+    __device__ __forceinline__ uint32_t top(bool& special) const {
+        float f[8];
+        get(f);
+        return f8_top(f, special);
     }
 };
 
@@ -72,12 +78,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
 #pragma unroll
     for (int n = 0; n < N; n++) {
         float f[8];
+        bool special;
         v[n].get(f);
-        uint32_t top = f8_top(f);
+        uint32_t top = v[n].top(special);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         const uint32_t se = f8_scale_exp(top);
-        const uint2 r = f8_pack8(f, f8_inverse(se));
+        const uint2 r = f8_pack8(f, f8_inverse(se), special);
         if (in[n]) *reinterpret_cast<uint2*>(q + at[n]) = r;
         const uint32_t g = g0 + n * 16;
         if (sub == 0 && g < groups) s[g] = __uint_as_float(se << 23);
@@ -103,11 +110,12 @@ __global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const
         else v[i].zero();
     }
     uint32_t top = 0;
+    bool special = false;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        float f[8];
-        v[i].get(f);
-        top = max(top, f8_top(f));
+        bool s8;
+        top = max(top, v[i].top(s8));
+        special |= s8;
     }
     top = __reduce_max_sync(0xffffffffu, top);
     if ((threadIdx.x & 31) == 0) top_s[threadIdx.x >> 5] = top;
@@ -121,7 +129,7 @@ __global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const
         const uint32_t r = r0 + (threadIdx.x >> 4) + 16 * i;
         float f[8];
         v[i].get(f);
-        if (r < rows && c < cols) *reinterpret_cast<uint2*>(q + base + (size_t)r * cols + c) = f8_pack8(f, inv);
+        if (r < rows && c < cols) *reinterpret_cast<uint2*>(q + base + (size_t)r * cols + c) = f8_pack8(f, inv, special);
     }
     if (threadIdx.x == 0) s[blockIdx.x] = __uint_as_float(se << 23);
 }

@@ -823,8 +823,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (live && f0 < a.N) {  // F is a multiple of 64
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const uint2 lo = f8_pack8(reinterpret_cast<const float(&)[8]>(acc[0][16 * j]), inv);
-                        const uint2 hi = f8_pack8(reinterpret_cast<const float(&)[8]>(acc[0][16 * j + 8]), inv);
+                        const uint2 lo = f8_pack8(reinterpret_cast<const float(&)[8]>(acc[0][16 * j]), inv, true);
+                        const uint2 hi = f8_pack8(reinterpret_cast<const float(&)[8]>(acc[0][16 * j + 8]), inv, true);
                         reinterpret_cast<uint4*>(a.aq + slot * a.N + f0)[j] = make_uint4(lo.x, lo.y, hi.x, hi.y);
                     }
                 }
