@@ -498,13 +498,14 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
 #pragma unroll
                             for (int h = 0; h < WB; h++) v[u][h] += j + u < mine ? red[((r * per + j + u) * WB + h) * 128 + tid] : 0.f;
 #pragma unroll
-                    for (int u = 0; u < U; u++) {  // columns behind the last are of no use and harmless
-                        v[u][0] = swiglu_f32(v[u][0], v[u][WB - 1]);
-                        if (j + u < mine) red[(j + u) * WB * 128 + tid] = v[u][0];
-                        uint32_t t = __float_as_uint(v[u][0]) & 0x7fffffffu;
-                        t = __reduce_max_sync(0xffffffffu, t < 0x7f800000u ? t : 0u);
-                        if (lane == 0 && j + u < mine) c.top[warp][j + u] = t;
-                    }
+                    for (int u = 0; u < U; u++)
+                        if (j + u < mine) {
+                            const float act = swiglu_f32(v[u][0], v[u][WB - 1]);
+                            red[(j + u) * WB * 128 + tid] = act;
+                            uint32_t t = __float_as_uint(act) & 0x7fffffffu;
+                            t = __reduce_max_sync(0xffffffffu, t < 0x7f800000u ? t : 0u);
+                            if (lane == 0) c.top[warp][j + u] = t;
+                        }
                 }
                 named_bar_sync(1, 128);
 #pragma unroll 1
