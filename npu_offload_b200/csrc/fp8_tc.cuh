@@ -240,11 +240,11 @@ struct FewCfg {
     static constexpr int kStage = WB * 16384 + NQ * 128;
     static constexpr int kMinCtas = 2;  // an SM
     static constexpr int kRed = WB * NQ * 128 * 4;  // the sums on their way to the CTA that finishes them
-    static constexpr int kBudget = 112 * 1024 - 2048 - (kFewScales) * NQ * 4;
+    static constexpr int kBudget = 112 * 1024 - 2048 - kFewScales * NQ * 4;
     static constexpr int kStages = (kBudget - kRed) / kStage > 8 ? 8 : (kBudget - kRed) / kStage;
     static constexpr int kTmemCols = 2 * WB * NQ < 32 ? 32 : 2 * WB * NQ;
     static constexpr int kSmem = kStages * kStage + kRed + 1024;  // 1 KB: alignment of the ring
-    static_assert(kStages >= 2 && kSmem + 1024 + (kFewScales) * NQ * 4 <= 227 * 1024 / kMinCtas, "stages");
+    static_assert(kStages >= 2 && kSmem + 1024 + kFewScales * NQ * 4 <= 227 * 1024 / kMinCtas, "stages");
 };
 
 constexpr int kFewChunk = 4, kFewSlots = 3;
@@ -356,6 +356,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
                     const int s = g % S, b = g & 1;
                     if (g >= 2) ok = f8_wait(&c.dempty[b], ((g >> 1) & 1) ^ 1, &c.abort, a);
                     ok = ok && f8_wait(&c.full[s], (g / S) & 1, &c.abort, a);
+                    ok = __all_sync(0xffffffffu, ok);  // the warp leaves its loop as a whole
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t dw = desc0 + (uint64_t)(s * (C::kStage >> 4)), dx = dw + WB * 1024;
@@ -709,6 +710,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const int s = g % S, b = ph & 1, p = kb % KP;
                     ok = f8_wait(&c.full[s], (g / S) & 1, &c.abort, a);
                     if (p == 0 && ph >= 2) ok = ok && f8_wait(&c.dempty[b], ((ph >> 1) & 1) ^ 1, &c.abort, a);
+                    ok = __all_sync(0xffffffffu, ok);  // the warp leaves its loop as a whole
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t dx = desc0 + (uint64_t)(s * (C::kStage >> 4)), dw = dx + 1024;

@@ -173,3 +173,31 @@ def test_views_streams_and_graphs(planes):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(l3, loss) and torch.equal(d3, d) and torch.equal(st3.counts, st.counts)
+
+
+def test_inside_an_autograd_function(planes):
+    """The explicit pair of calls as a training program wraps it: the gradient reaches the logits' producer."""
+    p = planes(8, 2, "softmax")
+
+    class Balance(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, logits, idx):
+            loss, ctx.stats = p.balance_loss(logits.detach(), idx)
+            ctx.save_for_backward(logits)
+            return loss
+
+        @staticmethod
+        def backward(ctx, grad):
+            (logits,) = ctx.saved_tensors
+            return p.balance_loss_backward(logits.detach(), ctx.stats, grad.contiguous()), None
+
+    g = gen(4)
+    x, w = torch.randn(20, 16, generator=g, device="cuda"), torch.randn(16, 8, generator=g, device="cuda", requires_grad=True)
+    idx = (x @ w).topk(2, -1)[1].int()
+    (0.5 * Balance.apply(x @ w, idx)).backward()
+    logits = (x @ w).detach()
+    d = balance64(logits, idx, None, None, "softmax", 0.5)[2]
+    want = x.double().T @ d
+    # the kernel's gradient, off by less than 200 half steps of its rows' largest, through a product of 20 terms in fp32
+    lim = (200 + 40) * EPS * (x.double().abs().T @ d.abs().amax(-1, keepdim=True).expand_as(d)) + 1e-12
+    assert bool(((w.grad.double() - want).abs() <= lim).all())
