@@ -2,7 +2,6 @@
 import pytest
 import torch
 
-from tests.conftest import has_gpu
 from tests.fp8_util import EPS, F8, ceil128, experts64, expand, matmul64, matmul_bound, quantize64, weight
 
 pytestmark = pytest.mark.gpu
