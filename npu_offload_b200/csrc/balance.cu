@@ -235,7 +235,6 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThread
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = (int)cl.block_rank(), E = a.E;
     const int e = r * 32 + lane, clusters = gridDim.x / kBalCluster;
-    griddep_launch_dependents();
     griddep_wait();
     for (int b = blockIdx.x / kBalCluster; b < a.B; b += clusters) {
         int first, last;
@@ -309,7 +308,6 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThread
 // A warp a row; rows of a warp are neighbours, so that it keeps its sequence's f in registers.
 template <int NE, bool SIG, bool V, bool FULL>
 __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceArgs a, int per_warp) {
-    griddep_launch_dependents();
     griddep_wait();
     const int E = a.E;
     const long t0 = ((long)blockIdx.x * kBalWarps + (threadIdx.x >> 5)) * per_warp;

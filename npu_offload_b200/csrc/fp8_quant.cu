@@ -61,8 +61,8 @@ struct Eight<true> {
 template <bool F32, int N>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, uint32_t groups, uint32_t per_row,
                                                             uint32_t cols, uint8_t* __restrict__ q, float* __restrict__ s) {
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const uint32_t sub = threadIdx.x & 15, g0 = blockIdx.x * 16 * N + (threadIdx.x >> 4);
     Eight<F32> v[N];
     size_t at[N];
@@ -97,8 +97,8 @@ __global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const
                                                               uint32_t rb, uint32_t cb, uint8_t* __restrict__ q,
                                                               float* __restrict__ s) {
     __shared__ uint32_t top_s[8];
-    griddep_launch_dependents();
     griddep_wait();
+    griddep_launch_dependents();
     const uint32_t b = blockIdx.x / cb, kb = blockIdx.x - b * cb, mat = b / rb, r0 = (b - mat * rb) * kF8Block;
     const uint32_t c = kb * kF8Block + (threadIdx.x & 15) * 8;
     const size_t base = (size_t)mat * rows * cols;

@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
     // groups are there: it may read them, and the weights, before it waits for the activations.
     if (MODE == kF8Down) griddep_launch_dependents();
     if (MODE != kF8Down || warp != 4) griddep_wait();
-    if (MODE != kF8Down) griddep_launch_dependents();
+    if (MODE == kF8GateUp) griddep_launch_dependents();
     const int items = f8_groups<MODE>(a, NQ) * a.nt;
 
     if (warp == 4) {
@@ -662,7 +662,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     tc_fence_after();
     const uint32_t tmem = c.tmem;
     griddep_wait();
-    griddep_launch_dependents();
+    if (MODE != kF8Dense) griddep_launch_dependents();
     const int groups = f8_groups<MODE>(a, 128), items = groups * a.nt, nkb = a.nkb;
 
     if (warp == kManyEpi) {

@@ -3,6 +3,9 @@
 // before it, in all its CTAs, ahead of its first access to memory that anything else in the stream may write
 // or read; so what it follows, and what follows it, see the order of the stream.  Launched one after the
 // other, a product's set-up (barriers, tensor memory, tensor maps) is off the critical path.
+// The last kernel of a call does not let the next kernel start before its end: the planner and the decode kernel
+// read router logits ahead of their wait, and a product or a sum may have written them.  The quantiser, whose
+// outputs no kernel reads ahead of its wait, lets the next one start once its own wait is over.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -476,6 +476,49 @@ def test_results_follow_the_order_of_the_stream(planes):
     assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(got))
 
 
+@pytest.mark.parametrize("between", ["nothing", "quantiser", "balance"])
+def test_logits_of_a_product_reach_the_layer_behind_it(between):
+    """The layer's planner reads its router logits early: a product that writes them, and whatever is
+    called between the two, must have let it start no sooner than the logits are there."""
+    from npu_offload_b200 import MoEDataPlane
+    H, F, E, K, T, KR = 512, 256, 64, 4, 2, 16384
+    p, g = MoEDataPlane(H, F, E, K, n_layers=1, max_tokens=16), gen(91)
+    try:
+        for e in range(E):
+            p.load_expert(0, e, *((randn(g, *sh) * 0.05).to(torch.bfloat16) for sh in ((F, H), (F, H), (H, F))))
+        x = randn(g, T, H).to(torch.bfloat16)
+        router = p.quantize_fp8(randn(g, E, KR) * KR ** -0.5, block_rows=128)
+        feats = [p.quantize_fp8(randn(g, T, KR)) for _ in range(6)]
+        side, logits = randn(g, 64, 4096), torch.zeros(T, E, device="cuda")
+        side_logits = randn(g, 4096, E)
+        side_idx = side_logits.topk(K).indices.to(torch.int32)
+
+        def step(f, sync):
+            p.matmul_fp8(f, router, out=logits)
+            if sync:
+                torch.cuda.synchronize()
+            if between == "quantiser":
+                p.quantize_fp8(side)
+            elif between == "balance":
+                p.balance_loss(side_logits, side_idx)
+            if sync:
+                torch.cuda.synchronize()
+            return p.forward(0, x, logits)
+
+        want = [step(f, True) for f in feats]
+        torch.cuda.synchronize()
+        assert not torch.equal(want[0], want[1])
+        got = [step(f, False) for f in feats * 20]
+        torch.cuda.synchronize()
+        # the plan may cut the sums elsewhere behind a running call: the same experts, not the same order of sums
+        for i, o in enumerate(got):
+            v = want[i % len(feats)]
+            assert float((o - v).abs().max()) <= 1e-4 * float(v.abs().max())
+        assert p.status() == 0
+    finally:
+        p.close()
+
+
 def test_a_wait_that_runs_out_is_reported_and_the_context_stays_usable():
     """The test hook makes the kernels wait for an arrival that nothing makes: they give up and return."""
     from npu_offload_b200 import Fp8, MoEDataPlane
