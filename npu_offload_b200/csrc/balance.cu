@@ -236,6 +236,7 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThread
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = (int)cl.block_rank(), E = a.E;
     const int e = r * 32 + lane, clusters = gridDim.x / kBalCluster;
     griddep_wait();
+    griddep_launch_dependents();
     for (int b = blockIdx.x / kBalCluster; b < a.B; b += clusters) {
         int first, last;
         sequence(a.offsets, b, a.T, first, last);

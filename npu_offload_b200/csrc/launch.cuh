@@ -4,8 +4,8 @@
 // or read; so what it follows, and what follows it, see the order of the stream.  Launched one after the
 // other, a product's set-up (barriers, tensor memory, tensor maps) is off the critical path.
 // The last kernel of a call does not let the next kernel start before its end: the planner and the decode kernel
-// read router logits ahead of their wait, and a product or a sum may have written them.  The quantiser, whose
-// outputs no kernel reads ahead of its wait, lets the next one start once its own wait is over.
+// read router logits ahead of their wait, and a product may have written them.  The quantiser and the loss, whose
+// outputs no kernel reads ahead of its wait, let the next one start once their own wait is over.
 #pragma once
 #include <cuda_runtime.h>
 
