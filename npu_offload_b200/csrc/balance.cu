@@ -235,6 +235,9 @@ __global__ void __cluster_dims__(kBalCluster, 1, 1) __launch_bounds__(kSumThread
     cg::cluster_group cl = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, r = (int)cl.block_rank(), E = a.E;
     const int e = r * 32 + lane, clusters = gridDim.x / kBalCluster;
+    // A CTA's shared memory may be written once that CTA runs, and the first store to CTA 0's is ahead of the loop's own
+    // barriers; met here, behind the kernel before this one, it costs nothing.
+    cl.sync();
     griddep_wait();
     griddep_launch_dependents();
     for (int b = blockIdx.x / kBalCluster; b < a.B; b += clusters) {
