@@ -426,6 +426,8 @@ class MoEDataPlane:
             raise ValueError(f"logits are {tuple(lg.shape)}, the context has {self.E} experts")
         T = lg.shape[0]
         b = None if bias is None else _as(bias, torch.float32, self.device)
+        if b is not None and b.numel() != self.E:
+            raise ValueError(f"bias is {tuple(b.shape)}, the context has {self.E} experts")
         idx = torch.empty(T, self.K, dtype=torch.int32, device=self.device)
         w = torch.empty(T, self.K, dtype=torch.float32, device=self.device)
         pairs = max(1, T * self.K)
