@@ -149,10 +149,17 @@ MOE_API int moe_forward_layers(moe_ctx* ctx, int n, const int32_t* layers, int T
 /* Router + token permutation alone (device pointers unless MOE_F_HOST; bias may be NULL):
  *   topk_idx/topk_w [T,K]; counts [E]; offsets [E+1] (expert-id order); perm [T*K] pair ids
  *   t*K+k grouped by expert, tokens ascending (runtime.py:343-347); job_order [E] experts in
- *   first-appearance order (the cpu_moe job list, runtime.py:352-354); n_jobs [1]. */
+ *   first-appearance order (the cpu_moe job list, runtime.py:352-354); n_jobs [1].
+ * The sorted lists are made in the context's buffers, as a layer's are: one such call at a time. */
 MOE_API int moe_route(moe_ctx* ctx, int T, const float* router_logits, const float* bias, int32_t* topk_idx, float* topk_w,
               int32_t* counts, int32_t* offsets, int32_t* perm, int32_t* job_order, int32_t* n_jobs, int flags,
               void* stream);
+
+/* The router alone, straight into topk_idx / topk_w [T,K] (device pointers; the same numbers as moe_route's).
+ * It uses none of the context's buffers but the device-side status (MOE_F_SYNC or moe_status), so calls on several
+ * streams, and captured graphs, may overlap; T is at most 2^24, whatever max_tokens is. */
+MOE_API int moe_route_topk(moe_ctx* ctx, int64_t T, const float* router_logits, const float* bias, int32_t* topk_idx,
+                           float* topk_w, int flags, void* stream);
 
 /* cpu_moe surface (cpu_moe.cpp:38-39) with caller-owned expert weights in device memory:
  *   x [T,H] bf16; job j uses gu[j] = [2F,H] (gate rows then up rows) and d[j] = [H,F];

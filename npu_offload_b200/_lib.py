@@ -56,6 +56,7 @@ _SIGS = {
     "moe_forward": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "moe_forward_layers": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp]),
     "moe_route": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "moe_route_topk": (_i, [_vp, _i64, _vp, _vp, _vp, _vp, _i, _vp]),
     "moe_experts": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
     "moe_ck_moe3": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i, _vp]),
     "moe_ck_moe_q8w": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp]),

@@ -8,7 +8,8 @@ namespace moe {
 constexpr int kMaxExperts = 256;
 constexpr int kMaxTopK = 16;
 constexpr int kMaxTokens = 4096;
-// Limits of the e4m3 and balance-loss calls, whose working memory is the caller's.
+// Limits of the calls whose working memory is the caller's: routing alone, e4m3, balance loss.
+constexpr int kRouteTopkMaxTokens = 1 << 24;
 constexpr int kF8MaxK = 16384;             // inner size of a scaled product
 constexpr int kF8MaxRows = 1 << 24;        // its M and N
 constexpr int kF8MaxPairs = 1 << 20;       // (token, expert) pairs of an expert call

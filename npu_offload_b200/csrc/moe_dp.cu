@@ -1096,6 +1096,31 @@ int moe_route(moe_ctx* c, int T, const float* logits, const float* bias, int32_t
     return MOE_OK;
 }
 
+int moe_route_topk(moe_ctx* c, int64_t T, const float* logits, const float* bias, int32_t* topk_idx, float* topk_w, int flags,
+                   void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "moe_route_topk takes device pointers and no flag but MOE_F_SYNC");
+    if (T < 0 || T > kRouteTopkMaxTokens) return fail(MOE_EINVAL, "T=%lld not in [0,%d]", (long long)T, kRouteTopkMaxTokens);
+    if (T && (!logits || !topk_idx || !topk_w)) return fail(MOE_EINVAL, "null argument");
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T) {
+        RouteArgs a{};
+        a.logits = logits;
+        a.bias = bias;
+        a.T = (int)T;
+        a.E = c->cfg.n_experts;
+        a.K = c->cfg.top_k;
+        a.scoring = c->cfg.scoring;
+        a.idx = topk_idx;
+        a.w = topk_w;
+        a.err = c->d_err;
+        CUDA_TRY(launch_route_topk(a, st));
+        c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
 // Shared body of the explicit-job surfaces (cpu_moe, ck_moe3, ck_moe_q8w).
 static int run_jobs(moe_ctx* c, int T, const uint16_t* x, const std::vector<Job>& jobs,
                     const std::vector<int32_t>& ptok, const float* pw_src, bool pw_host, const std::vector<int32_t>& comb_off,

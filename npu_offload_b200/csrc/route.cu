@@ -345,6 +345,14 @@ cudaError_t launch_route(const RouteArgs& a, cudaStream_t st, int* launches) {
     return cudaGetLastError();
 }
 
+// A warp a token, whatever their number: the context's buffers, and the one block of route_fused_kernel, are for the
+// permutation alone.
+cudaError_t launch_route_topk(const RouteArgs& a, cudaStream_t st) {
+    if (a.T <= 0) return cudaSuccess;
+    route_topk_kernel<<<(a.T + 7) / 8, 256, 0, st>>>(a);
+    return cudaGetLastError();
+}
+
 // The router's exponential over an array (tests compare it with the CPU oracle over every float of
 // the domain the softmax sees).
 __global__ void __launch_bounds__(256) router_exp_kernel(const float* x, float* y, long long n) {

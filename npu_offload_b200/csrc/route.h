@@ -32,6 +32,8 @@ struct RouteArgs {
 constexpr size_t route_scratch_ints(int T, int E) { return (size_t)(T + 31) / 32 * E + 3 * (size_t)E; }
 
 cudaError_t launch_route(const RouteArgs& a, cudaStream_t st, int* launches);
+// idx and w alone, without the permutation: logits, bias, T, E, K, scoring, idx, w and err of `a`; any T.
+cudaError_t launch_route_topk(const RouteArgs& a, cudaStream_t st);
 cudaError_t route_set_smem_limits();
 // y[i] = router_exp(x[i]) for i < n (device pointers).
 cudaError_t launch_router_exp(const float* x, float* y, long long n, int sms, cudaStream_t st);

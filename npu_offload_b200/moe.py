@@ -380,8 +380,8 @@ class MoEDataPlane:
         return q, sc, rs
 
     # ---- 8-bit floating point: e4m3 values with one scale for each 128 ----
-    # Checks, allocation and the C calls of these methods are in _torch_binding: at one token the GPU takes a few
-    # microseconds, and Python with ctypes took longer than that.
+    # Checks, allocation and the C calls of these methods (but route_topk) are in _torch_binding: at one token the GPU
+    # takes a few microseconds, and Python with ctypes took longer than that.
     def quantize_fp8(self, x, block_rows=1, stream=None):
         """x [..., rows, cols] bf16 or fp32 -> Fp8(q, scale): one scale for each 128 columns of a row
         (block_rows=1, activations) or of 128 rows (block_rows=128, weights).  Scales are powers of two;
@@ -417,7 +417,10 @@ class MoEDataPlane:
                                   _raw_stream(self._index))
 
     def route_topk(self, logits, bias=None, stream=None):
-        """The router alone, on the device and without a wait: (idx [T, top_k] int32, w [T, top_k] fp32)."""
+        """The router alone, on the device and without a wait: (idx [T, top_k] int32, w [T, top_k] fp32).
+
+        Written straight into the results: calls on several streams or in captured graphs may overlap, and T
+        is not bound by max_tokens."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.route_topk(logits, bias)
@@ -430,11 +433,7 @@ class MoEDataPlane:
             raise ValueError(f"bias is {tuple(b.shape)}, the context has {self.E} experts")
         idx = torch.empty(T, self.K, dtype=torch.int32, device=self.device)
         w = torch.empty(T, self.K, dtype=torch.float32, device=self.device)
-        pairs = max(1, T * self.K)
-        n = torch.empty(3 * self.E + 2 + pairs, dtype=torch.int32, device=self.device)
-        counts, offsets, perm, order, jobs = n.split([self.E, self.E + 1, pairs, self.E, 1])
-        check(lib().moe_route(self._h, T, _vp(lg), _vp(b), _vp(idx), _vp(w), _vp(counts), _vp(offsets), _vp(perm), _vp(order),
-                              _vp(jobs), 0, _raw_stream(self._index)))
+        check(lib().moe_route_topk(self._h, T, _vp(lg), _vp(b), _vp(idx), _vp(w), 0, _raw_stream(self._index)))
         return idx, w
 
     # ---- the router's load-balance loss ----
