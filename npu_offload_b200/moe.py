@@ -387,7 +387,7 @@ class MoEDataPlane:
         (block_rows=1, activations) or of 128 rows (block_rows=128, weights).  Scales are powers of two;
         infinities and NaN become NaN.  cols must be a multiple of 16."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with self._on(stream):
                 return self.quantize_fp8(x, block_rows)
         p = self._plane or self._bind()
         return Fp8(*_calls.quantize_fp8(p, _tensor("x", x), block_rows, _raw_stream(self._index)))
@@ -396,7 +396,7 @@ class MoEDataPlane:
         """out [M, N] = x [M, K] . w [N, K]^T with fp32 sums.  x: Fp8 with a scale per row and 128 columns
         (or a bf16 / fp32 tensor, which is quantised first); w: Fp8 with a scale per 128 x 128 block."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with self._on(stream):
                 return self.matmul_fp8(x, w, out_dtype, out)
         if type(x) is not Fp8:
             x = self.quantize_fp8(x)
@@ -410,7 +410,7 @@ class MoEDataPlane:
         128 x 128 block; idx [T, top_k] int32 (negative: no expert) and w [T, top_k] fp32, as
         route_topk() gives them.  Tokens and SwiGLU activations are quantised per row and 128 columns."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with self._on(stream):
                 return self.experts_fp8(x, gate_up, down, idx, w, out_dtype, out, accumulate)
         p = self._plane or self._bind()
         return _calls.experts_fp8(p, x, *_fp8("gate_up", gate_up), *_fp8("down", down), idx, w, out_dtype, out, accumulate,
@@ -422,7 +422,7 @@ class MoEDataPlane:
         Written straight into the results: calls on several streams or in captured graphs may overlap, and T
         is not bound by max_tokens."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with self._on(stream):
                 return self.route_topk(logits, bias)
         lg = _as(logits, torch.float32, self.device)
         if lg.dim() != 2 or lg.shape[1] != self.E:
@@ -445,7 +445,7 @@ class MoEDataPlane:
         loss = mean over sequences of sum_e f_e P_e, f_e = E * share of the choices, P_e = mean score.
         No autograd graph is recorded: the gradient is balance_loss_backward()."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with self._on(stream):
                 return self.balance_loss(logits, idx, offsets, mask)
         p = self._plane or self._bind()
         loss, *stats = _calls.balance_loss(p, logits, idx, offsets, mask, _raw_stream(self._index))
@@ -455,10 +455,15 @@ class MoEDataPlane:
         """dlogits [T, E] fp32 = grad * d loss / d logits (grad: a device fp32 scalar; None: 1), zero for
         tokens that do not count.  logits and stats are those of balance_loss()."""
         if stream is not None:
-            with torch.cuda.stream(stream):
+            with self._on(stream):
                 return self.balance_loss_backward(logits, stats, grad, out)
         p = self._plane or self._bind()
         return _calls.balance_loss_backward(p, logits, *stats, grad, out, _raw_stream(self._index))
+
+    def _on(self, stream):
+        if stream.device != self.device:
+            raise ValueError(f"stream is on {stream.device}, the context on {self.device}")
+        return torch.cuda.stream(stream)
 
     def _bind(self):
         """What the calls of _torch_binding need of this context; dropped with it by close()."""
