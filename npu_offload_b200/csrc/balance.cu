@@ -150,15 +150,17 @@ struct Row {
 };
 
 // Scores of one token: e[k] = exp(l - max l) or sigmoid(l) of the lane's expert k (0 behind the last),
-// and 1 / their sum.
-template <int NE, bool SIG, bool V, bool FULL>
-__device__ __forceinline__ float scores(const float (&l)[NE], int E, float (&e)[NE]) {
+// and 1 / their sum.  slope (GRAD): e of the softmax, s (1 - s) of the sigmoid as x / (1 + x)^2 with x = exp(-|l|), since
+// 1 - s of a rounded s near 1 is off by 17 % at l = 15, and 0 from 17 on.
+template <int NE, bool SIG, bool V, bool FULL, bool GRAD>
+__device__ __forceinline__ float scores(const float (&l)[NE], int E, float (&e)[NE], float (&slope)[NE]) {
     float sum = 0.f;
     if (SIG) {
 #pragma unroll
         for (int k = 0; k < NE; k++) {
             const float x = exp_nonpositive(-fabsf(l[k])), q = inverse_of_1_to_2(1.f + x);
             e[k] = FULL || expert_of<V>(k) < E ? (l[k] < 0.f ? x * q : q) : 0.f;
+            if (GRAD) slope[k] = x * q * q;
             sum += e[k];
         }
         return 1.f / (warp_sum(sum) + 1e-20f);
@@ -172,6 +174,7 @@ __device__ __forceinline__ float scores(const float (&l)[NE], int E, float (&e)[
 #pragma unroll
     for (int k = 0; k < NE; k++) {
         e[k] = FULL || expert_of<V>(k) < E ? exp2_approx((l[k] - m) * kLog2e) : 0.f;
+        if (GRAD) slope[k] = e[k];
         sum += e[k];
     }
     return 1.f / warp_sum(sum);
@@ -219,10 +222,10 @@ __global__ void __launch_bounds__(kBalThreads) balance_units_kernel(BalanceArgs 
         const int x = next_x;
         ahead(t + kBalWarps);
         if (!row.counts) continue;
-        float e[NE];
+        float e[NE], none[NE];
         if (x >= E) bad = true;
         else if (x >= 0) atomicAdd(&c_s[x], 1);
-        const float r = scores<NE, SIG, V, FULL>(row.l, E, e);
+        const float r = scores<NE, SIG, V, FULL, false>(row.l, E, e, none);
 #pragma unroll
         for (int k = 0; k < NE; k++) acc[k] = fmaf(e[k], r, acc[k]);
         n++;
@@ -378,13 +381,13 @@ __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceAr
 #pragma unroll
             for (int j = 0; j < NE; j++) d[j] = 0.f;
         } else {
-            float e[NE], inner = 0.f;
-            const float r = scores<NE, SIG, V, FULL>(row.l, E, e);
+            float e[NE], slope[NE], inner = 0.f;
+            const float r = scores<NE, SIG, V, FULL, true>(row.l, E, e, slope);
 #pragma unroll
             for (int j = 0; j < NE; j++) inner = fmaf(f[j], e[j], inner);
             inner = warp_sum(inner) * r;
 #pragma unroll
-            for (int j = 0; j < NE; j++) d[j] = (SIG ? e[j] * (1.f - e[j]) : e[j]) * r * (f[j] - inner);
+            for (int j = 0; j < NE; j++) d[j] = slope[j] * r * (f[j] - inner);
         }
         float* out = a.dlogits + (size_t)t * E;
 #pragma unroll

@@ -54,3 +54,31 @@ def test_a_score_is_off_by_a_few_half_steps(plane, E):
     span = (logits.amax(-1) - logits.amin(-1)).double()
     limit = 4 + 1.25 * span + (4 + 4) + 9 if p.scoring == "softmax" else 8 + 8 + 9
     assert bool((off <= limit).all()), float((off - limit).max())
+
+
+@pytest.mark.parametrize("low,high", [(12.0, 20.0), (-20.0, 20.0), (60.0, 80.0), (-2.0, 2.0)])
+@pytest.mark.parametrize("E,K", [(128, 8), (60, 4)])
+def test_gradients_of_saturated_scores(plane, E, K, low, high):
+    """1 - s of a sigmoid near 1 is as exact as s: each gradient against its own slope p (softmax) or s (1 - s) / S.
+
+    Half steps: s 8, 1 - s 8, their product one; S 8 for its terms, 14 for the sum (8 values a lane, then 5 steps, 1e-20);
+    its inverse and the product with it one each: 41 for the slope (softmax 4 + 1.25 |d| and 1 |d| for d itself, twice, and
+    16).  f: three.  f . p: 8 and 14 for the sum, 32 for p: 54.  Their difference one.  Below
+    2^-126 numbers are 2^-149 apart: two roundings of the slope and one of the gradient, of half that each."""
+    p = plane(E, K)
+    g = torch.Generator(device="cuda").manual_seed(E)
+    logits = low + (high - low) * torch.rand(300, E, generator=g, device="cuda")
+    idx = logits.topk(K, -1)[1].int()
+    _, st = p.balance_loss(logits, idx)
+    d = p.balance_loss_backward(logits, st).double()
+    l = logits.double()
+    f = st.counts.double()[0] * E / (K * 300) / 300
+    pr = scores64(logits, p.scoring)
+    slope, far = pr, 2.25 * 2 * (l.amax(-1, keepdim=True) - l.amin(-1, keepdim=True))
+    if p.scoring == "sigmoid":
+        slope, far = torch.sigmoid(-l) * pr, 0.0
+    inner = (f * pr).sum(-1, keepdim=True)
+    limit = EPS * slope * ((42 + far) * (f - inner).abs() + 3 * f + (55 + far) * inner) + 1.5 * 2.0 ** -149
+    off = (d - slope * (f - inner)).abs()
+    assert bool((off <= limit).all()), float((off / limit).max())
+    assert p.status() == 0
