@@ -59,6 +59,12 @@ std::string name_of(at::ScalarType t) {
     }
 }
 
+// No call records an autograd graph: a gradient that one would drop in silence is refused.
+void no_gradient(const char* name, const Tensor& t) {
+    if (t.requires_grad() && at::GradMode::is_enabled())
+        refuse(name, " requires a gradient, and this call records no autograd graph: pass it detached, or call under torch.no_grad()");
+}
+
 // t as a contiguous tensor of the plane's device, at a multiple of `align` bytes; other types and ranks are refused.
 Tensor operand(const Plane& p, const char* name, Tensor t, std::initializer_list<at::ScalarType> types, int dims, int align = 1) {
     if (!t.defined() || t.device() != p.device) refuse(name, " must be a tensor on ", p.device);
@@ -66,6 +72,7 @@ Tensor operand(const Plane& p, const char* name, Tensor t, std::initializer_list
     for (at::ScalarType s : types) ok |= t.scalar_type() == s;
     if (!ok) refuse(name, " is ", name_of(t.scalar_type()), ", not ", name_of(*types.begin()));
     if (dims >= 0 && t.dim() != dims) refuse(name, " has ", t.dim(), " dimensions, not ", dims);
+    no_gradient(name, t);
     if (!t.is_contiguous()) t = t.contiguous();
     if (align > 1 && (uintptr_t)t.data_ptr() % align) t = t.clone();
     return t;
@@ -94,6 +101,7 @@ Tensor output(const Plane& p, const c10::optional<Tensor>& out, at::IntArrayRef 
     if (out->device() != p.device || (t != at::kFloat && !(bf16 && t == at::kBFloat16)) || out->sizes() != sizes || !out->is_contiguous() ||
         (uintptr_t)out->data_ptr() % 16)
         refuse("out must be a contiguous, 16-byte aligned ", shape(sizes), bf16 ? " bf16 or fp32" : " fp32", " tensor on ", p.device);
+    no_gradient("out", *out);
     return *out;
 }
 
@@ -168,9 +176,9 @@ struct Sequences {
     int64_t T, B;
 };
 Sequences sequences(const Plane& p, Tensor logits, c10::optional<Tensor> offsets, c10::optional<Tensor> mask) {
-    logits = operand(p, "logits", std::move(logits), {at::kFloat}, 2);
-    if (logits.requires_grad() && at::GradMode::is_enabled())
+    if (logits.defined() && logits.requires_grad() && at::GradMode::is_enabled())
         refuse("balance_loss records no autograd graph: pass logits.detach() and use balance_loss_backward");
+    logits = operand(p, "logits", std::move(logits), {at::kFloat}, 2);
     if (logits.size(1) != p.E) refuse("logits have ", logits.size(1), " columns, the context ", p.E, " experts");
     Sequences s{logits, {}, {}, logits.size(0), 1};
     if (offsets) {

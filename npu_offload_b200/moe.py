@@ -424,6 +424,8 @@ class MoEDataPlane:
         if stream is not None:
             with self._on(stream):
                 return self.route_topk(logits, bias)
+        if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
+            raise ValueError("route_topk records no autograd graph: pass logits.detach(), or call under torch.no_grad()")
         lg = _as(logits, torch.float32, self.device)
         if lg.dim() != 2 or lg.shape[1] != self.E:
             raise ValueError(f"logits are {tuple(lg.shape)}, the context has {self.E} experts")
