@@ -83,7 +83,11 @@ struct Fp8 {
 };
 Fp8 fp8(const Plane& p, const char* name, const Tensor& q, const Tensor& scale, int dims, int64_t block_rows) {
     const std::string qn = std::string(name) + ".q", sn = std::string(name) + ".scale";
-    if (block_rows > 1 && q.defined() && !q.is_contiguous()) refuse(qn, " must be contiguous");
+    // Weights are read in place: a copy of them on every call would cost more than the call.
+    if (block_rows > 1 && q.defined() && q.device() == p.device) {
+        if (!q.is_contiguous()) refuse(qn, " must be contiguous");
+        if ((uintptr_t)q.data_ptr() % 16) refuse(qn, " must be 16-byte aligned: clone it once");
+    }
     Fp8 m{operand(p, qn.c_str(), q, {at::kFloat8_e4m3fn}, dims, 16), operand(p, sn.c_str(), scale, {at::kFloat}, dims)};
     const int64_t rows = m.q.size(-2), cols = m.q.size(-1);
     bool ok = m.scale.size(-2) == (rows + block_rows - 1) / block_rows && m.scale.size(-1) == (cols + 127) / 128;
