@@ -159,7 +159,7 @@ struct PrepLoad {
 };
 __device__ __forceinline__ uint4 prep_load(const PrepArgs& a, const PrepLoad& l, uint32_t g) {
     const uint32_t row = g / l.per_row, c = (g - row * l.per_row) * 128 + (threadIdx.x & 15) * 8;
-    return g < l.groups && c < (uint32_t)a.H ? ldg_stream(a.x + (size_t)row * a.H + c) : make_uint4(0, 0, 0, 0);
+    return g < l.groups && c < (uint32_t)a.H ? ld_cg_u4(a.x + (size_t)row * a.H + c) : make_uint4(0, 0, 0, 0);
 }
 __device__ __forceinline__ PrepLoad prep_begin(const PrepArgs& a) {
     PrepLoad l;
@@ -350,7 +350,7 @@ __global__ void __cluster_dims__(kPlanCluster, 1, 1) __launch_bounds__(kPrepThre
 }
 __global__ void __launch_bounds__(kPrepThreads) f8_scatter_kernel(PrepArgs a) {
     griddep_launch_dependents();
-    const PrepLoad l = prep_begin(a);
+    const PrepLoad l = prep_begin(a);  // tokens from before the plan kernel, past L1 (launch.cuh)
     griddep_wait();
     prep_rows(a, l, a.pos);
 }
@@ -362,20 +362,20 @@ __global__ void __launch_bounds__(256) f8_combine_kernel(const float* __restrict
                                                          bool accumulate) {
     const int per = H / 4;
     const int64_t n = (int64_t)T * per;
-    bool waited = false;  // the slots are there when this kernel starts, the rows after the wait
+    bool waited = false;  // slots, weights and out are there when this kernel starts (launch.cuh), the rows after the wait
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
         const int64_t t = i / per;
         const int h = (int)(i - t * per) * 4;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (accumulate) v = *reinterpret_cast<const float4*>(static_cast<const float*>(out) + t * H + h);
+        if (accumulate) v = __ldcg(reinterpret_cast<const float4*>(static_cast<const float*>(out) + t * H + h));
         for (int k0 = 0; k0 < K; k0 += 8) {
             int s[8];
             float c[8];
             float4 a[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
-                s[k] = k0 + k < K ? __ldg(pos + t * K + k0 + k) : -1;
-                c[k] = k0 + k < K ? __ldg(w + t * K + k0 + k) : 0.f;
+                s[k] = k0 + k < K ? __ldcg(pos + t * K + k0 + k) : -1;
+                c[k] = k0 + k < K ? __ldcg(w + t * K + k0 + k) : 0.f;
             }
             if (!waited) griddep_wait();
             waited = true;

@@ -221,7 +221,14 @@ __device__ __forceinline__ F8Group f8_group(const F8Gemm& a, int g, int height) 
 }
 template <int MODE>
 __device__ __forceinline__ int f8_groups(const F8Gemm& a, int height) {
-    return MODE == kF8Dense ? (a.M + height - 1) / height : __ldg(a.n_groups);
+    return MODE == kF8Dense ? (a.M + height - 1) / height : __ldcg(a.n_groups);
+}
+// The same group for the warp that reads it ahead of the wait: past L1 (launch.cuh).
+template <int MODE>
+__device__ __forceinline__ F8Group f8_group_early(const F8Gemm& a, int g, int height) {
+    if (MODE != kF8Down) return f8_group<MODE>(a, g, height);
+    const uint4 v = ld_cg_u4(a.groups + g);
+    return F8Group{(int32_t)v.x, (int32_t)v.y, (int32_t)v.z, (int32_t)v.w};
 }
 // Scales of the 128-row weight block `block` of the matrix a group uses (gate/up: g = 0 gate, 1 up).
 template <int MODE>
@@ -302,7 +309,7 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
         const uint64_t pol_w = l2_evict_first(), pol_x = l2_evict_last();
         for (int item = cid; ok && item < items; item += n_clusters) {
             const int n = item % a.nt;
-            const F8Group grp = f8_group<MODE>(a, item / a.nt, NQ);
+            const F8Group grp = f8_group_early<MODE>(a, item / a.nt, NQ);
             auto load_w = [&](int kb, int s) {
                 unsigned char* st = ring + (size_t)s * C::kStage;
                 mbar_arrive_expect_tx(&c.full[s], C::kStage);
@@ -316,8 +323,10 @@ __global__ void __launch_bounds__(kFewThreads, FewCfg<MODE, NQ>::kMinCtas)
             int kb = kb0;
             if (MODE == kF8Down && g == 0) {  // the first stages' weights ahead of the wait
                 const int ahead = min(S, kb1 - kb0);
-                if (lane == 0)
+                if (lane == 0) {
+                    fence_proxy_async_global();  // the weights may have been written by a kernel just before the call
                     for (int k = 0; k < ahead; k++) load_w(kb0 + k, k);
+                }
                 griddep_wait();
                 if (lane == 0)
                     for (int k = 0; k < ahead; k++) load_x(kb0 + k, k);
