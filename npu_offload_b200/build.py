@@ -1,5 +1,5 @@
-"""Build libmoe_dp.so (the C-ABI library) in-tree with nvcc for sm_100a, and _torch_binding.so (the torch
-side of the e4m3 and balance-loss calls) with the host compiler.
+"""Build libmoe_dp.so (the C-ABI library) in-tree with nvcc for sm_100a, and the torch side of the e4m3 and
+balance-loss calls (_torch_binding.<Python>-torch<version>.so) with the host compiler.
 
     python -m npu_offload_b200.build [--force]
 
@@ -14,7 +14,6 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libmoe_dp.so")
-BINDING = os.path.join(HERE, "_torch_binding.so")
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
 CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
@@ -54,11 +53,19 @@ def up_to_date():
     return all(os.path.getmtime(d) <= t for d in sources()[1])
 
 
+def binding_path():
+    """Where the binding for the running Python and torch is: one of another version of either may differ in the
+    layout of every object that it is handed, and is never loaded."""
+    import torch
+    return os.path.join(HERE, f"_torch_binding.{sys.implementation.cache_tag}-torch{torch.__version__}.so")
+
+
 def build_binding(force=False):
-    """Compiles _torch_binding.so, linked to the library beside it, where it is older than what it is made of."""
+    """Compiles the binding, linked to the library beside it, where it is older than what it is made of."""
+    path = binding_path()
     deps = [BINDING_SOURCE, os.path.join(ROOT, "include", "moe_dp.h")]
-    if not force and os.path.exists(BINDING) and all(os.path.getmtime(d) <= os.path.getmtime(BINDING) for d in deps):
-        return BINDING
+    if not force and os.path.exists(path) and all(os.path.getmtime(d) <= os.path.getmtime(path) for d in deps):
+        return path
     import sysconfig
 
     import torch
@@ -67,11 +74,11 @@ def build_binding(force=False):
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_torch_binding"]
     for d in [*ext.include_paths(), sysconfig.get_paths()["include"]]:
         cmd += ["-isystem", d]
-    cmd += [BINDING_SOURCE, "-o", BINDING + ".tmp", *["-L" + d for d in ext.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu",
+    cmd += [BINDING_SOURCE, "-o", path + ".tmp", *["-L" + d for d in ext.library_paths()], "-lc10", "-ltorch", "-ltorch_cpu",
             "-ltorch_python", "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
     subprocess.check_call(cmd)
-    os.replace(BINDING + ".tmp", BINDING)
-    return BINDING
+    os.replace(path + ".tmp", path)
+    return path
 
 
 def build(force=False, verbose=False, extra=(), out=None):

@@ -11,6 +11,8 @@
 PyTorch only provides device memory and streams here; every computation runs in libmoe_dp.so.
 """
 import ctypes
+import importlib.util
+import os
 from typing import NamedTuple
 
 import numpy as np
@@ -19,6 +21,7 @@ import torch
 from . import _lib
 from ._lib import (MOE_F_ACCUMULATE, MOE_F_HOST, MOE_F_SYNC, MOE_SCORING_SIGMOID, MOE_SCORING_SOFTMAX,
                    MoeConfig, check, lib)
+from .build import binding_path
 
 __all__ = ["MoEDataPlane", "Fp8", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"]
 
@@ -472,7 +475,7 @@ class MoEDataPlane:
         global _calls
         if _calls is None:
             lib()  # the library first: the binding is linked to it
-            from . import _torch_binding as _calls
+            _calls = _load_binding()
         self._plane = _calls.Plane(self._h.value if self._h else 0, self.device, self.H, self.F, self.E, self.K)
         return self._plane
 
@@ -504,6 +507,16 @@ class MoEDataPlane:
         n = ctypes.c_int64()
         check(lib().moe_profile_read(self._h, ms, n_stages, ctypes.byref(n)))
         return list(ms), int(n.value)
+
+
+def _load_binding():
+    path = binding_path()
+    if not os.path.exists(path):
+        raise ImportError(f"{path} is missing: build it with `python -m npu_offload_b200.build` for this Python and torch")
+    spec = importlib.util.spec_from_file_location(__package__ + "._torch_binding", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def _tensor(name, t):
