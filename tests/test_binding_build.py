@@ -28,3 +28,19 @@ def test_a_binding_of_another_version_is_not_loaded(monkeypatch, what):
     monkeypatch.setattr(moe, "_raw_stream", lambda index: 0)
     with pytest.raises(ImportError, match="npu_offload_b200.build"):
         p.quantize_fp8(torch.zeros(4, 32))
+
+
+@pytest.mark.parametrize("lacking", ["compiler", "torch", "headers"])
+def test_the_library_builds_without_what_the_binding_needs(monkeypatch, lacking, capsys):
+    """Only the e4m3 and balance-loss calls from Python need the binding."""
+    monkeypatch.setattr(build, "build_library", lambda *a, **k: "the library")
+    if lacking == "compiler":
+        monkeypatch.setattr(build, "CXX", "/nowhere/g++")
+    elif lacking == "torch":
+        monkeypatch.setitem(sys.modules, "torch", None)
+    else:
+        monkeypatch.setattr(build, "CXX", "false")  # what a compiler returns that finds no headers
+    assert build.build(force=True) == "the library"
+    assert "binding" in capsys.readouterr().err
+    with pytest.raises(Exception):
+        build.build_binding(force=True)
