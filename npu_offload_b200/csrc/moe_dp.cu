@@ -216,10 +216,12 @@ int map_err(uint32_t bits) {
     return MOE_OK;
 }
 
-// Reads and clears the device error word (the stream must be synchronised by the caller after).
-void queue_err_readback(moe_ctx* c, cudaStream_t st) {
-    cudaMemcpyAsync(c->h_err, c->d_err, sizeof(uint32_t), cudaMemcpyDeviceToHost, st);
-    cudaMemsetAsync(c->d_err, 0, sizeof(uint32_t), st);
+// Reads and clears the device error word, in one step: kernels on other streams may raise errors at that time, and one
+// between a copy and a clear was lost.  (The stream must be synchronised by the caller after.)
+__global__ void take_errors_kernel(uint32_t* d_err, uint32_t* h_err) { *h_err = atomicExch(d_err, 0u); }
+cudaError_t queue_err_readback(moe_ctx* c, cudaStream_t st) {
+    take_errors_kernel<<<1, 1, 0, st>>>(c->d_err, c->h_err);
+    return cudaGetLastError();
 }
 
 // After a fused call gave up, its counts fall short: every call so far counts as finished.
@@ -234,7 +236,7 @@ int reset_counters(moe_ctx* c) {
 }
 
 int finish_sync(moe_ctx* c, cudaStream_t st) {
-    queue_err_readback(c, st);
+    CUDA_TRY(queue_err_readback(c, st));
     CUDA_TRY(cudaStreamSynchronize(st));
     uint32_t bits = *c->h_err | c->latched;
     c->latched = 0;
