@@ -24,7 +24,10 @@
  *    host buffer goes through the library's own pinned staging.
  *  - Device-pointer calls are asynchronous on `stream` (a cudaStream_t; NULL = legacy default
  *    stream).  Device-side errors (non-finite router input, a bounded wait that gave up) are
- *    latched in the context and returned by the next MOE_F_SYNC call or by moe_status().
+ *    latched in the context and returned, once, by the next MOE_F_SYNC call or by moe_status(), whichever
+ *    call raised them; one that a call still running on another stream raises later comes with a later
+ *    status.  (MOE_F_HOST calls return those of layer calls alone, and leave the errors of the routing, e4m3
+ *    and balance-loss calls to the others.)
  *  - One context per GPU per process.  Calls on one context must be serialised by the caller
  *    (like the reference engine's single caller thread, main.rs:149); distinct contexts are
  *    independent.

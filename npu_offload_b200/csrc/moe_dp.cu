@@ -118,8 +118,8 @@ struct moe_ctx {
     Job* d_jobs = nullptr;
     uint16_t* d_act = nullptr;
     float* d_y = nullptr;
-    uint32_t* d_err = nullptr;
-    uint32_t* h_err = nullptr;  // pinned
+    uint32_t* d_err = nullptr;  // [2] of the layer calls; of the calls that may overlap them (call_err)
+    uint32_t* h_err = nullptr;  // [2] pinned
     uint32_t* h_errsnap = nullptr;  // pinned, written by the decode kernel on host-buffer calls
     // MOE_F_HOST staging
     uint16_t* d_hidden = nullptr;
@@ -216,9 +216,11 @@ int map_err(uint32_t bits) {
     return MOE_OK;
 }
 
-// Reads and clears the device error word, in one step: kernels on other streams may raise errors at that time, and one
+// Reads and clears the device error words, each in one step: kernels on other streams may raise errors at that time, and one
 // between a copy and a clear was lost.  (The stream must be synchronised by the caller after.)
-__global__ void take_errors_kernel(uint32_t* d_err, uint32_t* h_err) { *h_err = atomicExch(d_err, 0u); }
+__global__ void take_errors_kernel(uint32_t* d_err, uint32_t* h_err) {
+    for (int i = 0; i < 2; i++) h_err[i] = atomicExch(d_err + i, 0u);
+}
 cudaError_t queue_err_readback(moe_ctx* c, cudaStream_t st) {
     take_errors_kernel<<<1, 1, 0, st>>>(c->d_err, c->h_err);
     return cudaGetLastError();
@@ -238,15 +240,19 @@ int reset_counters(moe_ctx* c) {
 int finish_sync(moe_ctx* c, cudaStream_t st) {
     CUDA_TRY(queue_err_readback(c, st));
     CUDA_TRY(cudaStreamSynchronize(st));
-    uint32_t bits = *c->h_err | c->latched;
+    uint32_t bits = c->h_err[0] | c->latched;
     c->latched = 0;
-    // a fused call that gave up may leave its grid-arrival counter short of the grid: clear both
+    // a fused call that gave up may leave its grid-arrival counter short of the grid: clear both.  (Not for a call of
+    // the other word, which counts nothing there: a fused call may be running, and would be counted twice.)
     if ((bits & kErrTimeout) && c->d_cnt) {
         int r = reset_counters(c);
         if (r) return r;
     }
-    return map_err(bits);
+    return map_err(bits | c->h_err[1]);
 }
+
+// The error word of the calls whose working memory is the caller's (routing alone, e4m3, balance loss).
+uint32_t* call_err(moe_ctx* c) { return c->d_err + 1; }
 
 template <class T>
 int dalloc(T** p, size_t n) {
@@ -690,7 +696,7 @@ int moe_create(const moe_config* cfg, moe_ctx** out) {
     if (!st) st = dalloc(&c->d_jobs, E);
     if (!st) st = dalloc(&c->d_act, NP * k.inter);
     if (!st) st = dalloc(&c->d_y, NP * k.hidden);
-    if (!st) st = dalloc(&c->d_err, 1);
+    if (!st) st = dalloc(&c->d_err, 2);
     if (!st) st = dalloc(&c->d_hidden, (size_t)k.max_tokens * k.hidden);
     if (!st) st = dalloc(&c->d_logits, (size_t)k.max_tokens * E);
     if (!st) st = dalloc(&c->d_out, (size_t)k.max_tokens * k.hidden);
@@ -705,7 +711,7 @@ int moe_create(const moe_config* cfg, moe_ctx** out) {
     if (!st && cudaMemset(c->d_hctr, 0, 2 * sizeof(uint32_t)) != cudaSuccess) st = fail(MOE_ECUDA, "memset failed");
     if (!st && cudaMemset(c->d_cnt, 0, sizeof(unsigned long long) * 4) != cudaSuccess)
         st = fail(MOE_ECUDA, "memset failed");
-    if (!st && cudaMallocHost((void**)&c->h_err, sizeof(uint32_t)) != cudaSuccess) st = fail(MOE_ENOMEM, "pinned error word");
+    if (!st && cudaMallocHost((void**)&c->h_err, 2 * sizeof(uint32_t)) != cudaSuccess) st = fail(MOE_ENOMEM, "pinned error word");
     if (!st && cudaMallocHost((void**)&c->h_errsnap, 16) != cudaSuccess) st = fail(MOE_ENOMEM, "pinned error word");
     if (!st && (cudaEventCreateWithFlags(&c->dec_ev, cudaEventDisableTiming) != cudaSuccess ||
                 cudaEventCreateWithFlags(&c->in_stage.ev, cudaEventDisableTiming) != cudaSuccess ||
@@ -714,7 +720,7 @@ int moe_create(const moe_config* cfg, moe_ctx** out) {
         st = fail(MOE_ECUDA, "event creation failed");
     if (!st && cudaMemcpy(c->d_desc, c->h_desc.data(), sizeof(ExpDesc) * c->h_desc.size(), cudaMemcpyHostToDevice) != cudaSuccess)
         st = fail(MOE_ECUDA, "descriptor upload failed");
-    if (!st && cudaMemset(c->d_err, 0, sizeof(uint32_t)) != cudaSuccess) st = fail(MOE_ECUDA, "memset failed");
+    if (!st && cudaMemset(c->d_err, 0, 2 * sizeof(uint32_t)) != cudaSuccess) st = fail(MOE_ECUDA, "memset failed");
     if (!st && cudaMemset(c->d_bias, 0, sizeof(float) * (size_t)L * E) != cudaSuccess) st = fail(MOE_ECUDA, "memset failed");
     if (!st) {
         cudaError_t e = decode_set_smem_limit();
@@ -1116,7 +1122,7 @@ int moe_route_topk(moe_ctx* c, int64_t T, const float* logits, const float* bias
         a.scoring = c->cfg.scoring;
         a.idx = topk_idx;
         a.w = topk_w;
-        a.err = c->d_err;
+        a.err = call_err(c);
         CUDA_TRY(launch_route_topk(a, st));
         c->launches++;
     }
@@ -1619,7 +1625,7 @@ int moe_matmul_fp8(moe_ctx* c, int64_t M, int64_t N, int64_t K, const uint8_t* x
     if (M && N) {
         if (!x || !x_scale || !w || !w_scale || !out) return fail(MOE_EINVAL, "null operand");
         if (!aligned16(x) || !aligned16(w) || !aligned16(out)) return fail(MOE_EINVAL, "x, w and out must be 16-byte aligned");
-        MatmulF8 a{x, x_scale, w, w_scale, M, N, (int)K, out, out_dtype == MOE_DT_F32, c->d_err, c->timeout_ns,
+        MatmulF8 a{x, x_scale, w, w_scale, M, N, (int)K, out, out_dtype == MOE_DT_F32, call_err(c), c->timeout_ns,
                    c->inject_timeout};
         CUDA_TRY(launch_matmul_fp8(a, c->sm_count, st));
         c->launches++;
@@ -1651,7 +1657,7 @@ int moe_experts_fp8(moe_ctx* c, int T, const uint16_t* x, const uint8_t* gate_up
         if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
         ExpertsF8 a{x, gate_up, gate_up_scale, down, down_scale, topk_idx, topk_w, T, c->cfg.hidden, c->cfg.inter,
                     c->cfg.n_experts, c->cfg.top_k, out, out_dtype == MOE_DT_F32, (flags & MOE_F_ACCUMULATE) != 0, workspace,
-                    c->d_err, c->timeout_ns, c->inject_timeout};
+                    call_err(c), c->timeout_ns, c->inject_timeout};
         int n = 0;
         CUDA_TRY(launch_experts_fp8(a, c->sm_count, st, &n));
         c->launches += n;
@@ -1687,7 +1693,7 @@ int moe_balance_loss(moe_ctx* c, int64_t T, const float* logits, const int32_t* 
     DeviceGuard dg(c->dev);
     cudaStream_t st = (cudaStream_t)stream;
     BalanceArgs a{logits, topk_idx, offsets, mask, (int)T, c->cfg.n_experts, c->cfg.top_k, B, c->cfg.scoring, counts, tokens, loss,
-                  nullptr, nullptr, workspace, c->d_err};
+                  nullptr, nullptr, workspace, call_err(c)};
     CUDA_TRY(launch_balance_loss(a, c->sm_count, st));
     c->launches += 2;
     return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
@@ -1703,7 +1709,7 @@ int moe_balance_loss_backward(moe_ctx* c, int64_t T, const float* logits, const 
     cudaStream_t st = (cudaStream_t)stream;
     if (T) {
         BalanceArgs a{logits, nullptr, offsets, mask, (int)T, c->cfg.n_experts, c->cfg.top_k, B, c->cfg.scoring,
-                      const_cast<int32_t*>(counts), const_cast<int32_t*>(tokens), nullptr, grad, dlogits, nullptr, c->d_err};
+                      const_cast<int32_t*>(counts), const_cast<int32_t*>(tokens), nullptr, grad, dlogits, nullptr, call_err(c)};
         CUDA_TRY(launch_balance_backward(a, c->sm_count, st));
         c->launches++;
     }

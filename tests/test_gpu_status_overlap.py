@@ -33,3 +33,40 @@ def test_an_error_is_reported_once_whatever_else_reads_the_status():
                 lost.append((i, seen))
         assert not lost, (len(lost), lost[:5])
         assert p.status() == MOE_OK
+
+
+def test_a_wait_that_gave_up_beside_a_running_layer_leaves_its_counts_alone():
+    """A product gives up (test hook) and its status is read while layer calls run on another stream: their grids count
+    arrivals over all calls, and go on from where they were."""
+    from npu_offload_b200 import Fp8, MoEDataPlane
+    from npu_offload_b200._lib import MOE_ETIMEOUT, MOE_OK, MOE_OPT_INJECT_WAIT_TIMEOUT, MOE_OPT_WAIT_TIMEOUT_US
+    H, F, E, K, T = 512, 256, 16, 4, 2
+    g = gen(2)
+    with MoEDataPlane(H, F, E, K, n_layers=1, max_tokens=16) as p:
+        for e in range(E):
+            p.load_expert(0, e, *((torch.randn(*s, generator=g, device="cuda") * 0.05).to(torch.bfloat16)
+                                  for s in ((F, H), (F, H), (H, F))))
+        xs = [torch.randn(T, H, generator=g, device="cuda").to(torch.bfloat16) for _ in range(4)]
+        lgs = [torch.randn(T, E, generator=g, device="cuda") for _ in range(4)]
+        rows, w = p.quantize_fp8(torch.randn(1, 1024, generator=g, device="cuda")), Fp8(*weight(g, 100, 1024))
+        want = [p.forward(0, x, lg) for x, lg in zip(xs, lgs)]
+        layers, products = torch.cuda.Stream(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        assert p.status() == MOE_OK
+        got = []
+        for i in range(30):
+            with torch.cuda.stream(layers):
+                torch.cuda._sleep(1_000_000 * (i % 5))
+                got += [p.forward(0, x, lg) for x, lg in zip(xs, lgs)]
+            p.set_option(MOE_OPT_WAIT_TIMEOUT_US, 1000)
+            p.set_option(MOE_OPT_INJECT_WAIT_TIMEOUT, 1)
+            p.matmul_fp8(rows, w, stream=products)
+            p.set_option(MOE_OPT_INJECT_WAIT_TIMEOUT, 0)
+            p.set_option(MOE_OPT_WAIT_TIMEOUT_US, 1_000_000)
+            assert p.status(products) == MOE_ETIMEOUT
+        torch.cuda.synchronize()
+        assert p.status() == MOE_OK
+        # the plan may cut the sums elsewhere behind a running call: the same experts, not the same order of sums
+        for i, y in enumerate(got):
+            v = want[i % 4]
+            assert float((y - v).abs().max()) <= 1e-4 * float(v.abs().max())
