@@ -360,6 +360,13 @@ cudaError_t launch_tc_items(const Job* jobs, const int* n_jobs, int E, const voi
 // ---- host side ----
 
 EncodeTiledFn tc_encode_fn() {
+    // The encoder is the driver's, and wants a context that is current in this thread: the runtime binds the device's
+    // with cudaSetDevice, or with a thread's first launch, which comes behind the encoding.
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+    }
     static EncodeTiledFn fn = nullptr;
     static bool tried = false;
     if (!tried) {
