@@ -367,18 +367,17 @@ EncodeTiledFn tc_encode_fn() {
         int dev = 0;
         bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
     }
-    static EncodeTiledFn fn = nullptr;
-    static bool tried = false;
-    if (!tried) {
-        tried = true;
+    // Looked up once, by whichever thread comes first, while others wait: with flags of our own, a thread that found the
+    // look-up begun and not done took it for failed.
+    static const EncodeTiledFn fn = [] {
         void* p = nullptr;
         cudaDriverEntryPointQueryResult q;
         if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
             q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeTiledFn>(p);
-        else
-            cudaGetLastError();
-    }
+            return reinterpret_cast<EncodeTiledFn>(p);
+        cudaGetLastError();
+        return static_cast<EncodeTiledFn>(nullptr);
+    }();
     return fn;
 }
 

@@ -43,3 +43,9 @@ def run(code, *args):
 def test_a_product_is_a_threads_first_call():
     """A thread that made no CUDA call yet."""
     run(FIRST, "1")
+
+
+def test_the_first_product_of_a_process_by_several_threads():
+    """Contexts are independent: the look-up of the tensor-map encoder, common to them, is one thread's alone."""
+    for _ in range(2):
+        run(FIRST, "12")
