@@ -126,7 +126,7 @@ struct moe_ctx {
     float* d_logits = nullptr;
     float* d_out = nullptr;
     Staging in_stage, out_stage, job_stage;
-    int64_t launches = 0;
+    std::atomic<int64_t> launches{0};  // (the calls that may overlap may come from several threads)
     uint32_t latched = 0;
     // fused decode kernel state
     unsigned long long* d_decide = nullptr;  // [4] fused decode: per-call share-cut decisions (call mod 4)
@@ -1733,7 +1733,7 @@ int moe_status(moe_ctx* c, void* stream) {
     return finish_sync(c, (cudaStream_t)stream);
 }
 
-int64_t moe_launch_count(moe_ctx* c) { return c ? c->launches + (c->shared ? c->shared->launches : 0) : -1; }
+int64_t moe_launch_count(moe_ctx* c) { return c ? c->launches.load() + (c->shared ? c->shared->launches.load() : 0) : -1; }
 
 static int set_option_one(moe_ctx* c, int option, int64_t value);
 

@@ -49,3 +49,36 @@ def test_the_first_product_of_a_process_by_several_threads():
     """Contexts are independent: the look-up of the tensor-map encoder, common to them, is one thread's alone."""
     for _ in range(2):
         run(FIRST, "12")
+
+
+def test_launches_of_several_threads_are_all_counted():
+    """The calls that may overlap on one context keep the launch count, each thread on its own stream."""
+    import ctypes
+    import threading
+
+    import torch
+
+    from npu_offload_b200 import MoEDataPlane, lib
+    with MoEDataPlane(64, 64, 8, 2, n_layers=1, max_tokens=16) as p:
+        logits = torch.randn(4, 8, device="cuda")
+        outs = [(torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, 2, device="cuda")) for _ in range(8)]
+        streams = [torch.cuda.Stream() for _ in outs]
+        want = p.route_topk(logits)
+        torch.cuda.synchronize()
+        before, n, bad = p.launch_count, 3000, []
+
+        def call(i):
+            a = [ctypes.c_void_p(t.data_ptr()) for t in (logits, *outs[i])]
+            for _ in range(n):
+                if lib().moe_route_topk(p._h, 4, a[0], None, a[1], a[2], 0, ctypes.c_void_p(streams[i].cuda_stream)):
+                    bad.append(i)
+
+        threads = [threading.Thread(target=call, args=(i,)) for i in range(len(outs))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        torch.cuda.synchronize()
+        assert not bad and p.launch_count - before == n * len(outs)
+        assert all(torch.equal(o[0], want[0]) and torch.equal(o[1], want[1]) for o in outs)
+        assert p.status() == 0
