@@ -254,7 +254,9 @@ MOE_API int moe_ep_import(moe_ctx* ctx, const void* records, int world);
  *
  * moe_matmul_fp8: out [M, N] (bf16 or fp32) = x . w^T with fp32 sums; x [M, K] scaled per row and 128
  * columns (x_scale [M, ceil(K / 128)]), w [N, K] per 128 x 128 block (w_scale [ceil(N / 128),
- * ceil(K / 128)]).  Any scales, not powers of two alone.  K a multiple of 16, at most 16384.
+ * ceil(K / 128)]).  Any scales, not powers of two alone; a block's sum is multiplied by x_scale * w_scale rounded
+ * to fp32, so where that product is infinite or below 2^-126 the block adds infinity, NaN or fewer bits.
+ * K a multiple of 16, at most 16384.
  *
  * moe_experts_fp8: the routed experts on e4m3 weights, with the caller's routing (moe_route's topk_idx
  * and topk_w [T, top_k]); H, F, E and top_k are the context's:

@@ -11,9 +11,9 @@
 // the same read as keeping them would.  Both passes are bounded by HBM: T E 4 bytes read, and T E 4
 // bytes written by the backward pass.
 //
-// Forward: unit u of a sequence is a run of kept chunk tokens; a CTA sums p over a unit (a warp a row,
-// a lane every 32nd expert, 32-bit sums over at most chunk / 8 rows, then the warps in order) and
-// counts its choices with integer atomics in shared memory, and stores both sums.  The second kernel,
+// Forward: unit u of a sequence is a run of chunk of its tokens, kept or not; a CTA sums p over a unit (a warp a row,
+// a lane every 32nd expert or four neighbours of every 128, 32-bit sums over at most chunk / kBalWarps rows, then the
+// warps in order) and counts its choices with integer atomics in shared memory, and stores both sums.  The second kernel,
 // a cluster of eight CTAs a sequence, adds the units in order (in 64 bits) and forms f . P; the last
 // cluster to finish adds the sequences in order.  No sum depends on timing.
 #include <cooperative_groups.h>

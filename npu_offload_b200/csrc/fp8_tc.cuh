@@ -8,8 +8,8 @@
 // applied that way in fp32 (the scaled MMA forms take powers of two only).
 //
 // Two forms, by the number of token rows:
-//   few rows   P = 128 weight rows (lanes), Q = 16, 32 or 64 token rows: each weight byte is loaded once, by
-//              TMA straight to the tensor core's shared memory, whatever the number of tokens.  A cluster
+//   few rows   P = 128 weight rows (lanes), Q = 16, 32 or 64 token rows: each weight byte is loaded once for
+//              a group of token rows, by TMA straight to the tensor core's shared memory.  A cluster
 //              of CTAs splits the inner dimension and adds its partial sums, in order, through distributed
 //              shared memory: enough loads are in flight with few tiles, and no sum depends on timing.
 //   many rows  P = 128 token rows, Q = 256 (or 128) weight rows, one persistent CTA an SM.  A block of the 128 x
