@@ -174,6 +174,12 @@ class MoEDataPlane:
         """Frees the expert's HBM slot (MOE_OPT_LAYER_SLOTS tables); it reads as not loaded afterwards."""
         check(lib().moe_evict_expert(self._h, layer, expert))
 
+    def _bias(self, bias, device=None):
+        b = _as(bias, torch.float32, device)
+        if b.numel() != self.E:
+            raise ValueError(f"bias is {tuple(b.shape)}, the context has {self.E} experts")
+        return b
+
     def expert_kind(self, layer, expert):
         return lib().moe_expert_kind(self._h, layer, expert)
 
@@ -181,7 +187,7 @@ class MoEDataPlane:
         if bias is None:
             check(lib().moe_set_bias(self._h, layer, None, 0))
             return
-        b = _as(bias, torch.float32)
+        b = self._bias(bias)
         check(lib().moe_set_bias(self._h, layer, _vp(b), 0 if b.is_cuda else MOE_F_HOST))
 
     # ---- hot path ----
@@ -312,7 +318,7 @@ class MoEDataPlane:
         """Router + permutation on the GPU; returns a dict of host numpy arrays (synchronous)."""
         lg = _as(logits, torch.float32, self.device)
         T = lg.shape[0]
-        b = None if bias is None else _as(bias, torch.float32, self.device)
+        b = None if bias is None else self._bias(bias, self.device)
         dev = self.device
         r = dict(idx=torch.empty(T, self.K, dtype=torch.int32, device=dev),
                  w=torch.empty(T, self.K, dtype=torch.float32, device=dev),
@@ -433,9 +439,7 @@ class MoEDataPlane:
         if lg.dim() != 2 or lg.shape[1] != self.E:
             raise ValueError(f"logits are {tuple(lg.shape)}, the context has {self.E} experts")
         T = lg.shape[0]
-        b = None if bias is None else _as(bias, torch.float32, self.device)
-        if b is not None and b.numel() != self.E:
-            raise ValueError(f"bias is {tuple(b.shape)}, the context has {self.E} experts")
+        b = None if bias is None else self._bias(bias, self.device)
         idx = torch.empty(T, self.K, dtype=torch.int32, device=self.device)
         w = torch.empty(T, self.K, dtype=torch.float32, device=self.device)
         check(lib().moe_route_topk(self._h, T, _vp(lg), _vp(b), _vp(idx), _vp(w), 0, _raw_stream(self._index)))

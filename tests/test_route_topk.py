@@ -24,6 +24,14 @@ def test_a_bias_of_another_size_is_refused(plane, shape):
         plane.route_topk(torch.zeros(3, 8), bias=torch.zeros(shape))
 
 
+@pytest.mark.parametrize("shape", [(7,), (9,), (0,), (8, 8)])
+def test_route_and_set_bias_refuse_it_too(plane, shape):
+    with pytest.raises(ValueError, match="bias is"):
+        plane.route(torch.zeros(3, 8), bias=torch.zeros(shape))
+    with pytest.raises(ValueError, match="bias is"):
+        plane.set_bias(0, torch.zeros(shape))
+
+
 def test_a_bias_of_the_experts_is_taken(plane):
     for bias in (None, torch.zeros(8), torch.zeros(1, 8), torch.zeros(8, dtype=torch.float64)):
         with pytest.raises(MoEError, match="null context"):
