@@ -222,8 +222,8 @@ __global__ void take_errors_kernel(uint32_t* d_err, uint32_t* h_err) {
     for (int i = 0; i < 2; i++) h_err[i] = atomicExch(d_err + i, 0u);
 }
 cudaError_t queue_err_readback(moe_ctx* c, cudaStream_t st) {
-    take_errors_kernel<<<1, 1, 0, st>>>(c->d_err, c->h_err);
-    return cudaGetLastError();
+    void* args[2] = {&c->d_err, &c->h_err};
+    return cudaLaunchKernel((const void*)take_errors_kernel, dim3(1), dim3(1), args, 0, st);  // (this launch's own error)
 }
 
 // After a fused call gave up, its counts fall short: every call so far counts as finished.

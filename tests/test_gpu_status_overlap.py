@@ -70,3 +70,19 @@ def test_a_wait_that_gave_up_beside_a_running_layer_leaves_its_counts_alone():
         for i, y in enumerate(got):
             v = want[i % 4]
             assert float((y - v).abs().max()) <= 1e-4 * float(v.abs().max())
+
+
+def test_the_status_is_not_that_of_another_runtime_call():
+    """A call of the CUDA runtime that failed before, and was dealt with, is no error of the plane."""
+    import ctypes
+
+    from npu_offload_b200 import MoEDataPlane
+    from npu_offload_b200._lib import MOE_OK
+    with MoEDataPlane(64, 64, 8, 2, n_layers=1, max_tokens=16) as p:
+        assert p.status() == MOE_OK
+        library = [line.split()[-1] for line in open("/proc/self/maps") if "libcudart.so" in line and "r-xp" in line]
+        for path in sorted(set(library)):
+            assert ctypes.CDLL(path).cudaSetDevice(10 ** 6) != 0  # no such device; leaves its code for cudaGetLastError
+        assert p.status() == MOE_OK
+        for path in sorted(set(library)):
+            ctypes.CDLL(path).cudaGetLastError()
