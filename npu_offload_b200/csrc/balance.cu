@@ -76,18 +76,18 @@ __device__ __forceinline__ void sequence(const int32_t* offsets, int b, int T, i
         first = 0, last = T;
         return;
     }
-    first = __ldg(offsets + b), last = __ldg(offsets + b + 1);
+    first = offsets[b], last = offsets[b + 1];
     if (first < 0 || last < first || last > T) first = last = 0;
 }
 __device__ __forceinline__ bool offsets_bad(const int32_t* offsets, int b, int T) {
     if (!offsets) return false;
-    const int first = __ldg(offsets + b), last = __ldg(offsets + b + 1);
+    const int first = offsets[b], last = offsets[b + 1];
     return first < 0 || last < first || last > T;
 }
 // The unit of chunk j of sequence b is offsets[b] / chunk + b + j: it grows with (b, j), and no two
 // have the same one, since a sequence has at most offsets[b + 1] / chunk - offsets[b] / chunk + 1.
 __device__ __forceinline__ int first_unit(const int32_t* offsets, int b, int chunk) {
-    return offsets ? max(__ldg(offsets + b), 0) / chunk + b : 0;
+    return offsets ? max(offsets[b], 0) / chunk + b : 0;
 }
 
 // 2^x of the hardware (2 ulp).
@@ -344,14 +344,14 @@ __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceAr
     if (t0 >= t1) return;
     Row<NE, V, FULL> next;
     next.load(a, t0);
-    const int full = __ldg(a.tokens + a.B);
-    const float grad = a.grad ? __ldg(a.grad) : 1.f;
+    const int full = a.tokens[a.B];
+    const float grad = a.grad ? *a.grad : 1.f;
     int b = 0;  // the sequence of token t is the last that begins at or before t, -1: none does
     if (a.offsets) {
         int lo = 0, hi = a.B;
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (__ldg(a.offsets + mid) <= t0) lo = mid + 1;
+            if (a.offsets[mid] <= t0) lo = mid + 1;
             else hi = mid;
         }
         b = lo - 1;
@@ -363,16 +363,16 @@ __global__ void __launch_bounds__(kBalThreads) balance_backward_kernel(BalanceAr
         if (t + 1 < t1) next.load(a, t + 1);
         bool in = true;
         if (a.offsets) {
-            while (b + 1 < a.B && __ldg(a.offsets + b + 1) <= t) b++;
-            in = b >= 0 && __ldg(a.offsets + b + 1) > t;
+            while (b + 1 < a.B && a.offsets[b + 1] <= t) b++;
+            in = b >= 0 && a.offsets[b + 1] > t;
         }
         if (in && b != have) {
-            n = __ldg(a.tokens + b);
+            n = a.tokens[b];
             const float k = n > 0 && full > 0 ? grad * (float)((double)E / ((double)a.K * n * (double)n * full)) : 0.f;
 #pragma unroll
             for (int j = 0; j < NE; j++) {
                 const int e = expert_of<V>(j);
-                f[j] = FULL || e < E ? k * (float)__ldg(a.counts + (size_t)b * E + e) : 0.f;
+                f[j] = FULL || e < E ? k * (float)a.counts[(size_t)b * E + e] : 0.f;
             }
             have = b;
         }

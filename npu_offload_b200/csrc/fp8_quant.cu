@@ -26,7 +26,7 @@ template <>
 struct Eight<false> {
     uint4 v;
     __device__ __forceinline__ void load(const void* x, size_t i) {
-        v = ldg_stream(static_cast<const uint16_t*>(x) + i);
+        v = ld_cg_u4(static_cast<const uint16_t*>(x) + i);
     }
     __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&f)[8]) const {
@@ -40,8 +40,8 @@ template <>
 struct Eight<true> {
     uint4 a, b;
     __device__ __forceinline__ void load(const void* x, size_t i) {
-        a = ldg_stream(static_cast<const float*>(x) + i);
-        b = ldg_stream(static_cast<const float*>(x) + i + 4);
+        a = ld_cg_u4(static_cast<const float*>(x) + i);
+        b = ld_cg_u4(static_cast<const float*>(x) + i + 4);
     }
     __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
     __device__ __forceinline__ void get(float (&f)[8]) const {
@@ -59,8 +59,8 @@ struct Eight<true> {
 // Rows: sixteen lanes hold a group, eight values each, and share its maximum by shuffles; N groups' loads
 // in flight for each half warp.
 template <bool F32, int N>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, uint32_t groups, uint32_t per_row,
-                                                            uint32_t cols, uint8_t* __restrict__ q, float* __restrict__ s) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* x, uint32_t groups, uint32_t per_row,
+                                                            uint32_t cols, uint8_t* q, float* s) {
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t sub = threadIdx.x & 15, g0 = blockIdx.x * 16 * N + (threadIdx.x >> 4);
@@ -93,9 +93,9 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restri
 
 // 128 x 128 blocks: one CTA a block, thread t columns 8 (t % 16) .. of rows t / 16 + 16 i.
 template <bool F32>
-__global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const void* __restrict__ x, uint32_t rows, uint32_t cols,
-                                                              uint32_t rb, uint32_t cb, uint8_t* __restrict__ q,
-                                                              float* __restrict__ s) {
+__global__ void __launch_bounds__(256, F32 ? 2 : 4) quantize_blocks_kernel(const void* x, uint32_t rows, uint32_t cols,
+                                                              uint32_t rb, uint32_t cb, uint8_t* q,
+                                                              float* s) {
     __shared__ uint32_t top_s[8];
     griddep_wait();
     griddep_launch_dependents();

@@ -14,6 +14,8 @@
 //   product) have ended and their writes are performed by then; the down product lets its successor start at once, but
 //   has itself started behind that point.  The wait that makes those writes visible was another grid's, so
 //   these reads go past L1, whose lines might be older, to L2 (ld.cg, TMA), where nothing older is left.
+// * No kernel launched this way uses non-coherent loads (__ldg, ld.global.nc, const __restrict__ pointers): its operands
+//   may be written while it is on the SMs already, and the compiler may move such loads ahead of the wait.
 // The last kernel of a call does not let the next kernel start before its end: the planner and the decode kernel
 // read router logits ahead of their wait, and a product may have written them.  The quantiser and the loss, whose
 // outputs no kernel reads ahead of its wait, let the next one start once their own wait is over.
