@@ -299,6 +299,31 @@ MOE_API int moe_balance_loss_backward(moe_ctx* ctx, int64_t T, const float* logi
                                       const uint8_t* mask, const int32_t* counts, const int32_t* tokens, const float* grad,
                                       float* dlogits, int flags, void* stream);
 
+/* ---- Residual addition with root-mean-square norm, to bf16 / fp32 and / or e4m3, and its gradients ----
+ *
+ * moe_add_norm, rows of C values (1 to 16384), T rows (at most 2^24):
+ *   sum = x + residual, rounded to the residual's type (residual NULL: the sum is x, and `sum` is NULL too)
+ *   rstd[t] = 1 / sqrt(mean_c sum[t]^2 + eps);   y = sum * rstd[t] * weight, rounded once, bf16 or fp32 (NULL: not wanted)
+ *   q, scale (both NULL: not wanted): y before its rounding as e4m3 with a scale for each 128 columns of a row, the smallest
+ *     power of two >= 2^-126 with max|y| <= 448 scale, 1 for zeros: what moe_matmul_fp8 takes as x.  C % 16 == 0.
+ * x, residual and weight are bf16 or fp32 each (their MOE_DT_*).  eps > 0.  Squares may leave fp32's range: such rows are
+ * summed in 64 bits.  A row with an infinity or NaN gives NaN and zeros as the formula does, and reaches no other row.
+ *
+ * moe_add_norm_backward: dy [T, C] (bf16 or fp32) the gradient of y, dsum (NULL: none) what flows into the sum besides, of the sum's
+ * type; with u = sum * rstd[t] and g = weight * dy
+ *   dx = rstd[t] * (g - u * mean_c(g u)) + dsum, of the sum's type, the gradient of x and of the residual alike
+ *   dweight [C] fp32 = sum_t dy u (NULL: not wanted)
+ * Results do not depend on timing.  workspace: moe_add_norm_backward_workspace bytes, 256-byte aligned (NULL without dweight).
+ *
+ * Device pointers, tensors 16-byte aligned; an output overlaps nothing.  Nothing is kept in the context. */
+MOE_API int moe_add_norm(moe_ctx* ctx, int64_t T, int64_t C, const void* x, int x_dtype, const void* residual, int stream_dtype,
+                         const void* weight, int weight_dtype, float eps, void* sum, void* y, int y_dtype, uint8_t* q,
+                         float* scale, float* rstd, int flags, void* stream);
+MOE_API int64_t moe_add_norm_backward_workspace(moe_ctx* ctx, int64_t T, int64_t C);
+MOE_API int moe_add_norm_backward(moe_ctx* ctx, int64_t T, int64_t C, const void* dy, int dy_dtype, const void* sum,
+                                  int stream_dtype, const void* dsum, const void* weight, int weight_dtype, const float* rstd,
+                                  void* dx, float* dweight, void* workspace, int64_t workspace_bytes, int flags, void* stream);
+
 /* The router's exponential, y[i] = exp(x[i]) rounded once to fp32 (correctly rounded), on the
  * calling thread's current device, asynchronously on `stream`; x and y are device pointers.  It is
  * the exp of the softmax numerators (host.rs.tpl:249, `(v - m).exp()`) and of the sigmoid

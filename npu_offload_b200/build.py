@@ -19,7 +19,8 @@ CXX = os.environ.get("CXX", "g++")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["moe_dp.cu", "route.cu", "experts.cu", "decode.cu", "noalloc.cu", "prefill.cu", "prefill_tc.cu",
-           "block.cu", "fp8_quant.cu", "fp8_gemm.cu", "balance.cu"]
+           "block.cu", "fp8_quant.cu", "fp8_gemm.cu", "balance.cu", "norm.cu",
+           "norm_backward.cu"]
 
 
 def cute_include():

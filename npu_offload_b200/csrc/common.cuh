@@ -15,6 +15,8 @@ constexpr int kF8MaxRows = 1 << 24;        // its M and N
 constexpr int kF8MaxPairs = 1 << 20;       // (token, expert) pairs of an expert call
 constexpr int kBalanceMaxTokens = 1 << 24;
 constexpr int kBalanceMaxSeqs = 1 << 16;
+constexpr int kNormMaxRows = 1 << 24;
+constexpr int kNormMaxCols = 16384;
 
 // Latched device-side error bits (ctx->dev_err); host maps them to MOE_E* codes.
 constexpr uint32_t kErrNonFinite = 1u;

@@ -42,4 +42,15 @@ cudaError_t launch_after(K kernel, int grid, int threads, int smem, int cluster,
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// The same for the norm, grouped routing and adapter kernels: each waits at its very start, reads nothing ahead of that
+// and lets nothing start before its end.  What overlaps the kernel before is the launch alone.
+struct Launch {
+    int grid, threads, smem, cluster;
+    cudaStream_t st;
+    template <class K, class... A>
+    cudaError_t run(K kernel, A... args) const {
+        return launch_after(kernel, grid, threads, smem, cluster, st, args...);
+    }
+};
+
 }  // namespace moe

@@ -17,6 +17,7 @@
 #include "block.h"
 #include "experts.h"
 #include "fp8.h"
+#include "norm.h"
 #include "route.h"
 
 using namespace moe;
@@ -1713,6 +1714,94 @@ int moe_balance_loss_backward(moe_ctx* c, int64_t T, const float* logits, const 
         CUDA_TRY(launch_balance_backward(a, c->sm_count, st));
         c->launches++;
     }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+// ---------------- residual addition and root-mean-square norm ----------------
+
+static bool float_dtype(int d) { return d == MOE_DT_BF16 || d == MOE_DT_F32; }
+static size_t dtype_bytes(int d) { return d == MOE_DT_F32 ? 4 : 2; }
+static bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    return a && b && na && nb && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
+
+static int norm_checks(moe_ctx* c, int64_t T, int64_t C, int flags) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "the norm takes device pointers and no flag but MOE_F_SYNC");
+    if (T < 0 || T > kNormMaxRows) return fail(MOE_EINVAL, "T=%lld not in [0,%d]", (long long)T, kNormMaxRows);
+    if (C < 1 || C > kNormMaxCols) return fail(MOE_EINVAL, "C=%lld not in [1,%d]", (long long)C, kNormMaxCols);
+    return MOE_OK;
+}
+
+int moe_add_norm(moe_ctx* c, int64_t T, int64_t C, const void* x, int x_dtype, const void* residual, int stream_dtype,
+                 const void* weight, int weight_dtype, float eps, void* sum, void* y, int y_dtype, uint8_t* q, float* scale,
+                 float* rstd, int flags, void* stream) {
+    int r = norm_checks(c, T, C, flags);
+    if (r) return r;
+    if (!float_dtype(x_dtype) || !float_dtype(stream_dtype) || !float_dtype(weight_dtype) || !float_dtype(y_dtype))
+        return fail(MOE_EINVAL, "a dtype is neither MOE_DT_BF16 nor MOE_DT_F32");
+    if (!(eps > 0.f) || !(eps < INFINITY)) return fail(MOE_EINVAL, "eps must be positive and finite");
+    if (q && C % 16) return fail(MOE_EINVAL, "C=%lld is not a multiple of 16, as e4m3 rows are", (long long)C);
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T) {
+        if (!x || !weight) return fail(MOE_EINVAL, "null x / weight");
+        if (!q != !scale) return fail(MOE_EINVAL, "q and scale go together");
+        if (!residual != !sum) return fail(MOE_EINVAL, "residual and sum go together");
+        if (!y && !q && !sum && !rstd) return fail(MOE_EINVAL, "no result is wanted");
+        const void* all[] = {x, residual, weight, sum, y, q};
+        for (const void* p : all)
+            if (!aligned16(p)) return fail(MOE_EINVAL, "x, residual, weight, sum, y and q must be 16-byte aligned");
+        const size_t n = (size_t)T * C;
+        const struct { const void* p; size_t bytes; } in[] = {{x, n * dtype_bytes(x_dtype)}, {residual, n * dtype_bytes(stream_dtype)},
+                                                              {weight, (size_t)C * dtype_bytes(weight_dtype)}},
+                                                      out[] = {{sum, n * dtype_bytes(stream_dtype)}, {y, n * dtype_bytes(y_dtype)}, {q, n},
+                                                               {scale, (size_t)T * ((C + 127) / 128) * 4}, {rstd, (size_t)T * 4}};
+        for (int i = 0; i < 5; i++) {
+            for (const auto& o : in)
+                if (overlap(out[i].p, out[i].bytes, o.p, o.bytes)) return fail(MOE_EINVAL, "a result overlaps an operand");
+            for (int j = 0; j < i; j++)
+                if (overlap(out[i].p, out[i].bytes, out[j].p, out[j].bytes)) return fail(MOE_EINVAL, "two results overlap");
+        }
+        NormArgs a{x, residual, weight, x_dtype == MOE_DT_F32, stream_dtype == MOE_DT_F32, weight_dtype == MOE_DT_F32,
+                   y_dtype == MOE_DT_F32, T, (int)C, eps, sum, y, q, scale, rstd};
+        CUDA_TRY(launch_add_norm(a, c->sm_count, st));
+        c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+int64_t moe_add_norm_backward_workspace(moe_ctx* c, int64_t T, int64_t C) {
+    if (!c || T < 0 || T > kNormMaxRows || C < 1 || C > kNormMaxCols) return -1;
+    return (int64_t)norm_backward_workspace(T, (int)C, c->sm_count);
+}
+
+int moe_add_norm_backward(moe_ctx* c, int64_t T, int64_t C, const void* dy, int dy_dtype, const void* sum, int stream_dtype,
+                          const void* dsum, const void* weight, int weight_dtype, const float* rstd, void* dx, float* dweight,
+                          void* workspace, int64_t workspace_bytes, int flags, void* stream) {
+    int r = norm_checks(c, T, C, flags);
+    if (r) return r;
+    if (!float_dtype(dy_dtype) || !float_dtype(stream_dtype) || !float_dtype(weight_dtype))
+        return fail(MOE_EINVAL, "a dtype is neither MOE_DT_BF16 nor MOE_DT_F32");
+    if (T && (!dy || !sum || !weight || !rstd || !dx)) return fail(MOE_EINVAL, "null argument");
+    if (!aligned16(dy) || !aligned16(sum) || !aligned16(dsum) || !aligned16(weight) || !aligned16(dx))
+        return fail(MOE_EINVAL, "dy, sum, dsum, weight and dx must be 16-byte aligned");
+    if (dweight) {
+        const int64_t need = moe_add_norm_backward_workspace(c, T, C);
+        if (!workspace || (uintptr_t)workspace & 255) return fail(MOE_EINVAL, "the workspace must be 256-byte aligned");
+        if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+    }
+    const size_t n = (size_t)T * C, nx = n * dtype_bytes(stream_dtype), nw = (size_t)C * dtype_bytes(weight_dtype);
+    if (overlap(dx, nx, dy, n * dtype_bytes(dy_dtype)) || overlap(dx, nx, sum, nx) || overlap(dx, nx, dsum, nx) ||
+        overlap(dx, nx, weight, nw) || overlap(dx, nx, rstd, (size_t)T * 4) || overlap(dx, nx, dweight, (size_t)C * 4))
+        return fail(MOE_EINVAL, "dx overlaps an operand");
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    NormBackwardArgs a{dy, sum, dsum, weight, rstd, dy_dtype == MOE_DT_F32, stream_dtype == MOE_DT_F32, weight_dtype == MOE_DT_F32, T,
+                       (int)C, dx, dweight, (float*)workspace};
+    int launched = 0;
+    CUDA_TRY(launch_add_norm_backward(a, c->sm_count, st, &launched));
+    c->launches += launched;
     return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
 }
 

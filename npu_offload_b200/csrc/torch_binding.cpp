@@ -1,4 +1,4 @@
-// Torch-side half of the e4m3 and balance-loss calls: checks, allocation of results and working memory, and
+// Torch-side half of the calls that allocate through torch (e4m3, balance loss, norm): checks, allocation of results and working memory, and
 // the call of the C ABI.  These calls take a few microseconds on the GPU at one token; through Python and
 // ctypes the host needed 11 us (quantiser, product) to 30 us (loss and gradient) for them.
 //
@@ -226,10 +226,81 @@ Tensor balance_loss_backward(const Plane& p, Tensor logits, Tensor counts, Tenso
     return o;
 }
 
+struct Rows {  // [..., C] as T rows
+    int64_t T, C;
+};
+Rows rows_of(const char* name, const Tensor& t) {
+    if (t.dim() < 1 || t.size(-1) < 1) refuse(name, " must be [..., C] with a column at least, not ", shape(t.sizes()));
+    return {t.numel() / t.size(-1), t.size(-1)};
+}
+Tensor norm_weight(const Plane& p, Tensor w, int64_t C) {
+    w = operand(p, "weight", std::move(w), {at::kBFloat16, at::kFloat}, 1, 16);
+    if (w.size(0) != C) refuse("weight has ", w.size(0), " values, the rows ", C);
+    return w;
+}
+
+std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>, Tensor, Tensor> add_norm(
+    const Plane& p, Tensor x, Tensor weight, c10::optional<Tensor> residual, double eps, c10::optional<at::ScalarType> out_dtype, bool fp8,
+    int64_t stream) {
+    x = operand(p, "x", std::move(x), {at::kBFloat16, at::kFloat}, -1, 16);
+    const Rows n = rows_of("x", x);
+    weight = norm_weight(p, std::move(weight), n.C);
+    if (residual) {
+        residual = operand(p, "residual", *residual, {at::kBFloat16, at::kFloat}, -1, 16);
+        if (residual->sizes() != x.sizes()) refuse("residual is ", shape(residual->sizes()), ", x ", shape(x.sizes()));
+    }
+    if (out_dtype && *out_dtype != at::kBFloat16 && *out_dtype != at::kFloat)
+        refuse("out_dtype ", name_of(*out_dtype), " is neither torch.bfloat16 nor torch.float32");
+    if (!out_dtype && !fp8) refuse("neither an out_dtype nor fp8 is wanted");
+    if (fp8 && n.C % 16) refuse("fp8 rows are a multiple of 16, not ", n.C, " columns");
+    const auto opt = at::TensorOptions(p.device);
+    c10::optional<Tensor> y, q, scale;
+    if (out_dtype) y = at::empty(x.sizes(), opt.dtype(*out_dtype));
+    if (fp8) {
+        auto sizes = x.sizes().vec();
+        sizes.back() = (n.C + 127) / 128;
+        q = at::empty(x.sizes(), opt.dtype(at::kFloat8_e4m3fn));
+        scale = at::empty(sizes, opt.dtype(at::kFloat));
+    }
+    const Tensor sum = residual ? at::empty(x.sizes(), opt.dtype(residual->scalar_type())) : x;
+    const Tensor rstd = at::empty(x.sizes().slice(0, x.dim() - 1), opt.dtype(at::kFloat));
+    check(moe_add_norm(p.ctx, n.T, n.C, x.data_ptr(), dtype_of(x), ptr<void>(residual), dtype_of(sum), weight.data_ptr(), dtype_of(weight),
+                       (float)eps, residual ? sum.data_ptr() : nullptr, ptr<void>(y), y ? dtype_of(*y) : MOE_DT_BF16, ptr<uint8_t>(q),
+                       ptr<float>(scale), ptr<float>(rstd), 0, (void*)stream));
+    return {y, q, scale, sum, rstd};
+}
+
+std::pair<Tensor, c10::optional<Tensor>> add_norm_backward(const Plane& p, Tensor dy, Tensor sum, Tensor weight, Tensor rstd,
+                                                          c10::optional<Tensor> dsum, bool weight_grad, int64_t stream) {
+    dy = operand(p, "dy", std::move(dy), {at::kBFloat16, at::kFloat}, -1, 16);
+    sum = operand(p, "sum", std::move(sum), {at::kBFloat16, at::kFloat}, -1, 16);
+    const Rows n = rows_of("sum", sum);
+    weight = norm_weight(p, std::move(weight), n.C);
+    rstd = operand(p, "rstd", std::move(rstd), {at::kFloat}, (int)sum.dim() - 1);
+    if (dy.sizes() != sum.sizes()) refuse("dy is ", shape(dy.sizes()), ", sum ", shape(sum.sizes()));
+    if (rstd.sizes() != sum.sizes().slice(0, sum.dim() - 1)) refuse("rstd is ", shape(rstd.sizes()), " for a sum of ", shape(sum.sizes()));
+    if (dsum) {
+        dsum = operand(p, "dsum", *dsum, {sum.scalar_type()}, -1, 16);
+        if (dsum->sizes() != sum.sizes()) refuse("dsum is ", shape(dsum->sizes()), ", sum ", shape(sum.sizes()));
+    }
+    const Tensor dx = at::empty(sum.sizes(), at::TensorOptions(p.device).dtype(sum.scalar_type()));
+    c10::optional<Tensor> dw;
+    int64_t bytes = 0;
+    if (weight_grad) {
+        dw = at::empty({n.C}, at::TensorOptions(p.device).dtype(at::kFloat));
+        bytes = moe_add_norm_backward_workspace(p.ctx, n.T, n.C);
+    }
+    const Tensor ws = workspace(p, bytes);
+    check(moe_add_norm_backward(p.ctx, n.T, n.C, dy.data_ptr(), dtype_of(dy), sum.data_ptr(), dtype_of(sum), ptr<void>(dsum),
+                                weight.data_ptr(), dtype_of(weight), ptr<float>(rstd), dx.data_ptr(), ptr<float>(dw), ws.data_ptr(), bytes,
+                                0, (void*)stream));
+    return {dx, dw};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
-    m.doc() = "Checks, allocation and calls of the e4m3 and balance-loss entry points of libmoe_dp.so.";
+    m.doc() = "Checks, allocation and calls of the entry points of libmoe_dp.so that allocate through torch.";
     py::class_<Plane>(m, "Plane").def(py::init([](int64_t ctx, at::Device device, int64_t H, int64_t F, int64_t E, int64_t K) {
         return Plane{(moe_ctx*)ctx, device, H, F, E, K};
     }));
@@ -238,4 +309,6 @@ PYBIND11_MODULE(_torch_binding, m) {
     m.def("experts_fp8", &experts_fp8);
     m.def("balance_loss", &balance_loss);
     m.def("balance_loss_backward", &balance_loss_backward);
+    m.def("add_norm", &add_norm);
+    m.def("add_norm_backward", &add_norm_backward);
 }

@@ -23,7 +23,7 @@ from ._lib import (MOE_F_ACCUMULATE, MOE_F_HOST, MOE_F_SYNC, MOE_SCORING_SIGMOID
                    MoeConfig, check, lib)
 from .build import binding_path
 
-__all__ = ["MoEDataPlane", "Fp8", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"]
+__all__ = ["MoEDataPlane", "Fp8", "Normed", "BalanceStats", "gpu_moe", "set_threads", "as_bf16"]
 
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # (a torch without CUDA has none, and no GPU path)
 _calls = None  # the module _torch_binding, from its first use on
@@ -33,6 +33,14 @@ class Fp8(NamedTuple):
     """e4m3 values with one fp32 scale for each 128 columns of one row, or of 128 rows; value = q * scale."""
     q: torch.Tensor      # [..., rows, cols] torch.float8_e4m3fn
     scale: torch.Tensor  # [..., ceil(rows / block_rows), ceil(cols / 128)] torch.float32
+
+
+class Normed(NamedTuple):
+    """What add_norm() gives."""
+    y: "torch.Tensor | None"  # sum * rstd * weight, of out_dtype (None: not asked for)
+    fp8: "Fp8 | None"         # the same in e4m3, a scale for each 128 columns of a row (None: not asked for)
+    sum: torch.Tensor         # x + residual, of the residual's type; without a residual, x itself
+    rstd: torch.Tensor        # [...] fp32: 1 / sqrt(mean sum^2 + eps)
 
 
 class BalanceStats(NamedTuple):
@@ -468,6 +476,31 @@ class MoEDataPlane:
                 return self.balance_loss_backward(logits, stats, grad, out)
         p = self._plane or self._bind()
         return _calls.balance_loss_backward(p, logits, *stats, grad, out, _raw_stream(self._index))
+
+    # ---- residual addition and root-mean-square norm ----
+    def add_norm(self, x, weight, residual=None, eps=1e-6, out_dtype=torch.bfloat16, fp8=False, stream=None):
+        """Normed(y, fp8, sum, rstd): sum = x + residual in the residual's type, y = sum / sqrt(mean sum^2 + eps) * weight.
+
+        x, residual [..., C] and weight [C] bf16 or fp32; C at most 16384.  out_dtype: bf16, fp32, or None for no y;
+        fp8: y also as e4m3 with a scale for each 128 columns (C a multiple of 16), as matmul_fp8 takes it, rounded
+        from y before that is.  No autograd graph is recorded: the gradient is add_norm_backward()."""
+        if stream is not None:
+            with self._on(stream):
+                return self.add_norm(x, weight, residual, eps, out_dtype, fp8)
+        p = self._plane or self._bind()
+        y, q, scale, total, rstd = _calls.add_norm(p, _tensor("x", x), _tensor("weight", weight), residual, eps, out_dtype, fp8,
+                                                   _raw_stream(self._index))
+        return Normed(y, None if q is None else Fp8(q, scale), total, rstd)
+
+    def add_norm_backward(self, dy, sum, weight, rstd, dsum=None, weight_grad=True, stream=None):
+        """(dx, dweight) of add_norm: dy [..., C] (bf16 or fp32) is the gradient of y, dsum (sum's type) what else flows into
+        the sum; dx, of sum's type, is the gradient of x and of the residual; dweight [C] fp32 (weight_grad=False: None)."""
+        if stream is not None:
+            with self._on(stream):
+                return self.add_norm_backward(dy, sum, weight, rstd, dsum, weight_grad)
+        p = self._plane or self._bind()
+        return _calls.add_norm_backward(p, _tensor("dy", dy), _tensor("sum", sum), _tensor("weight", weight), _tensor("rstd", rstd), dsum,
+                                        weight_grad, _raw_stream(self._index))
 
     def _on(self, stream):
         if stream.device != self.device:
