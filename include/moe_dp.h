@@ -299,6 +299,28 @@ MOE_API int moe_balance_loss_backward(moe_ctx* ctx, int64_t T, const float* logi
                                       const uint8_t* mask, const int32_t* counts, const int32_t* tokens, const float* grad,
                                       float* dlogits, int flags, void* stream);
 
+/* ---- Routing limited to the best groups of experts, and the gradient of routing weights ----
+ *
+ * moe_route_groups: logits [T, E] fp32; E, top_k and the scoring are the context's, T as moe_route_topk's.  Experts come in
+ * `groups` (1 to 32, a divisor of E) groups of E / groups neighbours; the best top_groups of them are open, and the choices are made in those.
+ *   key: the logit (softmax), or s + bias in fp32, s as moe_route_topk forms it (sigmoid; bias [E] or NULL, NULL for softmax)
+ *   a group's score: its largest key (softmax), the fp32 sum of its two largest (sigmoid; of the one, in groups of one)
+ *   best groups, and in them the top_k best keys: the larger first, ties to the lower index
+ *   topk_w = scale * v, divided by the sum of the chosen v (sigmoid: + 1e-20) where renormalize is set; v = softmax over all E, or s
+ * -inf masks an expert: it comes last.  NaN logits or biases, a softmax of +inf or of nothing but -inf: MOE_ENONFINITE in the
+ * device-side status; that token's weights are NaN, its experts distinct.  top_k <= top_groups * E / groups.
+ *
+ * moe_route_backward: dlogits [T, E] = the gradient of the logits from dw [T, top_k], that of topk_w (of moe_route_topk too:
+ * renormalize = 1, scale = 1), at the choices topk_idx (negative: none; one of E or more is skipped, MOE_EINVAL in the device-side
+ * status; an expert twice in a token counts twice).  Choices are constants.  MOE_F_ACCUMULATE: dlogits +=, as behind
+ * moe_balance_loss_backward.
+ *
+ * Both use nothing of the context but the device-side status. */
+MOE_API int moe_route_groups(moe_ctx* ctx, int64_t T, const float* router_logits, const float* bias, int groups, int top_groups,
+                             int renormalize, float scale, int32_t* topk_idx, float* topk_w, int flags, void* stream);
+MOE_API int moe_route_backward(moe_ctx* ctx, int64_t T, const float* router_logits, const int32_t* topk_idx, const float* dw,
+                               int renormalize, float scale, float* dlogits, int flags, void* stream);
+
 /* ---- Residual addition with root-mean-square norm, to bf16 / fp32 and / or e4m3, and its gradients ----
  *
  * moe_add_norm, rows of C values (1 to 16384), T rows (at most 2^24):

@@ -72,6 +72,8 @@ _SIGS = {
     "moe_balance_loss_workspace": (_i64, [_vp, _i64, _i]),
     "moe_balance_loss": (_i, [_vp, _i64, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
     "moe_balance_loss_backward": (_i, [_vp, _i64, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i, _vp]),
+    "moe_route_groups": (_i, [_vp, _i64, _vp, _vp, _i, _i, _i, ctypes.c_float, _vp, _vp, _i, _vp]),
+    "moe_route_backward": (_i, [_vp, _i64, _vp, _vp, _vp, _i, ctypes.c_float, _vp, _i, _vp]),
     "moe_add_norm": (_i, [_vp, _i64, _i64, _vp, _i, _vp, _i, _vp, _i, ctypes.c_float, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp]),
     "moe_add_norm_backward_workspace": (_i64, [_vp, _i64, _i64]),
     "moe_add_norm_backward": (_i, [_vp, _i64, _i64, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i64, _i, _vp]),

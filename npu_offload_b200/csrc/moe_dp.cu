@@ -19,6 +19,7 @@
 #include "fp8.h"
 #include "norm.h"
 #include "route.h"
+#include "route_groups.h"
 
 using namespace moe;
 
@@ -1802,6 +1803,52 @@ int moe_add_norm_backward(moe_ctx* c, int64_t T, int64_t C, const void* dy, int 
     int launched = 0;
     CUDA_TRY(launch_add_norm_backward(a, c->sm_count, st, &launched));
     c->launches += launched;
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+// ---------------- routing limited to groups, and the weights' gradient ----------------
+
+int moe_route_groups(moe_ctx* c, int64_t T, const float* logits, const float* bias, int groups, int top_groups, int renormalize,
+                     float scale, int32_t* topk_idx, float* topk_w, int flags, void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "moe_route_groups takes device pointers and no flag but MOE_F_SYNC");
+    if (T < 0 || T > kRouteTopkMaxTokens) return fail(MOE_EINVAL, "T=%lld not in [0,%d]", (long long)T, kRouteTopkMaxTokens);
+    const int E = c->cfg.n_experts, K = c->cfg.top_k;
+    if (groups < 1 || groups > kRouteMaxGroups || E % groups)
+        return fail(MOE_EINVAL, "%d groups: a divisor of the %d experts in [1,%d] is needed", groups, E, kRouteMaxGroups);
+    if (top_groups < 1 || top_groups > groups) return fail(MOE_EINVAL, "top_groups=%d not in [1,%d]", top_groups, groups);
+    if (top_groups * (E / groups) < K) return fail(MOE_EINVAL, "%d groups of %d experts have no %d choices", top_groups, E / groups, K);
+    if (bias && c->cfg.scoring == MOE_SCORING_SOFTMAX) return fail(MOE_EINVAL, "softmax scoring takes no bias");
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(MOE_EINVAL, "scale must be finite");
+    if (T && (!logits || !topk_idx || !topk_w)) return fail(MOE_EINVAL, "null argument");
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T) {
+        RouteGroupsArgs a{logits, bias, T, E, K, c->cfg.scoring, groups, top_groups, renormalize != 0, scale, topk_idx, topk_w, call_err(c)};
+        CUDA_TRY(launch_route_groups(a, c->sm_count, st));
+        c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+int moe_route_backward(moe_ctx* c, int64_t T, const float* logits, const int32_t* topk_idx, const float* dw, int renormalize, float scale,
+                       float* dlogits, int flags, void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~(MOE_F_SYNC | MOE_F_ACCUMULATE)) return fail(MOE_EINVAL, "moe_route_backward takes device pointers");
+    if (T < 0 || T > kRouteTopkMaxTokens) return fail(MOE_EINVAL, "T=%lld not in [0,%d]", (long long)T, kRouteTopkMaxTokens);
+    if (!(scale > -INFINITY && scale < INFINITY)) return fail(MOE_EINVAL, "scale must be finite");
+    if (T && (!logits || !topk_idx || !dw || !dlogits)) return fail(MOE_EINVAL, "null argument");
+    const size_t n = (size_t)T * c->cfg.n_experts * 4, k = (size_t)T * c->cfg.top_k * 4;
+    if (overlap(dlogits, n, logits, n) || overlap(dlogits, n, topk_idx, k) || overlap(dlogits, n, dw, k))
+        return fail(MOE_EINVAL, "dlogits overlaps an operand");
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T) {
+        RouteBackwardArgs a{logits, topk_idx, dw, T, c->cfg.n_experts, c->cfg.top_k, c->cfg.scoring, renormalize != 0,
+                            (flags & MOE_F_ACCUMULATE) != 0, scale, dlogits, call_err(c)};
+        CUDA_TRY(launch_route_backward(a, c->sm_count, st));
+        c->launches++;
+    }
     return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
 }
 

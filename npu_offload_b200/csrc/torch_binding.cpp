@@ -1,4 +1,4 @@
-// Torch-side half of the calls that allocate through torch (e4m3, balance loss, norm): checks, allocation of results and working memory, and
+// Torch-side half of the calls that allocate through torch (e4m3, routing in groups, balance loss, norm): checks, allocation of results and working memory, and
 // the call of the C ABI.  These calls take a few microseconds on the GPU at one token; through Python and
 // ctypes the host needed 11 us (quantiser, product) to 30 us (loss and gradient) for them.
 //
@@ -297,6 +297,43 @@ std::pair<Tensor, c10::optional<Tensor>> add_norm_backward(const Plane& p, Tenso
     return {dx, dw};
 }
 
+Tensor router_logits(const Plane& p, Tensor t) {
+    t = operand(p, "logits", std::move(t), {at::kFloat}, 2);
+    if (t.size(1) != p.E) refuse("logits are ", shape(t.sizes()), ", the context has ", p.E, " experts");
+    return t;
+}
+
+std::pair<Tensor, Tensor> route_groups(const Plane& p, Tensor logits, int64_t groups, int64_t top_groups, c10::optional<Tensor> bias,
+                                       bool renormalize, double scale, int64_t stream) {
+    logits = router_logits(p, std::move(logits));
+    if (bias) {
+        bias = operand(p, "bias", bias->detach(), {at::kFloat}, 1);  // (it only selects: no gradient is lost)
+        if (bias->size(0) != p.E) refuse("bias is ", shape(bias->sizes()), ", the context has ", p.E, " experts");
+    }
+    if (groups < INT32_MIN || groups > INT32_MAX || top_groups < INT32_MIN || top_groups > INT32_MAX) refuse("groups are out of range");
+    const int64_t T = logits.size(0);
+    const Tensor idx = at::empty({T, p.K}, at::TensorOptions(p.device).dtype(at::kInt));
+    const Tensor w = at::empty({T, p.K}, at::TensorOptions(p.device).dtype(at::kFloat));
+    check(moe_route_groups(p.ctx, T, ptr<float>(logits), ptr<float>(bias), (int)groups, (int)top_groups, renormalize, (float)scale,
+                           ptr<int32_t>(idx), ptr<float>(w), 0, (void*)stream));
+    return {idx, w};
+}
+
+Tensor route_backward(const Plane& p, Tensor logits, Tensor idx, Tensor dw, bool renormalize, double scale, const c10::optional<Tensor>& out,
+                      bool accumulate, int64_t stream) {
+    logits = router_logits(p, std::move(logits));
+    const int64_t T = logits.size(0), pairs[2] = {T, p.K};
+    idx = operand(p, "idx", std::move(idx), {at::kInt}, 2);
+    dw = operand(p, "dw", std::move(dw), {at::kFloat}, 2);
+    if (idx.sizes() != at::IntArrayRef(pairs) || dw.sizes() != at::IntArrayRef(pairs))
+        refuse("idx ", shape(idx.sizes()), " and dw ", shape(dw.sizes()), " must be ", shape(pairs));
+    if (accumulate && !out) refuse("accumulate needs an out to add to");
+    const Tensor o = output(p, out, {T, p.E}, at::kFloat, false);
+    check(moe_route_backward(p.ctx, T, ptr<float>(logits), ptr<int32_t>(idx), ptr<float>(dw), renormalize, (float)scale, ptr<float>(o),
+                             accumulate ? MOE_F_ACCUMULATE : 0, (void*)stream));
+    return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
@@ -309,6 +346,8 @@ PYBIND11_MODULE(_torch_binding, m) {
     m.def("experts_fp8", &experts_fp8);
     m.def("balance_loss", &balance_loss);
     m.def("balance_loss_backward", &balance_loss_backward);
+    m.def("route_groups", &route_groups);
+    m.def("route_backward", &route_backward);
     m.def("add_norm", &add_norm);
     m.def("add_norm_backward", &add_norm_backward);
 }

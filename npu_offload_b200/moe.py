@@ -453,6 +453,29 @@ class MoEDataPlane:
         check(lib().moe_route_topk(self._h, T, _vp(lg), _vp(b), _vp(idx), _vp(w), 0, _raw_stream(self._index)))
         return idx, w
 
+    def route_groups(self, logits, groups, top_groups, bias=None, renormalize=True, scale=1.0, stream=None):
+        """The router limited to the best groups of experts: (idx [T, top_k] int32, w [T, top_k] fp32), on the device.
+
+        logits [T, E] fp32; `groups` groups of E / groups neighbours, of which the top_groups best are open: by their largest
+        logit (softmax scoring), or by the sum of their two largest s + bias (sigmoid; bias [E] fp32 only selects).  Then the
+        top_k best experts of those, the best first, ties to the lower index; w = scale * softmax probability or s, divided by
+        the chosen ones' sum where renormalize is set.  The weights' gradient is route_backward()."""
+        if stream is not None:
+            with self._on(stream):
+                return self.route_groups(logits, groups, top_groups, bias, renormalize, scale)
+        p = self._plane or self._bind()
+        return _calls.route_groups(p, _tensor("logits", logits), groups, top_groups, bias, renormalize, scale, _raw_stream(self._index))
+
+    def route_backward(self, logits, idx, dw, renormalize=True, scale=1.0, out=None, accumulate=False, stream=None):
+        """dlogits [T, E] fp32 from dw [T, top_k], the gradient of route_groups()'s or route_topk()'s weights at idx (negative:
+        no choice); renormalize and scale as they were routed with.  accumulate: out +=, as behind balance_loss_backward()."""
+        if stream is not None:
+            with self._on(stream):
+                return self.route_backward(logits, idx, dw, renormalize, scale, out, accumulate)
+        p = self._plane or self._bind()
+        return _calls.route_backward(p, _tensor("logits", logits), _tensor("idx", idx), _tensor("dw", dw), renormalize, scale, out, accumulate,
+                                     _raw_stream(self._index))
+
     # ---- the router's load-balance loss ----
     def balance_loss(self, logits, idx, offsets=None, mask=None, stream=None):
         """(loss, BalanceStats): the router's load-balance loss over each sequence, and per-expert counts.
