@@ -346,6 +346,21 @@ MOE_API int moe_add_norm_backward(moe_ctx* ctx, int64_t T, int64_t C, const void
                                   int stream_dtype, const void* dsum, const void* weight, int weight_dtype, const float* rstd,
                                   void* dx, float* dweight, void* workspace, int64_t workspace_bytes, int flags, void* stream);
 
+/* ---- Low-rank adapters of many requests beside a shared projection ----
+ *
+ * moe_add_lora: x [T, K] bf16, the projection's input; base [T, N] its result (moe_matmul_fp8's, say), bf16 or fp32; n adapters,
+ * a [n, r, K] and b [n, N, r] bf16; ids [T]: each token's adapter, negative for none; scale [n] fp32 (NULL: 1)
+ *   out[t] = base[t] + scale[i] * (x[t] . a[i]^T) . b[i]^T,  i = ids[t];   out[t] = base[t] without an adapter
+ * with fp32 sums, rounded once, of base's type.  out may be base (tokens without an adapter are then not touched) and else overlaps
+ * nothing.  An id of n or more is none, and MOE_EINVAL in the device-side status.  T at most 2^20, K and r multiples of 8, K and N
+ * at most 2^20, r at most 128, n 1 to 4096.  Device pointers; x, a, b, base and out 16-byte aligned.  A token's result does not depend on
+ * the others of the call in more than its sums' order, nor on timing.  workspace: moe_add_lora_workspace bytes, 256-byte aligned
+ * (-1: out of range). */
+MOE_API int64_t moe_add_lora_workspace(moe_ctx* ctx, int64_t T, int64_t n);
+MOE_API int moe_add_lora(moe_ctx* ctx, int64_t T, int64_t K, int64_t N, int64_t r, int64_t n, const void* base, const uint16_t* x,
+                         const uint16_t* a, const uint16_t* b, const int32_t* ids, const float* scale, void* out, int out_dtype,
+                         void* workspace, int64_t workspace_bytes, int flags, void* stream);
+
 /* The router's exponential, y[i] = exp(x[i]) rounded once to fp32 (correctly rounded), on the
  * calling thread's current device, asynchronously on `stream`; x and y are device pointers.  It is
  * the exp of the softmax numerators (host.rs.tpl:249, `(v - m).exp()`) and of the sigmoid

@@ -17,6 +17,10 @@ constexpr int kBalanceMaxTokens = 1 << 24;
 constexpr int kBalanceMaxSeqs = 1 << 16;
 constexpr int kNormMaxRows = 1 << 24;
 constexpr int kNormMaxCols = 16384;
+constexpr int kLoraMaxTokens = 1 << 20;
+constexpr int kLoraMaxCols = 1 << 20;      // K and N
+constexpr int kLoraMaxRank = 128;
+constexpr int kLoraMaxAdapters = 4096;
 
 // Latched device-side error bits (ctx->dev_err); host maps them to MOE_E* codes.
 constexpr uint32_t kErrNonFinite = 1u;

@@ -17,6 +17,7 @@
 #include "block.h"
 #include "experts.h"
 #include "fp8.h"
+#include "lora.h"
 #include "norm.h"
 #include "route.h"
 #include "route_groups.h"
@@ -1848,6 +1849,45 @@ int moe_route_backward(moe_ctx* c, int64_t T, const float* logits, const int32_t
                             (flags & MOE_F_ACCUMULATE) != 0, scale, dlogits, call_err(c)};
         CUDA_TRY(launch_route_backward(a, c->sm_count, st));
         c->launches++;
+    }
+    return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
+}
+
+// ---------------- low-rank adapters ----------------
+
+int64_t moe_add_lora_workspace(moe_ctx* c, int64_t T, int64_t n) {
+    if (!c || T < 0 || T > kLoraMaxTokens || n < 1 || n > kLoraMaxAdapters) return -1;
+    return (int64_t)lora_workspace((int)T, (int)n);
+}
+
+int moe_add_lora(moe_ctx* c, int64_t T, int64_t K, int64_t N, int64_t r, int64_t n, const void* base, const uint16_t* x, const uint16_t* a,
+                 const uint16_t* b, const int32_t* ids, const float* scale, void* out, int out_dtype, void* workspace,
+                 int64_t workspace_bytes, int flags, void* stream) {
+    if (!c) return fail(MOE_EINVAL, "null context");
+    if (flags & ~MOE_F_SYNC) return fail(MOE_EINVAL, "moe_add_lora takes device pointers and no flag but MOE_F_SYNC");
+    if (!float_dtype(out_dtype)) return fail(MOE_EINVAL, "out_dtype %d is neither MOE_DT_BF16 nor MOE_DT_F32", out_dtype);
+    if (T < 0 || T > kLoraMaxTokens) return fail(MOE_EINVAL, "T=%lld not in [0,%d]", (long long)T, kLoraMaxTokens);
+    if (K < 8 || K % 8 || K > kLoraMaxCols) return fail(MOE_EINVAL, "K=%lld is not a multiple of 8 in [8,%d]", (long long)K, kLoraMaxCols);
+    if (N < 0 || N > kLoraMaxCols) return fail(MOE_EINVAL, "N=%lld not in [0,%d]", (long long)N, kLoraMaxCols);
+    if (r < 8 || r % 8 || r > kLoraMaxRank) return fail(MOE_EINVAL, "r=%lld is not a multiple of 8 in [8,%d]", (long long)r, kLoraMaxRank);
+    if (n < 1 || n > kLoraMaxAdapters) return fail(MOE_EINVAL, "n=%lld not in [1,%d]", (long long)n, kLoraMaxAdapters);
+    DeviceGuard dg(c->dev);
+    cudaStream_t st = (cudaStream_t)stream;
+    if (T && N) {
+        if (!base || !x || !a || !b || !ids || !out) return fail(MOE_EINVAL, "null argument");
+        if (!aligned16(base) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out))
+            return fail(MOE_EINVAL, "base, x, a, b and out must be 16-byte aligned");
+        const size_t no = (size_t)T * N * dtype_bytes(out_dtype);
+        if ((out != base && overlap(out, no, base, no)) || overlap(out, no, x, (size_t)T * K * 2) || overlap(out, no, a, (size_t)n * r * K * 2) ||
+            overlap(out, no, b, (size_t)n * N * r * 2) || overlap(out, no, ids, (size_t)T * 4) || overlap(out, no, scale, (size_t)n * 4))
+            return fail(MOE_EINVAL, "out overlaps an operand");
+        const int64_t need = moe_add_lora_workspace(c, T, n);
+        if (need && (!workspace || (uintptr_t)workspace & 255)) return fail(MOE_EINVAL, "the workspace must be 256-byte aligned");
+        if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+        LoraArgs l{base, x, a, b, ids, scale, (int)T, (int)K, (int)N, (int)r, (int)n, out, out_dtype == MOE_DT_F32, workspace, call_err(c)};
+        int launched = 0;
+        CUDA_TRY(launch_add_lora(l, c->sm_count, st, &launched));
+        c->launches += launched;
     }
     return (flags & MOE_F_SYNC) ? finish_sync(c, st) : MOE_OK;
 }

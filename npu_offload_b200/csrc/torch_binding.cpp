@@ -1,4 +1,4 @@
-// Torch-side half of the calls that allocate through torch (e4m3, routing in groups, balance loss, norm): checks, allocation of results and working memory, and
+// Torch-side half of the calls that allocate through torch (e4m3, routing in groups, balance loss, norm, adapters): checks, allocation of results and working memory, and
 // the call of the C ABI.  These calls take a few microseconds on the GPU at one token; through Python and
 // ctypes the host needed 11 us (quantiser, product) to 30 us (loss and gradient) for them.
 //
@@ -334,6 +334,39 @@ Tensor route_backward(const Plane& p, Tensor logits, Tensor idx, Tensor dw, bool
     return o;
 }
 
+// Read in place, like the e4m3 weights: never copied.
+Tensor adapter(const Plane& p, const char* name, const Tensor& t) {
+    if (t.defined() && t.device() == p.device) {
+        if (!t.is_contiguous()) refuse(name, " must be contiguous");
+        if ((uintptr_t)t.data_ptr() % 16) refuse(name, " must be 16-byte aligned: clone it once");
+    }
+    return operand(p, name, t, {at::kBFloat16}, 3, 16);
+}
+
+Tensor add_lora(const Plane& p, Tensor base, Tensor x, const Tensor& at_a, const Tensor& at_b, Tensor ids, c10::optional<Tensor> scale,
+                const c10::optional<Tensor>& out, int64_t stream) {
+    base = operand(p, "base", std::move(base), {at::kBFloat16, at::kFloat}, 2, 16);
+    x = operand(p, "x", std::move(x), {at::kBFloat16}, 2, 16);
+    const Tensor a = adapter(p, "a", at_a), b = adapter(p, "b", at_b);
+    const int64_t T = x.size(0), K = x.size(1), N = b.size(1), r = a.size(1), n = a.size(0);
+    if (a.size(2) != K) refuse("a is ", shape(a.sizes()), " for x of ", K, " columns");
+    if (b.size(0) != n || b.size(2) != r) refuse("b is ", shape(b.sizes()), " beside a of ", shape(a.sizes()));
+    if (base.size(0) != T || base.size(1) != N) refuse("base is ", shape(base.sizes()), ", not (", T, ", ", N, ")");
+    ids = operand(p, "ids", std::move(ids), {at::kInt}, 1);
+    if (ids.size(0) != T) refuse("ids has ", ids.size(0), " tokens, x ", T);
+    if (scale) {
+        scale = operand(p, "scale", *scale, {at::kFloat}, 1);
+        if (scale->size(0) != n) refuse("scale has ", scale->size(0), " values for ", n, " adapters");
+    }
+    const Tensor o = output(p, out, {T, N}, base.scalar_type(), true);
+    if (o.scalar_type() != base.scalar_type()) refuse("out is ", name_of(o.scalar_type()), ", base ", name_of(base.scalar_type()));
+    const int64_t bytes = moe_add_lora_workspace(p.ctx, T, n);
+    const Tensor ws = workspace(p, bytes);
+    check(moe_add_lora(p.ctx, T, K, N, r, n, base.data_ptr(), ptr<uint16_t>(x), ptr<uint16_t>(a), ptr<uint16_t>(b), ptr<int32_t>(ids),
+                       ptr<float>(scale), o.data_ptr(), dtype_of(o), ws.data_ptr(), bytes, 0, (void*)stream));
+    return o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_binding, m) {
@@ -348,6 +381,7 @@ PYBIND11_MODULE(_torch_binding, m) {
     m.def("balance_loss_backward", &balance_loss_backward);
     m.def("route_groups", &route_groups);
     m.def("route_backward", &route_backward);
+    m.def("add_lora", &add_lora);
     m.def("add_norm", &add_norm);
     m.def("add_norm_backward", &add_norm_backward);
 }

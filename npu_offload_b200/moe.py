@@ -525,6 +525,20 @@ class MoEDataPlane:
         return _calls.add_norm_backward(p, _tensor("dy", dy), _tensor("sum", sum), _tensor("weight", weight), _tensor("rstd", rstd), dsum,
                                         weight_grad, _raw_stream(self._index))
 
+    # ---- low-rank adapters beside a shared projection ----
+    def add_lora(self, base, x, a, b, ids, scale=None, out=None, stream=None):
+        """out [T, N] = base + scale[i] * (x . a[i]^T) . b[i]^T for each token's adapter i = ids[t] (negative: base alone).
+
+        base [T, N] (bf16 or fp32) is the shared projection of x [T, K] bf16, matmul_fp8()'s result for instance; a [n, r, K]
+        and b [n, N, r] bf16, contiguous; K and r multiples of 8, r at most 128; ids [T] int32; scale [n] fp32 (None: 1).
+        fp32 sums, one rounding.  out may be base: tokens without an adapter are then left as they are."""
+        if stream is not None:
+            with self._on(stream):
+                return self.add_lora(base, x, a, b, ids, scale, out)
+        p = self._plane or self._bind()
+        return _calls.add_lora(p, _tensor("base", base), _tensor("x", x), _tensor("a", a), _tensor("b", b), _tensor("ids", ids), scale, out,
+                               _raw_stream(self._index))
+
     def _on(self, stream):
         if stream.device != self.device:
             raise ValueError(f"stream is on {stream.device}, the context on {self.device}")
