@@ -20,7 +20,7 @@ NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 SOURCES = ["moe_dp.cu", "route.cu", "experts.cu", "decode.cu", "noalloc.cu", "prefill.cu", "prefill_tc.cu",
            "block.cu", "fp8_quant.cu", "fp8_gemm.cu", "balance.cu", "norm.cu",
-           "norm_backward.cu", "route_groups.cu", "lora.cu"]
+           "norm_backward.cu", "route_groups.cu", "lora.cu", "lora_many.cu"]
 
 
 def cute_include():

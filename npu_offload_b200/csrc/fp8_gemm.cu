@@ -32,18 +32,6 @@ bool encode2(EncodeTiledFn enc, CUtensorMap* m, const void* base, int64_t cols, 
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Lets a kernel use `bytes` of dynamic shared memory, on every device that it runs on.
-template <auto kernel>
-cudaError_t allow_smem(int bytes) {
-    static unsigned long long done = 0;  // a bit a device; setting it twice does no harm
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1))) return e;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
-    return e;
-}
-
 template <int MODE, int NQ>
 struct Few {
     using C = FewCfg<MODE, NQ>;

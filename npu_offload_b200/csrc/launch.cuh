@@ -42,6 +42,18 @@ cudaError_t launch_after(K kernel, int grid, int threads, int smem, int cluster,
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// Lets a kernel use `bytes` of dynamic shared memory, on every device that it runs on.
+template <auto kernel>
+cudaError_t allow_smem(int bytes) {
+    static unsigned long long done = 0;  // a bit a device; setting it twice does no harm
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) >> dev & 1))) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) __atomic_fetch_or(&done, 1ull << dev, __ATOMIC_RELAXED);
+    return e;
+}
+
 // The same for the norm, grouped routing and adapter kernels: each waits at its very start, reads nothing ahead of that
 // and lets nothing start before its end.  What overlaps the kernel before is the launch alone.
 struct Launch {

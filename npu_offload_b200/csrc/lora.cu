@@ -114,10 +114,17 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
     }
 }
 
-size_t lora_workspace(int T, int n) { return 0; }
+// Calls of at most so many tokens take a cluster a token.
+#ifndef LORA_FEW
+#define LORA_FEW 128
+#endif
+constexpr int kLoraFewTokens = LORA_FEW;
+
+size_t lora_workspace(int T, int n) { return T <= kLoraFewTokens ? 0 : lora_many_workspace(T, n); }
 
 cudaError_t launch_add_lora(const LoraArgs& a, int sm_count, cudaStream_t st, int* launches) {
     if (a.T <= 0 || a.N <= 0) return cudaSuccess;
+    if (a.T > kLoraFewTokens) return launch_lora_many(a, st, launches);
     const Launch l{a.T * kLoraCluster, kLoraThreads, 0, 0, st};
     ++*launches;
     if (a.r <= 8) return l.run(lora_few_kernel<1>, a);

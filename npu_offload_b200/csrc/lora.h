@@ -20,6 +20,8 @@ struct LoraArgs {
     uint32_t* err;
 };
 size_t lora_workspace(int T, int n);
+size_t lora_many_workspace(int T, int n);
+cudaError_t launch_lora_many(const LoraArgs& a, cudaStream_t st, int* launches);  // two kernels, any T
 cudaError_t launch_add_lora(const LoraArgs& a, int sm_count, cudaStream_t st, int* launches);
 
 }  // namespace moe
