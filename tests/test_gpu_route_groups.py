@@ -276,3 +276,83 @@ def test_the_library_refuses():
                                (dict(flags=1), "device pointers")):
                 assert back(**kw) == _lib.MOE_EINVAL and needle in _lib.last_error(), kw
             assert p.launch_count == 0
+
+
+# ---------------------------------------------------------------- calls of many tokens (another kernel, by size)
+
+def sorted_choice(logits, groups, top, K, bias, scoring):
+    """choose() by stable sorts on the GPU, for many tokens (NaN as -inf)."""
+    key = torch.from_numpy(keys(logits, bias, scoring)).cuda()
+    key = torch.where(key.isnan(), float("-inf"), key)
+    T, E = key.shape
+    best = key.view(T, groups, E // groups).sort(dim=-1, descending=True)[0]
+    score = best[..., 0] if scoring == "softmax" or E == groups else best[..., 0] + best[..., 1]
+    score = torch.where(score.isnan(), float("-inf"), score)
+    chosen = score.sort(dim=-1, descending=True, stable=True)[1][:, :top]
+    open_ = torch.zeros_like(score, dtype=torch.bool).scatter(1, chosen, True).repeat_interleave(E // groups, 1)
+    first = open_.float().sort(dim=-1, descending=True, stable=True)[1]  # open experts in front, in order
+    inside = key.gather(1, first)[:, : top * (E // groups)]
+    return first.gather(1, inside.sort(dim=-1, descending=True, stable=True)[1])[:, :K].int()
+
+
+MANY = [(32, 2, 8, 3), (32, 8, 1, 1), (64, 6, 8, 2), (64, 8, 4, 4), (96, 4, 4, 1), (128, 8, 8, 3), (128, 1, 2, 1), (160, 6, 8, 3), (192, 8, 2, 1), (224, 5, 8, 8),
+        (256, 8, 8, 4), (256, 8, 1, 1), (256, 8, 4, 2), (256, 8, 8, 1), (256, 9, 8, 4), (248, 8, 8, 4), (240, 8, 16, 4)]
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,K,groups,top", MANY)
+def test_many_tokens_of_all_kinds(E, K, groups, top, scoring):
+    """Random logits, few values, values a step apart, biases that decide, masked experts; numbers of tokens that leave a rest."""
+    with plane(E, K, scoring) as p:
+        g = gen(7 * E + K)
+        for T in (9602, 9475):
+            rnd = torch.randn(T, E, generator=g, device="cuda")
+            kinds = [rnd, (rnd * 2).round() / 2, 1 + torch.randint(0, 9, (T, E), generator=g, device="cuda") * 2.0 ** -23, rnd * 1e-3 - 15]
+            if scoring == "softmax":
+                kinds.append(torch.where(rnd > 1, float("-inf"), rnd))
+            for logits in kinds:
+                bias = 0.05 * torch.randn(E, generator=g, device="cuda") if scoring == "sigmoid" else None
+                for b in ({None} if bias is None else {None, bias, 1e4 * bias, torch.where(bias > 0.05, float("-inf"), bias)}):
+                    for renormalize in (True, False):
+                        idx, w = p.route_groups(logits, groups, top, bias=b, renormalize=renormalize, scale=1.5)
+                        assert torch.equal(idx, sorted_choice(logits, groups, top, K, b, scoring))
+                        want = weights64(logits, idx, scoring, renormalize, 1.5)
+                        assert ((w.double() - want).abs() <= WEIGHT * want + 1e-37).all()
+        assert p.status() == 0
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_many_tokens_with_errors_among_them(scoring):
+    from npu_offload_b200._lib import MOE_ENONFINITE, MOE_OK
+    with plane(128, 8, scoring) as p:
+        T = 9503
+        logits = torch.randn(T, 128, generator=gen(21), device="cuda")
+        want = p.route_groups(logits, 8, 3)
+        bad = torch.zeros(T, dtype=torch.bool, device="cuda")
+        for t in (0, 5, 1502, T - 1):
+            logits[t, (t * 7) % 128] = float("nan")
+            bad[t] = True
+        if scoring == "softmax":
+            logits[9] = float("-inf")
+            logits[10, 3] = float("inf")
+            bad[9] = bad[10] = True
+        idx, w = p.route_groups(logits, 8, 3)
+        assert p.status() == MOE_ENONFINITE and p.status() == MOE_OK
+        assert torch.equal(idx[~bad], want[0][~bad]) and torch.equal(w[~bad], want[1][~bad]) and w[bad].isnan().all()
+        assert torch.equal(idx, sorted_choice(logits, 8, 3, 8, None, scoring))
+        if scoring == "sigmoid":
+            logits = torch.randn(T, 128, generator=gen(22), device="cuda")
+            bias = torch.zeros(128, device="cuda")
+            bias[17] = float("nan")
+            w = p.route_groups(logits, 8, 3, bias=bias)[1]
+            assert p.status() == MOE_ENONFINITE and w.isnan().all()
+
+
+def test_few_and_many_tokens_agree():
+    """The same rows in a call of few and in one of many: the same choices and weights to the last steps."""
+    for scoring in ("softmax", "sigmoid"):
+        with plane(256, 8, scoring) as p:
+            logits = torch.randn(10000, 256, generator=gen(23), device="cuda")
+            many = p.route_groups(logits, 8, 4)
+            few = p.route_groups(logits[:100].clone(), 8, 4)
+            assert torch.equal(many[0][:100], few[0]) and (many[1][:100] - few[1]).abs().max() <= WEIGHT
