@@ -605,123 +605,195 @@ cudaError_t launch_route_groups(const RouteGroupsArgs& a, int sm_count, cudaStre
 //   softmax: dL/dl_e = v_e (dL/dv_e - sum_j dL/dv_j v_j);   sigmoid: dL/dl_e = dL/dv_e s_e (1 - s_e)
 // Where weights are renormalised, or sigmoids, the chosen experts alone have a gradient and only their logits are read:
 // p = v / W gives (softmax) p_k (g_k - sum g p), (sigmoid) (1 - s_k) p_k (g_k - sum g p), g_k s_k (1 - s_k) without.
-// A warp a token: the choices on lanes 0 to K - 1, their values put in place through a row in shared memory, which is
-// then written as it lies.  Bounded by HBM: T E 4 bytes written, and read where the softmax needs its sum.
-template <int V, bool DENSE>
+// Four tokens a warp, whose four rows are one run of memory, 8 lanes a token (K <= 8; else 16, two tokens after two): zeros go out
+// while choices and chosen logits are on their way, the values over them (they meet in L2; a run put together in shared memory
+// first: 23.6 us at 65536 x 256, so 21.3).  Where the softmax needs the sum over its row (route_dense_kernel), a warp a token.
+// Bounded by HBM: T E 4 bytes written, and read where the softmax needs its sum.
+
+// Choices and their gradients: the same expert twice on the lanes of one token: its first lane takes the sum, in the
+// choices' order, and `first` is false on the others.  All lanes of the warp; lanes of other tokens never match.
+template <int LANES>
+__device__ __forceinline__ void merge_repeated(int key, bool in, float& d, bool& first) {
+    const unsigned same = __match_any_sync(0xffffffffu, key);
+    first = in;
+    if (!__any_sync(0xffffffffu, in && __popc(same) > 1)) return;
+    const int lane = threadIdx.x & 31, at = lane & ~(LANES - 1);
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < LANES; k++) {
+        const float dk = __shfl_sync(0xffffffffu, d, at + k);
+        if (same >> (at + k) & 1) sum += dk;
+    }
+    if (in) d = sum;
+    first = in && __ffs(same) - 1 == lane;
+}
+template <int LANES>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+struct Choice {
+    int i;       // the expert; -1: none
+    float g, x;  // scale dL/dw, logit
+};
+// dL/dl of a token's choices, on LANES lanes.
+template <int LANES>
+__device__ __forceinline__ float choice_gradient(const RouteBackwardArgs& a, const Choice& c) {
+    const bool in = c.i >= 0;
+    float d;
+    if (a.scoring == 0) {
+        const float x = in ? c.x : -INFINITY;
+        float m = x;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const float v = in ? expf(x - m) : 0.f, total = lanes_sum<LANES>(v), p = in ? __fdiv_rn(v, total) : 0.f;
+        d = p * (c.g - lanes_sum<LANES>(in ? c.g * p : 0.f));
+    } else {
+        // s and 1 - s from exp(-|l|), so that neither loses bits where the other is near 1
+        const float x = in ? c.x : 0.f, q = expf(-fabsf(x)), big = __fdiv_rn(1.f, 1.f + q), small = q * big;
+        const float s = x >= 0.f ? big : small, rest = x >= 0.f ? small : big;
+        if (a.renormalize) {
+            const float total = lanes_sum<LANES>(in ? s : 0.f) + 1e-20f, p = in ? __fdiv_rn(s, total) : 0.f;
+            d = rest * p * (c.g - lanes_sum<LANES>(in ? c.g * p : 0.f));
+        } else {
+            d = c.g * s * rest;
+        }
+    }
+    return in ? d : 0.f;
+}
+
+template <int LANES>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_backward_kernel(RouteBackwardArgs a, bool vec) {
+    griddep_wait();
+    constexpr int kPasses = LANES / 8;  // of 32 / LANES tokens
+    const int lane = threadIdx.x & 31, E = a.E, K = a.K, k = lane & (LANES - 1);
+    const int64_t set = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+    if (set * 4 >= a.T) return;  // the whole warp
+    auto token = [&](int pass) { return set * 4 + pass * (32 / LANES) + lane / LANES; };
+    float* out = a.dlogits + set * 4 * E;
+    Choice c[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; p++) {
+        const int64_t t = token(p);
+        c[p] = Choice{-1, 0.f, 0.f};
+        if (t < a.T && k < K) c[p].i = a.idx[t * K + k], c[p].g = a.dw[t * K + k] * a.scale;
+    }
+    if (!a.accumulate) {
+        const int n = (int)min((int64_t)4, a.T - set * 4) * E;
+        if (vec) {
+            for (int i = lane * 4; i + 4 <= n; i += 128) *reinterpret_cast<float4*>(out + i) = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (lane < (n & 3)) out[(n & ~3) + lane] = 0.f;
+        } else {
+            for (int i = lane; i < n; i += 32) out[i] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; p++) {
+        if (c[p].i >= E) {
+            atomicOr(a.err, kErrBadIndex);
+            c[p].i = -1;
+        }
+        if (c[p].i >= 0) c[p].x = a.logits[token(p) * E + c[p].i];
+    }
+    __syncwarp();  // the zeros come before the values
+#pragma unroll
+    for (int p = 0; p < kPasses; p++) {
+        const int row = p * (32 / LANES) + lane / LANES;
+        float d = choice_gradient<LANES>(a, c[p]);
+        bool first;
+        merge_repeated<LANES>(c[p].i >= 0 ? row * E + c[p].i : -1 - lane, c[p].i >= 0, d, first);
+        float* at = out + row * E + c[p].i;
+        if (first) *at = a.accumulate ? __fadd_rn(*at, d) : d;  // (the gradient's own bits, added: not fused with its last product)
+    }
+}
+
+// Softmax probabilities as they are: every expert has a gradient.
+template <int V>
+__global__ void __launch_bounds__(kRouteWarps * 32) route_dense_kernel(RouteBackwardArgs a) {
     __shared__ __align__(16) float rows[kRouteWarps][32 * V];
     griddep_wait();
     const int lane = threadIdx.x & 31, E = a.E, K = a.K;
     float* s_row = rows[threadIdx.x >> 5];
-    for (int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5); t < a.T; t += (int64_t)gridDim.x * kRouteWarps) {
-        const float* row = a.logits + t * E;
-        float* out = a.dlogits + t * E;
-        int i = -1;
-        float g = 0.f;
-        if (lane < K) {
-            i = a.idx[t * K + lane];
-            g = a.dw[t * K + lane] * a.scale;
-        }
-        float l[V];
-        if (DENSE) {
 #pragma unroll
-            for (int j = 0; j < V; j++) l[j] = lane + 32 * j < E ? row[lane + 32 * j] : -INFINITY;
-        }
+    for (int j = 0; j < V; j++) s_row[lane + 32 * j] = 0.f;
+    __syncwarp();
+    const int64_t stride = (int64_t)gridDim.x * kRouteWarps;
+    int64_t t = (int64_t)blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+    float next[V], g_next = 0.f;
+    int i_next = -1;
+    auto ask = [&](int64_t t) {
+        const float* row = a.logits + t * E;
+        i_next = -1, g_next = 0.f;
+        if (t >= a.T) return;
+#pragma unroll
+        for (int j = 0; j < V; j++) next[j] = lane + 32 * j < E ? row[lane + 32 * j] : -INFINITY;
+        if (lane < K) i_next = a.idx[t * K + lane], g_next = a.dw[t * K + lane];
+    };
+    ask(t);
+    for (; t < a.T; t += stride) {
+        float* out = a.dlogits + t * E;
+        float l[V];
+        int i = i_next;
+        float g = g_next * a.scale;
+#pragma unroll
+        for (int j = 0; j < V; j++) l[j] = next[j];
+        ask(t + stride);
         if (i >= E) {
             atomicOr(a.err, kErrBadIndex);
             i = -1;
         }
         const bool in = i >= 0;
-        float d = 0.f;  // what goes to expert i: dL/dl, or (DENSE) dL/dv
-        float inv = 0.f, most = 0.f, dot = 0.f;
-        if (DENSE) {
-            most = l[0];
+        if (!in) g = 0.f;
+        float most = l[0];
 #pragma unroll
-            for (int j = 1; j < V; j++) most = fmaxf(most, l[j]);
+        for (int j = 1; j < V; j++) most = fmaxf(most, l[j]);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            float z = 0.f;
+        for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        float z = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                l[j] = exp2_hw((l[j] - most) * 1.44269504f);
-                z += l[j];
-            }
-            inv = __fdiv_rn(1.f, warp_sum(z));
-            d = in ? g : 0.f;
-            dot = warp_sum(in ? g * (exp2_hw((row[i] - most) * 1.44269504f) * inv) : 0.f);
-        } else if (a.scoring == 0) {
-            const float x = in ? row[i] : -INFINITY;
-            float m = x;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const float v = in ? expf(x - m) : 0.f, total = warp_sum(v), p = in ? __fdiv_rn(v, total) : 0.f;
-            d = p * (g - warp_sum(in ? g * p : 0.f));
-        } else {
-            // s and 1 - s from exp(-|l|), so that neither loses bits where the other is near 1
-            const float x = in ? row[i] : 0.f, q = expf(-fabsf(x)), big = __fdiv_rn(1.f, 1.f + q), small = q * big;
-            const float s = x >= 0.f ? big : small, rest = x >= 0.f ? small : big;
-            if (a.renormalize) {
-                const float total = warp_sum(in ? s : 0.f) + 1e-20f, p = in ? __fdiv_rn(s, total) : 0.f;
-                d = rest * p * (g - warp_sum(in ? g * p : 0.f));
-            } else {
-                d = g * s * rest;
-            }
+        for (int j = 0; j < V; j++) {
+            l[j] = exp2_hw((l[j] - most) * 1.44269504f);
+            z += l[j];
         }
-        if (!in) d = 0.f;
-        // the same expert twice: its first lane takes the sum, in the choices' order
-        const unsigned same = __match_any_sync(0xffffffffu, in ? i : -1 - lane);
-        bool first = in;
-        if (__any_sync(0xffffffffu, __popc(same) > 1)) {
-            float sum = 0.f;
-            for (int k = 0; k < K; k++) {
-                const float dk = __shfl_sync(0xffffffffu, d, k);
-                if (same >> k & 1) sum += dk;
-            }
-            if (in) d = sum;
-            first = in && __ffs(same) - 1 == lane;
-        }
-        if (!DENSE && a.accumulate) {
-            if (first) out[i] = __fadd_rn(out[i], d);  // (the gradient's own bits, added: not fused with its last product)
-            continue;
-        }
-#pragma unroll
-        for (int j = 0; j < V; j++) s_row[lane + 32 * j] = 0.f;
+        bool first;
+        merge_repeated<32>(in ? i : -1 - lane, in, g, first);
+        if (first) s_row[i] = g;
         __syncwarp();
-        if (first) s_row[i] = d;
-        __syncwarp();
-        if (DENSE) {
+        float dot = 0.f;
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const int e = lane + 32 * j;
-                if (e < E) {
-                    const float v = l[j] * inv * (s_row[e] - dot);
-                    out[e] = a.accumulate ? __fadd_rn(out[e], v) : v;
-                }
+        for (int j = 0; j < V; j++) dot = fmaf(s_row[lane + 32 * j], l[j], dot);
+        const float inv = __fdiv_rn(1.f, warp_sum(z));
+        dot = warp_sum(dot) * inv;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int e = lane + 32 * j;
+            if (e < E) {
+                const float v = l[j] * inv * (s_row[e] - dot);
+                out[e] = a.accumulate ? __fadd_rn(out[e], v) : v;
             }
-        } else if (V >= 4 && vec) {
-            for (int e = lane * 4; e < E; e += 128) *reinterpret_cast<float4*>(out + e) = *reinterpret_cast<const float4*>(s_row + e);
-        } else {
-#pragma unroll
-            for (int j = 0; j < V; j++)
-                if (lane + 32 * j < E) out[lane + 32 * j] = s_row[lane + 32 * j];
         }
+        __syncwarp();
+        if (first) s_row[i] = 0.f;
         __syncwarp();
     }
 }
 
 cudaError_t launch_route_backward(const RouteBackwardArgs& a, int sm_count, cudaStream_t st) {
     if (a.T <= 0) return cudaSuccess;
-    const int64_t blocks = (a.T + kRouteWarps - 1) / kRouteWarps;
-    const Launch l{(int)std::min<int64_t>(blocks, (int64_t)sm_count * 8), kRouteWarps * 32, 0, 0, st};
-    const bool dense = a.scoring == 0 && !a.renormalize, vec = a.E % 4 == 0 && (uintptr_t)a.dlogits % 16 == 0;
-#define ROUTE_BACKWARD(V) \
-    if (a.E <= 32 * V) return dense ? l.run(route_backward_kernel<V, true>, a, vec) : l.run(route_backward_kernel<V, false>, a, vec)
-    ROUTE_BACKWARD(1);
-    ROUTE_BACKWARD(2);
-    ROUTE_BACKWARD(4);
-    ROUTE_BACKWARD(8);
-#undef ROUTE_BACKWARD
-    return cudaErrorInvalidValue;
+    if (a.scoring == 0 && !a.renormalize) {
+        const int64_t blocks = (a.T + kRouteWarps - 1) / kRouteWarps;
+        const Launch l{(int)std::min<int64_t>(blocks, (int64_t)sm_count * 6), kRouteWarps * 32, 0, 0, st};
+        if (a.E <= 32) return l.run(route_dense_kernel<1>, a);
+        if (a.E <= 64) return l.run(route_dense_kernel<2>, a);
+        if (a.E <= 128) return l.run(route_dense_kernel<4>, a);
+        return l.run(route_dense_kernel<8>, a);
+    }
+    const bool vec = (uintptr_t)a.dlogits % 16 == 0;  // (four rows are a multiple of 16 bytes)
+    const int64_t blocks = ((a.T + 3) / 4 + kRouteWarps - 1) / kRouteWarps;
+    const Launch l{(int)blocks, kRouteWarps * 32, 0, 0, st};
+    return a.K <= 8 ? l.run(route_backward_kernel<8>, a, vec) : l.run(route_backward_kernel<16>, a, vec);
 }
 
 }  // namespace moe
