@@ -356,7 +356,7 @@ MOE_API int moe_add_norm_backward(moe_ctx* ctx, int64_t T, int64_t C, const void
  * at most 2^20, r at most 128, n 1 to 4096.  Device pointers; x, a, b, base and out 16-byte aligned.  A token's result does not depend on
  * the others of the call in more than its sums' order, nor on timing.  workspace: moe_add_lora_workspace bytes, 256-byte aligned
  * (-1: out of range). */
-MOE_API int64_t moe_add_lora_workspace(moe_ctx* ctx, int64_t T, int64_t n);
+MOE_API int64_t moe_add_lora_workspace(moe_ctx* ctx, int64_t T, int64_t r, int64_t n);
 MOE_API int moe_add_lora(moe_ctx* ctx, int64_t T, int64_t K, int64_t N, int64_t r, int64_t n, const void* base, const uint16_t* x,
                          const uint16_t* a, const uint16_t* b, const int32_t* ids, const float* scale, void* out, int out_dtype,
                          void* workspace, int64_t workspace_bytes, int flags, void* stream);

@@ -77,7 +77,7 @@ _SIGS = {
     "moe_add_norm": (_i, [_vp, _i64, _i64, _vp, _i, _vp, _i, _vp, _i, ctypes.c_float, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp]),
     "moe_add_norm_backward_workspace": (_i64, [_vp, _i64, _i64]),
     "moe_add_norm_backward": (_i, [_vp, _i64, _i64, _vp, _i, _vp, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i64, _i, _vp]),
-    "moe_add_lora_workspace": (_i64, [_vp, _i64, _i64]),
+    "moe_add_lora_workspace": (_i64, [_vp, _i64, _i64, _i64]),
     "moe_add_lora": (_i, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _vp, _i64, _i, _vp]),
     "moe_load_shared": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _i]),
     "moe_shared_router": (_i, [_vp, _i, _i, _vp, _vp, _vp, _vp, _i, _vp]),

@@ -54,8 +54,10 @@ cudaError_t allow_smem(int bytes) {
     return e;
 }
 
-// The same for the norm, grouped routing and adapter kernels: each waits at its very start, reads nothing ahead of that
-// and lets nothing start before its end.  What overlaps the kernel before is the launch alone.
+// The same for the norm, grouped routing and adapter kernels.  Each waits at its very start, but for lora_out_kernel, which reads tiles, base
+// and B ahead of its wait, past L1: it starts behind the waits of all CTAs of lora_low_kernel, so behind the end of the planning
+// kernel and of all before that.  Of a call's kernels all but the last let the next start once their own wait is over; the last
+// lets nothing start before its end.
 struct Launch {
     int grid, threads, smem, cluster;
     cudaStream_t st;

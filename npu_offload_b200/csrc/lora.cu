@@ -4,9 +4,10 @@
 //
 // One launch: a cluster of eight CTAs a token.  Each takes an eighth of the inner dimension of A for all r rows (a warp a
 // row, 16-byte loads), the partial sums go to all eight through distributed shared memory and are added there in order,
-// and each then takes an eighth of the columns of B, a thread a column, whose first rows are in registers by then.  All
-// sums are fp32; the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the
-// store), by the adapters' bytes for a batch of requests with adapters of their own.
+// and each then takes an eighth of the columns of B, whose first are in registers by then: a row of B is read by as many
+// neighbouring lanes as it has 16-byte words (a thread a row: 10.6 instead of 7.5 us at 32 tokens, r = 64).  All sums are fp32; the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the
+// store), by the adapters' bytes out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.7 us; 1280 x 32 x 4096, 48 tokens of 32
+// adapters: 6.6 us, 1.6 of them for the bytes from HBM.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -32,7 +33,7 @@ __device__ __forceinline__ void lora_store(const LoraArgs& a, size_t i, float v)
     else static_cast<uint16_t*>(a.out)[i] = f8_bf16(v);
 }
 
-// R: rank rows of A a warp, and 16-byte words of a row of B; r <= 8 R.
+// R: rank rows of A a warp, and 16-byte words of a row of B; r <= 8 R, R a power of two.
 template <int R>
 __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThreads) lora_few_kernel(LoraArgs a) {
     __shared__ float part[kLoraCluster][kLoraMaxRank], own[kLoraMaxRank], low[kLoraMaxRank];
@@ -52,13 +53,21 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
     const uint16_t* A = a.a + (size_t)id * r * a.K;
     const uint16_t* B = a.b + (size_t)id * a.N * r;
     const uint16_t* x = a.x + (size_t)t * a.K;
-    uint4 first[R];
-    float base = 0.f;
-    if (n0 + (int)threadIdx.x < n1) {
-        base = lora_load(a, out_row + n0 + threadIdx.x);
+    // Columns of B, 32 a warp: R neighbouring lanes a row of B, 16 bytes each, R rows after one another; the first are on their way early.
+    const int chunk = lane % R, g1 = (n1 - n0 + 31) / 32;
+    uint4 bv[R];
+    auto ask = [&](int g) {
 #pragma unroll
-        for (int k = 0; k < R; k++)
-            if (k * 8 < r) first[k] = ld_cg_u4(B + (size_t)(n0 + threadIdx.x) * r + k * 8);
+        for (int i = 0; i < R; i++) {
+            const int n = n0 + g * 32 + lane / R + 32 / R * i;
+            bv[i] = n < n1 && chunk * 8 < r ? ld_cg_u4(B + (size_t)n * r + chunk * 8) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    const int mine = lane / R + 32 / R * chunk;  // the column of 32 whose sum this lane ends up with
+    float base = 0.f;
+    if (warp < g1) {
+        ask(warp);
+        if (n0 + warp * 32 + mine < n1) base = lora_load(a, out_row + n0 + warp * 32 + mine);
     }
     float acc[R];
 #pragma unroll
@@ -92,39 +101,50 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
         low[threadIdx.x] = v * (a.scale ? a.scale[id] : 1.f);
     }
     __syncthreads();
-    for (int n = n0 + threadIdx.x; n < n1; n += kLoraThreads) {
-        if (n != n0 + (int)threadIdx.x) {
-            base = lora_load(a, out_row + n);
+    float l8[8];
 #pragma unroll
-            for (int k = 0; k < R; k++)
-                if (k * 8 < r) first[k] = ld_cg_u4(B + (size_t)n * r + k * 8);
+    for (int k = 0; k < 8; k++) l8[k] = chunk * 8 < r ? low[chunk * 8 + k] : 0.f;
+    for (int g = warp; g < g1; g += kLoraWarps) {
+        const int n = n0 + g * 32 + mine;
+        if (g != warp) {
+            ask(g);
+            if (n < n1) base = lora_load(a, out_row + n);
         }
-        float v = 0.f;
+        float v[R];
 #pragma unroll
-        for (int k = 0; k < R; k++)
-            if (k * 8 < r) {
-                const uint32_t w[4] = {first[k].x, first[k].y, first[k].z, first[k].w};
+        for (int i = 0; i < R; i++) {
+            const uint32_t w[4] = {bv[i].x, bv[i].y, bv[i].z, bv[i].w};
+            v[i] = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    v = fmaf(bf_lo(w[j]), low[k * 8 + 2 * j], v);
-                    v = fmaf(bf_hi(w[j]), low[k * 8 + 2 * j + 1], v);
-                }
+            for (int k = 0; k < 4; k++) {
+                v[i] = fmaf(bf_lo(w[k]), l8[2 * k], v[i]);
+                v[i] = fmaf(bf_hi(w[k]), l8[2 * k + 1], v[i]);
             }
-        lora_store(a, out_row + n, base + v);
+        }
+        // R sums over R lanes, one left on each: sum i on the lane with chunk i
+#pragma unroll
+        for (int o = R / 2; o > 0; o /= 2) {
+            const bool up = lane & o;
+#pragma unroll
+            for (int k = 0; k < o; k++) {
+                const float give = up ? v[k] : v[k + o];
+                v[k] = (up ? v[k + o] : v[k]) + __shfl_xor_sync(0xffffffffu, give, o);
+            }
+        }
+        if (n < n1) lora_store(a, out_row + n, base + v[0]);
     }
 }
 
-// Calls of at most so many tokens take a cluster a token.
-#ifndef LORA_FEW
-#define LORA_FEW 128
-#endif
-constexpr int kLoraFewTokens = LORA_FEW;
+// Calls of at most so many tokens take a cluster a token, others the kernels of lora_many.cu, us (a cluster a token / the others):
+//   r = 16: 64 tokens 5.8 / 11.3, 128: 11.4 / 11.3, 192: 16.1 / 12.0 (4096 x 2560)     r = 32: 64: 7.2 / 14.3, 128: 12.9 / 15.4 (1280 x 4096)
+//   r = 64: 32: 7.5 / 15.2, 64: 13.7 / 15.5, 96: 19.9 / 15.5 (1280 x 4096)              r = 128: 24: 19.8 / 20.4, 32: 21.7 / 20.5 (4096 x 2560)
+static int lora_few_tokens(int r) { return r <= 32 ? 128 : r <= 64 ? 64 : 24; }
 
-size_t lora_workspace(int T, int n) { return T <= kLoraFewTokens ? 0 : lora_many_workspace(T, n); }
+size_t lora_workspace(int T, int n, int r) { return T <= lora_few_tokens(r) ? 0 : lora_many_workspace(T, n, r); }
 
 cudaError_t launch_add_lora(const LoraArgs& a, int sm_count, cudaStream_t st, int* launches) {
     if (a.T <= 0 || a.N <= 0) return cudaSuccess;
-    if (a.T > kLoraFewTokens) return launch_lora_many(a, st, launches);
+    if (a.T > lora_few_tokens(a.r)) return launch_lora_many(a, sm_count, st, launches);
     const Launch l{a.T * kLoraCluster, kLoraThreads, 0, 0, st};
     ++*launches;
     if (a.r <= 8) return l.run(lora_few_kernel<1>, a);

@@ -19,9 +19,9 @@ struct LoraArgs {
     void* ws;               // lora_workspace bytes, 256-byte aligned
     uint32_t* err;
 };
-size_t lora_workspace(int T, int n);
-size_t lora_many_workspace(int T, int n);
-cudaError_t launch_lora_many(const LoraArgs& a, cudaStream_t st, int* launches);  // two kernels, any T
+size_t lora_workspace(int T, int n, int r);
+size_t lora_many_workspace(int T, int n, int r);
+cudaError_t launch_lora_many(const LoraArgs& a, int sm_count, cudaStream_t st, int* launches);  // three kernels, any T
 cudaError_t launch_add_lora(const LoraArgs& a, int sm_count, cudaStream_t st, int* launches);
 
 }  // namespace moe

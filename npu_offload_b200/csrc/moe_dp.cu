@@ -1855,9 +1855,9 @@ int moe_route_backward(moe_ctx* c, int64_t T, const float* logits, const int32_t
 
 // ---------------- low-rank adapters ----------------
 
-int64_t moe_add_lora_workspace(moe_ctx* c, int64_t T, int64_t n) {
-    if (!c || T < 0 || T > kLoraMaxTokens || n < 1 || n > kLoraMaxAdapters) return -1;
-    return (int64_t)lora_workspace((int)T, (int)n);
+int64_t moe_add_lora_workspace(moe_ctx* c, int64_t T, int64_t r, int64_t n) {
+    if (!c || T < 0 || T > kLoraMaxTokens || r < 8 || r > kLoraMaxRank || n < 1 || n > kLoraMaxAdapters) return -1;
+    return (int64_t)lora_workspace((int)T, (int)n, (int)r);
 }
 
 int moe_add_lora(moe_ctx* c, int64_t T, int64_t K, int64_t N, int64_t r, int64_t n, const void* base, const uint16_t* x, const uint16_t* a,
@@ -1881,7 +1881,7 @@ int moe_add_lora(moe_ctx* c, int64_t T, int64_t K, int64_t N, int64_t r, int64_t
         if ((out != base && overlap(out, no, base, no)) || overlap(out, no, x, (size_t)T * K * 2) || overlap(out, no, a, (size_t)n * r * K * 2) ||
             overlap(out, no, b, (size_t)n * N * r * 2) || overlap(out, no, ids, (size_t)T * 4) || overlap(out, no, scale, (size_t)n * 4))
             return fail(MOE_EINVAL, "out overlaps an operand");
-        const int64_t need = moe_add_lora_workspace(c, T, n);
+        const int64_t need = moe_add_lora_workspace(c, T, r, n);
         if (need && (!workspace || (uintptr_t)workspace & 255)) return fail(MOE_EINVAL, "the workspace must be 256-byte aligned");
         if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
         LoraArgs l{base, x, a, b, ids, scale, (int)T, (int)K, (int)N, (int)r, (int)n, out, out_dtype == MOE_DT_F32, workspace, call_err(c)};

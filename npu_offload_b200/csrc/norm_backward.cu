@@ -19,6 +19,7 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackwardArgs
     __shared__ float part[2][32];
     constexpr bool kAhead = THREADS <= kNormThreads;
     griddep_wait();
+    if (shares) griddep_launch_dependents();  // the shares' sum waits for this kernel's end before it does anything
     const int step = V ? 1 : blockDim.x, C = a.C;
     float w[N][8], dw[N][8];
 #pragma unroll

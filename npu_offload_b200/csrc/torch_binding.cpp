@@ -360,7 +360,7 @@ Tensor add_lora(const Plane& p, Tensor base, Tensor x, const Tensor& at_a, const
     }
     const Tensor o = output(p, out, {T, N}, base.scalar_type(), true);
     if (o.scalar_type() != base.scalar_type()) refuse("out is ", name_of(o.scalar_type()), ", base ", name_of(base.scalar_type()));
-    const int64_t bytes = moe_add_lora_workspace(p.ctx, T, n);
+    const int64_t bytes = moe_add_lora_workspace(p.ctx, T, r, n);
     const Tensor ws = workspace(p, bytes);
     check(moe_add_lora(p.ctx, T, K, N, r, n, base.data_ptr(), ptr<uint16_t>(x), ptr<uint16_t>(a), ptr<uint16_t>(b), ptr<int32_t>(ids),
                        ptr<float>(scale), o.data_ptr(), dtype_of(o), ws.data_ptr(), bytes, 0, (void*)stream));

@@ -166,4 +166,5 @@ def test_the_library_refuses(plane):
                        (dict(flags=2), "flag")):
         assert call(**kw) == _lib.MOE_EINVAL and needle in _lib.last_error(), kw
     assert plane.launch_count == before
-    assert L.moe_add_lora_workspace(plane.handle, 1 << 21, 1) == -1 and L.moe_add_lora_workspace(plane.handle, 1, 0) == -1
+    for bad in ((1 << 21, 8, 1), (1, 8, 0), (1, 0, 1), (-1, 8, 1)):
+        assert L.moe_add_lora_workspace(plane.handle, *bad) == -1

@@ -81,5 +81,5 @@ def test_a_stream_of_another_device_is_refused(plane, monkeypatch):
 
 def test_c_entry_points_report_a_null_context():
     L = nob.lib()
-    assert L.moe_add_lora_workspace(None, 1, 1) == -1
+    assert L.moe_add_lora_workspace(None, 1, 8, 1) == -1
     assert L.moe_add_lora(None, 1, 8, 8, 8, 1, None, None, None, None, None, None, None, 0, None, 0, 0, None) == _lib.MOE_EINVAL
