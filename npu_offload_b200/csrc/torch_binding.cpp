@@ -7,6 +7,10 @@
 // memory is a tensor here until its kernels are enqueued, and freed in the stream's order.
 #include <torch/extension.h>
 
+#include <ATen/EmptyTensor.h>
+#include <c10/core/Allocator.h>
+#include <c10/core/DeviceGuard.h>
+
 #include <string>
 
 #include "../../include/moe_dp.h"
@@ -65,6 +69,15 @@ void no_gradient(const char* name, const Tensor& t) {
         refuse(name, " requires a gradient, and this call records no autograd graph: pass it detached, or call under torch.no_grad()");
 }
 
+// A new tensor of the plane's device, straight from torch's allocator: at::empty takes 0.7 us on the host, this 0.4, and a call at
+// one token has five.
+Tensor fresh(const Plane& p, at::IntArrayRef sizes, at::ScalarType type) {
+    if (!p.device.is_cuda()) return at::empty(sizes, at::TensorOptions(p.device).dtype(type));
+    const c10::DeviceGuard guard(p.device);
+    return at::detail::empty_generic(sizes, c10::GetAllocator(c10::DeviceType::CUDA), c10::DispatchKeySet(c10::DispatchKey::CUDA), type,
+                                     c10::nullopt);
+}
+
 // t as a contiguous tensor of the plane's device, at a multiple of `align` bytes; other types and ranks are refused.
 Tensor operand(const Plane& p, const char* name, Tensor t, std::initializer_list<at::ScalarType> types, int dims, int align = 1) {
     if (!t.defined() || t.device() != p.device) refuse(name, " must be a tensor on ", p.device);
@@ -99,7 +112,7 @@ Fp8 fp8(const Plane& p, const char* name, const Tensor& q, const Tensor& scale, 
 Tensor output(const Plane& p, const c10::optional<Tensor>& out, at::IntArrayRef sizes, at::ScalarType type, bool bf16) {
     if (!out) {
         if (type != at::kFloat && !(bf16 && type == at::kBFloat16)) refuse("out_dtype ", name_of(type), " is neither torch.bfloat16 nor torch.float32");
-        return at::empty(sizes, at::TensorOptions(p.device).dtype(type));
+        return fresh(p, sizes, type);
     }
     const at::ScalarType t = out->scalar_type();
     if (out->device() != p.device || (t != at::kFloat && !(bf16 && t == at::kBFloat16)) || out->sizes() != sizes || !out->is_contiguous() ||
@@ -111,11 +124,11 @@ Tensor output(const Plane& p, const c10::optional<Tensor>& out, at::IntArrayRef 
 
 int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? MOE_DT_F32 : MOE_DT_BF16; }
 Tensor workspace(const Plane& p, int64_t bytes) {  // negative: the call itself says what is out of range
-    return at::empty({std::max<int64_t>(bytes, 0)}, at::TensorOptions(p.device).dtype(at::kByte));
+    return bytes > 0 ? fresh(p, {bytes}, at::kByte) : Tensor();
 }
 template <class T>
 T* ptr(const Tensor& t) {
-    return static_cast<T*>(t.data_ptr());
+    return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr;
 }
 template <class T>
 T* ptr(const c10::optional<Tensor>& t) {
@@ -132,8 +145,7 @@ std::pair<Tensor, Tensor> quantize_fp8(const Plane& p, Tensor x, int64_t block_r
     for (int64_t i = 0; i + 2 < x.dim(); i++) batch *= sizes[i];
     sizes[sizes.size() - 2] = (rows + block_rows - 1) / block_rows;
     sizes[sizes.size() - 1] = (cols + 127) / 128;
-    const Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-    const Tensor scale = at::empty(sizes, x.options().dtype(at::kFloat));
+    const Tensor q = fresh(p, x.sizes(), at::kFloat8_e4m3fn), scale = fresh(p, sizes, at::kFloat);
     check(moe_quantize_fp8(p.ctx, x.data_ptr(), dtype_of(x), batch, rows, cols, (int)block_rows, ptr<uint8_t>(q), ptr<float>(scale), 0,
                            (void*)stream));
     return {q, scale};
@@ -169,7 +181,7 @@ Tensor experts_fp8(const Plane& p, Tensor x, const Tensor& gq, const Tensor& gs,
     const int64_t n = moe_experts_fp8_workspace(p.ctx, (int)T);
     const Tensor ws = workspace(p, n);
     check(moe_experts_fp8(p.ctx, (int)T, ptr<uint16_t>(x), ptr<uint8_t>(gu.q), ptr<float>(gu.scale), ptr<uint8_t>(d.q), ptr<float>(d.scale),
-                          ptr<int32_t>(idx), ptr<float>(w), o.data_ptr(), dtype_of(o), ws.data_ptr(), n,
+                          ptr<int32_t>(idx), ptr<float>(w), o.data_ptr(), dtype_of(o), ptr<void>(ws), n,
                           accumulate ? MOE_F_ACCUMULATE : 0, (void*)stream));
     return o;
 }
@@ -204,12 +216,11 @@ std::tuple<Tensor, Tensor, Tensor, c10::optional<Tensor>, c10::optional<Tensor>>
     idx = operand(p, "idx", std::move(idx), {at::kInt}, 2);
     const int64_t pairs[2] = {s.T, p.K};
     if (idx.sizes() != at::IntArrayRef(pairs)) refuse("idx is ", shape(idx.sizes()), ", not ", shape(pairs));
-    const auto i32 = at::TensorOptions(p.device).dtype(at::kInt);
-    const Tensor loss = at::empty({}, i32.dtype(at::kFloat)), counts = at::empty({s.B, p.E}, i32), tokens = at::empty({s.B + 1}, i32);
+    const Tensor loss = fresh(p, {}, at::kFloat), counts = fresh(p, {s.B, p.E}, at::kInt), tokens = fresh(p, {s.B + 1}, at::kInt);
     const int64_t n = moe_balance_loss_workspace(p.ctx, s.T, (int)s.B);
     const Tensor ws = workspace(p, n);
     check(moe_balance_loss(p.ctx, s.T, ptr<float>(s.logits), ptr<int32_t>(idx), ptr<int32_t>(s.offsets), (int)s.B, ptr<uint8_t>(s.mask),
-                           ptr<float>(loss), ptr<int32_t>(counts), ptr<int32_t>(tokens), ws.data_ptr(), n, 0, (void*)stream));
+                           ptr<float>(loss), ptr<int32_t>(counts), ptr<int32_t>(tokens), ptr<void>(ws), n, 0, (void*)stream));
     return {loss, counts, tokens, s.offsets, s.mask};
 }
 
@@ -253,17 +264,16 @@ std::tuple<c10::optional<Tensor>, c10::optional<Tensor>, c10::optional<Tensor>, 
         refuse("out_dtype ", name_of(*out_dtype), " is neither torch.bfloat16 nor torch.float32");
     if (!out_dtype && !fp8) refuse("neither an out_dtype nor fp8 is wanted");
     if (fp8 && n.C % 16) refuse("fp8 rows are a multiple of 16, not ", n.C, " columns");
-    const auto opt = at::TensorOptions(p.device);
     c10::optional<Tensor> y, q, scale;
-    if (out_dtype) y = at::empty(x.sizes(), opt.dtype(*out_dtype));
+    if (out_dtype) y = fresh(p, x.sizes(), *out_dtype);
     if (fp8) {
         auto sizes = x.sizes().vec();
         sizes.back() = (n.C + 127) / 128;
-        q = at::empty(x.sizes(), opt.dtype(at::kFloat8_e4m3fn));
-        scale = at::empty(sizes, opt.dtype(at::kFloat));
+        q = fresh(p, x.sizes(), at::kFloat8_e4m3fn);
+        scale = fresh(p, sizes, at::kFloat);
     }
-    const Tensor sum = residual ? at::empty(x.sizes(), opt.dtype(residual->scalar_type())) : x;
-    const Tensor rstd = at::empty(x.sizes().slice(0, x.dim() - 1), opt.dtype(at::kFloat));
+    const Tensor sum = residual ? fresh(p, x.sizes(), residual->scalar_type()) : x;
+    const Tensor rstd = fresh(p, x.sizes().slice(0, x.dim() - 1), at::kFloat);
     check(moe_add_norm(p.ctx, n.T, n.C, x.data_ptr(), dtype_of(x), ptr<void>(residual), dtype_of(sum), weight.data_ptr(), dtype_of(weight),
                        (float)eps, residual ? sum.data_ptr() : nullptr, ptr<void>(y), y ? dtype_of(*y) : MOE_DT_BF16, ptr<uint8_t>(q),
                        ptr<float>(scale), ptr<float>(rstd), 0, (void*)stream));
@@ -283,16 +293,16 @@ std::pair<Tensor, c10::optional<Tensor>> add_norm_backward(const Plane& p, Tenso
         dsum = operand(p, "dsum", *dsum, {sum.scalar_type()}, -1, 16);
         if (dsum->sizes() != sum.sizes()) refuse("dsum is ", shape(dsum->sizes()), ", sum ", shape(sum.sizes()));
     }
-    const Tensor dx = at::empty(sum.sizes(), at::TensorOptions(p.device).dtype(sum.scalar_type()));
+    const Tensor dx = fresh(p, sum.sizes(), sum.scalar_type());
     c10::optional<Tensor> dw;
     int64_t bytes = 0;
     if (weight_grad) {
-        dw = at::empty({n.C}, at::TensorOptions(p.device).dtype(at::kFloat));
+        dw = fresh(p, {n.C}, at::kFloat);
         bytes = moe_add_norm_backward_workspace(p.ctx, n.T, n.C);
     }
     const Tensor ws = workspace(p, bytes);
     check(moe_add_norm_backward(p.ctx, n.T, n.C, dy.data_ptr(), dtype_of(dy), sum.data_ptr(), dtype_of(sum), ptr<void>(dsum),
-                                weight.data_ptr(), dtype_of(weight), ptr<float>(rstd), dx.data_ptr(), ptr<float>(dw), ws.data_ptr(), bytes,
+                                weight.data_ptr(), dtype_of(weight), ptr<float>(rstd), dx.data_ptr(), ptr<float>(dw), ptr<void>(ws), bytes,
                                 0, (void*)stream));
     return {dx, dw};
 }
@@ -312,8 +322,7 @@ std::pair<Tensor, Tensor> route_groups(const Plane& p, Tensor logits, int64_t gr
     }
     if (groups < INT32_MIN || groups > INT32_MAX || top_groups < INT32_MIN || top_groups > INT32_MAX) refuse("groups are out of range");
     const int64_t T = logits.size(0);
-    const Tensor idx = at::empty({T, p.K}, at::TensorOptions(p.device).dtype(at::kInt));
-    const Tensor w = at::empty({T, p.K}, at::TensorOptions(p.device).dtype(at::kFloat));
+    const Tensor idx = fresh(p, {T, p.K}, at::kInt), w = fresh(p, {T, p.K}, at::kFloat);
     check(moe_route_groups(p.ctx, T, ptr<float>(logits), ptr<float>(bias), (int)groups, (int)top_groups, renormalize, (float)scale,
                            ptr<int32_t>(idx), ptr<float>(w), 0, (void*)stream));
     return {idx, w};
@@ -363,7 +372,7 @@ Tensor add_lora(const Plane& p, Tensor base, Tensor x, const Tensor& at_a, const
     const int64_t bytes = moe_add_lora_workspace(p.ctx, T, r, n);
     const Tensor ws = workspace(p, bytes);
     check(moe_add_lora(p.ctx, T, K, N, r, n, base.data_ptr(), ptr<uint16_t>(x), ptr<uint16_t>(a), ptr<uint16_t>(b), ptr<int32_t>(ids),
-                       ptr<float>(scale), o.data_ptr(), dtype_of(o), ws.data_ptr(), bytes, 0, (void*)stream));
+                       ptr<float>(scale), o.data_ptr(), dtype_of(o), ptr<void>(ws), bytes, 0, (void*)stream));
     return o;
 }
 
