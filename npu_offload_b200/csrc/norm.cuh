@@ -102,10 +102,15 @@ __device__ __forceinline__ float cta_sum(float v, float (*part)[32], int turn) {
 // How a row of C <= 16384 columns is spread: eights a thread (1 or 2), and threads of a CTA.  Rows of more than 8192 columns
 // take 1024 threads; with the 64 registers that such a CTA leaves each, the next row's words are not asked for ahead.
 inline int norm_eights(int C) { return C <= 2048 ? 1 : 2; }
-inline int norm_threads(int C) {
-    const int each = norm_eights(C), n = ((C + 7) / 8 + each - 1) / each;
+inline int norm_threads(int C, int eights) {
+    const int n = ((C + 7) / 8 + eights - 1) / eights;
     return (n + 31) / 32 * 32;
 }
 constexpr int kNormThreads = 512;
+// CTAs for T rows where `most` fit at once: no more than the longest of them needs.
+inline int norm_grid(int64_t T, int64_t most) {
+    const int64_t rows = (T + most - 1) / most;
+    return (int)((T + rows - 1) / rows);
+}
 
 }  // namespace moe

@@ -105,16 +105,16 @@ __global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* shares,
 }
 
 static int backward_grid(int64_t T, int C, int sm_count) {
-    return (int)std::min<int64_t>(T, (int64_t)sm_count * std::max(1, 512 / norm_threads(C)));
+    return T > 0 ? norm_grid(T, (int64_t)sm_count * std::max(1, 512 / norm_threads(C, norm_eights(C)))) : 1;
 }
 size_t norm_backward_workspace(int64_t T, int C, int sm_count) {
-    return (size_t)backward_grid(std::max<int64_t>(T, 1), C, sm_count) * C * sizeof(float);
+    return (size_t)backward_grid(T, C, sm_count) * C * sizeof(float);
 }
 
 template <bool S32, bool D32, bool DS>
 static cudaError_t backward_for(const NormBackwardArgs& a, int grid, cudaStream_t st) {
     float* shares = a.dweight ? a.ws : nullptr;
-    const int threads = norm_threads(a.C);
+    const int threads = norm_threads(a.C, norm_eights(a.C));
     const Launch l{grid, threads, 0, 0, st};
     if (threads > kNormThreads) return l.run(a.C % 8 ? norm_backward_kernel<S32, D32, DS, 2, false, 1024> : norm_backward_kernel<S32, D32, DS, 2, true, 1024>, a, shares);
     if (a.C % 8) return l.run(norm_backward_kernel<S32, D32, DS, 2, false, kNormThreads>, a, shares);
