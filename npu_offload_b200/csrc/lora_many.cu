@@ -304,7 +304,7 @@ __global__ void __cluster_dims__(kLowCluster, 1, 1) __launch_bounds__(kLowThread
 #pragma unroll
             for (int part = 0; part < PARTS; part++) {
                 const uint32_t b = f8_bf16x2(v0, v1);
-                v0 -= bf_lo(b), v1 -= bf_hi(b);
+                v0 = fabsf(bf_lo(b)) < INFINITY ? v0 - bf_lo(b) : 0.f, v1 = fabsf(bf_hi(b)) < INFINITY ? v1 - bf_hi(b) : 0.f;  // (an infinity stays one)
                 to[part * 128] = b;
             }
         }

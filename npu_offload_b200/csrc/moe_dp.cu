@@ -1754,6 +1754,7 @@ int moe_add_norm(moe_ctx* c, int64_t T, int64_t C, const void* x, int x_dtype, c
         const void* all[] = {x, residual, weight, sum, y, q};
         for (const void* p : all)
             if (!aligned16(p)) return fail(MOE_EINVAL, "x, residual, weight, sum, y and q must be 16-byte aligned");
+        if (((uintptr_t)scale | (uintptr_t)rstd) & 3) return fail(MOE_EINVAL, "scale and rstd must be 4-byte aligned");
         const size_t n = (size_t)T * C;
         const struct { const void* p; size_t bytes; } in[] = {{x, n * dtype_bytes(x_dtype)}, {residual, n * dtype_bytes(stream_dtype)},
                                                               {weight, (size_t)C * dtype_bytes(weight_dtype)}},
@@ -1788,6 +1789,7 @@ int moe_add_norm_backward(moe_ctx* c, int64_t T, int64_t C, const void* dy, int 
     if (T && (!dy || !sum || !weight || !rstd || !dx)) return fail(MOE_EINVAL, "null argument");
     if (!aligned16(dy) || !aligned16(sum) || !aligned16(dsum) || !aligned16(weight) || !aligned16(dx))
         return fail(MOE_EINVAL, "dy, sum, dsum, weight and dx must be 16-byte aligned");
+    if (((uintptr_t)rstd | (uintptr_t)dweight) & 3) return fail(MOE_EINVAL, "rstd and dweight must be 4-byte aligned");
     if (dweight) {
         const int64_t need = moe_add_norm_backward_workspace(c, T, C);
         if (!workspace || (uintptr_t)workspace & 255) return fail(MOE_EINVAL, "the workspace must be 256-byte aligned");
@@ -1822,6 +1824,11 @@ int moe_route_groups(moe_ctx* c, int64_t T, const float* logits, const float* bi
     if (bias && c->cfg.scoring == MOE_SCORING_SOFTMAX) return fail(MOE_EINVAL, "softmax scoring takes no bias");
     if (!(scale > -INFINITY && scale < INFINITY)) return fail(MOE_EINVAL, "scale must be finite");
     if (T && (!logits || !topk_idx || !topk_w)) return fail(MOE_EINVAL, "null argument");
+    if (((uintptr_t)logits | (uintptr_t)bias | (uintptr_t)topk_idx | (uintptr_t)topk_w) & 3) return fail(MOE_EINVAL, "operands must be 4-byte aligned");
+    const size_t nl = (size_t)T * E * 4, nk = (size_t)T * K * 4, nb = (size_t)E * 4;
+    if (overlap(topk_idx, nk, logits, nl) || overlap(topk_w, nk, logits, nl) || overlap(topk_idx, nk, topk_w, nk) || overlap(topk_idx, nk, bias, nb) ||
+        overlap(topk_w, nk, bias, nb))
+        return fail(MOE_EINVAL, "a result overlaps an operand or the other result");
     DeviceGuard dg(c->dev);
     cudaStream_t st = (cudaStream_t)stream;
     if (T) {
@@ -1842,6 +1849,7 @@ int moe_route_backward(moe_ctx* c, int64_t T, const float* logits, const int32_t
     const size_t n = (size_t)T * c->cfg.n_experts * 4, k = (size_t)T * c->cfg.top_k * 4;
     if (overlap(dlogits, n, logits, n) || overlap(dlogits, n, topk_idx, k) || overlap(dlogits, n, dw, k))
         return fail(MOE_EINVAL, "dlogits overlaps an operand");
+    if (((uintptr_t)logits | (uintptr_t)topk_idx | (uintptr_t)dw | (uintptr_t)dlogits) & 3) return fail(MOE_EINVAL, "operands must be 4-byte aligned");
     DeviceGuard dg(c->dev);
     cudaStream_t st = (cudaStream_t)stream;
     if (T) {
@@ -1877,6 +1885,7 @@ int moe_add_lora(moe_ctx* c, int64_t T, int64_t K, int64_t N, int64_t r, int64_t
         if (!base || !x || !a || !b || !ids || !out) return fail(MOE_EINVAL, "null argument");
         if (!aligned16(base) || !aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(out))
             return fail(MOE_EINVAL, "base, x, a, b and out must be 16-byte aligned");
+        if (((uintptr_t)ids | (uintptr_t)scale) & 3) return fail(MOE_EINVAL, "ids and scale must be 4-byte aligned");
         const size_t no = (size_t)T * N * dtype_bytes(out_dtype);
         if ((out != base && overlap(out, no, base, no)) || overlap(out, no, x, (size_t)T * K * 2) || overlap(out, no, a, (size_t)n * r * K * 2) ||
             overlap(out, no, b, (size_t)n * N * r * 2) || overlap(out, no, ids, (size_t)T * 4) || overlap(out, no, scale, (size_t)n * 4))

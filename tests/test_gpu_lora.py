@@ -103,6 +103,10 @@ def test_special_values_stay_in_their_token(plane, T):
     want = plane.add_lora(**m)
     got = plane.add_lora(**{**m, "x": x, "a": a})
     assert not got[0].isfinite().all() and torch.equal(got[1:], want[1:])
+    # an infinity in x: low is one, of a sign or the other, or NaN, and so is the sum of its products with B
+    low = (x[0].double()[None] @ m["a"][1].double().T) * float(m["scale"][1])
+    exact = m["base"][0].double() + (low @ m["b"][1].double().T)[0]
+    assert torch.equal(got[0].isnan(), exact.isnan()) and torch.equal(got[0][~exact.isnan()].double(), exact[~exact.isnan()])
 
 
 def test_strides_no_tokens_and_wide_rows(plane):

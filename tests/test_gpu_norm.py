@@ -54,7 +54,7 @@ def check(n, x, w, residual, eps, out_dtype, fp8):
         assert ((n.fp8.q.double() * s - y).abs() <= (2.0 ** -4 + 2 * WORK) * y.abs() + 2.0 ** -10 * s).all()
 
 
-SHAPES = [(1, 1), (1, 16), (3, 8), (5, 7), (2, 127), (7, 128), (4, 129), (9, 1000), (33, 1280), (17, 1283), (300, 2048), (5, 2056), (1, 4096),
+SHAPES = [(1, 1), (1, 16), (6, 144), (150, 1040), (4, 2064), (149, 4112), (3, 8176), (3, 8), (5, 7), (2, 127), (7, 128), (4, 129), (9, 1000), (33, 1280), (17, 1283), (300, 2048), (5, 2056), (1, 4096),
           (700, 4096), (3, 4100), (2, 8192), (2, 8200), (3, 8193), (2, 16384), (1, 16383)]
 
 
@@ -237,7 +237,7 @@ def test_the_c_calls_refuse_what_would_overlap(plane):
     for kw, needle in ((dict(T=-1), "T="), (dict(T=1 << 25), "T="), (dict(C=0), "C="), (dict(C=16385), "C="), (dict(y=p(x)), "overlaps"),
                        (dict(res=p(z), total=p(z)), "overlaps"), (dict(res=p(z)), "together"), (dict(q=p(z)), "together"),
                        (dict(C=24, q=p(z), s=p(z)), "multiple of 16"), (dict(eps=0.0), "eps"), (dict(eps=float("nan")), "eps"),
-                       (dict(eps=float("inf")), "eps"), (dict(flags=1), "flag"), (dict(xp=p(x) + 4), "aligned"), (dict(xp=None), "null")):
+                       (dict(eps=float("inf")), "eps"), (dict(y=p(z), q=p(z) + 1024, s=p(rstd) + 2), "4-byte"), (dict(flags=1), "flag"), (dict(xp=p(x) + 4), "aligned"), (dict(xp=None), "null")):
         assert call(**kw) == _lib.MOE_EINVAL and needle in _lib.last_error(), kw
     dw, ws = torch.zeros(32, device="cuda"), torch.zeros(1 << 20, device="cuda")
 

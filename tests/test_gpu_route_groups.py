@@ -255,15 +255,16 @@ def test_no_tokens_strides_streams_and_graphs():
 def test_the_library_refuses():
     from npu_offload_b200 import _lib
     L, t = nob.lib(), torch.zeros(4, 16, device="cuda")
-    idx = torch.zeros(4, 4, device="cuda", dtype=torch.int32)
+    idx, w0 = torch.zeros(4, 4, device="cuda", dtype=torch.int32), torch.zeros(4, 4, device="cuda")
     for scoring in ("softmax", "sigmoid"):
         with plane(16, 4, scoring) as p:
-            def call(T=4, lg=t.data_ptr(), bias=None, groups=4, top=2, scale=1.0, i=idx.data_ptr(), w=t.data_ptr(), flags=0):
+            def call(T=4, lg=t.data_ptr(), bias=None, groups=4, top=2, scale=1.0, i=idx.data_ptr(), w=w0.data_ptr(), flags=0):
                 return L.moe_route_groups(p.handle, T, lg, bias, groups, top, 1, scale, i, w, flags, None)
 
             for kw, needle in ((dict(T=-1), "T="), (dict(T=1 << 25), "T="), (dict(groups=0), "groups"), (dict(groups=3), "divisor"), (dict(groups=33), "divisor"),
                                (dict(top=0), "top_groups"), (dict(top=5), "top_groups"), (dict(groups=16, top=3), "choices"), (dict(scale=float("nan")), "scale"),
-                               (dict(lg=None), "null"), (dict(i=None), "null"), (dict(flags=2), "flag")):
+                               (dict(lg=None), "null"), (dict(i=None), "null"), (dict(flags=2), "flag"), (dict(w=idx.data_ptr()), "overlaps"),
+                               (dict(lg=t.data_ptr() + 2), "4-byte"), (dict(w=t.data_ptr()), "overlaps")):
                 assert call(**kw) == _lib.MOE_EINVAL and needle in _lib.last_error(), kw
             if scoring == "softmax":
                 assert call(bias=t.data_ptr()) == _lib.MOE_EINVAL and "bias" in _lib.last_error()
