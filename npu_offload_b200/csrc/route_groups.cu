@@ -173,7 +173,7 @@ __device__ __forceinline__ float inverse(float y) {
 // A sigmoid's keys on a grid of 2^23 steps for the range that the biases allow: 2^23 + 1 + (s + bias - least bias) * grid, an
 // fp32 number with the steps for its last bits.
 struct RouteGrid {
-    float grid = 0.f, low = 0.f, slack = 0.f;
+    float grid = 0.f, low = 0.f, apart = 0.f;  // apart: how far two words must be (below)
     bool wild = false;  // a bias is not finite: nothing lies on the grid
     __device__ __forceinline__ void set(const float* bias, int E) {  // by a warp
         float least = bias ? INFINITY : 0.f, most = bias ? -INFINITY : 0.f;
@@ -192,7 +192,7 @@ struct RouteGrid {
         wild = __any_sync(0xffffffffu, wild) || !(range < 1e30f);
         grid = wild ? 0.f : 8388608.f / range;
         low = wild ? 0.f : least;
-        slack = grid * fmaxf(fabsf(least), fabsf(most) + 1.f) * 0x1p-23f + 4.f;
+        apart = grid * (0x1p-19f + fmaxf(fabsf(least), fabsf(most) + 1.f) * 0x1p-23f) + 4.f;
     }
     __device__ __forceinline__ float shift(const float* bias, int e) const {  // (what s * grid is added to)
         return wild ? 8388608.f : 8388609.f + ((bias ? bias[e] : 0.f) - low) * grid;
@@ -201,11 +201,12 @@ struct RouteGrid {
 
 // Margins.
 // Softmax: the words leave out the last bits of the logit; equal words but for the place are too close.
-// Sigmoid, in steps of the grid (2^-23 of the range; `grid` steps make 1): the product l log2 e is off by |l| 2^-24 / ln 2 in the exponent, 2^x and
-// the reciprocal by 2^-22 each, the additions by 2^-24, so s by s (|l| 2^-24 + 2^-21) at most; with s <= smax, and smax >
-// 2^-20 (else the token is done exactly), s |l| <= 14 smax, so that s is off by less than smax 2^-19.  The bias's place on the grid is off by
-// 1.5 steps, the sum by half a step, and the key of the definition by 2^-24 of its size, kmax at most.  Two keys:
-// grid (smax 2^-18 + kmax 2^-23) + 4; two groups of two keys: twice that, and a step of 2^-23 of a score, 2 kmax, each, for the sums' rounding.
+// Sigmoid, in steps of the grid (2^-23 of the range; `grid` steps make 1): the product l log2 e is off by |l| 2^-24 / ln 2 in the
+// exponent, 2^x and the reciprocal by 2^-22 each, the additions by 2^-24, so s by s (1 - s) |l| 2^-24 + s 2^-21 at most, and, since
+// s (1 - s) |l| < 0.23, by less than 2^-20.  The bias's place on the grid is off by 1.5 steps, the sum by half a step, and the key
+// of the definition by 2^-24 of its size, kmax at most.  Two keys: grid (2^-19 + kmax 2^-23) + 4; two groups of two keys: twice that,
+// and a step of 2^-23 of a score, 2 kmax, each, for the sums' rounding.  (Scores that are all far below 2^-19 are told apart by
+// their biases; without those, exactly.)
 // A NaN, like a bias that is not finite, leaves the range of words and is left to the exact choice.
 // FULL: every lane has V experts.
 template <int V, bool SIG, bool FULL>
@@ -242,13 +243,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 4) route_groups_kernel(Route
                 if (FULL || j < n) l[j] = row[e0 + j];
         }
         bool nan = SIG && on.wild;
-        float lmax = -INFINITY;
         uint32_t u[V];
 #pragma unroll
         for (int j = 0; j < V; j++) {
             float k = FULL || j < n ? l[j] : -INFINITY;
             if (SIG) {  // (from 2^23 to 2^24: the exponent's bits leave on the left)
-                lmax = fmaxf(lmax, k);
                 const float on_grid = fmaf(rcp_hw(1.f + exp2_hw(k * -1.44269504f)), on.grid, shift[j]);
                 u[j] = __float_as_uint(on_grid) * kPlaces + (place - j);
                 nan |= V > 8 && on_grid != on_grid;
@@ -264,12 +263,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 4) route_groups_kernel(Route
 #pragma unroll
         for (int j = 0; j < V; j++) list[j * 32] = u[j];
         bool again = nan, mixed = false;
-        float apart = 0.f;
-        if (SIG) {
-            const float smax = rcp_hw(1.f + exp2_hw(from_ordered(__reduce_max_sync(0xffffffffu, ordered_bits(lmax))) * -1.44269504f));
-            again |= !(smax > 0x1p-20f);
-            apart = fmaf(on.grid * smax, 0x1p-18f, on.slack);
-        }
+        const float apart = on.apart;
         const uint32_t* step = list;
         if (a.top < a.groups) {
             uint32_t score = u[0] / kPlaces, second = V > 1 ? u[V > 1 ? 1 : 0] / kPlaces : 0;
@@ -408,7 +402,6 @@ __global__ void __launch_bounds__(kOctetWarps * 32, kOctetCtas) route_octet_kern
         const float* shift = s.shift + at8 * kPitch;
         const uint32_t place = (7 - at8) * 32 + 31;
         bool nan = SIG && on.wild;
-        float lmax = -INFINITY;
         uint32_t u[V];
 #pragma unroll
         for (int i = 0; i < V; i += 4) {
@@ -422,7 +415,6 @@ __global__ void __launch_bounds__(kOctetWarps * 32, kOctetCtas) route_octet_kern
             for (int k = 0; k < 4; k++) {
                 const int j = i + k;
                 if (SIG) {
-                    lmax = fmaxf(lmax, lk[k]);
                     u[j] = __float_as_uint(fmaf(rcp_hw(1.f + exp2_hw(lk[k] * -1.44269504f)), on.grid, hk[k])) * 256 + (place - j);
                 } else {
                     const float x = lk[k] + 0.f;
@@ -456,14 +448,7 @@ __global__ void __launch_bounds__(kOctetWarps * 32, kOctetCtas) route_octet_kern
 #pragma unroll
         for (int j = 0; j < kKept; j++) list[j * 32] = u[j];
         bool again = nan;
-        float apart = 0.f;
-        if (SIG) {
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) lmax = fmaxf(lmax, __shfl_xor_sync(0xffffffffu, lmax, o));
-            const float smax = rcp_hw(1.f + exp2_hw(lmax * -1.44269504f));
-            again |= !(smax > 0x1p-20f);
-            apart = fmaf(on.grid * smax, 0x1p-18f, on.slack);
-        }
+        const float apart = on.apart;
         const uint32_t* step = list;
         if (a.top < a.groups) {
             uint32_t score = u[0] >> 8, second = u[1] >> 8;
