@@ -24,41 +24,35 @@ namespace moe {
 
 // ---- Rare paths, from memory and out of line, so that they cost the rows' path no registers.
 
-// Eight values of the sum, from the 8 (V) or every `step`-th column on.
+// Eight values of the sum, from column c on.
 template <bool X32, int R, bool V>
-__device__ __forceinline__ void sum8(const NormArgs& a, size_t row, int c, int step, float (&h)[8]) {
+__device__ __forceinline__ void sum8(const NormArgs& a, size_t row, int c, float (&h)[8]) {
     Raw8<X32> x;
-    x.template load<V>(a.x, row, c, step, a.C);
+    const size_t end = (size_t)a.T * a.C;
+    x.template load<V>(a.x, row, c, a.C, end);
     x.get(h);
     if (R) {
         Raw8<R == 2> res;
         float r[8];
-        res.template load<V>(a.residual, row, c, step, a.C);
+        res.template load<V>(a.residual, row, c, a.C, end);
         res.get(r);
 #pragma unroll
         for (int k = 0; k < 8; k++) h[k] = R == 1 ? bf2f(f8_bf16(h[k] + r[k])) : h[k] + r[k];
     }
+    keep_row<V>(h, c, a.C);
 }
 template <bool V>
-__device__ __forceinline__ void weight8(const NormArgs& a, int c, int step, float (&w)[8]) {
-    if (a.weight_f32) {
-        Raw8<true> r;
-        r.template load<V>(a.weight, 0, c, step, a.C);
-        r.get(w);
-    } else {
-        Raw8<false> r;
-        r.template load<V>(a.weight, 0, c, step, a.C);
-        r.get(w);
-    }
+__device__ __forceinline__ void weight8(const NormArgs& a, int c, float (&w)[8]) {
+    norm_weight<V>(a.weight, a.weight_f32, c, a.C, w);
 }
 // One row's 1 / sqrt(mean h^2 + eps) in 64 bits, by one warp.
 template <bool X32, int R, bool V>
 __device__ __forceinline__ double rstd_64(const NormArgs& a, size_t row) {
     double s = 0;
 #pragma unroll 2
-    for (int c = V ? (threadIdx.x & 31) * 8 : threadIdx.x & 31; c < a.C; c += 256) {
+    for (int c = (int)(threadIdx.x & 31) * 8 - (int)(V ? 0 : row % 8); c < a.C; c += 256) {
         float h[8];
-        sum8<X32, R, V>(a, row, c, V ? 1 : 32, h);
+        sum8<X32, R, V>(a, row, c, h);
 #pragma unroll
         for (int k = 0; k < 8; k++) s += (double)h[k] * (double)h[k];
     }
@@ -70,8 +64,8 @@ __device__ __forceinline__ double rstd_64(const NormArgs& a, size_t row) {
 template <bool X32, int R>
 __device__ __forceinline__ bool over_border(const NormArgs& a, size_t row, int c, double rstd, double border) {
     float h[8], w[8];
-    sum8<X32, R, true>(a, row, c, 1, h);
-    weight8<true>(a, c, 1, w);
+    sum8<X32, R, true>(a, row, c, h);
+    weight8<true>(a, c, w);
     double most = 0;
 #pragma unroll
     for (int k = 0; k < 8; k++) {
@@ -95,18 +89,18 @@ template <bool X32, int R, int N, bool V>
 __device__ __noinline__ void wide_row(const NormArgs* p, int64_t t) {
     const NormArgs& a = *p;
     const size_t row = (size_t)t * a.C;
-    const int step = V ? 1 : blockDim.x;
+    const int lead = V ? 0 : row % 8;
     const double rstd = rstd_64<X32, R, V>(a, row);
     if (threadIdx.x == 0 && a.rstd) a.rstd[t] = (float)rstd;
 #pragma unroll 1
     for (int i = 0; i < N; i++) {
-        const int c = norm_col<V>(i);
+        const int c = norm_col(i, lead);
         float h[8], w[8], y[8];
-        sum8<X32, R, V>(a, row, c, step, h);
-        weight8<V>(a, c, step, w);
+        sum8<X32, R, V>(a, row, c, h);
+        weight8<V>(a, c, w);
 #pragma unroll
         for (int k = 0; k < 8; k++) y[k] = (float)((double)h[k] * rstd * (double)w[k]);
-        if (a.y) store8<V>(a.y, a.y_f32, row, c, step, a.C, y);
+        if (a.y) store8<V>(a.y, a.y_f32, row, c, a.C, y);
         if (V && a.q) {
             bool special;
             uint32_t top = f8_top(y, special);
@@ -131,17 +125,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) add_norm_kern
     __shared__ float part[2][32];
     constexpr bool kAhead = THREADS <= kNormThreads;
     griddep_wait();
-    const int step = V ? 1 : blockDim.x, C = a.C, groups = (C + kF8Block - 1) / kF8Block;
+    const int C = a.C, lead = V ? 0 : (int)((int64_t)blockIdx.x * C % 8), groups = (C + kF8Block - 1) / kF8Block;
     float w[N][8];
 #pragma unroll
-    for (int i = 0; i < N; i++) weight8<V>(a, norm_col<V>(i), step, w[i]);
+    for (int i = 0; i < N; i++) weight8<V>(a, norm_col(i, lead), w[i]);
+    const size_t end = (size_t)a.T * C;
     Raw8<X32> x[N];
     Raw8<R == 2> res[N];
     auto ask = [&](int64_t t) {
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            x[i].template load<V>(a.x, (size_t)t * C, norm_col<V>(i), step, C);
-            if (R) res[i].template load<V>(a.residual, (size_t)t * C, norm_col<V>(i), step, C);
+            x[i].template load<V>(a.x, (size_t)t * C, norm_col(i, lead), C, end);
+            if (R) res[i].template load<V>(a.residual, (size_t)t * C, norm_col(i, lead), C, end);
         }
     };
     int turn = 0;
@@ -165,13 +160,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) add_norm_kern
                         h[i][k] = bf_lo(b), h[i][k + 1] = bf_hi(b);
                     }
             }
+            keep_row<V>(h[i], norm_col(i, lead), C);
 #pragma unroll
             for (int k = 0; k < 8; k++) ss = fmaf(h[i][k], h[i][k], ss);
         }
         if (kAhead && t + gridDim.x < a.T) ask(t + gridDim.x);
         if (R)
 #pragma unroll
-            for (int i = 0; i < N; i++) store8<V>(a.sum, R == 2, row, norm_col<V>(i), step, C, h[i]);
+            for (int i = 0; i < N; i++) store8<V>(a.sum, R == 2, row, norm_col(i, lead), C, h[i]);
         ss = cta_sum(ss, part, turn);
         if (!(ss < 1e37f) || ss < tiny) {  // the whole CTA
             wide_row<X32, R, N, V>(&a, t);
@@ -181,11 +177,11 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) add_norm_kern
         if (threadIdx.x == 0 && a.rstd) a.rstd[t] = rstd;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const int c = norm_col<V>(i);
+            const int c = norm_col(i, lead);
             float y[8];
 #pragma unroll
             for (int k = 0; k < 8; k++) y[k] = h[i][k] * rstd * w[i][k];
-            if (a.y) store8<V>(a.y, a.y_f32, row, c, step, C, y);
+            if (a.y) store8<V>(a.y, a.y_f32, row, c, C, y);
             if (Q) {
                 bool special;
                 uint32_t top = f8_top(y, special);
@@ -212,11 +208,12 @@ static cudaError_t add_norm_for(const NormArgs& a, int sm_count, cudaStream_t st
     // instead of 89).  CTAs for as many rows as fit on the SMs at once, the next row's words asked for ahead: a CTA a row without that
     // took 106 us, three CTAs of 80 registers 141 (spills).
     const int eights = a.T <= sm_count && a.C <= 4096 ? 1 : norm_eights(a.C), threads = norm_threads(a.C, eights);
-    const int grid = norm_grid(a.T, sm_count * std::max(1, 512 / threads));
+    const int grid = norm_grid(a.T, sm_count * std::max(1, 512 / threads), a.C);
     const Launch l{grid, threads, 0, 0, st};
     if constexpr (!Q)
         if (a.C % 8) {
-            if (threads > 512) return l.run(add_norm_kernel<X32, R, false, 2, false, 1024>, a, tiny);
+            if (threads > 512) return l.run(eights == 3 ? add_norm_kernel<X32, R, false, 3, false, 1024> : add_norm_kernel<X32, R, false, 2, false, 1024>, a, tiny);
+            if (eights == 1) return l.run(threads > 256 ? add_norm_kernel<X32, R, false, 1, false, 512> : add_norm_kernel<X32, R, false, 1, false, 256>, a, tiny);
             return l.run(threads > 256 ? add_norm_kernel<X32, R, false, 2, false, 512> : add_norm_kernel<X32, R, false, 2, false, 256>, a, tiny);
         }
     if (threads > 512) return l.run(add_norm_kernel<X32, R, Q, 2, true, 1024>, a, tiny);

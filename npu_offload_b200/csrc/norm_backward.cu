@@ -20,22 +20,15 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackwardArgs
     constexpr bool kAhead = THREADS <= kNormThreads;
     griddep_wait();
     if (shares) griddep_launch_dependents();  // the shares' sum waits for this kernel's end before it does anything
-    const int step = V ? 1 : blockDim.x, C = a.C;
+    const int C = a.C, lead = V ? 0 : (int)((int64_t)blockIdx.x * C % 8);
     float w[N][8], dw[N][8];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if (a.weight_f32) {
-            Raw8<true> r;
-            r.template load<V>(a.weight, 0, norm_col<V>(i), step, C);
-            r.get(w[i]);
-        } else {
-            Raw8<false> r;
-            r.template load<V>(a.weight, 0, norm_col<V>(i), step, C);
-            r.get(w[i]);
-        }
+        norm_weight<V>(a.weight, a.weight_f32, norm_col(i, lead), C, w[i]);
 #pragma unroll
         for (int k = 0; k < 8; k++) dw[i][k] = 0.f;
     }
+    const size_t end = (size_t)a.T * C;
     Raw8<S32> h[N], ds[N];
     Raw8<D32> dy[N];
     float rstd_next = 0.f;
@@ -43,9 +36,9 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackwardArgs
         rstd_next = a.rstd[t];
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            h[i].template load<V>(a.sum, (size_t)t * C, norm_col<V>(i), step, C);
-            dy[i].template load<V>(a.dy, (size_t)t * C, norm_col<V>(i), step, C);
-            if (DS) ds[i].template load<V>(a.dsum, (size_t)t * C, norm_col<V>(i), step, C);
+            h[i].template load<V>(a.sum, (size_t)t * C, norm_col(i, lead), C, end);
+            dy[i].template load<V>(a.dy, (size_t)t * C, norm_col(i, lead), C, end);
+            if (DS) ds[i].template load<V>(a.dsum, (size_t)t * C, norm_col(i, lead), C, end);
         }
     };
     int turn = 0;
@@ -59,6 +52,8 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackwardArgs
         for (int i = 0; i < N; i++) {
             h[i].get(u[i]);
             dy[i].get(g[i]);
+            keep_row<V>(u[i], norm_col(i, lead), C);
+            keep_row<V>(g[i], norm_col(i, lead), C);
             if (DS) dst[i] = ds[i];
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -81,12 +76,12 @@ __global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackwardArgs
 #pragma unroll
                 for (int k = 0; k < 8; k++) o[k] += d[k];
             }
-            store8<V>(a.dx, S32, (size_t)t * C, norm_col<V>(i), step, C, o);
+            store8<V>(a.dx, S32, (size_t)t * C, norm_col(i, lead), C, o);
         }
     }
     if (shares)
 #pragma unroll
-        for (int i = 0; i < N; i++) store8<V>(shares, true, (size_t)blockIdx.x * C, norm_col<V>(i), step, C, dw[i]);
+        for (int i = 0; i < N; i++) store8<V>(shares, true, (size_t)blockIdx.x * C, norm_col(i, lead), C, dw[i]);
 }
 
 // dw = the shares' sum: 32 columns a CTA, 32 warps each every 32nd share, then the warps in order.
@@ -105,7 +100,7 @@ __global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* shares,
 }
 
 static int backward_grid(int64_t T, int C, int sm_count) {
-    return T > 0 ? norm_grid(T, (int64_t)sm_count * std::max(1, 512 / norm_threads(C, norm_eights(C)))) : 1;
+    return T > 0 ? norm_grid(T, (int64_t)sm_count * std::max(1, 512 / norm_threads(C, norm_eights(C))), C) : 1;
 }
 size_t norm_backward_workspace(int64_t T, int C, int sm_count) {
     return (size_t)backward_grid(T, C, sm_count) * C * sizeof(float);
@@ -116,8 +111,10 @@ static cudaError_t backward_for(const NormBackwardArgs& a, int grid, cudaStream_
     float* shares = a.dweight ? a.ws : nullptr;
     const int threads = norm_threads(a.C, norm_eights(a.C));
     const Launch l{grid, threads, 0, 0, st};
-    if (threads > kNormThreads) return l.run(a.C % 8 ? norm_backward_kernel<S32, D32, DS, 2, false, 1024> : norm_backward_kernel<S32, D32, DS, 2, true, 1024>, a, shares);
-    if (a.C % 8) return l.run(norm_backward_kernel<S32, D32, DS, 2, false, kNormThreads>, a, shares);
+    if (threads > kNormThreads && a.C % 8)
+        return l.run(norm_eights(a.C) == 3 ? norm_backward_kernel<S32, D32, DS, 3, false, 1024> : norm_backward_kernel<S32, D32, DS, 2, false, 1024>, a, shares);
+    if (threads > kNormThreads) return l.run(norm_backward_kernel<S32, D32, DS, 2, true, 1024>, a, shares);
+    if (a.C % 8) return l.run(norm_eights(a.C) == 1 ? norm_backward_kernel<S32, D32, DS, 1, false, kNormThreads> : norm_backward_kernel<S32, D32, DS, 2, false, kNormThreads>, a, shares);
     return l.run(norm_eights(a.C) == 1 ? norm_backward_kernel<S32, D32, DS, 1, true, kNormThreads> : norm_backward_kernel<S32, D32, DS, 2, true, kNormThreads>, a, shares);
 }
 

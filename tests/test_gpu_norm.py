@@ -55,7 +55,7 @@ def check(n, x, w, residual, eps, out_dtype, fp8):
 
 
 SHAPES = [(1, 1), (1, 16), (6, 144), (150, 1040), (4, 2064), (149, 4112), (3, 8176), (3, 8), (5, 7), (2, 127), (7, 128), (4, 129), (9, 1000), (33, 1280), (17, 1283), (300, 2048), (5, 2056), (1, 4096),
-          (700, 4096), (3, 4100), (2, 8192), (2, 8200), (3, 8193), (2, 16384), (1, 16383)]
+          (700, 4096), (3, 4100), (2, 8192), (2, 8200), (3, 8193), (2, 16384), (1, 16383), (9, 16381), (400, 130), (1000, 2047), (301, 4095), (600, 4), (5000, 3), (333, 1)]
 
 
 @pytest.mark.parametrize("T,C", SHAPES)
@@ -76,7 +76,7 @@ def test_forward(plane, T, C, x_dtype, r_dtype):
                                                         (F32, BF, False), (BF, F32, False)])
 def test_backward(plane, T, C, dy_dtype, s_dtype, with_dsum):
     """dx: every term of the formula is off by the work's few steps of its own size (C of them in the mean: 26 steps), the
-    result by half a step.  dweight: rows after one another on a CTA (5 at most here), then 10 levels."""
+    result by half a step.  dweight: rows after one another on a CTA (12 at most here), then at most 14 shares and 5 levels."""
     g = gen(T * 17 + C)
     h, dy = rows(g, T, C, dtype=s_dtype), rows(g, T, C, dtype=dy_dtype)
     w = (1 + 0.3 * torch.randn(C, generator=g, device="cuda")).to(BF if T % 2 else F32)
