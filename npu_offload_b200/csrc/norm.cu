@@ -121,7 +121,7 @@ __device__ __noinline__ void wide_row(const NormArgs* p, int64_t t) {
 
 // R: the residual is none (0), bf16 (1) or fp32 (2).
 template <bool X32, int R, bool Q, int N, bool V, int THREADS>
-__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 2 : 1) add_norm_kernel(const __grid_constant__ NormArgs a, float tiny) {
+__global__ void __launch_bounds__(THREADS, THREADS != 256 ? 1 : N == 1 && !X32 && R != 2 ? 3 : 2) add_norm_kernel(const __grid_constant__ NormArgs a, float tiny) {
     __shared__ float part[2][32];
     constexpr bool kAhead = THREADS <= kNormThreads;
     griddep_wait();
@@ -208,7 +208,7 @@ static cudaError_t add_norm_for(const NormArgs& a, int sm_count, cudaStream_t st
     // instead of 89).  CTAs for as many rows as fit on the SMs at once, the next row's words asked for ahead: a CTA a row without that
     // took 106 us, three CTAs of 80 registers 141 (spills).
     const int eights = a.T <= sm_count && a.C <= 4096 ? 1 : norm_eights(a.C), threads = norm_threads(a.C, eights);
-    const int grid = norm_grid(a.T, sm_count * std::max(1, 512 / threads), a.C);
+    const int grid = norm_grid(a.T, sm_count * std::max(1, (eights == 1 && threads <= 256 && !X32 && R != 2 ? 768 : 512) / threads), a.C);
     const Launch l{grid, threads, 0, 0, st};
     if constexpr (!Q)
         if (a.C % 8) {

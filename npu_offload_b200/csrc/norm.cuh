@@ -12,7 +12,7 @@ namespace moe {
 // Eight neighbouring values as they come from memory, from column c of the row that begins at value `row` on; row + c is a multiple of
 // eight, so that every word of 16 bytes lies at its boundary.  V: rows are multiples of eight values, c is 0 or more.  Else c may be
 // negative, and the first and last eight of a row hold values of its neighbours, for keep_row to take out (nothing waits for a word
-// before it is used: put together from single values, the next row's words were waited for at once, 64 instead of MEASURED_ODD us at
+// before it is used: put together from single values, the next row's words were waited for at once, 64 instead of 38 us at
 // 4000 x 4099); the one word that may reach behind the tensor's end comes value by value.  0 where c is behind the row.
 template <bool F32>
 struct Raw8 {

@@ -15,7 +15,7 @@
 namespace moe {
 
 template <bool S32, bool D32, bool DS, int N, bool V, int THREADS>
-__global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackwardArgs a, float* shares) {
+__global__ void __launch_bounds__(THREADS, N == 1 && !S32 && !D32 ? 2 : 1) norm_backward_kernel(NormBackwardArgs a, float* shares) {
     __shared__ float part[2][32];
     constexpr bool kAhead = THREADS <= kNormThreads;
     griddep_wait();
@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* shares,
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float v = 0.f;
     if (c < C)
+#pragma unroll 8
         for (int r = warp; r < n; r += 32) v += shares[(size_t)r * C + c];
     s[warp][lane] = v;
     __syncthreads();
@@ -99,11 +100,13 @@ __global__ void __launch_bounds__(1024) norm_dweight_kernel(const float* shares,
     if (lane == 0 && o < C) dweight[o] = v;
 }
 
-static int backward_grid(int64_t T, int C, int sm_count) {
-    return T > 0 ? norm_grid(T, (int64_t)sm_count * std::max(1, 512 / norm_threads(C, norm_eights(C))), C) : 1;
+// (64 registers a thread of bf16 rows of one eight a thread, else up to 128; narrow rows have fewer CTAs than fit, for their shares' sake)
+static int backward_grid(int64_t T, int C, bool narrow_type, int sm_count) {
+    const int threads = norm_threads(C, norm_eights(C)), fit = norm_eights(C) == 1 && narrow_type && threads >= 64 ? 1024 : 512;
+    return T > 0 ? norm_grid(T, (int64_t)sm_count * std::max(1, fit / threads), C) : 1;
 }
 size_t norm_backward_workspace(int64_t T, int C, int sm_count) {
-    return (size_t)backward_grid(T, C, sm_count) * C * sizeof(float);
+    return (size_t)std::max(backward_grid(T, C, true, sm_count), backward_grid(T, C, false, sm_count)) * C * sizeof(float);
 }
 
 template <bool S32, bool D32, bool DS>
@@ -120,7 +123,7 @@ static cudaError_t backward_for(const NormBackwardArgs& a, int grid, cudaStream_
 
 cudaError_t launch_add_norm_backward(const NormBackwardArgs& a, int sm_count, cudaStream_t st, int* launches) {
     if (a.C <= 0) return cudaSuccess;
-    const int grid = backward_grid(a.T, a.C, sm_count);
+    const int grid = backward_grid(a.T, a.C, !a.stream_f32 && !a.dy_f32, sm_count);
     cudaError_t e = cudaSuccess;
     if (a.T > 0) {
         const int kind = (a.stream_f32 ? 4 : 0) | (a.dy_f32 ? 2 : 0) | (a.dsum ? 1 : 0);
