@@ -1,5 +1,5 @@
-"""Build libmoe_dp.so (the C-ABI library) in-tree with nvcc for sm_100a, and the torch side of the e4m3 and
-balance-loss calls (_torch_binding.<Python>-torch<version>.so) with the host compiler.
+"""Build libmoe_dp.so (the C-ABI library) in-tree with nvcc for sm_100a, and the torch side of the calls that allocate through
+torch (_torch_binding.<Python>-torch<version>.so) with the host compiler.
 
     python -m npu_offload_b200.build [--force]
 
@@ -90,7 +90,7 @@ def build(force=False, verbose=False, extra=(), out=None):
         try:
             build_binding(force)
         except (ImportError, OSError, subprocess.CalledProcessError) as e:
-            print(f"torch binding not built, the e4m3 and balance-loss calls need it: {e}", file=sys.stderr)
+            print(f"torch binding not built, the calls that allocate through torch need it: {e}", file=sys.stderr)
     return lib
 
 
