@@ -1795,10 +1795,11 @@ int moe_add_norm_backward(moe_ctx* c, int64_t T, int64_t C, const void* dy, int 
         if (!workspace || (uintptr_t)workspace & 255) return fail(MOE_EINVAL, "the workspace must be 256-byte aligned");
         if (workspace_bytes < need) return fail(MOE_EINVAL, "workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
     }
-    const size_t n = (size_t)T * C, nx = n * dtype_bytes(stream_dtype), nw = (size_t)C * dtype_bytes(weight_dtype);
-    if (overlap(dx, nx, dy, n * dtype_bytes(dy_dtype)) || overlap(dx, nx, sum, nx) || overlap(dx, nx, dsum, nx) ||
-        overlap(dx, nx, weight, nw) || overlap(dx, nx, rstd, (size_t)T * 4) || overlap(dx, nx, dweight, (size_t)C * 4))
-        return fail(MOE_EINVAL, "dx overlaps an operand");
+    const size_t n = (size_t)T * C, nx = n * dtype_bytes(stream_dtype), nw = (size_t)C * dtype_bytes(weight_dtype), ng = (size_t)C * 4;
+    const struct { const void* p; size_t bytes; } in[] = {{dy, n * dtype_bytes(dy_dtype)}, {sum, nx}, {dsum, nx}, {weight, nw}, {rstd, (size_t)T * 4}};
+    for (const auto& o : in)
+        if (overlap(dx, nx, o.p, o.bytes) || overlap(dweight, ng, o.p, o.bytes)) return fail(MOE_EINVAL, "a result overlaps an operand");
+    if (overlap(dx, nx, dweight, ng)) return fail(MOE_EINVAL, "two results overlap");
     DeviceGuard dg(c->dev);
     cudaStream_t st = (cudaStream_t)stream;
     NormBackwardArgs a{dy, sum, dsum, weight, rstd, dy_dtype == MOE_DT_F32, stream_dtype == MOE_DT_F32, weight_dtype == MOE_DT_F32, T,

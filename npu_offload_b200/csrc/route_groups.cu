@@ -19,8 +19,8 @@
 // exponential in double); where the last chosen and the next, or two groups, do, the token is done again with 64-bit words
 // of key and index: the result is always that of the definition.
 //
-// Bounded by the instructions a token takes and their latency: 262 a token at 65536 x 256, 8 groups, top 8, sigmoid, with four tokens a
-// warp (route_octet_kernel; 490 with one), 32 us, of which reading the logits needs 11.
+// Bounded by the instructions a token takes and their latency: 258 a token at 65536 x 256, 8 groups, top 8, sigmoid, with four tokens a
+// warp (route_octet_kernel; 490 with one), 31 us, of which reading the logits needs 11.
 #include <algorithm>
 
 #include "common.cuh"
@@ -558,7 +558,7 @@ cudaError_t launch_route_groups(const RouteGroupsArgs& a, int sm_count, cudaStre
     const bool vec = sp.each % 4 == 0 && sp.size % 4 == 0 && (uintptr_t)a.logits % 16 == 0;  // (a lane has a multiple of four, then)
     // Four tokens a warp where there are tokens for more than one round of it.  With it and without, us (sigmoid, 8 groups, top 8;
     // E = 64: softmax, 4 groups, top 4):  2400 tokens: 7.3 / 5.9 (E = 256), 5.3 / 4.2 (128), 2.6 / 2.4 (64);  4800: 8.6 / 7.3, 6.0 / 5.8,
-    // 2.8 / 3.5;  9600: 11.9 / 11.7, 6.8 / 8.5, 3.5 / 5.3;  19200: 15.9 / 17.7, 10.4 / 14.0, 5.0 / 8.6;  65536: 32 / 44 (256).
+    // 2.8 / 3.5;  9600: 11.9 / 11.7, 6.8 / 8.5, 3.5 / 5.3;  19200: 15.9 / 17.7, 10.4 / 14.0, 5.0 / 8.6;  65536: 31 / 44 (256).
     if (a.E % 32 == 0 && a.K <= 8 && 8 % a.groups == 0 && a.top * (8 / a.groups) >= 2 && a.T >= (a.E <= 64 ? 32ll : 64ll) * sm_count && (uintptr_t)a.logits % 16 == 0) {
         if (a.E <= 32) return octets<4>(a, sp, sm_count, st);
         if (a.E <= 64) return octets<8>(a, sp, sm_count, st);

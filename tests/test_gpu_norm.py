@@ -248,3 +248,16 @@ def test_the_c_calls_refuse_what_would_overlap(plane):
                        (dict(work=p(ws) + 16), "workspace")):
         assert back(**kw) == _lib.MOE_EINVAL and needle in _lib.last_error(), kw
     assert plane.launch_count == before
+
+
+def test_the_weights_gradient_overlaps_nothing(plane):
+    """dweight on an operand: written while other rows may still be read.  Nothing is launched."""
+    from npu_offload_b200 import _lib
+    L, f = nob.lib(), lambda *shape: torch.zeros(*shape, device="cuda")
+    dy, total, dsum, w, rstd, dx, ws = f(4, 32), f(4, 32), f(4, 32), f(32), f(64), f(4, 32), f(1 << 20)
+    p, before = lambda t: t.data_ptr(), plane.launch_count
+    for t in (dy, total, dsum, w, rstd, dx):
+        for at in (p(t), p(t) + 4, p(t) - 124):
+            assert L.moe_add_norm_backward(plane.handle, 4, 32, p(dy), 1, p(total), 1, p(dsum), p(w), 1, p(rstd), p(dx), at, p(ws), 1 << 22,
+                                           0, None) == _lib.MOE_EINVAL and "overlap" in _lib.last_error()
+    assert plane.launch_count == before
