@@ -4,9 +4,10 @@
 //
 // One launch: a cluster of eight CTAs a token.  Each takes an eighth of the inner dimension of A for all r rows (a warp a
 // row, 16-byte loads), the partial sums go to all eight through distributed shared memory and are added there in order,
-// and each then takes an eighth of the columns of B, whose first are in registers by then: a row of B is read by as many
-// neighbouring lanes as it has 16-byte words (a thread a row: 10.6 instead of 7.5 us at 32 tokens, r = 64).  All sums are fp32; the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the
-// store), by the adapters' bytes out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.7 us; 1280 x 32 x 4096, 48 tokens of 32
+// and each then takes an eighth of the columns of B, whose first are in registers by then up to r = 32: a row of B is read by as
+// many neighbouring lanes as it has 16-byte words (a thread a row: 10.6 instead of 7.5 us at 32 tokens, r = 64).  All sums are fp32;
+// the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the store), by the adapters' bytes
+// out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.6 us; 1280 x 32 x 4096, 48 tokens of 32
 // adapters: 6.6 us, 1.6 of them for the bytes from HBM.
 #include <cooperative_groups.h>
 
@@ -35,7 +36,7 @@ __device__ __forceinline__ void lora_store(const LoraArgs& a, size_t i, float v)
 
 // R: rank rows of A a warp, and 16-byte words of a row of B; r <= 8 R, R a power of two.
 template <int R>
-__global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThreads) lora_few_kernel(LoraArgs a) {
+__global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThreads, R == 16 ? 2 : R == 8 ? 3 : 4) lora_few_kernel(LoraArgs a) {
     __shared__ float part[kLoraCluster][kLoraMaxRank], own[kLoraMaxRank], low[kLoraMaxRank];
     griddep_wait();
     cg::cluster_group cl = cg::this_cluster();
@@ -55,6 +56,9 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
     const uint16_t* x = a.x + (size_t)t * a.K;
     // Columns of B, 32 a warp: R neighbouring lanes a row of B, 16 bytes each, R rows after one another; the first are on their way early.
     const int chunk = lane % R, g1 = (n1 - n0 + 31) / 32;
+    // (Held that early, eight words a lane cost a CTA of each SM: 7.5 / 7.8 us with / without at 32 tokens, 13.3 / 8.8 at 48; sixteen: 20.2 / 13.3
+    // at 24.  Asking L2 for them instead: 7.9, 9.1; 13.9.)
+    constexpr bool kEarly = R < 8;
     uint4 bv[R];
     auto ask = [&](int g) {
 #pragma unroll
@@ -66,7 +70,7 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
     const int mine = lane / R + 32 / R * chunk;  // the column of 32 whose sum this lane ends up with
     float base = 0.f;
     if (warp < g1) {
-        ask(warp);
+        if (kEarly) ask(warp);
         if (n0 + warp * 32 + mine < n1) base = lora_load(a, out_row + n0 + warp * 32 + mine);
     }
     float acc[R];
@@ -106,10 +110,8 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
     for (int k = 0; k < 8; k++) l8[k] = chunk * 8 < r ? low[chunk * 8 + k] : 0.f;
     for (int g = warp; g < g1; g += kLoraWarps) {
         const int n = n0 + g * 32 + mine;
-        if (g != warp) {
-            ask(g);
-            if (n < n1) base = lora_load(a, out_row + n);
-        }
+        if (!kEarly || g != warp) ask(g);
+        if (g != warp && n < n1) base = lora_load(a, out_row + n);
         float v[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
@@ -136,9 +138,9 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
 }
 
 // Calls of at most so many tokens take a cluster a token, others the kernels of lora_many.cu, us (a cluster a token / the others):
-//   r = 16: 64 tokens 5.8 / 11.3, 128: 11.4 / 11.3, 192: 16.1 / 12.0 (4096 x 2560)     r = 32: 64: 7.2 / 14.3, 128: 12.9 / 15.4 (1280 x 4096)
-//   r = 64: 32: 7.5 / 15.2, 64: 13.7 / 15.5, 96: 19.9 / 15.5 (1280 x 4096)              r = 128: 24: 19.8 / 20.4, 32: 21.7 / 20.5 (4096 x 2560)
-static int lora_few_tokens(int r) { return r <= 32 ? 128 : r <= 64 ? 64 : 24; }
+//   r = 16: 64 tokens 5.8 / 11.3, 128: 11.4 / 11.3, 192: 16.1 / 12.0 (4096 x 2560)     r = 32: 64: 7.0 / 13.2, 128: 12.7 / 13.0 (1280 x 4096)
+//   r = 64: 48: 8.8 / 14.7, 64: 14.5 / 14.9, 96: 16.0 / 14.9 (1280 x 4096)              r = 128: 32: 13.7 / 20.6, 48: 23.8 / 22.2 (4096 x 2560)
+static int lora_few_tokens(int r) { return r <= 32 ? 128 : r <= 64 ? 64 : 32; }
 
 size_t lora_workspace(int T, int n, int r) { return T <= lora_few_tokens(r) ? 0 : lora_many_workspace(T, n, r); }
 

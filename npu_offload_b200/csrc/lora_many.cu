@@ -13,11 +13,11 @@
 // rows (gathered) and of A's r rows a stage, cp.async, a warp 16 tokens; the sums go to the CTA that owns the tokens, which adds them
 // in order, multiplies by the scale and splits each into bf16 parts (two for a bf16 result: 2^-17 of low; three for an fp32 one:
 // 2^-24), stored as the fragments that the matrix instruction takes, 16 bytes a lane.
-// lora_out_kernel, a CTA 32 tokens and four warps' columns: out.  A warp reads and writes 16 bytes of four lanes a row, whole
+// lora_out_kernel, a CTA 32 tokens (64 from r = 64 on) and four warps' columns: out.  A warp reads and writes 16 bytes of four lanes a row, whole
 // sectors: the columns of B are dealt to the matrix instruction so that a lane's results are neighbours, as are its inner values,
 // eight bytes of a row of B.  base and B are asked for ahead of the wait for lora_low_kernel.
 //
-// 4093 tokens, 4096 x 16 x 2560: 24 us, 13 of them the first two kernels; x, base and out alone take 11.8 at a copy's rate.  (One
+// 4093 tokens, 4096 x 16 x 2560: 23 us, 12 of them the first two kernels; x, base and out alone take 11.8 at a copy's rate.  (One
 // kernel for low and out, the cluster going on to its columns: 26 to 29 us, since all CTAs load, exchange and store at the same time.)
 #include <cooperative_groups.h>
 
@@ -211,7 +211,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
 // cluster is through with those.
 template <int R>
 struct LowSmem {
-    static constexpr int kStages = 4;
+    static constexpr int kStages = R <= 32 ? 4 : 3;  // (four CTAs an SM at r = 64: the 576 of 4093 tokens in one round, 34.6 instead of 43.6 us; two: 35.8)
     static constexpr int kStageBytes = (kTile + R) * kStageCols * 2;
     static constexpr int kOffTok = kStages * kStageBytes;
     static constexpr int kBytes = kOffTok + kTile * 4;
@@ -312,48 +312,53 @@ __global__ void __cluster_dims__(kLowCluster, 1, 1) __launch_bounds__(kLowThread
     }
 }
 
-// A warp's columns: 16 bytes of four lanes' results.  An item is 32 tokens and some column blocks of a CTA; the next blocks' base and
+// A warp's columns: 16 bytes of four lanes' results.  An item is 32 or 64 tokens and some column blocks of a CTA; the next blocks' base and
 // B are on their way into shared memory while one is worked on (in registers, a block ahead: 17 us of 30 at 4093 tokens, since
 // 16 warps an SM had too little on its way).
 template <int R, bool F32>
 struct OutSmem {
-    static constexpr int kStages = R <= 16 ? 4 : R <= 64 ? 3 : 2;
+    // Halves of a tile.  Both with the same stage of B, four warps each, leave twice the warps an SM where B takes most of shared memory:
+    // r = 64: 43.6 us / with one, in three stages, 46.3 (4093 tokens, 4096 x 2560), r = 128: 60.6 / 66.4 (2048 tokens, 4096 x 4096); at r = 16 one is enough: 25.9 / 23.2.
+    static constexpr int kHalves = R <= 32 ? 1 : 2;
+    static constexpr int kRows = 32 * kHalves, kThreads = kOutThreads * kHalves;
+    static constexpr int kStages = R <= 16 ? 4 : R <= 32 ? 3 : 2;
     static constexpr int W = F32 ? 4 : 8, kGroup = 4 * W, kCols = kGroup * kOutThreads / 32;
     static constexpr int kBasePitch = 256 + 16;                    // of a token's 256 bytes of a block
     static constexpr int kBPitch = R * 2 + (R > 16 ? 32 : 0);      // of a column's r values: eight bytes of four rows on different banks
-    static constexpr int kStageBytes = 32 * kBasePitch + kCols * kBPitch;
+    static constexpr int kStageBytes = kRows * kBasePitch + kCols * kBPitch;
     static constexpr bool kHoldLow = R <= 32;                      // low's fragments in registers, else behind the stages
-    static constexpr int kLowBytes = kHoldLow ? 0 : 2 * (R / 16) * (F32 ? 3 : 2) * 512;
+    static constexpr int kLowBytes = kHoldLow ? 0 : kRows / 16 * (R / 16) * (F32 ? 3 : 2) * 512;
     static constexpr int kBytes = kStages * kStageBytes + kLowBytes;
 };
 template <int R, bool F32>
-__global__ void __launch_bounds__(kOutThreads) lora_out_kernel(LoraArgs a, LoraWs ws) {
+__global__ void __launch_bounds__((OutSmem<R, F32>::kThreads)) lora_out_kernel(LoraArgs a, LoraWs ws) {
     using S = OutSmem<R, F32>;
     extern __shared__ __align__(128) unsigned char smem[];
     constexpr int W = S::W, kGroup = S::kGroup, kCols = S::kCols, PARTS = F32 ? 3 : 2, NT = W / 2, kSize = F32 ? 4 : 2;
+    constexpr int kRows = S::kRows, kThreads = S::kThreads, kPieces = kTile / kRows;
     constexpr bool kHoldLow = S::kHoldLow;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, q = lane & 3, i8 = lane >> 2, r = a.r, N = a.N;
+    const int tid = threadIdx.x, warp = tid >> 5 & 3, m0 = tid >> 7 << 1, lane = tid & 31, q = lane & 3, i8 = lane >> 2, r = a.r, N = a.N;
     const bool vec = N % W == 0;
     const int blocks = (N + kCols - 1) / kCols;
     const uint32_t s_base = smem_u32(smem);
     // Written before lora_low_kernel let this one start: the tiles (its own wait was for them), base and B.  Past L1.
-    const int halves = __ldcg(ws.n_tiles) * 2;
-    // a half tile's blocks in as many chunks as leave no CTA with two
-    const int most = max(1, min(blocks, (int)gridDim.x / max(1, halves))), per = (blocks + most - 1) / most, chunks = (blocks + per - 1) / per;
+    const int pieces = __ldcg(ws.n_tiles) * kPieces;
+    // a piece's (a tile's, or half a tile's) blocks in as many chunks as leave no CTA with two
+    const int most = max(1, min(blocks, (int)gridDim.x / max(1, pieces))), per = (blocks + most - 1) / most, chunks = (blocks + per - 1) / per;
     bool waited = false;
 #pragma unroll 1
-    for (int item = blockIdx.x; item < halves * chunks; item += gridDim.x) {
-        const int half_tile = item / chunks, i_tile = half_tile >> 1, row0 = (half_tile & 1) * 32;
+    for (int item = blockIdx.x; item < pieces * chunks; item += gridDim.x) {
+        const int piece = item / chunks, i_tile = piece / kPieces, row0 = piece % kPieces * kRows;
         const int* order = ws.order + i_tile * kTile + row0;
         const int2 tile = __ldcg(reinterpret_cast<const int2*>(ws.tiles + i_tile));
-        // of this thread: the tokens of its results, and of the rows that it copies (tid / 16 + 8 i)
+        // of this thread: the tokens of its results, and of the rows that it copies
         int token[4], copied[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) token[i] = __ldcg(order + i * 8 + i8), copied[i] = __ldcg(order + i * 8 + (tid >> 4));
+        for (int i = 0; i < 4; i++) token[i] = __ldcg(order + m0 * 16 + i * 8 + i8), copied[i] = __ldcg(order + i * 8 * S::kHalves + (tid >> 4));
         const int rows = tile.y - row0;
         if (rows <= 0) continue;
         const uint16_t* B = a.b + (size_t)max(tile.x, 0) * N * r;
-        const int block0 = (item - half_tile * chunks) * per, block1 = min(block0 + per, blocks);
+        const int block0 = (item - piece * chunks) * per, block1 = min(block0 + per, blocks);
         auto ask = [&](int block) {
             if (block < block1) {
                 const uint32_t buf = s_base + (block - block0) % S::kStages * S::kStageBytes;
@@ -361,19 +366,19 @@ __global__ void __launch_bounds__(kOutThreads) lora_out_kernel(LoraArgs a, LoraW
                 if (vec)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const int row = i * 8 + (tid >> 4);
+                        const int row = i * 8 * S::kHalves + (tid >> 4);
                         const bool in = row < rows && col < N;
                         cp_async16_or_zero(buf + row * S::kBasePitch + word * 16,
                                            static_cast<const char*>(a.base) + (in ? ((size_t)copied[i] * N + col) * kSize : 0), in);
                     }
                 if (tile.x >= 0)
 #pragma unroll
-                    for (int i = 0; i < kCols * (R / 8) / kOutThreads; i++) {
-                        const int at = tid + i * kOutThreads, n = at / (R / 8), w = at % (R / 8);
+                    for (int i = 0; i < kCols * (R / 8) / kThreads; i++) {
+                        const int at = tid + i * kThreads, n = at / (R / 8), w = at % (R / 8);
                         // column n of a group goes where the instruction's rows i8 of product j are neighbours
                         const int in_group = n % kGroup, pos = n - in_group + in_group % W / 2 * 8 + in_group / W * 2 + (in_group & 1);
                         const bool in = block * kCols + n < N && w * 8 < r;
-                        cp_async16_or_zero(buf + 32 * S::kBasePitch + pos * S::kBPitch + w * 16, in ? B + (size_t)(block * kCols + n) * r + w * 8 : a.b, in);
+                        cp_async16_or_zero(buf + kRows * S::kBasePitch + pos * S::kBPitch + w * 16, in ? B + (size_t)(block * kCols + n) * r + w * 8 : a.b, in);
                     }
             }
             cp_async_commit();
@@ -389,7 +394,7 @@ __global__ void __launch_bounds__(kOutThreads) lora_out_kernel(LoraArgs a, LoraW
         const uint4* low_s = reinterpret_cast<const uint4*>(smem + S::kStages * S::kStageBytes) + lane;
         if (!kHoldLow && tile.x >= 0) {
 #pragma unroll 1
-            for (int i = tid; i < S::kLowBytes / 16; i += kOutThreads) cp_async16(s_base + S::kStages * S::kStageBytes + i * 16, low + i);
+            for (int i = tid; i < S::kLowBytes / 16; i += kThreads) cp_async16(s_base + S::kStages * S::kStageBytes + i * 16, low + i);
             cp_async_wait_all();  // (the loop's first barrier shows it to all)
         }
         uint4 la[kHoldLow ? 2 : 1][kHoldLow ? R / 16 : 1][kHoldLow ? PARTS : 1];
@@ -400,43 +405,49 @@ __global__ void __launch_bounds__(kOutThreads) lora_out_kernel(LoraArgs a, LoraW
                 for (int k = 0; k < R / 16; k++)
 #pragma unroll
                     for (int part = 0; part < PARTS; part++)
-                        la[m][k][part] = tile.x >= 0 && m * 16 < rows ? low[((m * (R / 16) + k) * PARTS + part) * 32 + lane] : make_uint4(0, 0, 0, 0);
+                        la[m][k][part] = tile.x >= 0 && (m0 + m) * 16 < rows ? low[(((m0 + m) * (R / 16) + k) * PARTS + part) * 32 + lane] : make_uint4(0, 0, 0, 0);
 #pragma unroll 1
         for (int block = block0; block < block1; block++) {
             cp_async_wait<S::kStages - 2>();
             __syncthreads();  // this block is there; the one before, whose buffer comes next, has been used
             ask(block + S::kStages - 1);
             const unsigned char* buf = smem + (block - block0) % S::kStages * S::kStageBytes;
-            const unsigned char* b_at = buf + 32 * S::kBasePitch + (warp * kGroup + i8) * S::kBPitch + q * 8;
+            const unsigned char* b_at = buf + kRows * S::kBasePitch + (warp * kGroup + i8) * S::kBPitch + q * 8;
             const int col = block * kCols + warp * kGroup + W * q;
+            if (m0 * 16 >= rows) continue;
+            float o[2][NT][4];
 #pragma unroll
-            for (int m = 0; m < 2; m++) {
-                if (m * 16 >= rows) break;
-                float o[NT][4];
+            for (int m = 0; m < 2; m++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-                if (tile.x >= 0)
+                for (int j = 0; j < NT; j++) o[m][j][0] = o[m][j][1] = o[m][j][2] = o[m][j][3] = 0.f;
+            if (tile.x >= 0)
 #pragma unroll
-                    for (int k = 0; k < R / 16; k++) {
-                        uint2 bv[NT];
+                for (int k = 0; k < R / 16; k++) {
+                    uint2 bv[NT];
 #pragma unroll
-                        for (int j = 0; j < NT; j++) bv[j] = *reinterpret_cast<const uint2*>(b_at + j * 8 * S::kBPitch + k * 32);
+                    for (int j = 0; j < NT; j++) bv[j] = *reinterpret_cast<const uint2*>(b_at + j * 8 * S::kBPitch + k * 32);
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        if ((m0 + m) * 16 >= rows) break;
 #pragma unroll
                         for (int part = 0; part < PARTS; part++) {
-                            const uint4 v = kHoldLow ? la[kHoldLow ? m : 0][kHoldLow ? k : 0][kHoldLow ? part : 0] : low_s[((m * (R / 16) + k) * PARTS + part) * 32];
+                            const uint4 v = kHoldLow ? la[kHoldLow ? m : 0][kHoldLow ? k : 0][kHoldLow ? part : 0] : low_s[(((m0 + m) * (R / 16) + k) * PARTS + part) * 32];
                             const uint32_t f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-                            for (int j = 0; j < NT; j++) mma_bf16(o[j], f, bv[j].x, bv[j].y);
+                            for (int j = 0; j < NT; j++) mma_bf16(o[m][j], f, bv[j].x, bv[j].y);
                         }
                     }
+                }
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const int row = m * 16 + h * 8 + i8;
+                    const int row = (m0 + m) * 16 + h * 8 + i8;
                     if (row >= rows || col >= N) continue;
                     const size_t to = (size_t)token[m * 2 + h] * N + col;
                     float v[W];
 #pragma unroll
-                    for (int j = 0; j < NT; j++) v[2 * j] = o[j][2 * h], v[2 * j + 1] = o[j][2 * h + 1];
+                    for (int j = 0; j < NT; j++) v[2 * j] = o[m][j][2 * h], v[2 * j + 1] = o[m][j][2 * h + 1];
                     if (vec) {
                         const uint4 was = *reinterpret_cast<const uint4*>(buf + row * S::kBasePitch + (warp * 4 + q) * 16);
                         const uint32_t b[4] = {was.x, was.y, was.z, was.w};
@@ -475,9 +486,9 @@ static cudaError_t many_for(const LoraArgs& a, const LoraWs& ws, int sm_count, c
     ++*launches;
     constexpr auto out = lora_out_kernel<R, F32>;
     if ((e = allow_smem<out>(OutSmem<R, F32>::kBytes)) != cudaSuccess) return e;
-    const int64_t items = 2ll * tiles * ((a.N + OutSmem<R, F32>::kCols - 1) / OutSmem<R, F32>::kCols);
+    const int64_t items = (int64_t)(kTile / OutSmem<R, F32>::kRows) * tiles * ((a.N + OutSmem<R, F32>::kCols - 1) / OutSmem<R, F32>::kCols);
     const int fit = std::max(1, std::min(8, 225 * 1024 / (OutSmem<R, F32>::kBytes + 1024)));  // CTAs that an SM has room for
-    const Launch o{(int)std::min<int64_t>(items, (int64_t)fit * sm_count), kOutThreads, OutSmem<R, F32>::kBytes, 0, st};
+    const Launch o{(int)std::min<int64_t>(items, (int64_t)fit * sm_count), OutSmem<R, F32>::kThreads, OutSmem<R, F32>::kBytes, 0, st};
     if ((e = o.run(out, a, ws)) == cudaSuccess) ++*launches;
     return e;
 }

@@ -172,3 +172,26 @@ def test_the_library_refuses(plane):
     assert plane.launch_count == before
     for bad in ((1 << 21, 8, 1), (1, 8, 0), (1, 0, 1), (-1, 8, 1)):
         assert L.moe_add_lora_workspace(plane.handle, *bad) == -1
+
+
+@pytest.mark.parametrize("r,tokens", [(32, 128), (64, 64), (128, 32)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("more", [0, 1])
+def test_on_both_sides_of_few_tokens(plane, r, tokens, dtype, more):
+    """One kernel on one side, three on the other; columns that end inside a warp's and a block's."""
+    m = make(gen(r + more), tokens + more, 328, 300, r, 3, dtype)
+    check(plane.add_lora(**m), **m)
+
+
+@pytest.mark.parametrize("r", [16, 64, 128])
+@pytest.mark.parametrize("last", [1, 16, 17, 32, 33, 48, 49, 64])
+def test_tiles_that_end_anywhere(plane, r, last):
+    """Tokens of one adapter beyond whole tiles of 64: rows behind a tile's last are no one's."""
+    T = 192 + last
+    m = make(gen(r + last), T, 136, 264, r, 2, BF)
+    m["ids"] = torch.zeros(T, dtype=torch.int32, device="cuda")
+    check(plane.add_lora(**m), **m)
+    m["ids"].fill_(1)
+    m["ids"][5] = -1
+    check(plane.add_lora(**m), **m)
+    assert plane.status() == 0
