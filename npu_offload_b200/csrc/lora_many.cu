@@ -9,7 +9,7 @@
 // Places within an adapter go by integer atomics and may differ from run to run; no result does, since a token's
 // sums do not depend on its place.
 //
-// lora_low_kernel, a cluster of eight CTAs a tile: low.  A CTA multiplies an eighth of the inner dimension, 64 columns of x's 64
+// lora_low_kernel, a cluster of eight or four CTAs a tile: low.  A CTA multiplies its share of the inner dimension, 64 columns of x's 64
 // rows (gathered) and of A's r rows a stage, cp.async, a warp 16 tokens; the sums go to the CTA that owns the tokens, which adds them
 // in order, multiplies by the scale and splits each into bf16 parts (two for a bf16 result: 2^-17 of low; three for an fp32 one:
 // 2^-24), stored as the fragments that the matrix instruction takes, 16 bytes a lane.
@@ -34,8 +34,7 @@ namespace cg = cooperative_groups;
 namespace moe {
 
 constexpr int kTile = 64;                    // tokens
-constexpr int kLowThreads = 128, kLowCluster = 8;
-constexpr int kOwned = kTile / kLowCluster;  // tokens whose sums a CTA adds
+constexpr int kLowThreads = 128;
 constexpr int kOutThreads = 128;
 constexpr int kStageCols = 64;
 constexpr int kPlanThreads = 1024;
@@ -215,22 +214,23 @@ struct LowSmem {
     static constexpr int kStageBytes = (kTile + R) * kStageCols * 2;
     static constexpr int kOffTok = kStages * kStageBytes;
     static constexpr int kBytes = kOffTok + kTile * 4;
-    static_assert(kLowCluster * kOwned * R * 4 <= kOffTok, "the sums fit in the stages");
+    static_assert(kTile * R * 4 <= kOffTok, "the sums fit in the stages");
 };
 
-template <int R, int PARTS>
-__global__ void __cluster_dims__(kLowCluster, 1, 1) __launch_bounds__(kLowThreads) lora_low_kernel(LoraArgs a, LoraWs ws) {
+template <int R, int PARTS, int CL>
+__global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kLowThreads) lora_low_kernel(LoraArgs a, LoraWs ws) {
     using S = LowSmem<R>;
+    constexpr int kOwned = kTile / CL;  // tokens whose sums a CTA adds
     extern __shared__ __align__(128) unsigned char smem[];
     griddep_wait();
     griddep_launch_dependents();  // lora_out_kernel waits for this one's end before it reads low
     cg::cluster_group cl = cg::this_cluster();
     const int c = (int)cl.block_rank(), tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = a.r;
     const int n_tiles = __ldcg(ws.n_tiles), U = a.K / 8;
-    const int u0 = (int)((int64_t)c * U / kLowCluster), u1 = (int)((int64_t)(c + 1) * U / kLowCluster), stages = (u1 - u0 + 7) / 8;
+    const int u0 = (int)((int64_t)c * U / CL), u1 = (int)((int64_t)(c + 1) * U / CL), stages = (u1 - u0 + 7) / 8;
     int* tok = reinterpret_cast<int*>(smem + S::kOffTok);
     const uint32_t s_base = smem_u32(smem);
-    for (int i_tile = blockIdx.x / kLowCluster; i_tile < n_tiles; i_tile += gridDim.x / kLowCluster) {  // the whole cluster alike
+    for (int i_tile = blockIdx.x / CL; i_tile < n_tiles; i_tile += gridDim.x / CL) {  // the whole cluster alike
         const int token = tid < kTile ? __ldcg(ws.order + i_tile * kTile + tid) : 0;  // (of no meaning behind the tile's count)
         const int2 tile = __ldcg(reinterpret_cast<const int2*>(ws.tiles + i_tile));   // adapter, count
         if (tile.x < 0) continue;
@@ -293,7 +293,7 @@ __global__ void __cluster_dims__(kLowCluster, 1, 1) __launch_bounds__(kLowThread
             const int owned = i / (R / 2), col = (i % (R / 2)) * 2, row = c * kOwned + owned;
             float v0 = 0.f, v1 = 0.f;
 #pragma unroll
-            for (int s = 0; s < kLowCluster; s++) {
+            for (int s = 0; s < CL; s++) {
                 const float2 p = *reinterpret_cast<const float2*>(slots + (size_t)(s * kOwned + owned) * R + col);
                 v0 += p.x, v1 += p.y;
             }
@@ -475,14 +475,22 @@ __global__ void __launch_bounds__((OutSmem<R, F32>::kThreads)) lora_out_kernel(L
     if (!waited) griddep_wait();
 }
 
+template <int R, bool F32, int CL>
+static cudaError_t low_for(const LoraArgs& a, const LoraWs& ws, int tiles, int sm_count, cudaStream_t st) {
+    constexpr auto low = lora_low_kernel<R, F32 ? 3 : 2, CL>;
+    const cudaError_t e = allow_smem<low>(LowSmem<R>::kBytes);
+    const Launch l{std::min(tiles, sm_count) * CL, kLowThreads, LowSmem<R>::kBytes, 0, st};
+    return e != cudaSuccess ? e : l.run(low, a, ws);
+}
 template <int R, bool F32>
 static cudaError_t many_for(const LoraArgs& a, const LoraWs& ws, int sm_count, cudaStream_t st, int* launches) {
-    constexpr auto low = lora_low_kernel<R, F32 ? 3 : 2>;
-    cudaError_t e = allow_smem<low>(LowSmem<R>::kBytes);
-    if (e != cudaSuccess) return e;
     const int tiles = lora_max_tiles(a.T, a.n);
-    const Launch l{std::min(tiles, sm_count) * kLowCluster, kLowThreads, LowSmem<R>::kBytes, 0, st};
-    if ((e = l.run(low, a, ws)) != cudaSuccess) return e;
+    cudaError_t e;
+    // Clusters of four where eights may not all run at once; up to r = 32 fours are not faster.  Four / eight, us, 4096 x 2560: r = 64,
+    // 4096 tokens of 32 adapters 41.8 / 46.9, 300 of 4 (2048 x 2560, fp32) 15.9 / 14.5; r = 16, 4096 of 32: 27.8 / 26.9.
+    if (R >= 64 && tiles * 8 > 225 * 1024 / (LowSmem<R>::kBytes + 1024) * sm_count) e = low_for<R, F32, R >= 64 ? 4 : 8>(a, ws, tiles, sm_count, st);
+    else e = low_for<R, F32, 8>(a, ws, tiles, sm_count, st);
+    if (e != cudaSuccess) return e;
     ++*launches;
     constexpr auto out = lora_out_kernel<R, F32>;
     if ((e = allow_smem<out>(OutSmem<R, F32>::kBytes)) != cudaSuccess) return e;

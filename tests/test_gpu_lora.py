@@ -195,3 +195,12 @@ def test_tiles_that_end_anywhere(plane, r, last):
     m["ids"][5] = -1
     check(plane.add_lora(**m), **m)
     assert plane.status() == 0
+
+
+@pytest.mark.parametrize("T,K,N,r,n", [(4096, 264, 136, 64, 32), (2500, 4096, 40, 128, 64), (5000, 136, 72, 104, 3)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_more_tiles_than_run_at_once(plane, T, K, N, r, n, dtype):
+    """Of higher ranks, a tile then has fewer CTAs and a CTA a larger share of the inner dimension."""
+    m = make(gen(T + r), T, K, N, r, n, dtype)
+    check(plane.add_lora(**m), **m)
+    assert plane.status() == 0
