@@ -204,9 +204,11 @@ struct RouteGrid {
 // Sigmoid, in steps of the grid (2^-23 of the range; `grid` steps make 1): the product l log2 e is off by |l| 2^-24 / ln 2 in the
 // exponent, 2^x and the reciprocal by 2^-22 each, the additions by 2^-24, so s by s (1 - s) |l| 2^-24 + s 2^-21 at most, and, since
 // s (1 - s) |l| < 0.23, by less than 2^-20.  The bias's place on the grid is off by 1.5 steps, the sum by half a step, and the key
-// of the definition by 2^-24 of its size, kmax at most.  Two keys: grid (2^-19 + kmax 2^-23) + 4; two groups of two keys: twice that,
-// and a step of 2^-23 of a score, 2 kmax, each, for the sums' rounding.  (Scores that are all far below 2^-19 are told apart by
-// their biases; without those, exactly.)
+// of the definition by 2^-24 of its size, kmax at most.  Two keys: grid (2^-19 + kmax 2^-23) + 4 = apart.  Two groups of two keys, in
+// the same terms: grid 2^-20 and 2 steps for each of the four keys; kmax 2^-24 for the rounding of each, half a unit of kmax 2^-23, two
+// units for the four; and 2 kmax 2^-24 for the rounding of each group's fp32 sum, two units for both: grid (2^-18 + 4 kmax 2^-23) + 8,
+// which 4 apart covers (with 3 apart biases near 128 that lie within 0.1 have opened a group that was not the definition's).
+// (Scores that are all far below 2^-19 are told apart by their biases; without those, exactly.)
 // A NaN, like a bias that is not finite, leaves the range of words and is left to the exact choice.
 // FULL: every lane has V experts.
 template <int V, bool SIG, bool FULL>
@@ -281,7 +283,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32, 4) route_groups_kernel(Route
                 if (score == last) open = true, score = 0;
             }
             const uint32_t next = __reduce_max_sync(0xffffffffu, score);
-            if (SIG) again |= !((float)(last / 32 - next / 32) > 3.f * apart);
+            if (SIG) again |= !((float)(last / 32 - next / 32) > 4.f * apart);
             else again |= last / 32 == next / 32;
             if (!open) step = list + V * 32;
         }
@@ -469,7 +471,7 @@ __global__ void __launch_bounds__(kOctetWarps * 32, kOctetCtas) route_octet_kern
                 last = min(last, __shfl_xor_sync(0xffffffffu, last, o));
                 next = max(next, __shfl_xor_sync(0xffffffffu, next, o));
             }
-            if (SIG) again |= !((float)(last / 32 - next / 32) > 3.f * apart);
+            if (SIG) again |= !((float)(last / 32 - next / 32) > 4.f * apart);
             else again |= last / 32 == next / 32;
             if (!open) step = list + (kKept + 1) * 32;
         }
