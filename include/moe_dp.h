@@ -312,8 +312,8 @@ MOE_API int moe_balance_loss_backward(moe_ctx* ctx, int64_t T, const float* logi
  *
  * moe_route_backward: dlogits [T, E] = the gradient of the logits from dw [T, top_k], that of topk_w (of moe_route_topk too:
  * renormalize = 1, scale = 1), at the choices topk_idx (negative: none; one of E or more is skipped, MOE_EINVAL in the device-side
- * status; an expert twice in a token counts twice).  Choices are constants.  MOE_F_ACCUMULATE: dlogits +=, as behind
- * moe_balance_loss_backward.
+ * status; an expert twice in a token counts twice).  Choices are constants; a token without one has a gradient of zeros, whatever its
+ * logits hold.  MOE_F_ACCUMULATE: dlogits +=, as behind moe_balance_loss_backward.
  *
  * Both use nothing of the context but the device-side status. */
 MOE_API int moe_route_groups(moe_ctx* ctx, int64_t T, const float* router_logits, const float* bias, int groups, int top_groups,

@@ -732,6 +732,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_dense_kernel(RouteBack
             i = -1;
         }
         const bool in = i >= 0;
+        if (!__any_sync(0xffffffffu, in)) {  // no choice, so no gradient, whatever the logits hold (padding, say)
+#pragma unroll
+            for (int j = 0; j < V; j++)
+                if (!a.accumulate && lane + 32 * j < E) out[lane + 32 * j] = 0.f;
+            continue;
+        }
         if (!in) g = 0.f;
         float most = l[0];
 #pragma unroll
