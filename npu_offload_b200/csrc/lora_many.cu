@@ -298,6 +298,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(kLowThreads) lora_l
                 v0 += p.x, v1 += p.y;
             }
             v0 *= scale, v1 *= scale;
+            if (col >= r) v0 = v1 = 0.f;  // (an infinity or NaN in x or the scale makes NaN of the zero rows behind A's r)
             // of 16 inner values 4 q + {0, 1, 2, 3} are lane q's: the first two where the instruction has 2 q, the others where it has 2 q + 8
             const int to_lane = (row & 7) * 4 + ((col & 15) >> 2), reg = (col & 2) + (row >> 3 & 1);
             uint32_t* to = reinterpret_cast<uint32_t*>(ws.low + (((size_t)i_tile * 4 + row / 16) * (R / 16) + col / 16) * PARTS * 32 + to_lane) + reg;
