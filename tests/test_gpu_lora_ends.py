@@ -62,3 +62,39 @@ def test_scales_that_are_no_numbers(plane, T, r, dtype):
     m["a"][0], m["b"][0], m["x"] = m["a"][0].abs() + 0.01, m["b"][0].abs() + 0.01, m["x"].abs() + 0.01
     m["scale"][0], m["scale"][2] = INF, float("nan")
     same_ends(plane.add_lora(**m), definition(**m))
+
+
+@pytest.mark.parametrize("T", [5, 150])
+@pytest.mark.parametrize("r,N", [(8, 77), (16, 64), (24, 136), (64, 264), (128, 33)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_infinities_in_b(plane, T, r, N, dtype):
+    """A finite inner sum times an infinity is one, whatever the inner sum is held in."""
+    m = make(r + N, T, 136, N, r, 3, dtype)
+    for n in range(0, N, 5):
+        m["b"][0, n, n % r] = INF if n % 2 else -INF
+    m["b"][0, 11, :] = INF  # of both signs among the products: NaN
+    m["x"][2] = 0  # 0 times an infinity
+    clean = plane.add_lora(**{**m, "b": torch.where(m["b"].isinf(), 0, m["b"])})
+    got, want = plane.add_lora(**m), definition(**m)
+    assert want[0].isinf().any() and want[2].isnan().any()
+    same_ends(got, want)
+    plain = [n for n in range(N) if n % 5 and n != 11]
+    assert torch.equal(got[:, plain], clean[:, plain])  # columns without one
+    others = m["ids"] != 0
+    assert torch.equal(got[others], clean[others])
+
+
+@pytest.mark.parametrize("T", [5, 150])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_inner_sums_beyond_the_largest_bf16(plane, T, dtype):
+    """Inner sums of 2^127 (2 - 2^-9), which bf16 rounds to an infinity; the result is 4 - 2^-8 beside a base of 0."""
+    m = make(1, T, 64, 40, 16, 2, dtype)
+    m["ids"].zero_()
+    m["base"].zero_(), m["x"].zero_(), m["a"].zero_(), m["b"].zero_()
+    m["x"][:, 0], m["x"][:, 1], m["a"][0, 3, :2], m["b"][0, :, 3], m["scale"][0] = 2.0 ** 127, 2.0 ** 119, 1.0, 2.0 ** -126, 1.0
+    m["a"][0, 3, 0], m["a"][0, 3, 1] = 2 - 2.0 ** -7, 1.5
+    want = definition(**m)
+    got = plane.add_lora(**m)
+    assert want[0, 0] == 2 * (2 - 2.0 ** -9)
+    # off by half a step of the result, and by 2^-16 of the sum where that is held in two parts
+    assert ((got.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + (2.0 ** -16 if dtype == BF else 2.0 ** -23)) * want).all()
