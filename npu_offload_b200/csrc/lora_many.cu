@@ -429,7 +429,7 @@ __global__ void __launch_bounds__((OutSmem<R, F32>::kThreads)) lora_out_kernel(L
 #pragma unroll
             for (int m = 0; m < 2; m++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) o[m][j][0] = o[m][j][1] = o[m][j][2] = o[m][j][3] = 0.f;
+                for (int j = 0; j < NT; j++) o[m][j][0] = o[m][j][1] = o[m][j][2] = o[m][j][3] = tile.x < 0 ? -0.f : 0.f;  // (base + -0 is base)
             if (tile.x >= 0)
 #pragma unroll
                 for (int k = 0; k < R / 16; k++) {

@@ -98,3 +98,18 @@ def test_inner_sums_beyond_the_largest_bf16(plane, T, dtype):
     assert want[0, 0] == 2 * (2 - 2.0 ** -9)
     # off by half a step of the result, and by 2^-16 of the sum where that is held in two parts
     assert ((got.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + (2.0 ** -16 if dtype == BF else 2.0 ** -23)) * want).all()
+
+
+@pytest.mark.parametrize("T", [5, 150])
+@pytest.mark.parametrize("N", [64, 77])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_base_alone_keeps_its_zeros(plane, T, N, dtype):
+    """Zeros of either sign and NaN among the tokens without an adapter."""
+    m = make(N, T, 72, N, 16, 3, dtype)
+    m["ids"][1::2] = -1
+    m["base"][:, ::3] = -0.0
+    m["base"][:, 1::7] = float("nan")
+    none, bits = m["ids"] < 0, torch.int16 if dtype == BF else torch.int32
+    out, base = plane.add_lora(**m)[none], m["base"][none]
+    assert torch.equal(out.isnan(), base.isnan())
+    assert torch.equal(torch.where(base.isnan(), 0, out).view(bits), torch.where(base.isnan(), 0, base).view(bits))
