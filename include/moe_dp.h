@@ -351,11 +351,13 @@ MOE_API int moe_add_norm_backward(moe_ctx* ctx, int64_t T, int64_t C, const void
  * moe_add_lora: x [T, K] bf16, the projection's input; base [T, N] its result (moe_matmul_fp8's, say), bf16 or fp32; n adapters,
  * a [n, r, K] and b [n, N, r] bf16; ids [T]: each token's adapter, negative for none; scale [n] fp32 (NULL: 1)
  *   out[t] = base[t] + scale[i] * (x[t] . a[i]^T) . b[i]^T,  i = ids[t];   out[t] = base[t] without an adapter
- * with fp32 sums, rounded once, of base's type.  out may be base (tokens without an adapter are then not touched) and else overlaps
+ * with fp32 sums, rounded at the end, of base's type.  out may be base (tokens without an adapter are then not touched) and else overlaps
  * nothing.  An id of n or more is none, and MOE_EINVAL in the device-side status.  T at most 2^20, K and r multiples of 8, K and N
- * at most 2^20, r at most 128, n 1 to 4096.  Device pointers; x, a, b, base and out 16-byte aligned.  A token's result does not depend on
- * the others of the call in more than its sums' order, nor on timing.  workspace: moe_add_lora_workspace bytes, 256-byte aligned
- * (-1: out of range). */
+ * at most 2^20, r at most 128, n 1 to 4096.  Device pointers; x, a, b, base and out 16-byte aligned.
+ * One rounding more: with a bf16 result, calls of many tokens (more than 128 up to r = 32, 64 up to r = 64, 32 beyond) hold the r values
+ * scale[i] * (x[t] . a[i]^T) to 2^-16 of each (fp32 results: all of fp32's bits), as the matrix instruction takes them.
+ * But for that, a token's result depends on the others of the call by its sums' order alone, and not on timing.
+ * workspace: moe_add_lora_workspace bytes, 256-byte aligned (-1: out of range). */
 MOE_API int64_t moe_add_lora_workspace(moe_ctx* ctx, int64_t T, int64_t r, int64_t n);
 MOE_API int moe_add_lora(moe_ctx* ctx, int64_t T, int64_t K, int64_t N, int64_t r, int64_t n, const void* base, const uint16_t* x,
                          const uint16_t* a, const uint16_t* b, const int32_t* ids, const float* scale, void* out, int out_dtype,

@@ -531,7 +531,8 @@ class MoEDataPlane:
 
         base [T, N] (bf16 or fp32) is the shared projection of x [T, K] bf16, matmul_fp8()'s result for instance; a [n, r, K]
         and b [n, N, r] bf16, contiguous; K and r multiples of 8, r at most 128; ids [T] int32; scale [n] fp32 (None: 1).
-        fp32 sums, one rounding.  out may be base: tokens without an adapter are then left as they are."""
+        fp32 sums, rounded at the end; for bf16 results calls of many tokens (more than 128 up to r = 32, 64 up to r = 64, 32 beyond)
+        hold scale[i] * (x . a[i]^T) to 2^-16.  out may be base: tokens without an adapter are then left as they are."""
         if stream is not None:
             with self._on(stream):
                 return self.add_lora(base, x, a, b, ids, scale, out)

@@ -113,3 +113,24 @@ def test_base_alone_keeps_its_zeros(plane, T, N, dtype):
     out, base = plane.add_lora(**m)[none], m["base"][none]
     assert torch.equal(out.isnan(), base.isnan())
     assert torch.equal(torch.where(base.isnan(), 0, out).view(bits), torch.where(base.isnan(), 0, base).view(bits))
+
+
+@pytest.mark.parametrize("T", [5, 150])
+@pytest.mark.parametrize("r", [16, 64])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_what_is_left_where_base_and_adapter_cancel(plane, T, r, dtype):
+    """fp32 sums (steps of 2^-24 of the sizes, as the other tests of this call count them), and for bf16 results of many tokens the inner
+    sums to 2^-16 of each: nothing of the size of a bf16 step of base reaches the result."""
+    m = make(r, T, 512, 96, r, 2, dtype)
+    m["ids"].clamp_(min=0)
+    m["base"].zero_()
+    m["base"] = (-definition(**m)).to(dtype)
+    got, want = plane.add_lora(**m), definition(**m)
+    i = m["ids"].long()
+    low = torch.einsum("t,tk,trk->tr", m["scale"][i].double(), m["x"].double(), m["a"][i].double()).abs()
+    size = torch.einsum("t,tk,trk,tnr->tn", m["scale"][i].double(), m["x"].double().abs(), m["a"][i].double().abs(), m["b"][i].double().abs())
+    held = torch.einsum("tr,tnr->tn", low, m["b"][i].double().abs())
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + (512 / 128 + r + 40) * 2.0 ** -24 * (size + m["base"].double().abs())
+    if dtype == BF and T == 150:
+        bound += 2.0 ** -16 * held
+    assert ((got.double() - want).abs() <= bound).all()
