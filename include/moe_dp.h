@@ -307,8 +307,11 @@ MOE_API int moe_balance_loss_backward(moe_ctx* ctx, int64_t T, const float* logi
  *   a group's score: its largest key (softmax), the fp32 sum of its two largest (sigmoid; of the one, in groups of one)
  *   best groups, and in them the top_k best keys: the larger first, ties to the lower index
  *   topk_w = scale * v, divided by the sum of the chosen v (sigmoid: + 1e-20) where renormalize is set; v = softmax over all E, or s
- * -inf masks an expert: it comes last.  NaN logits or biases, a softmax of +inf or of nothing but -inf: MOE_ENONFINITE in the
- * device-side status; that token's weights are NaN, its experts distinct.  top_k <= top_groups * E / groups.
+ * Masks: under softmax a logit of -inf, whose expert comes last.  Under sigmoid such a logit has s = 0, so its bias alone for a key, which
+ * may be among the best (with a weight of 0); there a bias of -inf masks (a group with fewer than two other experts then scores
+ * -inf), or any bias well below the others' (-10, say), which keeps the fast path, unlike one of -inf.
+ * NaN logits or biases, a softmax of +inf or of nothing but -inf: MOE_ENONFINITE in the device-side status; that token's weights are
+ * NaN, its experts distinct.  top_k <= top_groups * E / groups.
  *
  * moe_route_backward: dlogits [T, E] = the gradient of the logits from dw [T, top_k], that of topk_w (of moe_route_topk too:
  * renormalize = 1, scale = 1), at the choices topk_idx (negative: none; one of E or more is skipped, MOE_EINVAL in the device-side
