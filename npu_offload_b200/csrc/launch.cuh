@@ -5,10 +5,11 @@
 // * Every kernel launched this way waits (griddep_wait) for the end of the kernel before it, in all its CTAs, before it
 //   writes to global memory and before it reads what that kernel writes.  As the kernel before did the same, all
 //   earlier ones have then ended too.
-// * Three kernels read ahead of that wait what older kernels wrote:
+// * Four kernels read ahead of that wait what older kernels wrote:
 //     f8_scatter_kernel       the tokens              behind f8_plan_kernel
 //     f8_few_kernel<kF8Down>  groups, down weights    behind f8_few_kernel<kF8GateUp>
 //     f8_combine_kernel       slots, weights w, out   behind the down product
+//     lora_out_kernel         tiles, base, B          behind lora_low_kernel (as Launch below says)
 //   A kernel starts when every CTA of the one before it has let it (griddep_launch_dependents) or ended.  The plan and
 //   the gate / up product let it after their own wait, so the caller's kernels (and the grouping, for the gate / up
 //   product) have ended and their writes are performed by then; the down product lets its successor start at once, but
