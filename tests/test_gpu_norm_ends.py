@@ -74,3 +74,12 @@ def test_special_values_stay_in_their_row(plane, C, T, dtype):
     exact, exact_w, size, size_w = norm_backward64(dy0, x, w, rstd)
     assert (dx[bad] == 0).all() and ((dx.double() - exact).abs() <= half_step(dtype) * exact.abs() + 2 * WORK * size + 1e-40).all()
     assert ((dw.double() - exact_w).abs() <= WORK * size_w + 1e-40).all()
+
+
+@pytest.mark.parametrize("C", [4097, 4098, 4100, 4099, 5121, 8191])
+def test_no_more_ctas_than_run_at_once(plane, C):
+    """Rows of that length have one CTA an SM, whose shares of the weight's gradient the workspace holds: a CTA more would run behind all others."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    for T in (1, 100, sms, sms + 1, 1000, 4000, 8192, 16384, 65536):
+        n = nob.lib().moe_add_norm_backward_workspace(plane.handle, T, C)
+        assert n % (4 * C) == 0 and 1 <= n // (4 * C) <= min(sms, T)
