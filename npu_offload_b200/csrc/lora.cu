@@ -5,9 +5,9 @@
 // One launch: a cluster of eight CTAs a token.  Each takes an eighth of the inner dimension of A for all r rows (a warp a
 // row, 16-byte loads), the partial sums go to all eight through distributed shared memory and are added there in order,
 // and each then takes an eighth of the columns of B, whose first are in registers by then up to r = 32: a row of B is read by as
-// many neighbouring lanes as it has 16-byte words (a thread a row: 10.6 instead of 7.5 us at 32 tokens, r = 64).  All sums are fp32;
-// the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the store), by the adapters' bytes
-// out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.6 us; 1280 x 32 x 4096, 48 tokens of 32
+// many neighbouring lanes as it has 16-byte words (a thread a row: 10.6 instead of 7.5 us at 32 tokens, r = 64, when its columns were held
+// early too; 7.9 as it is, below).  All sums are fp32; the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the store), by the adapters' bytes
+// out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.6 us (r = 64: 5.3, r = 128: 8.2); 1280 x 32 x 4096, 48 tokens of 32
 // adapters: 6.6 us, 1.6 of them for the bytes from HBM.
 #include <cooperative_groups.h>
 
@@ -56,8 +56,8 @@ __global__ void __cluster_dims__(kLoraCluster, 1, 1) __launch_bounds__(kLoraThre
     const uint16_t* x = a.x + (size_t)t * a.K;
     // Columns of B, 32 a warp: R neighbouring lanes a row of B, 16 bytes each, R rows after one another; the first are on their way early.
     const int chunk = lane % R, g1 = (n1 - n0 + 31) / 32;
-    // (Held that early, eight words a lane cost a CTA of each SM: 7.5 / 7.8 us with / without at 32 tokens, 13.3 / 8.8 at 48; sixteen: 20.2 / 13.3
-    // at 24.  Asking L2 for them instead: 7.9, 9.1; 13.9.)
+    // (Held that early, eight words a lane cost a CTA of each SM: r = 64, 1280 x 4096, 7.5 / 7.8 us with / without at 32 tokens, 13.3 / 8.8 at 48, and
+    // 4096 x 2560 8.3 / 8.9 and 14.8 / 9.9; sixteen, r = 128, 20.2 / 13.3 at 24.  Asking L2 for them instead: 7.9, 9.1; 13.9.)
     constexpr bool kEarly = R < 8;
     uint4 bv[R];
     auto ask = [&](int g) {

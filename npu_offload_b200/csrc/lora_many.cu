@@ -18,7 +18,7 @@
 // sectors: the columns of B are dealt to the matrix instruction so that a lane's results are neighbours, as are its inner values,
 // eight bytes of a row of B.  base and B are asked for ahead of the wait for lora_low_kernel.
 //
-// 4093 tokens, 4096 x 16 x 2560: 23 us, 12 of them the first two kernels; x, base and out alone take 11.8 at a copy's rate.  (One
+// 4093 tokens, 4096 x 16 x 2560: 23.4 us, 12 of them the first two kernels; x, base and out alone take 11.8 at a copy's rate.  (One
 // kernel for low and out, the cluster going on to its columns: 26 to 29 us, since all CTAs load, exchange and store at the same time.)
 #include <cooperative_groups.h>
 

@@ -6,6 +6,9 @@
 // CTA, the next row's words already asked for.  A CTA takes every gridDim-th row and keeps its rows' share of dw in
 // registers (a column is always the same thread's), writes it once, and a second kernel adds the CTAs' shares in order: no
 // sum depends on timing.
+//
+// Bounded by HBM: 8191 x 4096, bf16 with the stream's gradient, 48 us, 85 % of a copy's rate; 8192 x 5120 71 (72 %), 7168 84 (86 %), fp32 4000 x 4096
+// 56 (72 %).  Where one CTA of few threads is all that an SM has, by what is on its way: fp32 4000 x 4099 110 us (36 %; it spills).
 #include <algorithm>
 
 #include "launch.cuh"
