@@ -459,7 +459,8 @@ class MoEDataPlane:
         logits [T, E] fp32; `groups` groups of E / groups neighbours, of which the top_groups best are open: by their largest
         logit (softmax scoring), or by the sum of their two largest s + bias (sigmoid; bias [E] fp32 only selects).  Then the
         top_k best experts of those, the best first, ties to the lower index; w = scale * softmax probability or s, divided by
-        the chosen ones' sum where renormalize is set.  The weights' gradient is route_backward()."""
+        the chosen ones' sum where renormalize is set.  A logit of -inf masks under softmax; under sigmoid a bias of -inf, or one well below
+        the others (faster), does.  The weights' gradient is route_backward()."""
         if stream is not None:
             with self._on(stream):
                 return self.route_groups(logits, groups, top_groups, bias, renormalize, scale)
