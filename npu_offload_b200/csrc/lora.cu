@@ -6,8 +6,8 @@
 // row, 16-byte loads), the partial sums go to all eight through distributed shared memory and are added there in order,
 // and each then takes an eighth of the columns of B, whose first are in registers by then up to r = 32: a row of B is read by as
 // many neighbouring lanes as it has 16-byte words (a thread a row: 10.6 instead of 7.5 us at 32 tokens, r = 64, when its columns were held
-// early too; 7.9 as it is, below).  All sums are fp32; the result is rounded once.  Bounded by latency for a token (ids, then x and A, the exchange, the store), by the adapters' bytes
-// out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.6 us (r = 64: 5.3, r = 128: 8.2); 1280 x 32 x 4096, 48 tokens of 32
+// early too; 7.9 as it is, below).  All sums are fp32; the result is rounded once.  Bounded by latency for a token (ids, then x and A,
+// the exchange, the store), by the adapters' bytes out of L2 for a batch of requests.  4096 x 16 x 2560, one token: 3.6 us (r = 64: 5.3, r = 128: 8.2); 1280 x 32 x 4096, 48 tokens of 32
 // adapters: 6.6 us, 1.6 of them for the bytes from HBM.
 #include <cooperative_groups.h>
 

@@ -208,7 +208,8 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
 }
 
 // The first bf16 part of v, in the upper half: v cut to eight bits, or, where nothing would be left, the next smaller.  So the rest has
-// v's sign and is 0 with v alone (from 2^-119 on, where all parts are within bf16's range), and an infinity of B times the parts is the infinity that it is times v; an infinite v is each part.
+// v's sign and is 0 with v alone (from 2^-119 on, where all parts are within bf16's range), and an infinity of B times
+// the parts is the infinity that it is times v; an infinite v is each part.
 __device__ __forceinline__ uint32_t lora_lead(float v) {
     const uint32_t u = __float_as_uint(v);
     return u & 0xffffu || (u << 1) == 0 || !(fabsf(v) < INFINITY) ? u & 0xffff0000u : u - 0x10000u;
